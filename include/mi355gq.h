@@ -443,6 +443,101 @@ MI355GQ_API int mi355gq_silu_mul_dt(const void* x, int64_t R, int64_t I, void* o
 MI355GQ_API int mi355gq_moe_combine_dt(const void* y, const void* slot_positions, const void* weights, int64_t T,
                            int64_t top_k, int64_t H, void* out, int model_dtype, mi355gq_stream_t stream);
 
+/* ---- 8-bit block-scaled models: e4m3 weights with a float32 scale per 128 x 128 block, activations in e4m3 groups ---- */
+
+/*
+ * Formats.  e4m3 is the 8-bit float with 4 exponent and 3 mantissa bits, no infinities, largest number 448.
+ *   activations q [rows, K], rows q_pitch bytes apart, scale float32 [ceil(K / 128), rows] (a group's scales lie side by side);
+ *   weights     q [N, K], rows w_pitch bytes apart, scale float32 [ceil(N / 128), ceil(K / 128)]; stacks of experts [experts, ...].
+ * The value of a number is q * scale.  Pitches are multiples of 16 and at least K; bases are 16-byte aligned.  What a row
+ * holds between K and its pitch is never used.
+ *
+ * mi355gq_fp8_quantize: x [rows, K] in model_dtype, dense -> q, scale.  A group's scale is the smallest power of two s
+ * with max|x| <= 448 s (at least 2^-126, and 1 for a group of zeros), q = x / s rounded to nearest, ties to even: one
+ * rounding, the same on any machine.  An infinity or NaN becomes NaN and leaves the scale to the group's other numbers.
+ * The bytes between K and the next multiple of 8 (at most the pitch) are written as zeros.
+ * mi355gq_fp8_silu_mul_quantize: the same of silu(x1) * x2, x = [x1, x2] [rows, 2 K], computed in float32.
+ * mi355gq_fp8_quantize_weight: w [mats, N, K] dense -> q, scale with one scale per block, chosen alike.
+ * mi355gq_fp8_dequantize: out [mats, rows, K] dense in out_dtype = q * scale; row_groups 1: the activations' scale (mats 1),
+ * 0: the weights'.
+ */
+MI355GQ_API int mi355gq_fp8_quantize(const void* x, int64_t rows, int64_t K, int model_dtype, void* q, int64_t q_pitch,
+                         void* scale, mi355gq_stream_t stream);
+MI355GQ_API int mi355gq_fp8_silu_mul_quantize(const void* x, int64_t rows, int64_t K, int model_dtype, void* q,
+                                  int64_t q_pitch, void* scale, mi355gq_stream_t stream);
+MI355GQ_API int mi355gq_fp8_quantize_weight(const void* w, int64_t mats, int64_t N, int64_t K, int model_dtype, void* q,
+                                int64_t q_pitch, void* scale, mi355gq_stream_t stream);
+MI355GQ_API int mi355gq_fp8_dequantize(const void* q, int64_t q_pitch, const void* scale, int64_t mats, int64_t rows,
+                           int64_t K, int row_groups, int out_dtype, void* out, mi355gq_stream_t stream);
+
+/*
+ * y[M, N] = x[M, K] . w[N, K]^T (+ bias[N]) (+ residual[M, N]) with both operands in e4m3: a block of 128 of K is
+ * summed, scaled by both its scales, which may be any float32 numbers, and joins a float32 sum; one rounding to out_dtype
+ * (MI355GQ_F16, MI355GQ_F32 or MI355GQ_BF16).
+ * precise 1: a block is summed in float32.  precise 0: it may be summed by the 8-bit matrix instructions, which drop what of a product
+ * lies more than about 17 bits below the largest of its step (about 1e-5 of a typical result, far below the rounding to a
+ * 16-bit type) and are faster.
+ * x_scale not null: x is e4m3 with rows x_pitch bytes apart and x_scale its scales.  x_scale null: x is dense in model_dtype
+ * and quantised on the way as mi355gq_fp8_quantize does; x_pitch is ignored.  bias and residual carry model_dtype;
+ * residual may be y itself where their types agree.  workspace: mi355gq_fp8_linear_workspace_bytes(M, N, K, x_scale != null) bytes,
+ * 16-byte aligned; MI355GQ_ERR_WORKSPACE where it is smaller.
+ */
+MI355GQ_API int64_t mi355gq_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_quantized);
+MI355GQ_API int mi355gq_fp8_linear(const void* x, int64_t x_pitch, const void* x_scale, const void* w, int64_t w_pitch,
+                       const void* w_scale, const void* bias, const void* residual, int64_t M, int64_t N, int64_t K,
+                       int model_dtype, int out_dtype, int precise, void* y, void* workspace, int64_t workspace_bytes,
+                       mi355gq_stream_t stream);
+
+/*
+ * The same product by expert segments: y[r] = x[x_row_index ? x_row_index[r] : r] . w[e]^T for indptr[e] <= r < indptr[e + 1]
+ * (indptr int32 [num_experts + 1], ascending from 0; x_row_index int32 [rows], clamped into x's x_rows rows).  x is e4m3 with
+ * x_scale [ceil(K / 128), x_rows]; y [rows, N] in out_dtype.  Rows outside every segment are left untouched.
+ */
+MI355GQ_API int mi355gq_fp8_group_gemm(const void* x, int64_t x_pitch, const void* x_scale, int64_t x_rows,
+                           const void* x_row_index, int64_t rows, const void* w, int64_t w_pitch, const void* w_scale,
+                           const void* indptr, int64_t num_experts, int64_t N, int64_t K, int out_dtype, int precise, void* y,
+                           mi355gq_stream_t stream);
+
+/*
+ * Router of such models: logits [T, num_experts] in model_dtype -> weights float32 [T, top_k], ids int32 [T, top_k] in
+ * descending order of
+ *   key = score + bias,  score = softmax over the row (MI355GQ_SCORE_SOFTMAX) or 1 / (1 + exp(-logit)) (MI355GQ_SCORE_SIGMOID),
+ * in float32; bias float32 [num_experts] or null moves the choice alone.  num_groups > 1: the experts are that many equal
+ * runs, a run stands by its best key (without a bias) or the sum of its two best (with one), and only the experts of the
+ * top_groups best runs are chosen from.  Ties keep the lower index.  weight = score of the chosen expert, divided by the chosen
+ * scores' sum where renormalize is not 0 (0 where that sum is 0), times scale.
+ * A NaN logit counts as score 0 and is chosen last.  num_experts <= 512, top_k <= 32, num_groups <= 64 and a divisor of
+ * num_experts, top_groups * (num_experts / num_groups) >= top_k.
+ */
+#define MI355GQ_SCORE_SOFTMAX 0
+#define MI355GQ_SCORE_SIGMOID 1
+MI355GQ_API int mi355gq_moe_gating(const void* logits, const void* bias, int64_t T, int64_t num_experts, int64_t top_k,
+                       int scoring, int64_t num_groups, int64_t top_groups, int renormalize, float scale, int model_dtype,
+                       void* weights, void* ids, mi355gq_stream_t stream);
+
+/*
+ * ids int32 [T, top_k] -> the slots t * top_k + j in the order of their expert, slot order within one: row_token int32 [T * top_k]
+ * (the token of each row), slot_row int32 [T * top_k] (the row of each slot; -1 for an id outside the experts, which has
+ * none), indptr int32 [num_experts + 1].
+ */
+MI355GQ_API int mi355gq_moe_plan(const void* ids, int64_t T, int64_t top_k, int64_t num_experts, void* row_token,
+                     void* slot_row, void* indptr, mi355gq_stream_t stream);
+
+/*
+ * One expert layer on routed tokens, x and out [T, hidden] in model_dtype (float16 or bfloat16):
+ *   out[t] = sum over j of weights[t, j] * w2[e] . q(silu(g) * u),  [g, u] = w13[e] . q(x[t]),  e = ids[t, j]
+ * q() quantises as mi355gq_fp8_quantize does; w13 [num_experts, 2 inter, hidden] (gate rows, then up rows), w2 [num_experts,
+ * hidden, inter], with their scales; weights float32 [T, top_k], ids int32 [T, top_k] (an id outside the experts adds nothing).
+ * Products sum as with precise 0 above, all other sums are in float32; an expert's output is rounded to model_dtype before it is weighted.  hidden and inter: multiples of 16.
+ * workspace: mi355gq_fp8_moe_workspace_bytes() bytes, 16-byte aligned.
+ */
+MI355GQ_API int64_t mi355gq_fp8_moe_workspace_bytes(int64_t T, int64_t hidden, int64_t inter, int64_t num_experts,
+                                        int64_t top_k);
+MI355GQ_API int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int64_t num_experts, int64_t top_k,
+                    const void* weights, const void* ids, const void* w13, int64_t w13_pitch, const void* w13_scale,
+                    const void* w2, int64_t w2_pitch, const void* w2_scale, int model_dtype, void* out, void* workspace,
+                    int64_t workspace_bytes, mi355gq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

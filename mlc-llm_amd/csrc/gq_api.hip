@@ -131,6 +131,16 @@ int launch_empty_k(const void* bias, const void* residual, void* y, int64_t rows
 
 }  // namespace
 
+namespace gq {
+int set_error(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+}  // namespace gq
+
 extern "C" {
 
 int mi355gq_version(void) { return MI355GQ_VERSION; }

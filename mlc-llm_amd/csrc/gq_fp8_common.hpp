@@ -1,0 +1,102 @@
+// Shared pieces of the 8-bit block-scaled kernels.
+//
+// An e4m3 group is 128 numbers of a row (activations) or a block of 128 x 128 (weights) and a float32 scale s: the value is
+// q s.  The quantisers here take the smallest power of two s with max|x| <= 448 s.  A power of two costs a floating format
+// no precision (but for the last octave of its subnormals), makes x / s and q s exact, and so leaves one rounding, the
+// one to e4m3, whose result does not depend on how the division is carried out.  The products take any float32 scale.
+#pragma once
+
+#include "gq_common.hpp"
+#include "gq_internal.hpp"
+
+namespace gq {
+
+constexpr int kFp8Block = 128;
+
+typedef int int4_t __attribute__((ext_vector_type(4)));
+typedef int int8_vt __attribute__((ext_vector_type(8)));
+
+// max|x| over the finite numbers of a group -> the bits of its scale: 448 = 1.75 2^8, so a top of 1.f 2^e takes
+// 2^(e-8) while 1.f <= 1.75 and 2^(e-7) beyond.  Not below 2^-126, and 1 for a group of zeros.
+__device__ __forceinline__ uint32_t fp8_scale_bits(float top) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, top);
+  const int e = static_cast<int>(u >> 23) - ((u & 0x7fffffu) <= 0x600000u ? 8 : 7);
+  return top > 0.f ? static_cast<uint32_t>(e < 1 ? 1 : e) << 23 : 0x3f800000u;
+}
+__device__ __forceinline__ float fp8_scale(float top) { return __builtin_bit_cast(float, fp8_scale_bits(top)); }
+// 1 / s of such a scale, exact (s lies in 2^-126 .. 2^120)
+__device__ __forceinline__ float fp8_inverse(uint32_t scale_bits) {
+  return __builtin_bit_cast(float, (254u << 23) - scale_bits);
+}
+// |x| where it is finite, 0 for an infinity or NaN: those become NaN in e4m3, and the scale is that of the others
+__device__ __forceinline__ float fp8_magnitude(float x) {
+  const float a = __builtin_fabsf(x);
+  return a <= 3.402823466e38f ? a : 0.f;
+}
+// two numbers, already divided by their scale, to e4m3 (nearest, ties to even) in the low half; not finite -> NaN
+__device__ __forceinline__ uint32_t fp8_pair(float a, float b) {
+  const float nan = __builtin_bit_cast(float, 0x7fc00000u);
+  a = __builtin_fabsf(a) <= 448.f ? a : nan;
+  b = __builtin_fabsf(b) <= 448.f ? b : nan;
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false)) & 0xffffu;
+}
+__device__ __forceinline__ uint32_t fp8_quad(float a, float b, float c, float d) {
+  return fp8_pair(a, b) | fp8_pair(c, d) << 16;
+}
+
+__device__ __forceinline__ float silu_mul_f32(float gate, float up) { return gate / (1.0f + expf(-gate)) * up; }
+
+// the largest of the 16 lanes of a DPP row, in every lane of it
+__device__ __forceinline__ float row_max16(float v) {
+  v = fmaxf(v, dpp_f<0xB1>(v));   // quad_perm [1,0,3,2]
+  v = fmaxf(v, dpp_f<0x4E>(v));   // quad_perm [2,3,0,1]
+  v = fmaxf(v, dpp_f<0x141>(v));  // row_half_mirror
+  return fmaxf(v, dpp_f<0x140>(v));  // row_mirror
+}
+
+// Arguments of an e4m3 product y[r, n] = sum over blocks g of xs[g, r] ws[n / 128, g] sum_k xq[r, k] wq[n, k].
+struct Fp8Args {
+  const uint8_t* x = nullptr;   // [x_rows, K], rows x_pitch bytes apart
+  const float* xs = nullptr;    // [ceil(K / 128), x_rows]
+  const uint8_t* w = nullptr;   // [experts, N, K], rows w_pitch bytes apart
+  const float* ws = nullptr;    // [experts, ceil(N / 128), ceil(K / 128)]
+  const void* bias = nullptr;      // [N] in model_dtype, or null
+  const void* residual = nullptr;  // [rows, N] in model_dtype, or null
+  void* y = nullptr;            // [rows, N] in out_dtype
+  const int32_t* indptr = nullptr;       // [experts + 1]: rows indptr[e] .. of expert e; null: one segment of all rows
+  const int32_t* x_row_index = nullptr;  // row r reads row x_row_index[r] of x; null: row r
+  int64_t rows = 0, x_rows = 0, N = 0, K = 0, x_pitch = 0, w_pitch = 0, experts = 1;
+  int model_dtype = 0, out_dtype = 0;
+  bool precise = false;  // blocks summed in float32, whatever the output type
+};
+hipError_t launch_fp8_gemm(const Fp8Args& a, hipStream_t s);
+
+// rows of x [rows, cols] (silu_mul: of x [rows, 2 cols], silu(first half) * second half) to e4m3 groups; the q bytes between
+// cols and pitch are written as zeros
+hipError_t launch_fp8_quantize(const void* x, int64_t rows, int64_t cols, int model_dtype, bool silu_mul, uint8_t* q,
+                               int64_t q_pitch, float* scale, hipStream_t s);
+hipError_t launch_fp8_quantize_weight(const void* w, int64_t mats, int64_t N, int64_t K, int model_dtype, uint8_t* q,
+                                      int64_t q_pitch, float* scale, hipStream_t s);
+hipError_t launch_fp8_dequantize(const uint8_t* q, int64_t q_pitch, const float* scale, int64_t mats, int64_t rows,
+                                 int64_t cols, bool row_groups, int out_dtype, void* out, hipStream_t s);
+
+// router logits [T, E] -> weights, ids [T, k]; see mi355gq_moe_gating
+struct GatingArgs {
+  const void* logits;
+  const float* bias;
+  int64_t T;
+  int E, k, sigmoid, groups, top_groups, renormalize, model_dtype;
+  float scale;
+  float* weights;
+  int32_t* ids;
+};
+hipError_t launch_moe_gating(const GatingArgs& a, hipStream_t s);
+// ids [slots] -> the slots in order of their expert, stable: row_token [slots] (slot / k), slot_row [slots] (-1 for an id
+// outside the experts), indptr [E + 1]
+hipError_t launch_moe_plan(const int32_t* ids, int64_t slots, int k, int E, int32_t* row_token, int32_t* slot_row,
+                           int32_t* indptr, hipStream_t s);
+// out[t] = sum over j of weights[t, j] y[row], row = slot_row[t k + j] (null: t k + j; negative: no such row), in float32
+hipError_t launch_moe_weighted_sum(const void* y, const int32_t* slot_row, const float* weights, int64_t T, int k, int64_t H,
+                                   int model_dtype, void* out, hipStream_t s);
+
+}  // namespace gq

@@ -56,6 +56,9 @@ void note_kernel(const char* fmt, A... a) {
   };
 }
 
+// sets the thread's message of mi355gq_last_error and returns `code`, for entry points outside gq_api.hip
+int set_error(int code, const char* fmt, ...);
+
 // hipFuncAttributeMaxDynamicSharedMemorySize = the CU's whole LDS, set once per (kernel, device) and remembered;
 // kernels whose dynamic LDS may exceed 64 KiB call it before launching.
 hipError_t allow_large_lds(const void* kernel);

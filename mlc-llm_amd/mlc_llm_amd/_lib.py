@@ -14,7 +14,7 @@ import importlib.util
 import os
 import re
 import warnings
-from ctypes import c_char_p, c_int, c_int64, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "lib", "libmi355gq.so")
@@ -27,8 +27,9 @@ F16, F32, BF16 = 0, 1, 2
 ROUND_HALF_AWAY, ROUND_HALF_EVEN = 0, 1
 I32, I64 = 0, 1
 EPILOGUE_NONE, EPILOGUE_SILU_MUL = 0, 1
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 
-_P, _I, _L = c_void_p, c_int, c_int64
+_P, _I, _L, _F = c_void_p, c_int, c_int64, c_float
 
 # name -> (restype, argtypes); mirrors include/mi355gq.h one to one
 SIGNATURES = {
@@ -89,6 +90,17 @@ SIGNATURES = {
     "mi355gq_moe_scatter_output": (_I, [_P, _P, _L, _L, _P, _P]),
     "mi355gq_silu_mul": (_I, [_P, _L, _L, _P, _P]),
     "mi355gq_moe_combine": (_I, [_P, _P, _L, _L, _L, _P, _P]),
+    "mi355gq_fp8_quantize": (_I, [_P, _L, _L, _I, _P, _L, _P, _P]),
+    "mi355gq_fp8_silu_mul_quantize": (_I, [_P, _L, _L, _I, _P, _L, _P, _P]),
+    "mi355gq_fp8_quantize_weight": (_I, [_P, _L, _L, _L, _I, _P, _L, _P, _P]),
+    "mi355gq_fp8_dequantize": (_I, [_P, _L, _P, _L, _L, _L, _I, _I, _P, _P]),
+    "mi355gq_fp8_linear_workspace_bytes": (_L, [_L, _L, _L, _I]),
+    "mi355gq_fp8_linear": (_I, [_P, _L, _P, _P, _L, _P, _P, _P, _L, _L, _L, _I, _I, _I, _P, _P, _L, _P]),
+    "mi355gq_fp8_group_gemm": (_I, [_P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _L, _L, _L, _I, _I, _P, _P]),
+    "mi355gq_moe_gating": (_I, [_P, _P, _L, _L, _L, _I, _L, _L, _I, _F, _I, _P, _P, _P]),
+    "mi355gq_moe_plan": (_I, [_P, _L, _L, _L, _P, _P, _P, _P]),
+    "mi355gq_fp8_moe_workspace_bytes": (_L, [_L, _L, _L, _L, _L]),
+    "mi355gq_fp8_moe": (_I, [_P, _L, _L, _L, _L, _L, _P, _P, _P, _L, _P, _P, _L, _P, _I, _P, _P, _L, _P]),
 }
 
 

@@ -645,3 +645,254 @@ def moe_combine(y: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
     _lib.call("mi355gq_moe_combine_dt", y.data_ptr(), None, weights.data_ptr(), t, k, h, out.data_ptr(),
               _MODEL_DTYPES[y.dtype], _stream())
     return out
+
+
+# ---- 8-bit block-scaled models ----
+#
+# An e4m3 tensor is a torch.float8_e4m3fn tensor whose rows lie a multiple of 16 bytes apart (its last dimension contiguous; rows
+# of a last size that is no multiple of 16 are a view of a wider allocation, as fp8_quantize and fp8_quantize_weight make them).
+
+FP8_BLOCK = 128
+_E4M3 = torch.float8_e4m3fn
+_SCORING = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
+
+
+def _fp8_empty(lead, k: int, device) -> torch.Tensor:
+    return torch.empty((*lead, -(-k // 16) * 16), dtype=_E4M3, device=device)[..., :k]
+
+
+def _chk_fp8(t: torch.Tensor, name: str, dims: int) -> int:
+    """The pitch of an e4m3 tensor's rows in bytes."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: must live on the GPU (got {t.device})")
+    if t.dtype != _E4M3:
+        raise TypeError(f"{name}: dtype {t.dtype}, expected {_E4M3}")
+    if t.dim() != dims:
+        raise ValueError(f"{name}: {t.dim()} dimensions, expected {dims}")
+    k = t.shape[-1]
+    pitch = t.stride(-2) if t.shape[-2] > 1 else max(t.stride(-2), -(-k // 16) * 16)
+    if t.numel() and ((k > 1 and t.stride(-1) != 1) or pitch < k or pitch % 16
+                      or (dims == 3 and t.shape[0] > 1 and t.stride(0) != t.shape[1] * pitch)):
+        raise ValueError(f"{name}: rows must be contiguous and lie a multiple of 16 bytes apart (strides {t.stride()}); "
+                         "fp8_quantize_weight makes such a tensor, torch.nn.functional.pad one of a checkpoint's")
+    if t.numel() and t.shape[-2] == 1 and k % 16 and t.untyped_storage().nbytes() - t.storage_offset() < pitch:
+        raise ValueError(f"{name}: a row of {k} bytes needs {pitch} of storage")
+    return max(pitch, -(-k // 16) * 16)
+
+
+def _chk_scale(t: torch.Tensor, shape, name: str) -> torch.Tensor:
+    _chk(t, torch.float32, name)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return t
+
+
+def fp8_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x [rows, K] -> e4m3 [rows, K] in groups of 128 along K, and their scales float32 [ceil(K / 128), rows]: the smallest
+    power of two that brings a group's largest magnitude to 448 or below."""
+    _chk(x, _FLOATS, "x")
+    if x.dim() != 2:
+        raise ValueError(f"fp8_quantize: x must be [rows, K], got {tuple(x.shape)}")
+    rows, k = x.shape
+    q = _fp8_empty((rows,), k, x.device)
+    scale = torch.empty((-(-k // FP8_BLOCK), rows), dtype=torch.float32, device=x.device)
+    _lib.call("mi355gq_fp8_quantize", x.data_ptr(), rows, k, _MODEL_DTYPES[x.dtype], q.data_ptr(), -(-k // 16) * 16, scale.data_ptr(),
+              _stream())
+    return q, scale
+
+
+def fp8_silu_mul_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp8_quantize of silu(x1) * x2, x [rows, 2 K] = [x1, x2], computed in float32."""
+    _chk(x, _FLOATS, "x")
+    if x.dim() != 2 or x.shape[1] % 2:
+        raise ValueError(f"fp8_silu_mul_quantize: x must be [rows, 2 K], got {tuple(x.shape)}")
+    rows, k = x.shape[0], x.shape[1] // 2
+    q = _fp8_empty((rows,), k, x.device)
+    scale = torch.empty((-(-k // FP8_BLOCK), rows), dtype=torch.float32, device=x.device)
+    _lib.call("mi355gq_fp8_silu_mul_quantize", x.data_ptr(), rows, k, _MODEL_DTYPES[x.dtype], q.data_ptr(), -(-k // 16) * 16,
+              scale.data_ptr(), _stream())
+    return q, scale
+
+
+def fp8_quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """w [..., N, K] -> e4m3 [..., N, K] and a scale for each block of 128 x 128, float32 [..., ceil(N / 128), ceil(K / 128)]."""
+    _chk(w, _FLOATS, "w")
+    if w.dim() not in (2, 3):
+        raise ValueError(f"fp8_quantize_weight: w must be [N, K] or [experts, N, K], got {tuple(w.shape)}")
+    lead, (n, k) = tuple(w.shape[:-2]), w.shape[-2:]
+    q = _fp8_empty((*lead, n), k, w.device)
+    scale = torch.empty((*lead, -(-n // FP8_BLOCK), -(-k // FP8_BLOCK)), dtype=torch.float32, device=w.device)
+    _lib.call("mi355gq_fp8_quantize_weight", w.data_ptr(), lead[0] if lead else 1, n, k, _MODEL_DTYPES[w.dtype], q.data_ptr(),
+              -(-k // 16) * 16, scale.data_ptr(), _stream())
+    return q, scale
+
+
+def fp8_dequantize(q: torch.Tensor, scale: torch.Tensor, out_dtype=torch.float32, row_groups: bool = False) -> torch.Tensor:
+    """q * scale of e4m3 weights [..., N, K] with their block scales, or (row_groups) of activations [rows, K] with theirs."""
+    pitch = _chk_fp8(q, "q", 2 if row_groups else q.dim() if isinstance(q, torch.Tensor) and q.dim() == 3 else 2)
+    lead, (n, k) = tuple(q.shape[:-2]), q.shape[-2:]
+    groups = -(-k // FP8_BLOCK)
+    _chk_scale(scale, (groups, n) if row_groups else (*lead, -(-n // FP8_BLOCK), groups), "scale")
+    if out_dtype not in _MODEL_DTYPES:
+        raise TypeError(f"out_dtype {out_dtype}")
+    out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+    _lib.call("mi355gq_fp8_dequantize", q.data_ptr(), pitch, scale.data_ptr(), lead[0] if lead else 1, n, k, 1 if row_groups else 0,
+              _MODEL_DTYPES[out_dtype], out.data_ptr(), _stream())
+    return out
+
+
+def fp8_linear(x, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None, out_dtype=None,
+               residual: Optional[torch.Tensor] = None, precise: Optional[bool] = None) -> torch.Tensor:
+    """y[..., N] = x[..., K] . (weight * weight_scale)^T (+ bias) (+ residual), both operands in e4m3.
+
+    x: a float16, bfloat16 or float32 tensor, which is quantised on the way as fp8_quantize does, or the pair (q, scale) that
+    fp8_quantize gives.  weight e4m3 [N, K], weight_scale float32 [ceil(N / 128), ceil(K / 128)].  bias and residual have x's
+    type (of a pair: the output's, float16 by default), the output out_dtype, or that type.
+
+    precise: blocks of 128 are summed in float32.  Without it they may be summed by the 8-bit matrix instructions, which drop what of
+    a product lies more than about 17 bits below the largest of its step: 1e-5 of a typical result.  None: a float32 output is precise, a
+    16-bit one, whose rounding is far larger, is not.  Blocks join one another in float32 either way."""
+    pair = isinstance(x, (tuple, list))
+    if pair:
+        if len(x) != 2:
+            raise ValueError("fp8_linear: x must be a tensor or the pair (q, scale)")
+        q, x_scale = x
+        x_pitch = _chk_fp8(q, "x", 2)
+        _chk_scale(x_scale, (-(-q.shape[1] // FP8_BLOCK), q.shape[0]), "x scale")
+        out_dtype = torch.float16 if out_dtype is None else out_dtype
+        dtype, x = out_dtype, q
+    else:
+        _chk(x, _FLOATS, "x")
+        x_scale, x_pitch, dtype = None, 0, x.dtype
+        out_dtype = dtype if out_dtype is None else out_dtype
+    if out_dtype not in _MODEL_DTYPES:
+        raise TypeError(f"out_dtype {out_dtype}")
+    w_pitch = _chk_fp8(weight, "weight", 2)
+    n, k = weight.shape
+    if x.dim() < 1 or x.shape[-1] != k or k == 0:
+        raise ValueError(f"fp8_linear: x {tuple(x.shape)} for a weight of {tuple(weight.shape)}")
+    _chk_scale(weight_scale, (-(-n // FP8_BLOCK), -(-k // FP8_BLOCK)), "weight_scale")
+    m = 1
+    for d in x.shape[:-1]:
+        m *= d
+    shape = (*x.shape[:-1], n)
+    if bias is not None:
+        _chk(bias, dtype, "bias")
+        if tuple(bias.shape) != (n,):
+            raise ValueError(f"bias shape {tuple(bias.shape)}, expected {(n,)}")
+    if residual is not None:
+        _chk(residual, dtype, "residual")
+        if tuple(residual.shape) != shape:
+            raise ValueError(f"residual shape {tuple(residual.shape)}, expected {shape}")
+    out = torch.empty(shape, dtype=out_dtype, device=x.device)
+    ws_bytes = _lib.lib().mi355gq_fp8_linear_workspace_bytes(m, n, k, 1 if pair else 0)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+    _lib.call("mi355gq_fp8_linear", x.data_ptr(), x_pitch, x_scale.data_ptr() if pair else None, weight.data_ptr(), w_pitch,
+              weight_scale.data_ptr(), bias.data_ptr() if bias is not None else None,
+              residual.data_ptr() if residual is not None else None, m, n, k, _MODEL_DTYPES[dtype], _MODEL_DTYPES[out_dtype],
+              1 if (out_dtype == torch.float32 if precise is None else precise) else 0, out.data_ptr(), ws.data_ptr() if ws is not None else None, ws_bytes, _stream())
+    return out
+
+
+def fp8_group_gemm(q: torch.Tensor, scale: torch.Tensor, x_row_index: Optional[torch.Tensor], weight: torch.Tensor,
+                   weight_scale: torch.Tensor, indptr: torch.Tensor, out_dtype=torch.float16, precise: Optional[bool] = None
+                   ) -> torch.Tensor:
+    """The product by expert segments: y[r] = x[x_row_index[r]] . weight[e]^T for indptr[e] <= r < indptr[e + 1]; q, scale as
+    fp8_quantize gives them, weight e4m3 [experts, N, K].  x_row_index None: row r of x.  Rows outside every segment are zeros.
+    precise: see fp8_linear."""
+    x_pitch, w_pitch = _chk_fp8(q, "q", 2), _chk_fp8(weight, "weight", 3)
+    experts, n, k = weight.shape
+    if q.shape[1] != k or k == 0:
+        raise ValueError(f"fp8_group_gemm: q {tuple(q.shape)} for weights of {tuple(weight.shape)}")
+    groups = -(-k // FP8_BLOCK)
+    _chk_scale(scale, (groups, q.shape[0]), "scale")
+    _chk_scale(weight_scale, (experts, -(-n // FP8_BLOCK), groups), "weight_scale")
+    _chk(indptr, torch.int32, "indptr")
+    if tuple(indptr.shape) != (experts + 1,):
+        raise ValueError(f"indptr shape {tuple(indptr.shape)}, expected {(experts + 1,)}")
+    if out_dtype not in _MODEL_DTYPES:
+        raise TypeError(f"out_dtype {out_dtype}")
+    rows = q.shape[0]
+    if x_row_index is not None:
+        _chk(x_row_index, torch.int32, "x_row_index")
+        rows = x_row_index.numel()
+    out = torch.zeros((rows, n), dtype=out_dtype, device=q.device)
+    _lib.call("mi355gq_fp8_group_gemm", q.data_ptr(), x_pitch, scale.data_ptr(), q.shape[0],
+              x_row_index.data_ptr() if x_row_index is not None else None, rows, weight.data_ptr(), w_pitch, weight_scale.data_ptr(),
+              indptr.data_ptr(), experts, n, k, _MODEL_DTYPES[out_dtype],
+              1 if (out_dtype == torch.float32 if precise is None else precise) else 0, out.data_ptr(), _stream())
+    return out
+
+
+def moe_gating(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: Optional[torch.Tensor] = None, num_groups: int = 1,
+               top_groups: int = 1, renormalize: bool = True, scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Router logits [T, experts] -> (weights float32 [T, top_k], ids int32 [T, top_k]), best first.
+
+    scoring: "softmax" over the row, or "sigmoid" of each logit.  bias float32 [experts] is added for the choice, not to the
+    weights.  num_groups > 1: only the experts of the top_groups best of that many equal runs of experts are chosen from; a
+    run stands by its best key, or with a bias by the sum of its two best.  renormalize: the chosen scores are divided by their
+    sum.  Ties keep the lower index; a NaN logit is chosen last."""
+    _chk(logits, _FLOATS, "logits")
+    if logits.dim() != 2:
+        raise ValueError(f"moe_gating: logits must be [T, experts], got {tuple(logits.shape)}")
+    if scoring not in _SCORING:
+        raise ValueError(f"moe_gating: scoring {scoring!r}, expected one of {sorted(_SCORING)}")
+    t, ne = logits.shape
+    if bias is not None:
+        _chk_scale(bias, (ne,), "bias")
+    weights = torch.empty((t, max(top_k, 0)), dtype=torch.float32, device=logits.device)
+    ids = torch.empty((t, max(top_k, 0)), dtype=torch.int32, device=logits.device)
+    _lib.call("mi355gq_moe_gating", logits.data_ptr(), bias.data_ptr() if bias is not None else None, t, ne, top_k, _SCORING[scoring],
+              num_groups, top_groups, 1 if renormalize else 0, float(scale), _MODEL_DTYPES[logits.dtype], weights.data_ptr(),
+              ids.data_ptr(), _stream())
+    return weights, ids
+
+
+def moe_plan(ids: torch.Tensor, num_experts: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """ids int32 [T, k] -> the slots in the order of their expert: (row_token [T * k], slot_row [T * k], indptr [experts + 1])."""
+    _chk(ids, torch.int32, "ids")
+    if ids.dim() != 2:
+        raise ValueError(f"moe_plan: ids must be [T, k], got {tuple(ids.shape)}")
+    t, k = ids.shape
+    row_token, slot_row = (torch.zeros((t * k,), dtype=torch.int32, device=ids.device) for _ in range(2))
+    indptr = torch.empty((max(num_experts, 0) + 1,), dtype=torch.int32, device=ids.device)
+    _lib.call("mi355gq_moe_plan", ids.data_ptr(), t, k, num_experts, row_token.data_ptr(), slot_row.data_ptr(), indptr.data_ptr(),
+              _stream())
+    return row_token, slot_row, indptr
+
+
+def fp8_moe_experts(x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor,
+                    w2: torch.Tensor, w2_scale: torch.Tensor) -> torch.Tensor:
+    """One expert layer on routed tokens: x [T, hidden] float16 or bfloat16, weights float32 [T, k] and ids int32 [T, k] as
+    moe_gating gives them, w13 e4m3 [experts, 2 inter, hidden] (gate rows, then up rows), w2 e4m3 [experts, hidden, inter].
+    An id outside the experts adds nothing."""
+    _chk(x, (torch.float16, torch.bfloat16), "x")
+    _chk(ids, torch.int32, "ids")
+    pitch13, pitch2 = _chk_fp8(w13, "w13", 3), _chk_fp8(w2, "w2", 3)
+    ne, hidden, inter = w2.shape
+    if tuple(w13.shape) != (ne, 2 * inter, hidden) or x.dim() != 2 or x.shape[1] != hidden:
+        raise ValueError(f"fp8_moe: x {tuple(x.shape)}, w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} do not belong together")
+    t = x.shape[0]
+    if ids.dim() != 2 or ids.shape[0] != t:
+        raise ValueError(f"fp8_moe: ids {tuple(ids.shape)} for {t} tokens")
+    _chk_scale(weights, ids.shape, "weights")
+    _chk_scale(w13_scale, (ne, -(-2 * inter // FP8_BLOCK), -(-hidden // FP8_BLOCK)), "w13_scale")
+    _chk_scale(w2_scale, (ne, -(-hidden // FP8_BLOCK), -(-inter // FP8_BLOCK)), "w2_scale")
+    k = ids.shape[1]
+    out = torch.empty_like(x)
+    ws_bytes = _lib.lib().mi355gq_fp8_moe_workspace_bytes(t, hidden, inter, ne, k)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+    _lib.call("mi355gq_fp8_moe", x.data_ptr(), t, hidden, inter, ne, k, weights.data_ptr(), ids.data_ptr(), w13.data_ptr(), pitch13,
+              w13_scale.data_ptr(), w2.data_ptr(), pitch2, w2_scale.data_ptr(), _MODEL_DTYPES[x.dtype], out.data_ptr(),
+              ws.data_ptr() if ws is not None else None, ws_bytes, _stream())
+    return out
+
+
+def fp8_moe(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor,
+            w2_scale: torch.Tensor, top_k: int, scoring: str = "softmax", bias: Optional[torch.Tensor] = None, num_groups: int = 1,
+            top_groups: int = 1, renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """moe_gating on the router's logits [T, experts], then fp8_moe_experts."""
+    weights, ids = moe_gating(logits, top_k, scoring, bias, num_groups, top_groups, renormalize, scale)
+    return fp8_moe_experts(x, weights, ids, w13, w13_scale, w2, w2_scale)

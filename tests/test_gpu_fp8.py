@@ -1,0 +1,463 @@
+"""8-bit block-scaled operators against their definitions in float64: quantisers bit for bit, products and the expert layer within
+bounds that follow from their roundings."""
+
+import numpy as np
+import pytest
+import torch
+
+import mlc_llm_amd as gq
+from mlc_llm_amd import ops
+
+E4M3 = torch.float8_e4m3fn
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+UNIT = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8, torch.float32: 2.0**-24}  # half a step, relative
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---- the definitions, on the CPU in float64 ----
+
+
+def e4m3(v):
+    _, power = torch.frexp(v)
+    step = torch.ldexp(torch.ones_like(v), (power - 4).clamp(min=-9))
+    return torch.where(v.abs() <= 464, torch.round(v / step) * step, torch.nan)
+
+
+def pow2_scale(top):
+    part, power = torch.frexp(top)
+    power = torch.where(part > 0.875, power - 8, power - 9).clamp(min=-126)
+    return torch.where(top > 0, torch.ldexp(torch.ones_like(top), power), 1.0)
+
+
+def quantized(x, rows_per_block=1):
+    """x float64 [R, K] -> (q, scale [ceil(R / rows_per_block), ceil(K / 128)], q * scale)."""
+    q, val = torch.empty_like(x), torch.empty_like(x)
+    r, k = x.shape
+    scale = torch.empty((-(-r // rows_per_block), -(-k // 128)), dtype=torch.float64)
+    for g in range(scale.shape[1]):
+        part = x[:, 128 * g : 128 * g + 128]
+        top = torch.where(part.isfinite(), part.abs(), 0.0).amax(1)
+        if rows_per_block > 1:
+            top = torch.stack([t.amax() for t in top.split(rows_per_block)])
+        s = pow2_scale(top)
+        scale[:, g] = s
+        s = s.repeat_interleave(rows_per_block)[:r, None]
+        q[:, 128 * g : 128 * g + 128] = e4m3(part / s)
+        val[:, 128 * g : 128 * g + 128] = q[:, 128 * g : 128 * g + 128] * s
+    return q, scale, val
+
+
+def block_values(q, scale):
+    n, k = q.shape
+    return q.double() * scale.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+
+
+def route(logits, bias, k, scoring, groups, top_groups, renorm, scale):
+    """By sorting, in float64: (weights, ids) of one batch."""
+    x = logits.double()
+    nan = x.isnan()
+    x = torch.where(nan, -torch.inf, x).clamp(max=3.402823466e38)
+    if scoring == "sigmoid":
+        score = torch.sigmoid(x)
+    else:
+        m = x.amax(1, keepdim=True)
+        e = torch.where(x == -torch.inf, 0.0, torch.exp(x - torch.where(m == -torch.inf, 0.0, m)))
+        score = e / e.sum(1, keepdim=True).clamp(min=1e-300)
+    key = score + (0 if bias is None else bias.double())
+    key = torch.where(nan | key.isnan(), -torch.inf, key)
+    t, ne = key.shape
+    weights, ids = torch.zeros(t, k, dtype=torch.float64), torch.zeros(t, k, dtype=torch.int64)
+    size = ne // groups
+    for i in range(t):
+        row = key[i].tolist()
+        allowed = range(ne)
+        if groups > 1:
+            stand = []
+            for g in range(groups):
+                part = sorted(row[g * size : g * size + size], reverse=True)
+                stand.append(part[0] if bias is None or size == 1 else part[0] + part[1])
+            best = sorted(range(groups), key=lambda g: (-stand[g], g))[:top_groups]
+            allowed = [e for e in range(ne) if e // size in best]
+        chosen = sorted(allowed, key=lambda e: (-row[e], e))[:k]
+        ids[i] = torch.tensor(chosen)
+        w = score[i, chosen]
+        if renorm:
+            w = w / w.sum() if w.sum() > 0 else w * 0
+        weights[i] = w * scale
+    return weights, ids
+
+
+def experts_layer(x, weights, ids, w13, s13, w2, s2):
+    """float64 expert layer on e4m3 inputs; also the sum of magnitudes that bounds its roundings."""
+    inter, ne = w2.shape[2], w2.shape[0]
+    xv = quantized(x.double())[2]
+    out, size = torch.zeros_like(xv), torch.zeros_like(xv)
+    for e in range(ne):
+        token, slot = torch.nonzero(ids == e, as_tuple=True)
+        if len(token) == 0:
+            continue
+        both = xv[token] @ block_values(w13[e], s13[e]).t()
+        gate, up = both[:, :inter], both[:, inter:]
+        h = quantized(gate * torch.sigmoid(gate) * up)[2]
+        down = block_values(w2[e], s2[e])
+        for i, (t, s) in enumerate(zip(token.tolist(), slot.tolist())):
+            out[t] += weights[t, s].double() * (h[i] @ down.t())
+            size[t] += weights[t, s].double().abs() * (h[i].abs() @ down.abs().t())
+    return out, size
+
+
+# ---- quantisers ----
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k", [(1, 128), (3, 1), (5, 127), (2, 129), (7, 4096), (33, 272), (1, 14336), (130, 1000), (0, 64), (4, 513)])
+def test_quantize_rows_bit_for_bit(dtype, rows, k):
+    g = _gen(rows * 10007 + k)
+    x = (torch.randn(rows, k, generator=g) * torch.exp(3 * torch.randn(rows, 1, generator=g))).to(dtype)
+    if rows > 2:
+        x[1] = 0  # groups of nothing but zeros
+        x[2] = torch.where(torch.rand(k, generator=g) < 0.5, x[2] * 2.0**-12, x[2])  # e4m3 subnormals
+    q, scale = ops.fp8_quantize(x.cuda())
+    assert q.shape == (rows, k) and q.dtype == E4M3 and scale.shape == (-(-k // 128), rows)
+    if rows == 0:
+        return
+    want_q, want_s, want_v = quantized(x.double())
+    assert torch.equal(scale.cpu().double().t(), want_s)
+    assert torch.equal(q.cpu().double(), want_q)
+    for out in DTYPES:
+        back = ops.fp8_dequantize(q, scale, out, row_groups=True).cpu()
+        assert torch.equal(back, want_v.to(torch.float32).to(out))
+
+
+def test_quantize_extremes():
+    x = torch.zeros(9, 256)
+    x[0, 0] = 448.0  # exactly the top: scale 1
+    x[1, 0] = float(np.nextafter(np.float32(448.0), np.float32(1e9)))  # past it: scale 2
+    x[2, :3] = torch.tensor([torch.inf, 3.0, torch.nan])
+    x[3, :] = torch.nan
+    x[4, 128] = 3.402823466e38
+    x[5, 0] = 1e-45  # the smallest subnormal
+    x[6, 0] = 2.0**-126
+    x[7, :4] = torch.tensor([448.0, 17.0, 19.0, 0.0009765625])  # ties: 17 -> 16, 19 -> 20; half of the smallest subnormal -> 0
+    x[8, :3] = torch.tensor([-448.0, -17.0, -0.0])
+    q, scale = ops.fp8_quantize(x.cuda())
+    want_q, want_s, _ = quantized(x.double())
+    assert torch.equal(scale.cpu().double().t(), want_s)
+    got = q.cpu().double()
+    assert torch.equal(got.isnan(), want_q.isnan()) and torch.equal(got.nan_to_num(), want_q.nan_to_num())
+    assert got[2, 0].isnan() and got[2, 2].isnan() and got[2, 1] == 384 and got[7, :4].tolist() == [448, 16, 20, 0]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("mats,n,k", [(None, 128, 128), (None, 1, 1), (None, 300, 400), (3, 130, 257), (None, 127, 2048), (2, 256, 72)])
+def test_quantize_weight_bit_for_bit(dtype, mats, n, k):
+    w = (0.02 * torch.randn(mats or 1, n, k, generator=_gen(n + k))).to(dtype)
+    q, scale = ops.fp8_quantize_weight(w.cuda() if mats else w[0].cuda())
+    q, scale = (q, scale) if mats else (q[None], scale[None])
+    back = ops.fp8_dequantize(q, scale, torch.float32).cpu().double()
+    for m in range(mats or 1):
+        want_q, want_s, want_v = quantized(w[m].double(), 128)
+        assert torch.equal(scale[m].cpu().double(), want_s)
+        assert torch.equal(q[m].cpu().double(), want_q) and torch.equal(back[m], want_v)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k", [(1, 128), (5, 200), (3, 13), (17, 1408)])
+def test_silu_mul_quantize(dtype, rows, k):
+    x = (2 * torch.randn(rows, 2 * k, generator=_gen(rows + k))).to(dtype)
+    q, scale = ops.fp8_silu_mul_quantize(x.cuda())
+    gate, up = x.double().chunk(2, 1)
+    exact = gate * torch.sigmoid(gate) * up
+    # float32 arithmetic is a few 2^-24 off before the rounding to e4m3, which moves a number by at most half a step: a sixteenth
+    # of it, or 2^-10 scales below the subnormals' start
+    s = scale.cpu().double().t().repeat_interleave(128, 1)[:, :k]
+    got = q.cpu().double() * s
+    assert (((got - exact).abs() <= exact.abs() * (2.0**-4 + 2.0**-20) + 2.0**-10 * s * (1 + 2.0**-10))).all()
+    top = torch.stack([p.abs().amax(1) for p in exact.split(128, 1)], 1)
+    ratio = top / scale.cpu().double().t()
+    assert (ratio <= 448 * (1 + 2.0**-20)).all() and (ratio > 224 * (1 - 2.0**-20)).all()
+
+
+# ---- products ----
+
+
+def _weights(n, k, seed, experts=None):
+    g = _gen(seed)
+    lead = () if experts is None else (experts,)
+    q = (100 * torch.randn(*lead, n, -(-k // 16) * 16, generator=g)).clamp(-448, 448).to(E4M3)
+    scale = 2e-4 * (0.5 + torch.rand(*lead, -(-n // 128), -(-k // 128), generator=g))
+    # what lies between K and the pitch is never used: NaN there
+    q.view(torch.uint8)[..., k:] = 0x7F
+    return q, scale
+
+
+def _linear_bound(xv, wv, want, out_dtype):
+    # float32 sums: at most (K / 128 + 16) additions in a row each 2^-24 of a partial sum, whose size the magnitudes bound, the two
+    # scales' product and its use (3 roundings); then one rounding to the output type
+    size = xv.abs() @ wv.abs().t()
+    return size * (xv.shape[1] / 128 + 20) * 2.0**-23 + want.abs() * UNIT[out_dtype] + 2.0**-24 * (out_dtype == torch.float16)
+
+
+SHAPES = [(1, 64, 128), (1, 1, 1), (1, 4096, 4096), (2, 300, 400), (3, 129, 1000), (5, 1000, 272), (8, 2056, 1544), (16, 512, 2048), (17, 136, 4096),
+          (24, 768, 1408), (32, 264, 14336), (33, 640, 528), (64, 256, 256), (65, 257, 129), (100, 1024, 4096), (128, 384, 1040), (200, 520, 2000),
+          (256, 512, 512), (300, 4096, 1024), (513, 776, 384), (1, 20008, 144), (7, 28672, 256), (40, 96, 5120)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear(m, n, k, dtype):
+    g = _gen(m + 3 * n + 7 * k)
+    x = (torch.randn(m, k, generator=g) * torch.exp(torch.randn(m, 1, generator=g))).to(dtype)
+    w, ws = _weights(n, k, n + k)
+    bias = torch.randn(n, generator=g).to(dtype)
+    residual = torch.randn(m, n, generator=g).to(dtype)
+    wd = w.cuda()[:, :k]
+    xv, wv = quantized(x.double())[2], block_values(w[:, :k].float().nan_to_num(), ws)
+    exact = xv @ wv.t()
+    out_dtypes = {dtype, torch.float32}
+    for out in out_dtypes:
+        y = ops.fp8_linear(x.cuda(), wd, ws.cuda(), out_dtype=out, precise=True).cpu().double()
+        assert ((y - exact).abs() <= _linear_bound(xv, wv, exact, out)).all(), (y - exact).abs().max()
+    q, s = ops.fp8_quantize(x.cuda())
+    y = ops.fp8_linear((q, s), wd, ws.cuda(), out_dtype=torch.float32).cpu().double()
+    assert ((y - exact).abs() <= _linear_bound(xv, wv, exact, torch.float32)).all()
+    want = exact + bias.double() + residual.double()
+    y = ops.fp8_linear(x.cuda(), wd, ws.cuda(), bias=bias.cuda(), residual=residual.cuda(), precise=True).cpu().double()
+    extra = (exact.abs() + bias.double().abs() + residual.double().abs()) * 2.0**-22
+    assert ((y - want).abs() <= _linear_bound(xv, wv, want, dtype) + extra).all()
+
+
+def test_linear_leading_dimensions_strides_and_scales():
+    w, ws = _weights(200, 384, 1)
+    wide = torch.zeros(200, 640, dtype=E4M3)
+    wide[:, :384] = w
+    x = torch.randn(2, 3, 384, generator=_gen(2)).to(torch.bfloat16).cuda()
+    y = ops.fp8_linear(x, wide.cuda()[:, :384], ws.cuda())
+    assert y.shape == (2, 3, 200) and torch.equal(y, ops.fp8_linear(x, w.cuda(), ws.cuda()))
+    # scales that are no powers of two, on both sides
+    q, s = ops.fp8_quantize(x.view(6, 384))
+    s = s * (1 + torch.rand(s.shape, generator=_gen(3)).cuda())
+    xv = q.cpu().double() * s.cpu().double().t().repeat_interleave(128, 1)
+    wv = block_values(w, ws)
+    exact = xv @ wv.t()
+    y = ops.fp8_linear((q, s), w.cuda(), ws.cuda(), out_dtype=torch.float32).cpu().double()
+    assert ((y - exact).abs() <= _linear_bound(xv, wv, exact, torch.float32)).all()
+    assert ops.fp8_linear(x[:0], w.cuda(), ws.cuda()).shape == (0, 3, 200)
+
+
+@pytest.mark.parametrize("m", [1, 20, 40, 300])
+def test_linear_keeps_what_is_not_finite_in_its_row(m):
+    w, ws = _weights(256, 512, 5)
+    x = torch.randn(m, 512, generator=_gen(6)).to(torch.float16)
+    clean = ops.fp8_linear(x.cuda(), w.cuda(), ws.cuda())
+    x[0, 300] = torch.inf
+    y = ops.fp8_linear(x.cuda(), w.cuda(), ws.cuda())
+    assert y[0].isnan().all() and torch.equal(y[1:], clean[1:])
+
+
+def test_linear_on_a_side_stream_and_in_a_graph():
+    w, ws = (t.cuda() for t in _weights(512, 1024, 8))
+    for m in (1, 24, 130):
+        x = torch.randn(m, 1024, generator=_gen(m)).to(torch.bfloat16).cuda()
+        want = ops.fp8_linear(x, w, ws)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = ops.fp8_linear(x, w, ws)
+        side.synchronize()
+        assert torch.equal(got, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = ops.fp8_linear(x, w, ws)
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+            assert torch.equal(ops.fp8_linear(x, w, ws), want)
+
+
+@pytest.mark.parametrize("counts,n,k", [([1], 64, 128), ([0, 0, 3, 0], 200, 256), ([5, 0, 70, 1, 64, 0], 96, 400), ([0, 0], 64, 128),
+                                        ([300, 1, 0, 129], 264, 384), ([1] * 40, 128, 272), ([17, 16, 15, 33], 512, 1408)])
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("out", DTYPES)
+def test_group_gemm(counts, n, k, gather, out):
+    rows, experts = sum(counts), len(counts)
+    w, ws = _weights(n, k, 11, experts)
+    indptr = torch.tensor([0] + counts).cumsum(0).to(torch.int32)
+    source = max(rows // 3, 1) if gather else rows
+    x = torch.randn(source, k, generator=_gen(rows + k)).to(torch.bfloat16)
+    index = torch.randint(0, source, (rows,), generator=_gen(1), dtype=torch.int32) if gather else None
+    q, s = ops.fp8_quantize(x.cuda())
+    y = ops.fp8_group_gemm(q, s, index.cuda() if gather else None, w.cuda()[..., :k], ws.cuda(), indptr.cuda(), out, True).cpu().double()
+    assert y.shape == (rows, n)
+    xv = quantized(x.double())[2]
+    xv = xv[index.long()] if gather else xv
+    for e in range(experts):
+        part = slice(int(indptr[e]), int(indptr[e + 1]))
+        wv = block_values(w[e, :, :k], ws[e])
+        exact = xv[part] @ wv.t()
+        assert ((y[part] - exact).abs() <= _linear_bound(xv[part], wv, exact, out)).all()
+
+
+def test_group_gemm_leaves_rows_outside_the_segments():
+    w, ws = _weights(64, 128, 3, 2)
+    q, s = ops.fp8_quantize(torch.randn(90, 128, generator=_gen(4)).half().cuda())
+    y = ops.fp8_group_gemm(q, s, None, w.cuda(), ws.cuda(), torch.tensor([0, 70, 75], dtype=torch.int32).cuda())
+    assert (y[75:] == 0).all() and (y[:75].abs().sum(1) > 0).all()
+
+
+# ---- routing ----
+
+
+@pytest.mark.parametrize("t,ne,k,groups,top_groups", [(1, 8, 2, 1, 1), (7, 64, 6, 1, 1), (33, 128, 8, 8, 4), (5, 256, 8, 8, 4), (9, 160, 6, 8, 3),
+                                                      (3, 1, 1, 1, 1), (2, 512, 32, 64, 40), (4, 100, 5, 20, 2), (6, 63, 7, 3, 1), (1, 65, 8, 1, 1),
+                                                      (5, 64, 8, 64, 9), (130, 8, 8, 2, 2)])
+@pytest.mark.parametrize("scoring,bias", [("softmax", False), ("softmax", True), ("sigmoid", False), ("sigmoid", True)])
+def test_gating(t, ne, k, groups, top_groups, scoring, bias):
+    g = _gen(t + ne + k)
+    # keys on a grid, far enough apart that no rounding of an exponential decides: distinct logits, a permutation a row
+    grid = torch.linspace(-4, 4, ne)
+    for dtype in DTYPES:
+        logits = torch.stack([grid[torch.randperm(ne, generator=g)] for _ in range(t)]).to(dtype)
+        b = (torch.randint(-3, 4, (ne,), generator=g) * 0.25).float() if bias else None
+        for renorm, scale in ((True, 1.0), (False, 2.5)):
+            want_w, want_i = route(logits, b, k, scoring, groups, top_groups, renorm, scale)
+            w, i = ops.moe_gating(logits.cuda(), k, scoring, b.cuda() if bias else None, groups, top_groups, renorm, scale)
+            assert w.dtype == torch.float32 and i.dtype == torch.int32
+            same = i.cpu().long() == want_i
+            # (two keys a few 2^-24 apart may change places: their keys then are as near)
+            if not same.all():
+                x = logits.double()
+                key = (torch.softmax(x, 1) if scoring == "softmax" else torch.sigmoid(x)) + (0 if b is None else b.double())
+                a, c = key.gather(1, i.cpu().long()), key.gather(1, want_i)
+                assert groups == 1 and ((a - c).abs() <= 2.0**-20 * (1 + c.abs())).all()
+            # the exponential, the sum (ne additions in six steps and eight), two divisions and a product
+            assert ((w.cpu().double() - want_w).abs()[same] <= 40 * 2.0**-24 * want_w[same].abs() + 1e-37).all()
+
+
+def test_gating_ties_and_numbers_that_are_none():
+    inf, nan = torch.inf, torch.nan
+    rows = torch.zeros(8, 64)
+    rows[1, 10:] = 1.0
+    rows[2] = -inf
+    rows[3, 5], rows[3, 6] = nan, 3.0
+    rows[4] = nan
+    rows[5, 20] = inf
+    rows[6, :60] = -inf
+    rows[7, 3], rows[7, 40] = inf, inf
+    for dtype in DTYPES:
+        for scoring in ("softmax", "sigmoid"):
+            for groups, top_groups in ((1, 1), (8, 2)):
+                want_w, want_i = route(rows.to(dtype), None, 6, scoring, groups, top_groups, True, 1.0)
+                w, i = ops.moe_gating(rows.to(dtype).cuda(), 6, scoring, None, groups, top_groups)
+                assert torch.equal(i.cpu().long(), want_i), (scoring, groups)
+                assert ((w.cpu().double() - want_w).abs() <= 2.0**-18).all()
+    bias = torch.zeros(64)
+    bias[7], bias[9], bias[50] = nan, inf, -inf
+    want_w, want_i = route(rows[:2], bias, 6, "sigmoid", 1, 1, True, 1.0)
+    w, i = ops.moe_gating(rows[:2].cuda(), 6, "sigmoid", bias.cuda())
+    assert torch.equal(i.cpu().long(), want_i) and w.isfinite().all()
+    lowest = torch.full((2, 16), torch.finfo(torch.float16).min, dtype=torch.float16)
+    lowest[1, 4] = 0
+    w, i = ops.moe_gating(lowest.cuda(), 4)
+    assert i[0].tolist() == [0, 1, 2, 3] and i[1, 0] == 4 and torch.equal(w[0].cpu(), torch.full((4,), 0.25)) and w[1, 0] == 1
+
+
+@pytest.mark.parametrize("t,k,ne", [(1, 1, 1), (1, 6, 64), (16, 8, 128), (100, 2, 8), (777, 8, 256), (5000, 2, 8), (3, 32, 512), (0, 2, 8)])
+def test_plan(t, k, ne):
+    ids = torch.stack([torch.randperm(ne, generator=_gen(i))[:k] for i in range(t)]).int() if t else torch.zeros(0, k, dtype=torch.int32)
+    if t > 2:
+        ids[1, 0], ids[2, 0] = -1, ne  # no such experts
+    token, row, indptr = (v.cpu().long() for v in ops.moe_plan(ids.cuda(), ne))
+    flat = ids.reshape(-1).long()
+    inside = (flat >= 0) & (flat < ne)
+    order = torch.sort(torch.where(inside, flat, ne), stable=True).indices[: int(inside.sum())]
+    assert torch.equal(token[: len(order)], order // k)
+    want = torch.full((t * k,), -1)
+    want[order] = torch.arange(len(order))
+    assert torch.equal(row, want)
+    assert torch.equal(indptr, torch.tensor([int((inside & (flat < e)).sum()) for e in range(ne + 1)]))
+
+
+# ---- the layer ----
+
+
+@pytest.mark.parametrize("t,hidden,inter,ne,k", [(1, 256, 128, 8, 2), (1, 2048, 1408, 64, 6), (3, 400, 272, 5, 3), (16, 512, 256, 128, 8), (40, 256, 384, 4, 1),
+                                                 (65, 272, 144, 16, 4), (200, 512, 128, 8, 2), (700, 256, 256, 3, 2), (2, 1040, 640, 9, 9)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_moe_layer(t, hidden, inter, ne, k, dtype):
+    g = _gen(t + hidden + inter)
+    x = torch.randn(t, hidden, generator=g).to(dtype)
+    logits = torch.randn(t, ne, generator=g)
+    w13, s13 = _weights(2 * inter, hidden, 1, ne)
+    w2, s2 = _weights(hidden, inter, 2, ne)
+    args = tuple(v.cuda() for v in (w13, s13, w2, s2))
+    y = ops.fp8_moe(x.cuda(), logits.cuda(), *args, k)
+    weights, ids = ops.moe_gating(logits.cuda(), k)
+    assert torch.equal(y, ops.fp8_moe_experts(x.cuda(), weights, ids, *args))
+    want, size = experts_layer(x, weights.cpu(), ids.cpu().long(), w13, s13, w2, s2)
+    # every expert's output and the sum are rounded to the type; a float32 difference of a few 2^-24 moves a number of the
+    # activation across a rounding boundary now and then, by a sixteenth: as noise, far below the sum of magnitudes
+    err = (y.cpu().double() - want).abs()
+    assert (err <= 3 * UNIT[dtype] * (want.abs() + size / 16) + size * 2.0**-9).all(), (err / size).max()
+    assert err.norm() <= 4 * UNIT[dtype] * want.norm() + 1e-3 * want.norm()
+
+
+def test_moe_layer_without_some_experts():
+    x = torch.randn(5, 256, generator=_gen(1)).half().cuda()
+    w13, s13 = _weights(256, 256, 1, 4)
+    w2, s2 = _weights(256, 128, 2, 4)
+    args = tuple(v.cuda() for v in (w13, s13, w2, s2))
+    weights = torch.rand(5, 2, generator=_gen(2)).cuda()
+    ids = torch.tensor([[0, 1], [-1, 3], [2, 4], [-7, 99], [3, 0]], dtype=torch.int32)
+    y = ops.fp8_moe_experts(x, weights, ids.cuda(), *args)
+    want, size = experts_layer(x.cpu(), weights.cpu(), ids.long(), w13, s13, w2, s2)
+    assert (y[3] == 0).all() and y.isfinite().all()
+    assert ((y.cpu().double() - want).abs() <= 3 * UNIT[torch.float16] * (want.abs() + size / 16) + size * 2.0**-9).all()
+    assert ops.fp8_moe_experts(x[:0], weights[:0], ids[:0].cuda(), *args).shape == (0, 256)
+
+
+# ---- refusals ----
+
+
+def test_refusals():
+    w, ws = (t.cuda() for t in _weights(64, 128, 1))
+    x = torch.zeros(2, 128, dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError, match="GPU"):
+        ops.fp8_quantize(x.cpu())
+    with pytest.raises(TypeError, match="dtype"):
+        ops.fp8_quantize(x.to(torch.int32))
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.fp8_quantize(x.t())
+    with pytest.raises(ValueError, match="rows, K"):
+        ops.fp8_quantize(x[0])
+    with pytest.raises(TypeError, match="float8"):
+        ops.fp8_linear(x, w.float(), ws)
+    with pytest.raises(ValueError, match="weight_scale"):
+        ops.fp8_linear(x, w, ws[:, :0])
+    with pytest.raises(ValueError, match="multiple of 16"):
+        ops.fp8_linear(x[:, :120].contiguous(), torch.zeros(64, 120, dtype=E4M3, device="cuda"), ws)
+    with pytest.raises(ValueError, match="fp8_linear"):
+        ops.fp8_linear(x[:, :64].contiguous(), w, ws)
+    with pytest.raises(TypeError, match="bias"):
+        ops.fp8_linear(x, w, ws, bias=torch.zeros(64, device="cuda"))
+    with pytest.raises(ValueError, match="residual"):
+        ops.fp8_linear(x, w, ws, residual=x)
+    with pytest.raises(TypeError, match="out_dtype"):
+        ops.fp8_linear(x, w, ws, out_dtype=torch.int32)
+    with pytest.raises(ValueError, match="scoring"):
+        ops.moe_gating(torch.zeros(2, 8, device="cuda"), 2, "tanh")
+    for bad in ((0, 1, 1), (9, 1, 1), (2, 3, 1), (5, 4, 2), (2, 4, 5)):
+        with pytest.raises(gq._lib.Mi355gqError) as err:
+            ops.moe_gating(torch.zeros(2, 8, device="cuda"), bad[0], num_groups=bad[1], top_groups=bad[2])
+        assert err.value.code == gq._lib.ERR_ARG
+    q, s = ops.fp8_quantize(x)
+    with pytest.raises(ValueError, match="indptr"):
+        ops.fp8_group_gemm(q, s, None, w[None], ws[None], torch.zeros(3, dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError, match="belong together"):
+        ops.fp8_moe_experts(x, torch.zeros(2, 1, device="cuda"), torch.zeros(2, 1, dtype=torch.int32, device="cuda"), w[None], ws[None], w[None], ws[None])
