@@ -54,6 +54,10 @@ int quantize(const void* x, int64_t rows, int64_t K, int model_dtype, bool silu,
                                             static_cast<float*>(scale), as_stream(stream)), what);
 }
 
+hipError_t product(const gq::Fp8Args& a, hipStream_t s) {
+  return a.precise ? gq::launch_fp8_gemm(a, s) : gq::launch_fp8_tile(a, s);
+}
+
 struct LinearWorkspace {
   uint8_t* q = nullptr;
   float* scale = nullptr;
@@ -187,7 +191,7 @@ int mi355gq_fp8_linear(const void* x, int64_t x_pitch, const void* x_scale, cons
   a.model_dtype = model_dtype;
   a.out_dtype = out_dtype;
   a.precise = precise != 0;
-  return hip_result(gq::launch_fp8_gemm(a, as_stream(stream)), "fp8_linear launch");
+  return hip_result(product(a, as_stream(stream)), "fp8_linear launch");
 }
 
 int mi355gq_fp8_group_gemm(const void* x, int64_t x_pitch, const void* x_scale, int64_t x_rows, const void* x_row_index,
@@ -222,7 +226,7 @@ int mi355gq_fp8_group_gemm(const void* x, int64_t x_pitch, const void* x_scale, 
   a.K = K;
   a.out_dtype = out_dtype;
   a.precise = precise != 0;
-  return hip_result(gq::launch_fp8_gemm(a, as_stream(stream)), "fp8_group_gemm launch");
+  return hip_result(product(a, as_stream(stream)), "fp8_group_gemm launch");
 }
 
 int mi355gq_moe_gating(const void* logits, const void* bias, int64_t T, int64_t num_experts, int64_t top_k, int scoring,
@@ -305,7 +309,7 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
   a.K = hidden;
   a.y = ws.both;
   a.out_dtype = MI355GQ_F32;
-  if (e == hipSuccess) e = gq::launch_fp8_gemm(a, s);
+  if (e == hipSuccess) e = product(a, s);
   if (e == hipSuccess) e = gq::launch_fp8_quantize(ws.both, slots, inter, MI355GQ_F32, true, ws.hq, inter, ws.hs, s);
   a.x = ws.hq;
   a.xs = ws.hs;
@@ -319,7 +323,7 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
   a.K = inter;
   a.y = ws.y;
   a.out_dtype = model_dtype;
-  if (e == hipSuccess) e = gq::launch_fp8_gemm(a, s);
+  if (e == hipSuccess) e = product(a, s);
   if (e == hipSuccess)
     e = gq::launch_moe_weighted_sum(ws.y, ws.slot_row, static_cast<const float*>(weights), T, static_cast<int>(top_k), hidden, model_dtype,
                                     out, s);

@@ -69,7 +69,8 @@ struct Fp8Args {
   int model_dtype = 0, out_dtype = 0;
   bool precise = false;  // blocks summed in float32, whatever the output type
 };
-hipError_t launch_fp8_gemm(const Fp8Args& a, hipStream_t s);
+hipError_t launch_fp8_gemm(const Fp8Args& a, hipStream_t s);  // float32 sums
+hipError_t launch_fp8_tile(const Fp8Args& a, hipStream_t s);  // 8-bit matrix instruction
 
 // rows of x [rows, cols] (silu_mul: of x [rows, 2 cols], silu(first half) * second half) to e4m3 groups; the q bytes between
 // cols and pitch are written as zeros
