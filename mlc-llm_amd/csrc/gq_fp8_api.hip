@@ -54,7 +54,41 @@ int quantize(const void* x, int64_t rows, int64_t K, int model_dtype, bool silu,
                                             static_cast<float*>(scale), as_stream(stream)), what);
 }
 
+// the few-row kernel's view of a product on quantised x
+gq::Fp8RowsArgs few_rows(const gq::Fp8Args& a) {
+  gq::Fp8RowsArgs r;
+  r.x = a.x;
+  r.xs = a.xs;
+  r.x_pitch = a.x_pitch;
+  r.x_rows = a.x_rows;
+  r.w = a.w;
+  r.ws = a.ws;
+  r.w_pitch = a.w_pitch;
+  r.N = a.N;
+  r.K = a.K;
+  r.experts = a.experts;
+  r.bias = a.bias;
+  r.residual = a.residual;
+  r.y = a.y;
+  r.rows = a.rows;
+  r.indptr = a.indptr;
+  r.x_row_index = a.x_row_index;
+  r.model_dtype = a.model_dtype;
+  r.out_dtype = a.out_dtype;
+  r.y_aligned = aligned16(a.y);
+  return r;
+}
+
+// rows of a segment up to which the weights' way from memory is what counts
+constexpr int64_t kFewRows = 64;
+
 hipError_t product(const gq::Fp8Args& a, hipStream_t s) {
+  const int64_t segments = a.indptr ? (a.rows < a.experts ? a.rows : a.experts) : 1;
+  if (a.rows <= kFewRows * segments / (a.indptr ? 2 : 1)) {
+    const int64_t rows_max = a.indptr ? a.rows * 3 / (2 * segments) + 1 : a.rows;
+    const hipError_t e = gq::launch_fp8_rows(few_rows(a), static_cast<int>(rows_max), s);
+    if (e != hipErrorNotSupported) return e;
+  }
   return a.precise ? gq::launch_fp8_gemm(a, s) : gq::launch_fp8_tile(a, s);
 }
 
@@ -72,6 +106,8 @@ LinearWorkspace linear_workspace(int64_t M, int64_t K, bool x_quantized, void* b
   w.bytes = c.used;
   return w;
 }
+
+constexpr int64_t kIdSlots = 1024;  // slots whose ids every workgroup looks through itself
 
 struct MoeWorkspace {
   uint8_t *xq, *hq;
@@ -168,17 +204,6 @@ int mi355gq_fp8_linear(const void* x, int64_t x_pitch, const void* x_scale, cons
       return set_error(MI355GQ_ERR_WORKSPACE, "fp8_linear: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)ws.bytes);
   }
   gq::Fp8Args a;
-  if (x_scale == nullptr) {
-    const hipError_t e = gq::launch_fp8_quantize(x, M, K, model_dtype, false, ws.q, up16(K), ws.scale, as_stream(stream));
-    if (e != hipSuccess) return hip_result(e, "fp8_linear: quantize launch");
-    a.x = ws.q;
-    a.xs = ws.scale;
-    a.x_pitch = up16(K);
-  } else {
-    a.x = static_cast<const uint8_t*>(x);
-    a.xs = static_cast<const float*>(x_scale);
-    a.x_pitch = x_pitch;
-  }
   a.w = static_cast<const uint8_t*>(w);
   a.ws = static_cast<const float*>(w_scale);
   a.w_pitch = w_pitch;
@@ -191,6 +216,24 @@ int mi355gq_fp8_linear(const void* x, int64_t x_pitch, const void* x_scale, cons
   a.model_dtype = model_dtype;
   a.out_dtype = out_dtype;
   a.precise = precise != 0;
+  if (x_scale == nullptr && M <= 16 && aligned16(x)) {  // the kernel quantises x itself
+    gq::Fp8RowsArgs r = few_rows(a);
+    r.x = x;
+    r.x_kind = model_dtype;
+    const hipError_t e = gq::launch_fp8_rows(r, static_cast<int>(M), as_stream(stream));
+    if (e != hipErrorNotSupported) return hip_result(e, "fp8_linear launch");
+  }
+  if (x_scale == nullptr) {
+    const hipError_t e = gq::launch_fp8_quantize(x, M, K, model_dtype, false, ws.q, up16(K), ws.scale, as_stream(stream));
+    if (e != hipSuccess) return hip_result(e, "fp8_linear: quantize launch");
+    a.x = ws.q;
+    a.xs = ws.scale;
+    a.x_pitch = up16(K);
+  } else {
+    a.x = static_cast<const uint8_t*>(x);
+    a.xs = static_cast<const float*>(x_scale);
+    a.x_pitch = x_pitch;
+  }
   return hip_result(product(a, as_stream(stream)), "fp8_linear launch");
 }
 
@@ -290,8 +333,51 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
     return set_error(MI355GQ_ERR_WORKSPACE, "fp8_moe: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)ws.bytes);
   const hipStream_t s = as_stream(stream);
   const int64_t slots = T * top_k;
-  hipError_t e = gq::launch_moe_plan(static_cast<const int32_t*>(ids), slots, static_cast<int>(top_k), static_cast<int>(num_experts),
-                                     ws.row_token, ws.slot_row, ws.indptr, s);
+  const int64_t segments = slots < num_experts ? slots : num_experts;
+  hipError_t e;
+  if (slots <= 16 * segments && slots <= kIdSlots) {
+    // a slot or a few an expert: the workgroups find their rows from the ids, x and the activation are quantised where they are read
+    gq::Fp8RowsArgs r;
+    r.x = x;
+    r.x_rows = T;
+    r.x_kind = model_dtype;
+    r.w = static_cast<const uint8_t*>(w13);
+    r.ws = static_cast<const float*>(w13_scale);
+    r.w_pitch = w13_pitch;
+    r.N = 2 * inter;
+    r.K = hidden;
+    r.experts = num_experts;
+    r.y = ws.both;
+    r.rows = slots;
+    r.ids = static_cast<const int32_t*>(ids);
+    r.x_div = static_cast<int>(top_k);
+    r.top_k = static_cast<int>(top_k);
+    r.silu = 1;
+    r.out_dtype = MI355GQ_F32;
+    r.y_aligned = 1;
+    e = gq::launch_fp8_rows(r, 16, s);
+    if (e == hipSuccess) {
+      r.x = ws.both;
+      r.x_rows = slots;
+      r.x_kind = MI355GQ_F32;
+      r.w = static_cast<const uint8_t*>(w2);
+      r.ws = static_cast<const float*>(w2_scale);
+      r.w_pitch = w2_pitch;
+      r.N = hidden;
+      r.K = inter;
+      r.y = ws.y;
+      r.x_div = 1;
+      r.silu = 0;
+      r.out_dtype = model_dtype;
+      e = gq::launch_fp8_rows(r, 16, s);
+      if (e == hipSuccess)
+        e = gq::launch_moe_weighted_sum(ws.y, nullptr, static_cast<const int32_t*>(ids), static_cast<int>(num_experts),
+                                        static_cast<const float*>(weights), T, static_cast<int>(top_k), hidden, model_dtype, out, s);
+    }
+    if (e != hipErrorNotSupported) return hip_result(e, "fp8_moe launch");
+  }
+  e = gq::launch_moe_plan(static_cast<const int32_t*>(ids), slots, static_cast<int>(top_k), static_cast<int>(num_experts),
+                          ws.row_token, ws.slot_row, ws.indptr, s);
   if (e == hipSuccess) e = gq::launch_fp8_quantize(x, T, hidden, model_dtype, false, ws.xq, hidden, ws.xs, s);
   gq::Fp8Args a;
   a.x = ws.xq;
@@ -309,8 +395,18 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
   a.K = hidden;
   a.y = ws.both;
   a.out_dtype = MI355GQ_F32;
-  if (e == hipSuccess) e = product(a, s);
-  if (e == hipSuccess) e = gq::launch_fp8_quantize(ws.both, slots, inter, MI355GQ_F32, true, ws.hq, inter, ws.hs, s);
+  a.precise = true;  // sums that are rounded to e4m3 again: an error of 1e-5 would move one in thousands by a sixteenth
+  bool activated = false;
+  if (e == hipSuccess && slots <= kFewRows / 2 * segments) {
+    gq::Fp8RowsArgs r = few_rows(a);
+    r.silu = 1;
+    const hipError_t done = gq::launch_fp8_rows(r, static_cast<int>(slots * 3 / (2 * segments) + 1), s);
+    activated = done == hipSuccess;
+    if (done != hipErrorNotSupported) e = done;
+  }
+  if (e == hipSuccess && !activated) e = product(a, s);
+  if (e == hipSuccess) e = gq::launch_fp8_quantize(ws.both, slots, inter, MI355GQ_F32, !activated, ws.hq, inter, ws.hs, s);
+  a.precise = false;
   a.x = ws.hq;
   a.xs = ws.hs;
   a.x_pitch = inter;
@@ -325,8 +421,8 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
   a.out_dtype = model_dtype;
   if (e == hipSuccess) e = product(a, s);
   if (e == hipSuccess)
-    e = gq::launch_moe_weighted_sum(ws.y, ws.slot_row, static_cast<const float*>(weights), T, static_cast<int>(top_k), hidden, model_dtype,
-                                    out, s);
+    e = gq::launch_moe_weighted_sum(ws.y, ws.slot_row, nullptr, 0, static_cast<const float*>(weights), T, static_cast<int>(top_k), hidden,
+                                    model_dtype, out, s);
   return hip_result(e, "fp8_moe launch");
 }
 

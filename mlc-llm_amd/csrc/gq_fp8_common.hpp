@@ -69,6 +69,31 @@ struct Fp8Args {
   int model_dtype = 0, out_dtype = 0;
   bool precise = false;  // blocks summed in float32, whatever the output type
 };
+
+// ... of few rows a segment, with what the kernel for them takes besides
+constexpr int kXFp8 = 3;  // kind of x: MODEL_F16, MODEL_F32 or MODEL_BF16 (dense [x_rows, K], quantised by the kernel), or e4m3 with its scales
+struct Fp8RowsArgs {
+  const void* x = nullptr;
+  const float* xs = nullptr;
+  int64_t x_pitch = 0, x_rows = 0;
+  int x_kind = kXFp8;
+  const uint8_t* w = nullptr;
+  const float* ws = nullptr;
+  int64_t w_pitch = 0, N = 0, K = 0, experts = 1;
+  const void* bias = nullptr;
+  const void* residual = nullptr;
+  void* y = nullptr;  // [rows, N] (silu: [rows, N / 2] = silu(first half) * second half)
+  int64_t rows = 0;
+  const int32_t* indptr = nullptr;       // segments as in Fp8Args, or
+  const int32_t* x_row_index = nullptr;
+  const int32_t* ids = nullptr;          // [rows] the expert of each row, in any order; row r reads row r / x_div of x
+  int x_div = 1, top_k = 0;              // rows <= top_k: one token, whose ids differ
+  int silu = 0, model_dtype = 0, out_dtype = 0;
+  int y_aligned = 0;  // y starts at 16 bytes
+};
+// rows_max: rows that the largest segment is expected to have (more are taken in passes); hipErrorNotSupported where no form applies
+hipError_t launch_fp8_rows(const Fp8RowsArgs& a, int rows_max, hipStream_t s);
+
 hipError_t launch_fp8_gemm(const Fp8Args& a, hipStream_t s);  // float32 sums
 hipError_t launch_fp8_tile(const Fp8Args& a, hipStream_t s);  // 8-bit matrix instruction
 
@@ -96,8 +121,9 @@ hipError_t launch_moe_gating(const GatingArgs& a, hipStream_t s);
 // outside the experts), indptr [E + 1]
 hipError_t launch_moe_plan(const int32_t* ids, int64_t slots, int k, int E, int32_t* row_token, int32_t* slot_row,
                            int32_t* indptr, hipStream_t s);
-// out[t] = sum over j of weights[t, j] y[row], row = slot_row[t k + j] (null: t k + j; negative: no such row), in float32
-hipError_t launch_moe_weighted_sum(const void* y, const int32_t* slot_row, const float* weights, int64_t T, int k, int64_t H,
-                                   int model_dtype, void* out, hipStream_t s);
+// out[t] = sum over j of weights[t, j] y[row] in float32: row = slot_row[t k + j] (negative: no such row), or without slot_row
+// t k + j where ids[t k + j] is one of E experts
+hipError_t launch_moe_weighted_sum(const void* y, const int32_t* slot_row, const int32_t* ids, int E, const float* weights, int64_t T,
+                                   int k, int64_t H, int model_dtype, void* out, hipStream_t s);
 
 }  // namespace gq

@@ -220,7 +220,7 @@ hipError_t launch_moe_plan(const int32_t* ids, int64_t slots, int k, int E, int3
 // One thread eight neighbouring columns of a token (H % 8 == 0) or one (any H); float32 throughout, one rounding at the end.
 template <int DT, int VEC>
 __global__ __launch_bounds__(256) void moe_weighted_sum_kernel(const void* __restrict__ y, const int32_t* __restrict__ slot_row,
-                                                               const float* __restrict__ weights, int64_t T, int k, int64_t H,
+                                                               const int32_t* __restrict__ ids, int E, const float* __restrict__ weights, int64_t T, int k, int64_t H,
                                                                void* __restrict__ out) {
   const int64_t per_row = H / VEC, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= T * per_row) return;
@@ -229,8 +229,9 @@ __global__ __launch_bounds__(256) void moe_weighted_sum_kernel(const void* __res
 #pragma unroll
   for (int v = 0; v < VEC; ++v) acc[v] = 0.f;
   for (int j = 0; j < k; ++j) {
-    const int64_t row = slot_row ? slot_row[t * k + j] : t * k + j;
-    if (row < 0) continue;
+    const int at = slot_row ? slot_row[t * k + j] : ids[t * k + j];
+    if (at < 0 || (!slot_row && at >= E)) continue;
+    const int64_t row = slot_row ? at : t * k + j;
     const float w = weights[t * k + j];
     if constexpr (VEC == 8) {
       float f[8];
@@ -258,12 +259,12 @@ __global__ __launch_bounds__(256) void moe_weighted_sum_kernel(const void* __res
   for (int v = 0; v < VEC; ++v) Elem<DT>::store(out, t * H + h + v, acc[v]);
 }
 
-hipError_t launch_moe_weighted_sum(const void* y, const int32_t* slot_row, const float* weights, int64_t T, int k, int64_t H,
-                                   int model_dtype, void* out, hipStream_t s) {
+hipError_t launch_moe_weighted_sum(const void* y, const int32_t* slot_row, const int32_t* ids, int E, const float* weights, int64_t T,
+                                   int k, int64_t H, int model_dtype, void* out, hipStream_t s) {
   auto go = [&](auto dt, auto vec) {
     const int64_t n = T * (H / decltype(vec)::value);
     hipLaunchKernelGGL((moe_weighted_sum_kernel<decltype(dt)::value, decltype(vec)::value>),
-                       dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s, y, slot_row, weights, T, k, H, out);
+                       dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s, y, slot_row, ids, E, weights, T, k, H, out);
   };
   auto by_type = [&](auto vec) {
     if (model_dtype == MODEL_F32) go(std::integral_constant<int, MODEL_F32>{}, vec);
