@@ -89,20 +89,24 @@ hipError_t product(const gq::Fp8Args& a, hipStream_t s) {
     const hipError_t e = gq::launch_fp8_rows(few_rows(a), static_cast<int>(rows_max), s);
     if (e != hipErrorNotSupported) return e;
   }
-  return a.precise ? gq::launch_fp8_gemm(a, s) : gq::launch_fp8_tile(a, s);
+  return gq::launch_fp8_tile(a, s);
 }
 
 struct LinearWorkspace {
   uint8_t* q = nullptr;
   float* scale = nullptr;
-  int64_t bytes = 0;
+  void* split = nullptr;  // sums of shares of K
+  int64_t split_bytes = 0, bytes = 0;
 };
-LinearWorkspace linear_workspace(int64_t M, int64_t K, bool x_quantized, void* base) {
+LinearWorkspace linear_workspace(int64_t M, int64_t N, int64_t K, bool x_quantized, void* base) {
   LinearWorkspace w;
-  if (x_quantized) return w;
   Carver c{static_cast<char*>(base)};
-  w.q = c.take<uint8_t>(M * up16(K));
-  w.scale = c.take<float>(M * groups_of(K));
+  if (!x_quantized) {
+    w.q = c.take<uint8_t>(M * up16(K));
+    w.scale = c.take<float>(M * groups_of(K));
+  }
+  w.split_bytes = M > kFewRows ? gq::fp8_tile_workspace_bytes(M, N, K) : 0;
+  w.split = c.take<char>(w.split_bytes);
   w.bytes = c.used;
   return w;
 }
@@ -178,7 +182,7 @@ int mi355gq_fp8_dequantize(const void* q, int64_t q_pitch, const void* scale, in
 
 int64_t mi355gq_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_quantized) {
   if (!dim_ok(M) || !dim_ok(N) || !dim_ok(K) || M == 0 || N == 0 || K == 0) return 0;
-  return linear_workspace(M, K, x_quantized != 0, nullptr).bytes;
+  return linear_workspace(M, N, K, x_quantized != 0, nullptr).bytes;
 }
 
 int mi355gq_fp8_linear(const void* x, int64_t x_pitch, const void* x_scale, const void* w, int64_t w_pitch,
@@ -197,7 +201,7 @@ int mi355gq_fp8_linear(const void* x, int64_t x_pitch, const void* x_scale, cons
   FP8_REQUIRE(aligned16(w) && aligned4(w_scale) && aligned4(x_scale) && (x_scale ? aligned16(x) : dtype_aligned(x, model_dtype)) &&
                   dtype_aligned(bias, model_dtype) && dtype_aligned(residual, model_dtype) && dtype_aligned(y, out_dtype),
               "fp8_linear: misaligned pointer (e4m3 tensors: 16 bytes)");
-  const LinearWorkspace ws = linear_workspace(M, K, x_scale != nullptr, workspace);
+  const LinearWorkspace ws = linear_workspace(M, N, K, x_scale != nullptr, workspace);
   if (ws.bytes > 0) {
     FP8_REQUIRE(workspace == nullptr || aligned16(workspace), "fp8_linear: workspace must be 16-byte aligned");
     if (workspace == nullptr || workspace_bytes < ws.bytes)
@@ -216,6 +220,8 @@ int mi355gq_fp8_linear(const void* x, int64_t x_pitch, const void* x_scale, cons
   a.model_dtype = model_dtype;
   a.out_dtype = out_dtype;
   a.precise = precise != 0;
+  a.workspace = ws.split;
+  a.workspace_bytes = ws.split_bytes;
   if (x_scale == nullptr && M <= 16 && aligned16(x)) {  // the kernel quantises x itself
     gq::Fp8RowsArgs r = few_rows(a);
     r.x = x;
@@ -252,6 +258,9 @@ int mi355gq_fp8_group_gemm(const void* x, int64_t x_pitch, const void* x_scale, 
   FP8_REQUIRE(x_rows > 0 && x && x_scale && w && w_scale && indptr && y, "fp8_group_gemm: null pointer");
   FP8_REQUIRE(aligned16(x) && aligned16(w) && aligned4(x_scale) && aligned4(w_scale) && aligned4(indptr) && aligned4(x_row_index) &&
                   dtype_aligned(y, out_dtype), "fp8_group_gemm: misaligned pointer (e4m3 tensors: 16 bytes)");
+  if (x_row_index != nullptr && x_rows >= (int64_t(1) << 32) / x_pitch)
+    return set_error(MI355GQ_ERR_UNSUPPORTED, "fp8_group_gemm: x of %lld rows of %lld bytes with a row index (4 GiB at most)", (long long)x_rows,
+                     (long long)x_pitch);
   gq::Fp8Args a;
   a.x = static_cast<const uint8_t*>(x);
   a.xs = static_cast<const float*>(x_scale);
@@ -304,7 +313,7 @@ int mi355gq_moe_plan(const void* ids, int64_t T, int64_t top_k, int64_t num_expe
 }
 
 static bool moe_sizes_ok(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t top_k) {
-  return dim_ok(T) && hidden > 0 && hidden % 16 == 0 && hidden < (1 << 24) && inter > 0 && inter % 16 == 0 && inter < (1 << 24) &&
+  return dim_ok(T) && T * hidden < (int64_t(1) << 32) && hidden > 0 && hidden % 16 == 0 && hidden < (1 << 24) && inter > 0 && inter % 16 == 0 && inter < (1 << 24) &&
          experts > 0 && experts <= 512 && top_k > 0 && top_k <= 32 && T * top_k / 64 + experts <= kMaxTiles;
 }
 
@@ -404,8 +413,18 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
     activated = done == hipSuccess;
     if (done != hipErrorNotSupported) e = done;
   }
-  if (e == hipSuccess && !activated) e = product(a, s);
-  if (e == hipSuccess) e = gq::launch_fp8_quantize(ws.both, slots, inter, MI355GQ_F32, !activated, ws.hq, inter, ws.hs, s);
+  bool quantized = false;
+  if (e == hipSuccess && !activated) {
+    a.q_out = ws.hq;
+    a.scale_out = ws.hs;
+    const hipError_t done = gq::launch_fp8_tile(a, s);
+    quantized = done == hipSuccess;
+    if (done != hipErrorNotSupported) e = done;
+    a.q_out = nullptr;
+    a.scale_out = nullptr;
+    if (e == hipSuccess && !quantized) e = gq::launch_fp8_tile(a, s);
+  }
+  if (e == hipSuccess && !quantized) e = gq::launch_fp8_quantize(ws.both, slots, inter, MI355GQ_F32, !activated, ws.hq, inter, ws.hs, s);
   a.precise = false;
   a.x = ws.hq;
   a.xs = ws.hs;

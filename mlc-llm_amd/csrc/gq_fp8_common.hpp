@@ -68,6 +68,10 @@ struct Fp8Args {
   int64_t rows = 0, x_rows = 0, N = 0, K = 0, x_pitch = 0, w_pitch = 0, experts = 1;
   int model_dtype = 0, out_dtype = 0;
   bool precise = false;  // blocks summed in float32, whatever the output type
+  uint8_t* q_out = nullptr;  // see launch_fp8_tile
+  float* scale_out = nullptr;
+  void* workspace = nullptr;
+  int64_t workspace_bytes = 0;
 };
 
 // ... of few rows a segment, with what the kernel for them takes besides
@@ -94,8 +98,66 @@ struct Fp8RowsArgs {
 // rows_max: rows that the largest segment is expected to have (more are taken in passes); hipErrorNotSupported where no form applies
 hipError_t launch_fp8_rows(const Fp8RowsArgs& a, int rows_max, hipStream_t s);
 
-hipError_t launch_fp8_gemm(const Fp8Args& a, hipStream_t s);  // float32 sums
-hipError_t launch_fp8_tile(const Fp8Args& a, hipStream_t s);  // 8-bit matrix instruction
+// Tiles, on the 8-bit matrix instruction or (precise) in float32 sums; K split over workgroups where the scratch for it is there.
+// silu: x [rows, K] times gate and up rows of w (N = 2 I), silu(gate) * up quantised into q_out [rows, I] and its scales
+// scale_out [I / 128, rows]; I a multiple of 128.
+hipError_t launch_fp8_tile(const Fp8Args& a, hipStream_t s);
+int64_t fp8_tile_workspace_bytes(int64_t rows, int64_t N, int64_t K);
+
+// CNT (4 or 8) neighbouring results from column n of row r: bias, residual, one rounding, store.  a: Fp8Args or Fp8RowsArgs.
+// vec: y and residual start at 16 bytes and N is a multiple of CNT.
+template <int CNT, class Args>
+__device__ __forceinline__ void fp8_store(const Args& a, int64_t r, int n, int N, bool vec, float (&o)[CNT]) {
+  const int64_t at = r * N + n;
+  const int count = N - n < CNT ? N - n : CNT;
+  auto add = [&](const void* q, int64_t from) {
+#pragma unroll
+    for (int v = 0; v < CNT; ++v)
+      if (v < count)
+        o[v] += a.model_dtype == MODEL_F32    ? static_cast<const float*>(q)[from + v]
+                : a.model_dtype == MODEL_BF16 ? bf2f(static_cast<const uint16_t*>(q)[from + v])
+                                              : h2f(static_cast<const uint16_t*>(q)[from + v]);
+  };
+  if (a.bias) add(a.bias, n);
+  if (a.residual) add(a.residual, at);
+  if (a.out_dtype == MODEL_F32) {
+    float* y = static_cast<float*>(a.y) + at;
+    if (vec) {
+#pragma unroll
+      for (int v = 0; v < CNT; v += 4) *reinterpret_cast<float4_t*>(y + v) = float4_t{o[v], o[v + 1], o[v + 2], o[v + 3]};
+    } else {
+#pragma unroll
+      for (int v = 0; v < CNT; ++v)
+        if (v < count) y[v] = o[v];
+    }
+  } else {
+    uint32_t h[CNT];
+#pragma unroll
+    for (int v = 0; v < CNT; ++v) h[v] = a.out_dtype == MODEL_BF16 ? f2bf(o[v]) : f2h(o[v]);
+    uint16_t* y = static_cast<uint16_t*>(a.y) + at;
+    if (vec) {
+      uint32_t u[CNT / 2];
+#pragma unroll
+      for (int v = 0; v < CNT / 2; ++v) u[v] = h[2 * v] | h[2 * v + 1] << 16;
+      if constexpr (CNT == 8) *reinterpret_cast<uint4*>(y) = uint4{u[0], u[1], u[2], u[3]};
+      else *reinterpret_cast<uint2*>(y) = uint2{u[0], u[1]};
+    } else {
+#pragma unroll
+      for (int v = 0; v < CNT; ++v)
+        if (v < count) y[v] = static_cast<uint16_t>(h[v]);
+    }
+  }
+}
+
+// eight e4m3 numbers as an operand of the bfloat16 matrix instruction (a bfloat16 holds them exactly)
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ bf16x8_t fp8_widen(uint32_t lo, uint32_t hi) {
+  const bf16x2_dot_t a = __builtin_bit_cast(bf16x2_dot_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+  const bf16x2_dot_t b = __builtin_bit_cast(bf16x2_dot_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+  const bf16x2_dot_t c = __builtin_bit_cast(bf16x2_dot_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+  const bf16x2_dot_t d = __builtin_bit_cast(bf16x2_dot_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+  return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
 
 // rows of x [rows, cols] (silu_mul: of x [rows, 2 cols], silu(first half) * second half) to e4m3 groups; the q bytes between
 // cols and pitch are written as zeros

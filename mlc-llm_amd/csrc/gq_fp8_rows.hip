@@ -18,21 +18,11 @@ namespace gq {
 
 namespace {
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 typedef uint32_t uint4_vt __attribute__((ext_vector_type(4)));
 
 constexpr int kRowWaves = 8;
 constexpr int kRowBlocks = 512;  // workgroups of a launch: two a CU
-
-// eight e4m3 numbers as an operand of the bfloat16 instruction
-__device__ __forceinline__ bf16x8_t widen(uint32_t lo, uint32_t hi) {
-  const bf16x2_dot_t a = __builtin_bit_cast(bf16x2_dot_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
-  const bf16x2_dot_t b = __builtin_bit_cast(bf16x2_dot_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
-  const bf16x2_dot_t c = __builtin_bit_cast(bf16x2_dot_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
-  const bf16x2_dot_t d = __builtin_bit_cast(bf16x2_dot_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
-  return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
 
 // sixteen neighbouring numbers as float32, of which the first `count` are there (a multiple of 8, or ends of K % 16)
 template <int DT>
@@ -68,37 +58,7 @@ __device__ __forceinline__ void store_rows(const Fp8RowsArgs& p, int64_t r, int 
   float o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = SILU ? silu_mul_f32(v[0][i], v[SILU ? 1 : 0][i]) : v[0][i];
-  const int64_t at = r * N + n;
-  const int count = N - n < 4 ? N - n : 4;
-  if (count <= 0) return;
-  auto add = [&](const void* q, int64_t from) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < count)
-        o[i] += p.model_dtype == MODEL_F32   ? Elem<MODEL_F32>::load(q, from + i)
-                : p.model_dtype == MODEL_BF16 ? Elem<MODEL_BF16>::load(q, from + i)
-                                              : Elem<MODEL_F16>::load(q, from + i);
-  };
-  if (p.bias) add(p.bias, n);
-  if (p.residual) add(p.residual, at);
-  if (p.out_dtype == MODEL_F32) {
-    float* y = static_cast<float*>(p.y) + at;
-    if (N % 4 == 0 && p.y_aligned) *reinterpret_cast<float4_t*>(y) = float4_t{o[0], o[1], o[2], o[3]};
-    else
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < count) y[i] = o[i];
-  } else {
-    uint16_t h[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = p.out_dtype == MODEL_BF16 ? f2bf(o[i]) : f2h(o[i]);
-    uint16_t* y = static_cast<uint16_t*>(p.y) + at;
-    if (N % 4 == 0 && p.y_aligned) *reinterpret_cast<uint2*>(y) = uint2{h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16};
-    else
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < count) y[i] = h[i];
-  }
+  if (n < N) fp8_store<4>(p, r, n, N, N % 4 == 0 && p.y_aligned, o);
 }
 
 }  // namespace
@@ -299,8 +259,8 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void fp8_rows_kernel(Fp8RowsArgs
         for (int i = 0; i < NR; ++i) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            a[i][2 * h] = widen(wq[i][b][h][0], wq[i][b][h][1]);
-            a[i][2 * h + 1] = widen(wq[i][b][h][2], wq[i][b][h][3]);
+            a[i][2 * h] = fp8_widen(wq[i][b][h][0], wq[i][b][h][1]);
+            a[i][2 * h + 1] = fp8_widen(wq[i][b][h][2], wq[i][b][h][3]);
           }
           load_w(s_next, ph_next, i, b);
           w_scale[i] = wsr[i][block_of(ph, b) < groups ? block_of(ph, b) : groups - 1];
@@ -309,7 +269,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void fp8_rows_kernel(Fp8RowsArgs
         for (int t = 0; t < MT; ++t) {
           int4_t x0 = xq[b][t][0], x1 = xq[b][t][1];
           if (MT * SB > 4) asm volatile("" : "+v"(x0), "+v"(x1));  // (widened anew each round: the registers would not hold all of it)
-          const bf16x8_t xw[4] = {widen(x0[0], x0[1]), widen(x0[2], x0[3]), widen(x1[0], x1[1]), widen(x1[2], x1[3])};
+          const bf16x8_t xw[4] = {fp8_widen(x0[0], x0[1]), fp8_widen(x0[2], x0[3]), fp8_widen(x1[0], x1[1]), fp8_widen(x1[2], x1[3])};
 #pragma unroll
           for (int i = 0; i < NR; ++i) {
             float4_t part = {};

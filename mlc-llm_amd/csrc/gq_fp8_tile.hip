@@ -8,6 +8,9 @@
 // What the instruction sums itself is one block of 128: of eight neighbouring products it drops what lies more than 13 bits below
 // the largest, and adds such sums in float32 (seen with single products over all positions and sizes); about 1e-5 of a typical
 // result, a fiftieth of a float16 rounding.  Blocks join in float32.
+//
+// Precise products sum in float32 throughout: the operands are widened to bfloat16 (which holds them exactly) on their way from
+// LDS, four instructions of 16 x 16 x 32 to a block, at half the rate.  So do products that are rounded to e4m3 again.
 #include "gq_fp8_common.hpp"
 #include "gq_topk.hpp"
 
@@ -15,7 +18,6 @@ namespace gq {
 
 namespace {
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 
 // 16 bytes per lane from global memory into LDS at lds + 16 * lane, past the registers.  The compiler does not wait for them: the
@@ -39,56 +41,29 @@ __device__ __forceinline__ int4_t mask_chunk(int4_t v, int left) {
   return v;
 }
 
-// eight neighbouring results of row r: bias, residual, one rounding; vec: rows of y and residual start at 16 bytes
-template <int OUT, int MODEL>
-__device__ __forceinline__ void store_run(const Fp8Args& p, int64_t r, int n, int N, bool vec, float (&o)[8]) {
-  const int64_t at = r * N + n;
-  const int count = N - n < 8 ? N - n : 8;
-#pragma unroll
-  for (int v = 0; v < 8; ++v) {
-    if (v < count) {
-      if (p.bias) o[v] += Elem<MODEL>::load(p.bias, n + v);
-      if (p.residual) o[v] += Elem<MODEL>::load(p.residual, at + v);
-    }
-  }
-  if (vec) {
-    if constexpr (OUT == MODEL_F32) {
-      float4_t* q = reinterpret_cast<float4_t*>(static_cast<float*>(p.y) + at);
-      q[0] = float4_t{o[0], o[1], o[2], o[3]};
-      q[1] = float4_t{o[4], o[5], o[6], o[7]};
-    } else {
-      uint32_t u[4];
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-        u[v] = OUT == MODEL_BF16 ? f2bf(o[2 * v]) | static_cast<uint32_t>(f2bf(o[2 * v + 1])) << 16
-                                 : f2h(o[2 * v]) | static_cast<uint32_t>(f2h(o[2 * v + 1])) << 16;
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + at) = uint4{u[0], u[1], u[2], u[3]};
-    }
-  } else {
-#pragma unroll
-    for (int v = 0; v < 8; ++v)
-      if (v < count) Elem<OUT>::store(p.y, at + v, o[v]);
-  }
-}
-
 }  // namespace
 
 // WN x WM waves, each TN x TM results of 16 x 16: a tile of BN = 16 WN TN rows of W by BM = 16 WM TM rows of x.
-template <int WN, int WM, int TN, int TM, int OUT, int MODEL>
-__global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, int n_tiles, int m_tiles) {
+// SILU: half of a wave's rows of W are gate rows and half the up rows that belong to them.
+template <int WN, int WM, int TN, int TM, bool PRECISE, bool SILU>
+__global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, int n_tiles, int m_tiles, int per_split) {
   constexpr int kWaves = WN * WM, BN = 16 * WN * TN, BM = 16 * WM * TM, kStage = (BN + BM) * 128;
   constexpr int kLoads = (BN + BM) / 8 / kWaves;  // of 1 KiB, eight rows, a wave and stage
+  constexpr int P = SILU ? 2 : 1, kPart = 16 * TN / P;  // parts of a wave's rows of W
   static_assert((BN + BM) / 8 % kWaves == 0 && BN / 8 % kWaves == 0, "whole loads");
+  static_assert(TN % 2 == 0, "the first row of a block uses fw[0]");
+  static_assert(kPart <= kFp8Block && kFp8Block % kPart == 0, "a part lies in one block of W");
+  static_assert(!SILU || BN == 2 * kFp8Block, "a tile holds one group of the activation");
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int K = static_cast<int>(p.K), N = static_cast<int>(p.N);
+  const int K = static_cast<int>(p.K), N = static_cast<int>(p.N), half = N / P;
   const int groups = (K + kFp8Block - 1) / kFp8Block, n_blocks = (N + kFp8Block - 1) / kFp8Block;
 
   // Workgroups go to the eight dies in turn; each die takes a run of tiles, x tiles fastest, so that what runs on it at a time
   // shares rows of W and of x in its L2.
   const int tiles = n_tiles * m_tiles, per = (tiles + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if ((blockIdx.x >> 3) >= per || id >= tiles) return;
-  const int nt = id / m_tiles, mt = id - nt * m_tiles, n0 = nt * BN;
+  const int nt = id / m_tiles, mt = id - nt * m_tiles, n0 = nt * (BN / P);
   int e = 0, r0 = mt * BM, r_end = static_cast<int>(p.rows);
   if (p.indptr != nullptr) {
     // tiles of segment e are numbered from indptr[e] / BM + e on: no two segments share a number, and some numbers have no tile
@@ -106,6 +81,8 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
     r_end = __builtin_amdgcn_readfirstlane(r_end);
   }
   if (r0 >= r_end || r0 < 0) return;
+  // this workgroup's blocks of K
+  const int first = blockIdx.y * per_split, last = (first + per_split < groups ? first + per_split : groups) - 1;
 
   const uint8_t* w0 = p.w + (static_cast<int64_t>(e) * N + n0) * p.w_pitch;
   const int k16 = (K + 15) & ~15;
@@ -119,6 +96,10 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
     if (gather) j = p.x_row_index[j];
     return j < 0 ? 0 : j < p.x_rows ? j : static_cast<int>(p.x_rows) - 1;
   };
+  auto w_row = [&](int row) {  // row of W, from n0, behind row `row` of the tile
+    const int part = row % (16 * TN) / kPart, n = row / (16 * TN) * kPart + row % kPart;
+    return (n0 + n < half ? n : half - 1 - n0) + part * half;
+  };
 
   // A row of a stage is 128 bytes, its chunk c of 16 at place c ^ (row & 7), and a lane loads the chunk that belongs at its
   // place.  An operand is chunks q and q + 4 of a row, q = lane / 16 (the order of K is free as long as both operands share it):
@@ -129,14 +110,14 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
     const int row = (i * kWaves + wave) * 8 + (lane >> 3), chunk = (lane & 7) ^ (lane >> 3);
-    if (i < BN / 8 / kWaves) voff[i] = static_cast<uint32_t>(n0 + row < N ? row : N - 1 - n0) * w_pitch + chunk * 16;
+    if (i < BN / 8 / kWaves) voff[i] = static_cast<uint32_t>(w_row(row)) * w_pitch + chunk * 16;
     else voff[i] = static_cast<uint32_t>(source(r0 + row - BN) - (gather ? 0 : r0)) * x_pitch + chunk * 16;
     asm volatile("" : "+v"(voff[i]));  // (kept as it is, not computed again at every load)
   }
   uint8_t* const lds0 = smem + wave * 1024;
   // Loads [from, to) of block g into its stage; past the last block, that one's again (nobody reads them).  A chunk past the row's
   // end is read from its start, and masked where it is used.  No branches: the loop below is to stay one run of instructions.
-  const int last = groups - 1, my_chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+  const int my_chunk = ((lane & 7) ^ (lane >> 3)) * 16;
   auto issue = [&](int g, int from, int to) {
     uint8_t* const at = lds0 + (g & 1) * kStage;
     const int k = (g < last ? g : last) * 128;
@@ -150,11 +131,13 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
   uint32_t xrow[TM];
 #pragma unroll
   for (int j = 0; j < TM; ++j) xrow[j] = source(r0 + wm + 16 * j + frow);
-  // a wave's rows of W lie in one block, or (64 rows and fewer) in part of one: tiles start at multiples of their size
-  static_assert(16 * TN <= kFp8Block && kFp8Block % (16 * TN) == 0, "one block of W a wave");
   typedef const __attribute__((address_space(4))) float* scalar_floats;  // read through the scalar cache
-  const int wb = (n0 + wn) / kFp8Block < n_blocks ? (n0 + wn) / kFp8Block : n_blocks - 1;
-  const scalar_floats ws = (scalar_floats)(p.ws + (static_cast<int64_t>(e) * n_blocks + wb) * groups);
+  scalar_floats ws[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int b = (n0 + (wave % WN) * kPart + i * half) / kFp8Block;
+    ws[i] = (scalar_floats)(p.ws + (static_cast<int64_t>(e) * n_blocks + (b < n_blocks ? b : n_blocks - 1)) * groups);
+  }
 
   float4_t acc[TN][TM];
 #pragma unroll
@@ -163,35 +146,49 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
     for (int j = 0; j < TM; ++j) acc[i][j] = float4_t{};
 
   // Scales are two blocks ahead, and asked for in front of a stage's loads: the wait for a load takes all before it as well.
-  float sx_next[TM], sw_next = 0.f;
+  float sx_next[TM], sw_next[P];
   auto scales = [&](int g) {
     g = g < last ? g : last;
 #pragma unroll
     for (int j = 0; j < TM; ++j) sx_next[j] = (p.xs + g * p.x_rows)[xrow[j]];
-    sw_next = ws[g];
+#pragma unroll
+    for (int i = 0; i < P; ++i) sw_next[i] = ws[i][g];
+  };
+  struct Operand {
+    int4_t a, b;  // chunks q and q + 4 of a row
   };
   auto frag = [&](int g, int row, auto tail) {
     const uint8_t* base = smem + (g & 1) * kStage + row * 128;
-    int4_t a = *reinterpret_cast<const int4_t*>(base + ((fquad ^ (row & 7)) << 4));
-    int4_t b = *reinterpret_cast<const int4_t*>(base + (((fquad + 4) ^ (row & 7)) << 4));
+    Operand o;
+    o.a = *reinterpret_cast<const int4_t*>(base + ((fquad ^ (row & 7)) << 4));
+    o.b = *reinterpret_cast<const int4_t*>(base + (((fquad + 4) ^ (row & 7)) << 4));
     if constexpr (decltype(tail)::value) {
-      a = mask_chunk(a, K - g * 128 - fquad * 16);
-      b = mask_chunk(b, K - g * 128 - fquad * 16 - 64);
+      o.a = mask_chunk(o.a, K - g * 128 - fquad * 16);
+      o.b = mask_chunk(o.b, K - g * 128 - fquad * 16 - 64);
     }
-    return int8_vt{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    return o;
   };
-  float4_t part[TM];                      // a row of results of one block, unscaled
-  float sc[TM], sc_old[TM], sc_next[TM];  // scales of this block, the one before and the one behind it
-  int8_vt fx[TM], fw[2];
+  struct Wide {
+    bf16x8_t v[4];
+  };
+  auto wide = [](const Operand& o) {
+    return Wide{{fp8_widen(o.a[0], o.a[1]), fp8_widen(o.a[2], o.a[3]), fp8_widen(o.b[0], o.b[1]), fp8_widen(o.b[2], o.b[3])}};
+  };
+  float4_t part[TM];                                   // a row of results of one block, unscaled
+  float sc[P][TM], sc_old[P][TM], sc_next[P][TM];  // scales of this block, the one before and the one behind it
+  Operand fx[TM], fw[2];
+  Wide wx[PRECISE ? TM : 1];
   // Waits for stage g and hands it over: every wave has read the stage before it, which may take the loads of block g + 1.
   auto hand_over = [&](int g) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
 #pragma unroll
-    for (int j = 0; j < TM; ++j) {
-      sc_next[j] = sw_next * sx_next[j];
-      asm volatile("" : "+v"(sc_next[j]));  // here, not behind the loads below
-    }
+    for (int i = 0; i < P; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        sc_next[i][j] = sw_next[i] * sx_next[j];
+        asm volatile("" : "+v"(sc_next[i][j]));  // here, not behind the loads below
+      }
     scales(g + 1);
   };
   // One block.  The multiply-adds of a result run beside the matrix instructions of the row of results behind it, and the last
@@ -199,8 +196,8 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
   // arrive while that row is computed.
   // The next block's loads go out kBurst at a time, the first behind the hand-over and the others in front of the rows: all at
   // once they fill the queue to the vector cache (16 cycles a load), and every wave waits there in front of its matrix instructions.
-  constexpr int kBurst = 2;
-  static_assert((TN - 1) * kBurst >= kLoads - kBurst, "every load has a row");
+  constexpr int kBurst = (kLoads + TN - 1) / TN > 2 ? (kLoads + TN - 1) / TN : 2;
+  auto burst = [&](int g, int i) { issue(g, i * kBurst < kLoads ? i * kBurst : kLoads, (i + 1) * kBurst < kLoads ? (i + 1) * kBurst : kLoads); };
   auto step = [&](int g, auto tail, auto next_tail, auto has_next) {
 #pragma unroll
     for (int i = 0; i < TN; ++i) {
@@ -209,115 +206,260 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
       } else if (decltype(has_next)::value) {
         hand_over(g + 1);
         fw[0] = frag(g + 1, wn + frow, next_tail);
-        issue(g + 2, 0, kBurst < kLoads ? kBurst : kLoads);
+        burst(g + 2, 0);
       }
-      if (decltype(has_next)::value && i + 1 < TN && (i + 1) * kBurst < kLoads)
-        issue(g + 1, (i + 1) * kBurst, (i + 2) * kBurst < kLoads ? (i + 2) * kBurst : kLoads);
+      if (decltype(has_next)::value && i + 1 < TN) burst(g + 1, i + 1);
+      Wide ww;
+      if constexpr (PRECISE) ww = wide(fw[i & 1]);
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
-        const float s = i == 0 ? sc_old[j] : sc[j];
-        float4_t& to = acc[i == 0 ? TN - 1 : i - 1][j];
+        const int prev = i == 0 ? TN - 1 : i - 1;
+        const float s = i == 0 ? sc_old[prev * P / TN][j] : sc[prev * P / TN][j];
+        float4_t& to = acc[prev][j];
 #pragma unroll
         for (int v = 0; v < 4; ++v) to[v] = __builtin_fmaf(part[j][v], s, to[v]);
         asm volatile("" : "+v"(to));  // here, not behind the last row with all partial results kept
-        part[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[i & 1], fx[j], float4_t{}, 0, 0, 0, 0, 0, 0);
+        if constexpr (PRECISE) {
+          if (i == 0) wx[j] = wide(fx[j]);
+          part[j] = float4_t{};
+#pragma unroll
+          for (int h = 0; h < 4; ++h) part[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww.v[h], wx[j].v[h], part[j], 0, 0, 0);
+        } else {
+          auto both = [](const Operand& o) { return int8_vt{o.a[0], o.a[1], o.a[2], o.a[3], o.b[0], o.b[1], o.b[2], o.b[3]}; };
+          part[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(both(fw[i & 1]), both(fx[j]), float4_t{}, 0, 0, 0, 0, 0, 0);
+        }
         if (i + 1 == TN && decltype(has_next)::value) fx[j] = frag(g + 1, BN + wm + 16 * j + frow, next_tail);
       }
       __builtin_amdgcn_sched_barrier(0);  // rows in this order: operands of all rows at once would not fit the registers
     }
 #pragma unroll
-    for (int j = 0; j < TM; ++j) {
-      sc_old[j] = sc[j];
-      sc[j] = sc_next[j];
-    }
+    for (int i = 0; i < P; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        sc_old[i][j] = sc[i][j];
+        sc[i][j] = sc_next[i][j];
+      }
   };
-  static_assert(TN % 2 == 0, "the first row of a block uses fw[0]");
   constexpr std::true_type yes{};
   constexpr std::false_type no{};
-  scales(0);
-  issue(0, 0, kLoads);
-  hand_over(0);
-  issue(1, 0, kBurst < kLoads ? kBurst : kLoads);
+  scales(first);
+  issue(first, 0, kLoads);
+  hand_over(first);
+  burst(first + 1, 0);
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
     part[j] = float4_t{};
-    sc_old[j] = 0.f;
-    sc[j] = sc_next[j];
-  }
-  auto first = [&](auto tail) {
-    fw[0] = frag(0, wn + frow, tail);
 #pragma unroll
-    for (int j = 0; j < TM; ++j) fx[j] = frag(0, BN + wm + 16 * j + frow, tail);
+    for (int i = 0; i < P; ++i) {
+      sc_old[i][j] = 0.f;
+      sc[i][j] = sc_next[i][j];
+    }
+  }
+  auto begin = [&](auto tail) {
+    fw[0] = frag(first, wn + frow, tail);
+#pragma unroll
+    for (int j = 0; j < TM; ++j) fx[j] = frag(first, BN + wm + 16 * j + frow, tail);
   };
   // the last block is masked, whether K ends inside it or not: one form of it, once a tile
-  if (last == 0) first(yes);
-  else first(no);
-  for (int g = 0; g < last - 1; ++g) step(g, no, no, yes);
-  if (last > 0) step(last - 1, no, yes, yes);
+  if (first == last) begin(yes);
+  else begin(no);
+  for (int g = first; g < last - 1; ++g) step(g, no, no, yes);
+  if (first < last) step(last - 1, no, yes, yes);
   step(last, yes, no, no);
 #pragma unroll
   for (int j = 0; j < TM; ++j)
 #pragma unroll
-    for (int v = 0; v < 4; ++v) acc[TN - 1][j][v] = __builtin_fmaf(part[j][v], sc_old[j], acc[TN - 1][j][v]);
-
-  // The results change hands through LDS, 16 rows of x at a time and each wave in a part of its own, so that a row's
-  // columns go out as runs of 16 bytes per lane; float32 until bias and residual are in.
-  constexpr int kCols = 16 * TN, kRow = kCols + 4, kLanes = kCols / 8, kRows = 64 / kLanes < 16 ? 64 / kLanes : 16;
+    for (int v = 0; v < 4; ++v) acc[TN - 1][j][v] = __builtin_fmaf(part[j][v], sc_old[P - 1][j], acc[TN - 1][j][v]);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads that nobody reads may still land in the stages
-  __syncthreads();
-  float* const mine = reinterpret_cast<float*>(smem) + wave * 16 * kRow;
-  const bool vec = N % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.residual)) & 15u) == 0;
+  __syncthreads();  // (and the last stage has been read)
+
+  if constexpr (SILU) {
+    // silu(gate) * up in place of the gates; a group is the tile's 128 columns, of which this wave has kPart
+    float* const tops = reinterpret_cast<float*>(smem);  // [WN][BM]
+    uint8_t* const bytes = smem + WN * BM * 4;           // [BM][kBytes]
+    constexpr int kBytes = kFp8Block + 16;
 #pragma unroll
-  for (int j = 0; j < TM; ++j) {
+    for (int j = 0; j < TM; ++j) {
+      float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < TN; ++i) *reinterpret_cast<float4_t*>(mine + frow * kRow + 16 * i + 4 * fquad) = acc[i][j];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+      for (int i = 0; i < TN / 2; ++i)
 #pragma unroll
-    for (int t = 0; t < 16 / kRows; ++t) {
-      const int row = t * kRows + lane / kLanes, col = (lane % kLanes) * 8;
-      const int64_t r = r0 + wm + 16 * j + row;
-      const int n = n0 + wn + col;
-      if (row < 16 && r < r_end && n < N) {
-        const float4_t a = *reinterpret_cast<const float4_t*>(mine + row * kRow + col), b = *reinterpret_cast<const float4_t*>(mine + row * kRow + col + 4);
-        float o[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-        store_run<OUT, MODEL>(p, r, n, N, vec, o);
-      }
+        for (int v = 0; v < 4; ++v) {
+          acc[i][j][v] = silu_mul_f32(acc[i][j][v], acc[i + TN / 2][j][v]);
+          top = fmaxf(top, fp8_magnitude(acc[i][j][v]));
+        }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (fquad == 0) tops[(wave % WN) * BM + wm + 16 * j + frow] = top;
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const int row = wm + 16 * j + frow;
+      float top = tops[row];
+#pragma unroll
+      for (int w = 1; w < WN; ++w) top = fmaxf(top, tops[w * BM + row]);
+      const uint32_t bits = fp8_scale_bits(top);
+      const float inv = fp8_inverse(bits);
+#pragma unroll
+      for (int i = 0; i < TN / 2; ++i)
+        *reinterpret_cast<uint32_t*>(bytes + row * kBytes + (wave % WN) * kPart + 16 * i + 4 * fquad) =
+            fp8_quad(acc[i][j][0] * inv, acc[i][j][1] * inv, acc[i][j][2] * inv, acc[i][j][3] * inv);
+      if (wave % WN == 0 && fquad == 0 && r0 + row < r_end)
+        p.scale_out[static_cast<int64_t>(nt) * p.rows + r0 + row] = __builtin_bit_cast(float, bits);
+    }
+    __syncthreads();
+    for (int c = tid; c < BM * 8; c += 64 * kWaves) {
+      const int row = c >> 3;
+      if (r0 + row < r_end)
+        *reinterpret_cast<uint4*>(p.q_out + static_cast<int64_t>(r0 + row) * half + n0 + (c & 7) * 16) =
+            *reinterpret_cast<const uint4*>(bytes + row * kBytes + (c & 7) * 16);
+    }
+  } else {
+    // The results change hands through LDS, 16 rows of x at a time and each wave in a part of its own, so that a row's
+    // columns go out as runs of 16 bytes per lane; float32 until bias and residual are in.
+    constexpr int kCols = 16 * TN, kRow = kCols + 4, kLanes = kCols / 8, kRows = 64 / kLanes < 16 ? 64 / kLanes : 16;
+    float* const mine = reinterpret_cast<float*>(smem) + wave * 16 * kRow;
+    Fp8Args to = p;
+    if (gridDim.y > 1) {  // a share of K: its sums go to the scratch as they are
+      to.y = static_cast<float*>(p.workspace) + blockIdx.y * p.rows * N;
+      to.out_dtype = MODEL_F32;
+      to.bias = to.residual = nullptr;
+    }
+    const bool vec = N % 8 == 0 && (reinterpret_cast<uintptr_t>(to.y) & 15u) == 0;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+#pragma unroll
+      for (int i = 0; i < TN; ++i) *reinterpret_cast<float4_t*>(mine + frow * kRow + 16 * i + 4 * fquad) = acc[i][j];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int t = 0; t < 16 / kRows; ++t) {
+        const int row = t * kRows + lane / kLanes, col = (lane % kLanes) * 8;
+        const int64_t r = r0 + wm + 16 * j + row;
+        const int n = n0 + wn + col;
+        if (row < 16 && r < r_end && n < N) {
+          const float4_t a = *reinterpret_cast<const float4_t*>(mine + row * kRow + col), b = *reinterpret_cast<const float4_t*>(mine + row * kRow + col + 4);
+          float o[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+          fp8_store<8>(to, r, n, N, vec, o);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
   }
 }
 
-template <int WN, int WM, int TN, int TM>
-static hipError_t launch_tile(const Fp8Args& a, hipStream_t s) {
-  constexpr int BN = 16 * WN * TN, BM = 16 * WM * TM;
-  constexpr size_t stages = size_t(2) * (BN + BM) * 128, results = size_t(WN * WM) * 16 * (16 * TN + 4) * 4;
-  constexpr size_t lds = stages > results ? stages : results;
-  const int64_t m_tiles = a.indptr ? a.rows / BM + a.experts : (a.rows + BM - 1) / BM, n_tiles = (a.N + BN - 1) / BN;
-  const unsigned grid = static_cast<unsigned>((n_tiles * m_tiles + 7) / 8 * 8);
-  note_kernel("fp8_tile %dx%d", BN, BM);
-  auto go = [&](auto out, auto model) {
-    auto* kern = fp8_tile_kernel<WN, WM, TN, TM, decltype(out)::value, decltype(model)::value>;
-    if (lds > 65536) {
-      const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kern));
-      if (e != hipSuccess) return e;
+// the sums of the shares of K, in their order; bias, residual and the one rounding
+__global__ __launch_bounds__(256) void fp8_join_kernel(Fp8Args p, int splits) {
+  const int N = static_cast<int>(p.N), runs = (N + 7) / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= p.rows * runs) return;
+  const int64_t r = i / runs;
+  const int n = static_cast<int>(i - r * runs) * 8;
+  const float* from = static_cast<const float*>(p.workspace) + r * N + n;
+  float o[8];
+  if (N % 8 == 0) {
+    float4_t a = {}, b = {};
+    for (int s = 0; s < splits; ++s, from += p.rows * N) {
+      a += *reinterpret_cast<const float4_t*>(from);
+      b += *reinterpret_cast<const float4_t*>(from + 4);
     }
-    hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * WN * WM), lds, s, a, static_cast<int>(n_tiles), static_cast<int>(m_tiles));
-    return hipGetLastError();
-  };
-  auto by_model = [&](auto out) {
-    if (a.model_dtype == MODEL_F32) return go(out, std::integral_constant<int, MODEL_F32>{});
-    if (a.model_dtype == MODEL_BF16) return go(out, std::integral_constant<int, MODEL_BF16>{});
-    return go(out, std::integral_constant<int, MODEL_F16>{});
-  };
-  if (a.out_dtype == MODEL_F32) return by_model(std::integral_constant<int, MODEL_F32>{});
-  if (a.out_dtype == MODEL_BF16) return by_model(std::integral_constant<int, MODEL_BF16>{});
-  return by_model(std::integral_constant<int, MODEL_F16>{});
+#pragma unroll
+    for (int v = 0; v < 4; ++v) o[v] = a[v], o[v + 4] = b[v];
+  } else {
+#pragma unroll
+    for (int v = 0; v < 8; ++v) o[v] = 0.f;
+    for (int s = 0; s < splits; ++s, from += p.rows * N)
+#pragma unroll
+      for (int v = 0; v < 8; ++v)
+        if (n + v < N) o[v] += from[v];
+  }
+  fp8_store<8>(p, r, n, N, N % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0, o);
+}
+
+namespace {
+
+// A tile form and the shares of K of a dense product.
+struct Plan {
+  int form = 0, splits = 1, per_split = 0;
+};
+// per block of K and round of workgroups, in ns (measured); workgroups that run at a time
+struct Form {
+  int bn, bm, at_a_time;
+  float block_ns;
+};
+constexpr Form kForms[] = {{256, 256, 256, 2050.f}, {256, 128, 256, 1250.f}, {128, 128, 512, 1300.f}, {128, 64, 512, 900.f}};
+Plan plan_of(int64_t rows, int64_t N, int64_t K) {
+  const int64_t groups = (K + kFp8Block - 1) / kFp8Block;
+  Plan best;
+  float best_ns = 0.f;
+  for (int f = 0; f < 4; ++f) {
+    if (options().gemm_variant >= 0 && options().gemm_variant < 4 && options().gemm_variant != f) continue;
+    const int64_t tiles = ((rows + kForms[f].bm - 1) / kForms[f].bm) * ((N + kForms[f].bn - 1) / kForms[f].bn);
+    for (int64_t want = 1; want <= 16 && want <= (groups < 4 ? 1 : groups / 4); ++want) {
+      if (options().gemm_split_k > 0 && options().gemm_split_k != want) continue;
+      const int64_t per = (groups + want - 1) / want, splits = (groups + per - 1) / per;
+      const int64_t rounds = (tiles * splits + kForms[f].at_a_time - 1) / kForms[f].at_a_time;
+      const float ns = rounds * (per * kForms[f].block_ns + 4000.f) + (splits > 1 ? 2500.f + splits * rows * N * 8 / 4000.f : 0.f);
+      if (best.per_split == 0 || ns < best_ns) {
+        best_ns = ns;
+        best.form = f;
+        best.splits = static_cast<int>(splits);
+        best.per_split = static_cast<int>(per);
+      }
+    }
+  }
+  return best;
+}
+
+template <int WN, int WM, int TN, int TM, bool PRECISE, bool SILU>
+hipError_t launch_tile(const Fp8Args& a, const Plan& plan, hipStream_t s) {
+  constexpr int BN = 16 * WN * TN, BM = 16 * WM * TM;
+  constexpr size_t stages = size_t(2) * (BN + BM) * 128, results = SILU ? size_t(BM) * (4 * WN + kFp8Block + 16) : size_t(WN * WM) * 16 * (16 * TN + 4) * 4;
+  constexpr size_t lds = stages > results ? stages : results;
+  const int64_t groups = (a.K + kFp8Block - 1) / kFp8Block;
+  const int64_t m_tiles = a.indptr ? a.rows / BM + a.experts : (a.rows + BM - 1) / BM, n_tiles = (a.N + BN - 1) / BN;
+  int splits = 1, per_split = static_cast<int>(groups);
+  if (plan.splits > 1 && a.workspace != nullptr && a.workspace_bytes >= plan.splits * a.rows * a.N * 4) {
+    splits = plan.splits;
+    per_split = plan.per_split;
+  }
+  auto* kern = fp8_tile_kernel<WN, WM, TN, TM, PRECISE, SILU>;
+  if (lds > 65536) {
+    const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kern));
+    if (e != hipSuccess) return e;
+  }
+  note_kernel("fp8_tile %dx%d%s, %d shares of K", BN, BM, PRECISE ? " float32 sums" : "", splits);
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((n_tiles * m_tiles + 7) / 8 * 8), splits), dim3(64 * WN * WM), lds, s, a,
+                     static_cast<int>(n_tiles), static_cast<int>(m_tiles), per_split);
+  if (splits > 1)
+    hipLaunchKernelGGL(fp8_join_kernel, dim3(static_cast<unsigned>((a.rows * ((a.N + 7) / 8) + 255) / 256)), dim3(256), 0, s, a, splits);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t fp8_tile_workspace_bytes(int64_t rows, int64_t N, int64_t K) {
+  const Plan p = plan_of(rows, N, K);
+  return p.splits > 1 ? p.splits * rows * N * 4 : 0;
 }
 
 hipError_t launch_fp8_tile(const Fp8Args& a, hipStream_t s) {
-  return launch_tile<2, 4, 8, 4>(a, s);
+  if (a.q_out != nullptr) {
+    if (a.N % (2 * kFp8Block) != 0 || static_cast<uint64_t>(a.N) * a.w_pitch >= 0xffffffffull) return hipErrorNotSupported;
+    return launch_tile<4, 2, 4, 4, true, true>(a, Plan{}, s);
+  }
+  if (a.precise) return launch_tile<4, 2, 4, 4, true, false>(a, Plan{}, s);
+  Plan plan;
+  if (!a.indptr) plan = plan_of(a.rows, a.N, a.K);
+  else plan.form = a.rows > 192 * a.experts ? 0 : a.rows > 64 * a.experts ? 1 : 3;
+  switch (plan.form) {
+    case 0: return launch_tile<2, 4, 8, 4, false, false>(a, plan, s);
+    case 1: return launch_tile<4, 2, 4, 4, false, false>(a, plan, s);
+    case 2: return launch_tile<2, 2, 4, 4, false, false>(a, plan, s);
+    default: return launch_tile<2, 2, 4, 2, false, false>(a, plan, s);
+  }
 }
 
 }  // namespace gq
