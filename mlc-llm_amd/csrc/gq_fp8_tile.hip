@@ -47,10 +47,11 @@ __device__ __forceinline__ int4_t mask_chunk(int4_t v, int left) {
 // SILU: half of a wave's rows of W are gate rows and half the up rows that belong to them.
 template <int WN, int WM, int TN, int TM, bool PRECISE, bool SILU>
 __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, int n_tiles, int m_tiles, int per_split) {
-  constexpr int kWaves = WN * WM, BN = 16 * WN * TN, BM = 16 * WM * TM, kStage = (BN + BM) * 128;
-  constexpr int kLoads = (BN + BM) / 8 / kWaves;  // of 1 KiB, eight rows, a wave and stage
+  constexpr int kWaves = WN * WM, BN = 16 * WN * TN, BM = 16 * WM * TM;
+  constexpr int kWLoads = BN / 8 / kWaves, kXLoads = BM / 8 / kWaves;  // of 1 KiB, eight rows, a wave and block of K
   constexpr int P = SILU ? 2 : 1, kPart = 16 * TN / P;  // parts of a wave's rows of W
-  static_assert((BN + BM) / 8 % kWaves == 0 && BN / 8 % kWaves == 0, "whole loads");
+  constexpr int kWStage = BN * 128, kXStage = BM * 128;  // three stages of W and two of x in LDS
+  static_assert(BM / 8 % kWaves == 0 && BN / 8 % kWaves == 0, "whole loads");
   static_assert(TN % 2 == 0, "the first row of a block uses fw[0]");
   static_assert(kPart <= kFp8Block && kFp8Block % kPart == 0, "a part lies in one block of W");
   static_assert(!SILU || BN == 2 * kFp8Block, "a tile holds one group of the activation");
@@ -106,25 +107,34 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
   // so the 16 lanes that LDS serves in a cycle, half of them of one quarter of the wave and half of the next, meet 16 places in
   // 16 different groups of banks.  With chunks 2 q and 2 q + 1 every read took two turns.
   const uint32_t w_pitch = static_cast<uint32_t>(p.w_pitch), x_pitch = static_cast<uint32_t>(p.x_pitch);
-  uint32_t voff[kLoads];
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int row = (i * kWaves + wave) * 8 + (lane >> 3), chunk = (lane & 7) ^ (lane >> 3);
-    if (i < BN / 8 / kWaves) voff[i] = static_cast<uint32_t>(w_row(row)) * w_pitch + chunk * 16;
-    else voff[i] = static_cast<uint32_t>(source(r0 + row - BN) - (gather ? 0 : r0)) * x_pitch + chunk * 16;
-    asm volatile("" : "+v"(voff[i]));  // (kept as it is, not computed again at every load)
-  }
-  uint8_t* const lds0 = smem + wave * 1024;
-  // Loads [from, to) of block g into its stage; past the last block, that one's again (nobody reads them).  A chunk past the row's
-  // end is read from its start, and masked where it is used.  No branches: the loop below is to stay one run of instructions.
+  uint32_t w_off[kWLoads], x_off[kXLoads];
   const int my_chunk = ((lane & 7) ^ (lane >> 3)) * 16;
-  auto issue = [&](int g, int from, int to) {
-    uint8_t* const at = lds0 + (g & 1) * kStage;
+#pragma unroll
+  for (int i = 0; i < kWLoads; ++i) {
+    w_off[i] = static_cast<uint32_t>(w_row((i * kWaves + wave) * 8 + (lane >> 3))) * w_pitch + my_chunk;
+    asm volatile("" : "+v"(w_off[i]));  // (kept as it is, not computed again at every load)
+  }
+#pragma unroll
+  for (int i = 0; i < kXLoads; ++i) {
+    x_off[i] = static_cast<uint32_t>(source(r0 + (i * kWaves + wave) * 8 + (lane >> 3)) - (gather ? 0 : r0)) * x_pitch + my_chunk;
+    asm volatile("" : "+v"(x_off[i]));
+  }
+  // Loads [from, to) of block g; past the last block, that one's again (nobody reads them).  A chunk past the row's end is
+  // read from its start, and masked where it is used.  No branches: the loop below is to stay one run of instructions.
+  auto shift_of = [&](int g) {
     const int k = (g < last ? g : last) * 128;
-    const int shift = k + my_chunk < k16 ? k : -my_chunk;
+    return k + my_chunk < k16 ? k : -my_chunk;
+  };
+  auto issue_w = [&](int g, int slot, int from, int to) {
+    const int shift = shift_of(g);
+#pragma unroll
+    for (int i = from; i < to; ++i) load_to_lds(w_rsrc, w_off[i] + shift, 0, smem + slot + (i * kWaves + wave) * 1024);
+  };
+  auto issue_x = [&](int g, int from, int to) {
+    const int shift = shift_of(g);
 #pragma unroll
     for (int i = from; i < to; ++i)
-      load_to_lds(i < BN / 8 / kWaves ? w_rsrc : x_rsrc, voff[i] + shift, 0, at + i * kWaves * 1024);
+      load_to_lds(x_rsrc, x_off[i] + shift, 0, smem + 3 * kWStage + (g & 1) * kXStage + (i * kWaves + wave) * 1024);
   };
 
   const int wn = (wave % WN) * 16 * TN, wm = (wave / WN) * 16 * TM, frow = lane & 15, fquad = lane >> 4;
@@ -157,8 +167,8 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
   struct Operand {
     int4_t a, b;  // chunks q and q + 4 of a row
   };
-  auto frag = [&](int g, int row, auto tail) {
-    const uint8_t* base = smem + (g & 1) * kStage + row * 128;
+  auto frag = [&](const uint8_t* stage, int g, int row, auto tail) {
+    const uint8_t* base = stage + row * 128;
     Operand o;
     o.a = *reinterpret_cast<const int4_t*>(base + ((fquad ^ (row & 7)) << 4));
     o.b = *reinterpret_cast<const int4_t*>(base + (((fquad + 4) ^ (row & 7)) << 4));
@@ -178,9 +188,14 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
   float sc[P][TM], sc_old[P][TM], sc_next[P][TM];  // scales of this block, the one before and the one behind it
   Operand fx[TM], fw[2];
   Wide wx[PRECISE ? TM : 1];
-  // Waits for stage g and hands it over: every wave has read the stage before it, which may take the loads of block g + 1.
+  int w_now = 0, w_then = kWStage, w_last = 2 * kWStage;  // stages of W of this block, the next and the one behind it
+  auto frag_w = [&](int g, int slot, int i, auto tail) { return frag(smem + slot, g, wn + 16 * i + frow, tail); };
+  auto frag_x = [&](int g, int j, auto tail) { return frag(smem + 3 * kWStage + (g & 1) * kXStage, g, wm + 16 * j + frow, tail); };
+  // Waits for block g's stages and hands them over.  Loads come back in order, and the last ones asked for are those of W for
+  // block g + 1, which may still be on their way: W comes from memory and is two blocks ahead, x from the L2 and one.  Every wave has
+  // read block g - 1 by then, whose stages take x of block g + 1 and W of block g + 2.
   auto hand_over = [&](int g) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kWLoads) : "memory");
     __builtin_amdgcn_s_barrier();
 #pragma unroll
     for (int i = 0; i < P; ++i)
@@ -196,19 +211,23 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
   // arrive while that row is computed.
   // The next block's loads go out kBurst at a time, the first behind the hand-over and the others in front of the rows: all at
   // once they fill the queue to the vector cache (16 cycles a load), and every wave waits there in front of its matrix instructions.
-  constexpr int kBurst = (kLoads + TN - 1) / TN > 2 ? (kLoads + TN - 1) / TN : 2;
-  auto burst = [&](int g, int i) { issue(g, i * kBurst < kLoads ? i * kBurst : kLoads, (i + 1) * kBurst < kLoads ? (i + 1) * kBurst : kLoads); };
+  constexpr int kBurst = 2, kBursts = (kXLoads + kWLoads) / kBurst;
+  static_assert(kXLoads % kBurst == 0 && kWLoads % kBurst == 0 && kBursts <= TN, "a burst is of one kind and every burst has a row");
+  auto burst = [&](int i, int g, int w_slot) {  // burst i of x of block g and W of block g + 1
+    if (i * kBurst < kXLoads) issue_x(g, i * kBurst, (i + 1) * kBurst);
+    else if (i < kBursts) issue_w(g + 1, w_slot, i * kBurst - kXLoads, (i + 1) * kBurst - kXLoads);
+  };
   auto step = [&](int g, auto tail, auto next_tail, auto has_next) {
 #pragma unroll
     for (int i = 0; i < TN; ++i) {
       if (i + 1 < TN) {
-        fw[(i + 1) & 1] = frag(g, wn + 16 * (i + 1) + frow, tail);
+        fw[(i + 1) & 1] = frag_w(g, w_now, i + 1, tail);
       } else if (decltype(has_next)::value) {
         hand_over(g + 1);
-        fw[0] = frag(g + 1, wn + frow, next_tail);
-        burst(g + 2, 0);
+        fw[0] = frag_w(g + 1, w_then, 0, next_tail);
+        burst(0, g + 2, w_now);
       }
-      if (decltype(has_next)::value && i + 1 < TN) burst(g + 1, i + 1);
+      if (decltype(has_next)::value && i + 1 < TN) burst(i + 1, g + 1, w_last);
       Wide ww;
       if constexpr (PRECISE) ww = wide(fw[i & 1]);
 #pragma unroll
@@ -228,10 +247,17 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
           auto both = [](const Operand& o) { return int8_vt{o.a[0], o.a[1], o.a[2], o.a[3], o.b[0], o.b[1], o.b[2], o.b[3]}; };
           part[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(both(fw[i & 1]), both(fx[j]), float4_t{}, 0, 0, 0, 0, 0, 0);
         }
-        if (i + 1 == TN && decltype(has_next)::value) fx[j] = frag(g + 1, BN + wm + 16 * j + frow, next_tail);
+        if (i + 1 == TN && decltype(has_next)::value) {
+          fx[j] = frag_x(g + 1, j, next_tail);
+          __builtin_amdgcn_sched_barrier(0);  // (at once, not behind the row's other instructions)
+        }
       }
       __builtin_amdgcn_sched_barrier(0);  // rows in this order: operands of all rows at once would not fit the registers
     }
+    const int freed = w_now;
+    w_now = w_then;
+    w_then = w_last;
+    w_last = freed;
 #pragma unroll
     for (int i = 0; i < P; ++i)
 #pragma unroll
@@ -243,9 +269,12 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
   constexpr std::true_type yes{};
   constexpr std::false_type no{};
   scales(first);
-  issue(first, 0, kLoads);
+  issue_w(first, w_now, 0, kWLoads);
+  issue_x(first, 0, kXLoads);
+  asm volatile("" ::: "memory");  // (in this order)
+  issue_w(first + 1, w_then, 0, kWLoads);
   hand_over(first);
-  burst(first + 1, 0);
+  burst(0, first + 1, w_last);
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
     part[j] = float4_t{};
@@ -256,9 +285,9 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
     }
   }
   auto begin = [&](auto tail) {
-    fw[0] = frag(first, wn + frow, tail);
+    fw[0] = frag_w(first, w_now, 0, tail);
 #pragma unroll
-    for (int j = 0; j < TM; ++j) fx[j] = frag(first, BN + wm + 16 * j + frow, tail);
+    for (int j = 0; j < TM; ++j) fx[j] = frag_x(first, j, tail);
   };
   // the last block is masked, whether K ends inside it or not: one form of it, once a tile
   if (first == last) begin(yes);
@@ -416,7 +445,7 @@ Plan plan_of(int64_t rows, int64_t N, int64_t K) {
 template <int WN, int WM, int TN, int TM, bool PRECISE, bool SILU>
 hipError_t launch_tile(const Fp8Args& a, const Plan& plan, hipStream_t s) {
   constexpr int BN = 16 * WN * TN, BM = 16 * WM * TM;
-  constexpr size_t stages = size_t(2) * (BN + BM) * 128, results = SILU ? size_t(BM) * (4 * WN + kFp8Block + 16) : size_t(WN * WM) * 16 * (16 * TN + 4) * 4;
+  constexpr size_t stages = size_t(3 * BN + 2 * BM) * 128, results = SILU ? size_t(BM) * (4 * WN + kFp8Block + 16) : size_t(WN * WM) * 16 * (16 * TN + 4) * 4;
   constexpr size_t lds = stages > results ? stages : results;
   const int64_t groups = (a.K + kFp8Block - 1) / kFp8Block;
   const int64_t m_tiles = a.indptr ? a.rows / BM + a.experts : (a.rows + BM - 1) / BM, n_tiles = (a.N + BN - 1) / BN;
