@@ -111,8 +111,6 @@ LinearWorkspace linear_workspace(int64_t M, int64_t N, int64_t K, bool x_quantiz
   return w;
 }
 
-constexpr int64_t kIdSlots = 1024;  // slots whose ids every workgroup looks through itself
-
 struct MoeWorkspace {
   uint8_t *xq, *hq;
   float *xs, *hs, *both;
@@ -344,8 +342,7 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
   const int64_t slots = T * top_k;
   const int64_t segments = slots < num_experts ? slots : num_experts;
   hipError_t e;
-  if (slots <= 16 * segments && slots <= kIdSlots) {
-    // a slot or a few an expert: the workgroups find their rows from the ids, x and the activation are quantised where they are read
+  if (T == 1) {  // one token: its slots are the segments, x and the activation are quantised where they are read
     gq::Fp8RowsArgs r;
     r.x = x;
     r.x_rows = T;
@@ -360,7 +357,6 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
     r.rows = slots;
     r.ids = static_cast<const int32_t*>(ids);
     r.x_div = static_cast<int>(top_k);
-    r.top_k = static_cast<int>(top_k);
     r.silu = 1;
     r.out_dtype = MI355GQ_F32;
     r.y_aligned = 1;
@@ -385,9 +381,8 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
     }
     if (e != hipErrorNotSupported) return hip_result(e, "fp8_moe launch");
   }
-  e = gq::launch_moe_plan(static_cast<const int32_t*>(ids), slots, static_cast<int>(top_k), static_cast<int>(num_experts),
-                          ws.row_token, ws.slot_row, ws.indptr, s);
-  if (e == hipSuccess) e = gq::launch_fp8_quantize(x, T, hidden, model_dtype, false, ws.xq, hidden, ws.xs, s);
+  e = gq::launch_moe_plan_quantize(static_cast<const int32_t*>(ids), slots, static_cast<int>(top_k), static_cast<int>(num_experts),
+                                   ws.row_token, ws.slot_row, ws.indptr, x, T, hidden, model_dtype, ws.xq, ws.xs, s);
   gq::Fp8Args a;
   a.x = ws.xq;
   a.xs = ws.xs;
@@ -405,26 +400,29 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
   a.y = ws.both;
   a.out_dtype = MI355GQ_F32;
   a.precise = true;  // sums that are rounded to e4m3 again: an error of 1e-5 would move one in thousands by a sixteenth
-  bool activated = false;
-  if (e == hipSuccess && slots <= kFewRows / 2 * segments) {
-    gq::Fp8RowsArgs r = few_rows(a);
-    r.silu = 1;
-    const hipError_t done = gq::launch_fp8_rows(r, static_cast<int>(slots * 3 / (2 * segments) + 1), s);
-    activated = done == hipSuccess;
-    if (done != hipErrorNotSupported) e = done;
+  const bool by_rows = slots <= kFewRows / 2 * segments;
+  const int rows_max = static_cast<int>(slots * 3 / (2 * segments) + 1);
+  if (e == hipSuccess) {
+    hipError_t done;
+    if (by_rows) {
+      gq::Fp8RowsArgs r = few_rows(a);
+      r.silu = 1;
+      r.q_out = ws.hq;
+      r.scale_out = ws.hs;
+      done = gq::launch_fp8_rows(r, rows_max, s);
+    } else {
+      a.q_out = ws.hq;
+      a.scale_out = ws.hs;
+      done = gq::launch_fp8_tile(a, s);
+      a.q_out = nullptr;
+      a.scale_out = nullptr;
+    }
+    if (done == hipErrorNotSupported) {  // inter is no multiple of 128: product and activation apart
+      done = product(a, s);
+      if (done == hipSuccess) done = gq::launch_fp8_quantize(ws.both, slots, inter, MI355GQ_F32, true, ws.hq, inter, ws.hs, s);
+    }
+    e = done;
   }
-  bool quantized = false;
-  if (e == hipSuccess && !activated) {
-    a.q_out = ws.hq;
-    a.scale_out = ws.hs;
-    const hipError_t done = gq::launch_fp8_tile(a, s);
-    quantized = done == hipSuccess;
-    if (done != hipErrorNotSupported) e = done;
-    a.q_out = nullptr;
-    a.scale_out = nullptr;
-    if (e == hipSuccess && !quantized) e = gq::launch_fp8_tile(a, s);
-  }
-  if (e == hipSuccess && !quantized) e = gq::launch_fp8_quantize(ws.both, slots, inter, MI355GQ_F32, !activated, ws.hq, inter, ws.hs, s);
   a.precise = false;
   a.x = ws.hq;
   a.xs = ws.hs;

@@ -54,6 +54,37 @@ __device__ __forceinline__ float row_max16(float v) {
   return fmaxf(v, dpp_f<0x140>(v));  // row_mirror
 }
 
+// eight neighbouring numbers of DT (MODEL_F16, MODEL_F32, MODEL_BF16) at a 16-byte boundary as float32
+template <int DT>
+__device__ __forceinline__ void fp8_load8(const void* p, int64_t i, float (&f)[8]) {
+  if constexpr (DT == MODEL_F32) {
+    const float4_t* q = reinterpret_cast<const float4_t*>(static_cast<const float*>(p) + i);
+    const float4_t a = q[0], b = q[1];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) f[v] = a[v], f[v + 4] = b[v];
+  } else {
+    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      f[2 * v] = DT == MODEL_BF16 ? bf2f(u[v] & 0xffffu) : h2f(u[v] & 0xffffu);
+      f[2 * v + 1] = DT == MODEL_BF16 ? bf2f(u[v] >> 16) : h2f(u[v] >> 16);
+    }
+  }
+}
+// eight numbers of each of 16 neighbouring lanes, a group: its e4m3 numbers of this lane and the bits of its scale
+__device__ __forceinline__ uint2 fp8_group(const float (&f)[8], uint32_t* bits) {
+  float top = 0.f;
+#pragma unroll
+  for (int v = 0; v < 8; ++v) top = fmaxf(top, fp8_magnitude(f[v]));
+  *bits = fp8_scale_bits(row_max16(top));
+  const float inv = fp8_inverse(*bits);
+  uint2 q;
+  q.x = fp8_quad(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+  q.y = fp8_quad(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+  return q;
+}
+
 // Arguments of an e4m3 product y[r, n] = sum over blocks g of xs[g, r] ws[n / 128, g] sum_k xq[r, k] wq[n, k].
 struct Fp8Args {
   const uint8_t* x = nullptr;   // [x_rows, K], rows x_pitch bytes apart
@@ -90,10 +121,12 @@ struct Fp8RowsArgs {
   int64_t rows = 0;
   const int32_t* indptr = nullptr;       // segments as in Fp8Args, or
   const int32_t* x_row_index = nullptr;
-  const int32_t* ids = nullptr;          // [rows] the expert of each row, in any order; row r reads row r / x_div of x
-  int x_div = 1, top_k = 0;              // rows <= top_k: one token, whose ids differ
+  const int32_t* ids = nullptr;          // [rows] the expert of each row, segments of one row; row r reads row r / x_div of x
+  int x_div = 1;
   int silu = 0, model_dtype = 0, out_dtype = 0;
   int y_aligned = 0;  // y starts at 16 bytes
+  uint8_t* q_out = nullptr;  // silu: the activation quantised, [rows, N / 2] and its scales [N / 256, rows], instead of y; N / 2 a
+  float* scale_out = nullptr;  // multiple of 128
 };
 // rows_max: rows that the largest segment is expected to have (more are taken in passes); hipErrorNotSupported where no form applies
 hipError_t launch_fp8_rows(const Fp8RowsArgs& a, int rows_max, hipStream_t s);
@@ -183,6 +216,10 @@ hipError_t launch_moe_gating(const GatingArgs& a, hipStream_t s);
 // outside the experts), indptr [E + 1]
 hipError_t launch_moe_plan(const int32_t* ids, int64_t slots, int k, int E, int32_t* row_token, int32_t* slot_row,
                            int32_t* indptr, hipStream_t s);
+// ... and in the same launch rows of x [rows, cols] (float16 or bfloat16, 16-byte aligned, cols a multiple of 16) to e4m3 groups
+hipError_t launch_moe_plan_quantize(const int32_t* ids, int64_t slots, int k, int E, int32_t* row_token, int32_t* slot_row,
+                                    int32_t* indptr, const void* x, int64_t rows, int64_t cols, int model_dtype, uint8_t* q, float* scale,
+                                    hipStream_t s);
 // out[t] = sum over j of weights[t, j] y[row] in float32: row = slot_row[t k + j] (negative: no such row), or without slot_row
 // t k + j where ids[t k + j] is one of E experts
 hipError_t launch_moe_weighted_sum(const void* y, const int32_t* slot_row, const int32_t* ids, int E, const float* weights, int64_t T,

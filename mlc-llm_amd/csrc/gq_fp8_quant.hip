@@ -6,31 +6,12 @@ namespace gq {
 
 namespace {
 
-// eight neighbouring numbers of a row as float32
-template <int DT>
-__device__ __forceinline__ void load8(const void* p, int64_t i, float (&f)[8]) {
-  if constexpr (DT == MODEL_F32) {
-    const float4_t* q = reinterpret_cast<const float4_t*>(static_cast<const float*>(p) + i);
-    const float4_t a = q[0], b = q[1];
-#pragma unroll
-    for (int v = 0; v < 4; ++v) f[v] = a[v], f[v + 4] = b[v];
-  } else {
-    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      f[2 * v] = DT == MODEL_BF16 ? bf2f(u[v] & 0xffffu) : h2f(u[v] & 0xffffu);
-      f[2 * v + 1] = DT == MODEL_BF16 ? bf2f(u[v] >> 16) : h2f(u[v] >> 16);
-    }
-  }
-}
-
-// ... of which those past `cols` count as zero; ALIGNED: rows start at 16 bytes and cols is a multiple of 8
+// eight neighbouring numbers of a row, of which those past `cols` count as zero; ALIGNED: rows start at 16 bytes and cols is a multiple of 8
 template <int DT, bool ALIGNED>
 __device__ __forceinline__ void load8_row(const void* p, int64_t row0, int col, int cols, float (&f)[8]) {
   if constexpr (ALIGNED) {
     if (col < cols) {
-      load8<DT>(p, row0 + col, f);
+      fp8_load8<DT>(p, row0 + col, f);
       return;
     }
 #pragma unroll
@@ -62,16 +43,9 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const void* __restric
   } else {
     load8_row<DT, ALIGNED>(x, row * cols, col, cols, f);
   }
-  float top = 0.f;
-#pragma unroll
-  for (int v = 0; v < 8; ++v) top = fmaxf(top, fp8_magnitude(f[v]));
-  top = row_max16(top);
-  const uint32_t bits = fp8_scale_bits(top);
-  const float inv = fp8_inverse(bits);
+  uint32_t bits;
+  const uint2 out = fp8_group(f, &bits);
   if (col < q_pitch) {  // pitch is a multiple of 16
-    uint2 out;
-    out.x = fp8_quad(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-    out.y = fp8_quad(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
     *reinterpret_cast<uint2*>(q + row * q_pitch + col) = out;
   }
   if ((lane & 15) == 0 && col < cols) scale[static_cast<int64_t>(col / kFp8Block) * rows + row] = __builtin_bit_cast(float, bits);

@@ -166,10 +166,31 @@ hipError_t launch_moe_gating(const GatingArgs& a, hipStream_t s) {
 // The slots in the order of their expert, and in slot order within one: a workgroup an expert, each of which reads all ids
 // (a few hundred KiB at most, from the L2) and counts those before its own, so no table of counts goes through memory and
 // one launch does it.  A wave takes a run of slots, 64 at a time; its offsets come from the waves before it through LDS.
+//
+// DT: with E workgroups for this, further ones quantise rows of x, which the expert layer needs at the same point; a wave four
+// groups of a row at a time.  kPlanOnly: none.
+constexpr int kPlanOnly = -1;
+template <int DT>
 __global__ __launch_bounds__(1024) void moe_plan_kernel(const int32_t* __restrict__ ids, int slots, int k, int E, int per_wave,
                                                         int32_t* __restrict__ row_token, int32_t* __restrict__ slot_row,
-                                                        int32_t* __restrict__ indptr) {
+                                                        int32_t* __restrict__ indptr, const void* __restrict__ x, int64_t rows, int cols,
+                                                        uint8_t* __restrict__ q, float* __restrict__ scale) {
   __shared__ int counts[2][16];
+  if constexpr (DT != kPlanOnly) {
+    if (static_cast<int>(blockIdx.x) >= E) {
+      const int runs = (cols + 511) / 512;
+      const int64_t at = static_cast<int64_t>(blockIdx.x - E) * (blockDim.x >> 6) + (threadIdx.x >> 6), row = at / runs;
+      const int col = static_cast<int>(at - row * runs) * 512 + (threadIdx.x & 63) * 8;
+      if (row >= rows) return;
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (col < cols) fp8_load8<DT == kPlanOnly ? MODEL_F16 : DT>(x, row * cols + col, f);
+      uint32_t bits;
+      const uint2 out = fp8_group(f, &bits);
+      if (col < cols) *reinterpret_cast<uint2*>(q + row * cols + col) = out;
+      if ((threadIdx.x & 15) == 0 && col < cols) scale[static_cast<int64_t>(col / kFp8Block) * rows + row] = __builtin_bit_cast(float, bits);
+      return;
+    }
+  }
   const int e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int begin = wave * per_wave, end = begin + per_wave < slots ? begin + per_wave : slots;
   int own = 0, before = 0;
@@ -208,13 +229,28 @@ __global__ __launch_bounds__(1024) void moe_plan_kernel(const int32_t* __restric
   }
 }
 
-hipError_t launch_moe_plan(const int32_t* ids, int64_t slots, int k, int E, int32_t* row_token, int32_t* slot_row,
-                           int32_t* indptr, hipStream_t s) {
+template <int DT>
+static hipError_t launch_plan(const int32_t* ids, int64_t slots, int k, int E, int32_t* row_token, int32_t* slot_row, int32_t* indptr,
+                              const void* x, int64_t rows, int64_t cols, uint8_t* q, float* scale, hipStream_t s) {
   const int n = static_cast<int>(slots);
   const int waves = n >= 4096 ? 16 : n >= 1024 ? 8 : 4;
   const int per_wave = ((n + waves - 1) / waves + 63) / 64 * 64;
-  hipLaunchKernelGGL(moe_plan_kernel, dim3(E), dim3(64 * waves), 0, s, ids, n, k, E, per_wave, row_token, slot_row, indptr);
+  const int64_t more = DT == kPlanOnly ? 0 : (rows * ((cols + 511) / 512) + waves - 1) / waves;
+  hipLaunchKernelGGL(moe_plan_kernel<DT>, dim3(static_cast<unsigned>(E + more)), dim3(64 * waves), 0, s, ids, n, k, E, per_wave, row_token,
+                     slot_row, indptr, x, rows, static_cast<int>(cols), q, scale);
   return hipGetLastError();
+}
+
+hipError_t launch_moe_plan(const int32_t* ids, int64_t slots, int k, int E, int32_t* row_token, int32_t* slot_row,
+                           int32_t* indptr, hipStream_t s) {
+  return launch_plan<kPlanOnly>(ids, slots, k, E, row_token, slot_row, indptr, nullptr, 0, 0, nullptr, nullptr, s);
+}
+
+hipError_t launch_moe_plan_quantize(const int32_t* ids, int64_t slots, int k, int E, int32_t* row_token, int32_t* slot_row,
+                                    int32_t* indptr, const void* x, int64_t rows, int64_t cols, int model_dtype, uint8_t* q, float* scale,
+                                    hipStream_t s) {
+  return model_dtype == MODEL_BF16 ? launch_plan<MODEL_BF16>(ids, slots, k, E, row_token, slot_row, indptr, x, rows, cols, q, scale, s)
+                                   : launch_plan<MODEL_F16>(ids, slots, k, E, row_token, slot_row, indptr, x, rows, cols, q, scale, s);
 }
 
 // One thread eight neighbouring columns of a token (H % 8 == 0) or one (any H); float32 throughout, one rounding at the end.
