@@ -79,14 +79,13 @@ gq::Fp8RowsArgs few_rows(const gq::Fp8Args& a) {
   return r;
 }
 
-// rows of a segment up to which the weights' way from memory is what counts
-constexpr int64_t kFewRows = 64;
+// rows (of a segment on average) up to which the kernel that streams the weights past sixteen rows of x is the faster
+constexpr int64_t kFewRows = 16, kFewRowsEach = 10;
 
 hipError_t product(const gq::Fp8Args& a, hipStream_t s) {
   const int64_t segments = a.indptr ? (a.rows < a.experts ? a.rows : a.experts) : 1;
-  if (a.rows <= kFewRows * segments / (a.indptr ? 2 : 1)) {
-    const int64_t rows_max = a.indptr ? a.rows * 3 / (2 * segments) + 1 : a.rows;
-    const hipError_t e = gq::launch_fp8_rows(few_rows(a), static_cast<int>(rows_max), s);
+  if (a.rows <= (a.indptr ? kFewRowsEach * segments : kFewRows)) {
+    const hipError_t e = gq::launch_fp8_rows(few_rows(a), s);
     if (e != hipErrorNotSupported) return e;
   }
   return gq::launch_fp8_tile(a, s);
@@ -220,11 +219,11 @@ int mi355gq_fp8_linear(const void* x, int64_t x_pitch, const void* x_scale, cons
   a.precise = precise != 0;
   a.workspace = ws.split;
   a.workspace_bytes = ws.split_bytes;
-  if (x_scale == nullptr && M <= 16 && aligned16(x)) {  // the kernel quantises x itself
+  if (x_scale == nullptr && M <= kFewRows && aligned16(x)) {  // the kernel quantises x itself
     gq::Fp8RowsArgs r = few_rows(a);
     r.x = x;
     r.x_kind = model_dtype;
-    const hipError_t e = gq::launch_fp8_rows(r, static_cast<int>(M), as_stream(stream));
+    const hipError_t e = gq::launch_fp8_rows(r, as_stream(stream));
     if (e != hipErrorNotSupported) return hip_result(e, "fp8_linear launch");
   }
   if (x_scale == nullptr) {
@@ -360,7 +359,7 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
     r.silu = 1;
     r.out_dtype = MI355GQ_F32;
     r.y_aligned = 1;
-    e = gq::launch_fp8_rows(r, 16, s);
+    e = gq::launch_fp8_rows(r, s);
     if (e == hipSuccess) {
       r.x = ws.both;
       r.x_rows = slots;
@@ -374,7 +373,7 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
       r.x_div = 1;
       r.silu = 0;
       r.out_dtype = model_dtype;
-      e = gq::launch_fp8_rows(r, 16, s);
+      e = gq::launch_fp8_rows(r, s);
       if (e == hipSuccess)
         e = gq::launch_moe_weighted_sum(ws.y, nullptr, static_cast<const int32_t*>(ids), static_cast<int>(num_experts),
                                         static_cast<const float*>(weights), T, static_cast<int>(top_k), hidden, model_dtype, out, s);
@@ -400,8 +399,7 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
   a.y = ws.both;
   a.out_dtype = MI355GQ_F32;
   a.precise = true;  // sums that are rounded to e4m3 again: an error of 1e-5 would move one in thousands by a sixteenth
-  const bool by_rows = slots <= kFewRows / 2 * segments;
-  const int rows_max = static_cast<int>(slots * 3 / (2 * segments) + 1);
+  const bool by_rows = slots <= kFewRowsEach * segments;
   if (e == hipSuccess) {
     hipError_t done;
     if (by_rows) {
@@ -409,7 +407,7 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
       r.silu = 1;
       r.q_out = ws.hq;
       r.scale_out = ws.hs;
-      done = gq::launch_fp8_rows(r, rows_max, s);
+      done = gq::launch_fp8_rows(r, s);
     } else {
       a.q_out = ws.hq;
       a.scale_out = ws.hs;

@@ -128,8 +128,8 @@ struct Fp8RowsArgs {
   uint8_t* q_out = nullptr;  // silu: the activation quantised, [rows, N / 2] and its scales [N / 256, rows], instead of y; N / 2 a
   float* scale_out = nullptr;  // multiple of 128
 };
-// rows_max: rows that the largest segment is expected to have (more are taken in passes); hipErrorNotSupported where no form applies
-hipError_t launch_fp8_rows(const Fp8RowsArgs& a, int rows_max, hipStream_t s);
+// Sixteen rows of a segment at a time; hipErrorNotSupported where the kernel does not apply.
+hipError_t launch_fp8_rows(const Fp8RowsArgs& a, hipStream_t s);
 
 // Tiles, on the 8-bit matrix instruction or (precise) in float32 sums; K split over workgroups where the scratch for it is there.
 // silu: x [rows, K] times gate and up rows of w (N = 2 I), silu(gate) * up quantised into q_out [rows, I] and its scales

@@ -1,4 +1,4 @@
-// e4m3 block-scaled products of few rows (up to 64 a segment): the weights stream through once, bound by HBM.
+// e4m3 block-scaled products of up to sixteen rows (a segment): the weights stream through once, bound by HBM.
 //
 //   y[r, n] = sum over blocks g of 128 of  xs[g, r] ws[n / 128, g] sum_{k in g} xq[r, k] wq[n, k]
 //
@@ -37,14 +37,13 @@ __device__ __forceinline__ void store_rows(const Fp8RowsArgs& p, int64_t r, int 
 
 }  // namespace
 
-// Sixteen rows of W a step (SILU: sixteen gate rows and their sixteen up rows), 16 MT rows of x a pass.
+// Sixteen rows of W a step (SILU: sixteen gate rows and their sixteen up rows), sixteen rows of x a pass.
 // nbw: blocks of K a wave and phase, a multiple of D; phase_blocks = KW nbw blocks of x lie in LDS at a time.
-template <int MT, int X, bool SILU>
-__global__ __launch_bounds__(64 * kRowWaves, MT == 1 ? 4 : 2) void fp8_rows_kernel(Fp8RowsArgs p, int kw_log2, int nbw, int steps, int phases) {
+template <int X, bool SILU>
+__global__ __launch_bounds__(64 * kRowWaves, 4) void fp8_rows_kernel(Fp8RowsArgs p, int kw_log2, int nbw, int steps, int phases) {
   constexpr int NR = SILU ? 2 : 1, D = kRowDepth / NR;
-  constexpr bool kTwice = NR * MT <= 2;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  int32_t* const source_of = reinterpret_cast<int32_t*>(smem);  // [16 MT] rows of x
+  int32_t* const source_of = reinterpret_cast<int32_t*>(smem);  // [16] rows of x
   uint8_t* const x_lds = smem + kRowHead;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int KW = 1 << kw_log2, NW = kRowWaves >> kw_log2, kw = wave & (KW - 1), nw = wave >> kw_log2;
@@ -113,15 +112,15 @@ __global__ __launch_bounds__(64 * kRowWaves, MT == 1 ? 4 : 2) void fp8_rows_kern
     }
   };
 
-  for (int pass = 0; pass < rows; pass += 16 * MT) {
+  for (int pass = 0; pass < rows; pass += 16) {
     load_scales(s_first, 0, 0);
 #pragma unroll
     for (int b = 0; b < D; ++b)
 #pragma unroll
       for (int i = 0; i < NR; ++i) load_w(row_at(s_first, i), 0, i, b, b);
 
-    const int here = rows - pass < 16 * MT ? rows - pass : 16 * MT;  // rows of x in LDS
-    float* const xs = reinterpret_cast<float*>(x_lds + 16 * MT * x_pitch);  // [phase_blocks][16 MT]
+    const int here = rows - pass < 16 ? rows - pass : 16;  // rows of x in LDS
+    float* const xs = reinterpret_cast<float*>(x_lds + 16 * x_pitch);  // [phase_blocks][16]
     auto y_row = [&](int m) -> int64_t { return r0 + pass + m; };  // row of y behind row m of the pass
     auto x_row = [&](int m) -> int64_t {
       int64_t r = y_row(m);
@@ -149,7 +148,7 @@ __global__ __launch_bounds__(64 * kRowWaves, MT == 1 ? 4 : 2) void fp8_rows_kern
         }
         for (int c = tid; c < phase_blocks * here; c += 64 * kRowWaves) {
           const int b = c / here, m = c - b * here;
-          xs[b * 16 * MT + m] = first + b < groups ? p.xs[(first + b) * p.x_rows + source_of[m]] : 0.f;
+          xs[b * 16 + m] = first + b < groups ? p.xs[(first + b) * p.x_rows + source_of[m]] : 0.f;
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       } else {
@@ -171,16 +170,14 @@ __global__ __launch_bounds__(64 * kRowWaves, MT == 1 ? 4 : 2) void fp8_rows_kern
               const int m = m0 + u, chunk = (lane & 15) >> 1;
               if (m < here) {
                 *reinterpret_cast<uint2*>(x_lds + m * x_pitch + b * kFp8Block + ((chunk ^ (m & 7)) << 4) + 8 * (lane & 1)) = out;
-                if ((lane & 15) == 0) xs[b * 16 * MT + m] = __builtin_bit_cast(float, bits);
+                if ((lane & 15) == 0) xs[b * 16 + m] = __builtin_bit_cast(float, bits);
               }
             }
           }
       }
     };
-    int x_at[MT];  // this lane's row of x in LDS, per tile of 16
-#pragma unroll
-    for (int t = 0; t < MT; ++t) x_at[t] = 16 * t + col < here ? 16 * t + col : here - 1;
-    float4_t* const sums = reinterpret_cast<float4_t*>(x_lds + 16 * MT * (x_pitch + phase_blocks * 4));  // [1 or 2][waves][NR][MT][64]
+    const int x_at = col < here ? col : here - 1;  // this lane's row of x in LDS
+    float4_t* const sums = reinterpret_cast<float4_t*>(x_lds + 16 * (x_pitch + phase_blocks * 4));  // [2][waves][NR][64]
     if (phases == 1) {
       stage_x(0);
       __syncthreads();
@@ -188,11 +185,9 @@ __global__ __launch_bounds__(64 * kRowWaves, MT == 1 ? 4 : 2) void fp8_rows_kern
 
     for (int round = 0; round < rounds; ++round) {
       const int s = s_first + round * stride;
-      float4_t acc[NR][MT];
+      float4_t acc[NR];
 #pragma unroll
-      for (int i = 0; i < NR; ++i)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) acc[i][t] = float4_t{};
+      for (int i = 0; i < NR; ++i) acc[i] = float4_t{};
       for (int ph = 0; ph < phases; ++ph) {
         if (phases > 1) {
           __syncthreads();  // (the phase before it has been read)
@@ -226,102 +221,83 @@ __global__ __launch_bounds__(64 * kRowWaves, MT == 1 ? 4 : 2) void fp8_rows_kern
               w_scale[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale_now[i]), b));
             }
             const int xb = kw * nbw + b0 + b;
+            const uint8_t* const x = x_lds + x_at * x_pitch + xb * kFp8Block;
+            const int4_t x0 = *reinterpret_cast<const int4_t*>(x + ((quad ^ (x_at & 7)) << 4));
+            const int4_t x1 = *reinterpret_cast<const int4_t*>(x + (((quad + 4) ^ (x_at & 7)) << 4));
+            const float x_scale = xs[xb * 16 + x_at];
+            const bf16x8_t xw[4] = {fp8_widen(x0[0], x0[1]), fp8_widen(x0[2], x0[3]), fp8_widen(x1[0], x1[1]), fp8_widen(x1[2], x1[3])};
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-              const uint8_t* const x = x_lds + x_at[t] * x_pitch + xb * kFp8Block;
-              const int4_t x0 = *reinterpret_cast<const int4_t*>(x + ((quad ^ (x_at[t] & 7)) << 4));
-              const int4_t x1 = *reinterpret_cast<const int4_t*>(x + (((quad + 4) ^ (x_at[t] & 7)) << 4));
-              const float x_scale = xs[xb * 16 * MT + x_at[t]];
-              const bf16x8_t xw[4] = {fp8_widen(x0[0], x0[1]), fp8_widen(x0[2], x0[3]), fp8_widen(x1[0], x1[1]), fp8_widen(x1[2], x1[3])};
+            for (int i = 0; i < NR; ++i) {
+              float4_t part = {};
 #pragma unroll
-              for (int i = 0; i < NR; ++i) {
-                float4_t part = {};
+              for (int h = 0; h < 4; ++h) part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][h], xw[h], part, 0, 0, 0);
+              const float scale = w_scale[i] * x_scale;
 #pragma unroll
-                for (int h = 0; h < 4; ++h) part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][h], xw[h], part, 0, 0, 0);
-                const float scale = w_scale[i] * x_scale;
-#pragma unroll
-                for (int v = 0; v < 4; ++v) acc[i][t][v] = __builtin_fmaf(part[v], scale, acc[i][t][v]);
-              }
+              for (int v = 0; v < 4; ++v) acc[i][v] = __builtin_fmaf(part[v], scale, acc[i][v]);
             }
           }
         }
       }
-      // the KW waves of a step add up, in LDS that the rounds take in turn while there is room for two: one barrier a round
+      // the KW waves of a step add up, in LDS that the rounds take in turn: one barrier a round
       if (KW > 1) {
-        float4_t* const buf = sums + (kTwice ? round & 1 : 0) * kRowWaves * NR * MT * 64;
+        float4_t* const buf = sums + (round & 1) * kRowWaves * NR * 64;
 #pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-          for (int t = 0; t < MT; ++t) buf[((wave * NR + i) * MT + t) * 64 + lane] = acc[i][t];
+        for (int i = 0; i < NR; ++i) buf[(wave * NR + i) * 64 + lane] = acc[i];
         __syncthreads();
-        for (int t = kw; t < MT; t += KW) {
+        if (kw == 0) {
           float4_t v[NR];
 #pragma unroll
           for (int i = 0; i < NR; ++i) {
-            v[i] = buf[(((nw << kw_log2) * NR + i) * MT + t) * 64 + lane];
-            for (int w = 1; w < KW; ++w) v[i] += buf[((((nw << kw_log2) + w) * NR + i) * MT + t) * 64 + lane];
+            v[i] = acc[i];
+            for (int w = 1; w < KW; ++w) v[i] += buf[((wave + w) * NR + i) * 64 + lane];
           }
-          if (16 * t + col < here && s < steps) store_rows<SILU>(p, y_row(16 * t + col), 16 * s + 4 * quad, SILU ? half : N, v);
+          if (col < here && s < steps) store_rows<SILU>(p, r0 + pass + col, 16 * s + 4 * quad, SILU ? half : N, v);
         }
-        if (!kTwice) __syncthreads();
       } else if (SILU && p.q_out != nullptr) {
         // the workgroup's eight steps are one group of the activation: its top goes from wave to wave through LDS
-        float* const tops = reinterpret_cast<float*>(sums);  // [waves][16 MT]
-        float h[MT][4];
+        float* const tops = reinterpret_cast<float*>(sums);  // [waves][16]
+        float h[4], top = 0.f;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          float top = 0.f;
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            h[t][v] = silu_mul_f32(acc[0][t][v], acc[NR - 1][t][v]);
-            top = fmaxf(top, fp8_magnitude(h[t][v]));
-          }
-          top = fmaxf(top, __shfl_xor(top, 16));
-          top = fmaxf(top, __shfl_xor(top, 32));
-          if (quad == 0) tops[wave * 16 * MT + 16 * t + col] = top;
+        for (int v = 0; v < 4; ++v) {
+          h[v] = silu_mul_f32(acc[0][v], acc[NR - 1][v]);
+          top = fmaxf(top, fp8_magnitude(h[v]));
         }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (quad == 0) tops[wave * 16 + col] = top;
         __syncthreads();
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          float top = tops[16 * t + col];
-          for (int w = 1; w < kRowWaves; ++w) top = fmaxf(top, tops[w * 16 * MT + 16 * t + col]);
-          const uint32_t bits = fp8_scale_bits(top);
-          const float inv = fp8_inverse(bits);
-          if (16 * t + col < here && s < steps) {
-            const int64_t r = y_row(16 * t + col);
-            *reinterpret_cast<uint32_t*>(p.q_out + r * half + 16 * s + 4 * quad) = fp8_quad(h[t][0] * inv, h[t][1] * inv, h[t][2] * inv, h[t][3] * inv);
-            if (wave == 0 && quad == 0) p.scale_out[static_cast<int64_t>(s / 8) * p.rows + r] = __builtin_bit_cast(float, bits);
-          }
+        top = tops[col];
+        for (int w = 1; w < kRowWaves; ++w) top = fmaxf(top, tops[w * 16 + col]);
+        const uint32_t bits = fp8_scale_bits(top);
+        const float inv = fp8_inverse(bits);
+        if (col < here && s < steps) {
+          const int64_t r = r0 + pass + col;
+          *reinterpret_cast<uint32_t*>(p.q_out + r * half + 16 * s + 4 * quad) = fp8_quad(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
+          if (wave == 0 && quad == 0) p.scale_out[static_cast<int64_t>(s / 8) * p.rows + r] = __builtin_bit_cast(float, bits);
         }
         __syncthreads();
       } else {
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          float4_t v[NR];
-#pragma unroll
-          for (int i = 0; i < NR; ++i) v[i] = acc[i][t];
-          if (16 * t + col < here && s < steps) store_rows<SILU>(p, y_row(16 * t + col), 16 * s + 4 * quad, SILU ? half : N, v);
-        }
+        if (col < here && s < steps) store_rows<SILU>(p, r0 + pass + col, 16 * s + 4 * quad, SILU ? half : N, acc);
       }
     }
-    if (pass + 16 * MT < rows) __syncthreads();  // (x, the slots and the sums of this pass have been read)
+    if (pass + 16 < rows) __syncthreads();  // (x, the slots and the sums of this pass have been read)
   }
 }
 
 // Work distribution.  KW: as few waves share K as keep about kRowTarget waves busy, and not fewer than D blocks a wave; phases of
 // K where x would not fit LDS; as many workgroups as run at a time (two a CU where registers and LDS allow), four times that
 // for segments, whose number and sizes vary, each with the same number of steps.
-template <int MT, int X, bool SILU>
+template <int X, bool SILU>
 static hipError_t launch_rows(const Fp8RowsArgs& a, hipStream_t s) {
   constexpr int NR = SILU ? 2 : 1, D = kRowDepth / NR;
   const int64_t groups = (a.K + kFp8Block - 1) / kFp8Block;
   const int steps = static_cast<int>(((SILU ? a.N / 2 : a.N) + 15) / 16);
   const int64_t segments = a.ids ? a.rows : a.indptr ? (a.rows < a.experts ? a.rows : a.experts) : 1;
-  constexpr int64_t kBlockBytes = 16 * MT * (kFp8Block + 4);
+  constexpr int64_t kBlockBytes = 16 * (kFp8Block + 4);
   static_assert(kRowLds / kBlockBytes >= D, "a wave's blocks fit");
   // blocks a wave and phase, as many as fit beside the sums
   const auto fit = [](int log2) {
-    const int sums = log2 > 0 ? (NR * MT <= 2 ? 2 : 1) * kRowWaves * NR * MT * 1024 : 0;
+    const int sums = log2 > 0 ? 2 * kRowWaves * NR * 1024 : 0;
     return ((kRowLds - sums) / kBlockBytes >> log2) / D * D;
   };
   const auto share = [&](int log2) { return (((groups + (1 << log2) - 1) >> log2) + D - 1) / D * D; };
@@ -331,42 +307,33 @@ static hipError_t launch_rows(const Fp8RowsArgs& a, hipStream_t s) {
     ++kw_log2;
   const int64_t phases = (share(kw_log2) + fit(kw_log2) - 1) / fit(kw_log2);
   const int64_t nbw = ((share(kw_log2) + phases - 1) / phases + D - 1) / D * D;
-  const size_t lds = kRowHead + kBlockBytes * (nbw << kw_log2) + (kw_log2 > 0 ? (NR * MT <= 2 ? 2 : 1) * kRowWaves * NR * MT * 1024 : kRowWaves * 16 * MT * 4);
-  const int64_t at_a_time = (segments > 1 ? 1024 : 256) * (MT == 1 && lds <= 76 * 1024 ? 2 : 1);
+  const size_t lds = kRowHead + kBlockBytes * (nbw << kw_log2) + (kw_log2 > 0 ? 2 * kRowWaves * NR * 1024 : kRowWaves * 16 * 4);
+  const int64_t at_a_time = (segments > 1 ? 1024 : 256) * (lds <= 78 * 1024 ? 2 : 1);
   const int nw = kRowWaves >> kw_log2, sets = (steps + nw - 1) / nw;
   const int64_t want = (at_a_time + segments - 1) / segments, rounds = (sets + want - 1) / want;
   const dim3 grid(static_cast<unsigned>((sets + rounds - 1) / rounds), static_cast<unsigned>(segments));
-  auto* kern = fp8_rows_kernel<MT, X, SILU>;
+  auto* kern = fp8_rows_kernel<X, SILU>;
   if (lds > 60 * 1024) {
     const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kern));
     if (e != hipSuccess) return e;
   }
-  note_kernel("fp8_rows %d rows, %d blocks x %d waves, %d phases", 16 * MT, static_cast<int>(nbw), 1 << kw_log2, static_cast<int>(phases));
+  note_kernel("fp8_rows %d blocks x %d waves, %d phases", static_cast<int>(nbw), 1 << kw_log2, static_cast<int>(phases));
   hipLaunchKernelGGL(kern, grid, dim3(64 * kRowWaves), lds, s, a, kw_log2, static_cast<int>(nbw), steps, static_cast<int>(phases));
   return hipGetLastError();
 }
 
-template <int X, bool SILU>
-static hipError_t launch_rows_by_rows(const Fp8RowsArgs& a, int rows_max, hipStream_t s) {
-  if constexpr (X == kXFp8) {
-    if (rows_max > 32) return launch_rows<4, X, SILU>(a, s);
-    if (rows_max > 16) return launch_rows<2, X, SILU>(a, s);
-  }
-  return launch_rows<1, X, SILU>(a, s);
-}
-
-hipError_t launch_fp8_rows(const Fp8RowsArgs& a, int rows_max, hipStream_t s) {
+hipError_t launch_fp8_rows(const Fp8RowsArgs& a, hipStream_t s) {
   if (a.K % 16 != 0 || (a.silu && a.N % 32 != 0) || (a.q_out != nullptr && a.N % (2 * kFp8Block) != 0) || static_cast<uint64_t>(a.N) * a.w_pitch >= 0xffffffffull) return hipErrorNotSupported;
   if (a.silu) {
-    if (a.x_kind == kXFp8) return launch_rows_by_rows<kXFp8, true>(a, rows_max, s);
-    if (a.x_kind == MODEL_BF16) return launch_rows_by_rows<MODEL_BF16, true>(a, rows_max, s);
-    if (a.x_kind == MODEL_F16) return launch_rows_by_rows<MODEL_F16, true>(a, rows_max, s);
-    return launch_rows_by_rows<MODEL_F32, true>(a, rows_max, s);
+    if (a.x_kind == kXFp8) return launch_rows<kXFp8, true>(a, s);
+    if (a.x_kind == MODEL_BF16) return launch_rows<MODEL_BF16, true>(a, s);
+    if (a.x_kind == MODEL_F16) return launch_rows<MODEL_F16, true>(a, s);
+    return launch_rows<MODEL_F32, true>(a, s);
   }
-  if (a.x_kind == kXFp8) return launch_rows_by_rows<kXFp8, false>(a, rows_max, s);
-  if (a.x_kind == MODEL_BF16) return launch_rows_by_rows<MODEL_BF16, false>(a, rows_max, s);
-  if (a.x_kind == MODEL_F16) return launch_rows_by_rows<MODEL_F16, false>(a, rows_max, s);
-  return launch_rows_by_rows<MODEL_F32, false>(a, rows_max, s);
+  if (a.x_kind == kXFp8) return launch_rows<kXFp8, false>(a, s);
+  if (a.x_kind == MODEL_BF16) return launch_rows<MODEL_BF16, false>(a, s);
+  if (a.x_kind == MODEL_F16) return launch_rows<MODEL_F16, false>(a, s);
+  return launch_rows<MODEL_F32, false>(a, s);
 }
 
 }  // namespace gq

@@ -211,11 +211,11 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
   // arrive while that row is computed.
   // The next block's loads go out kBurst at a time, the first behind the hand-over and the others in front of the rows: all at
   // once they fill the queue to the vector cache (16 cycles a load), and every wave waits there in front of its matrix instructions.
-  constexpr int kBurst = 2, kBursts = (kXLoads + kWLoads) / kBurst;
-  static_assert(kXLoads % kBurst == 0 && kWLoads % kBurst == 0 && kBursts <= TN, "a burst is of one kind and every burst has a row");
+  constexpr int kBurst = 2, kXBursts = (kXLoads + kBurst - 1) / kBurst, kBursts = kXBursts + kWLoads / kBurst;
+  static_assert(kWLoads % kBurst == 0 && kBursts <= TN, "every burst has a row");
   auto burst = [&](int i, int g, int w_slot) {  // burst i of x of block g and W of block g + 1
-    if (i * kBurst < kXLoads) issue_x(g, i * kBurst, (i + 1) * kBurst);
-    else if (i < kBursts) issue_w(g + 1, w_slot, i * kBurst - kXLoads, (i + 1) * kBurst - kXLoads);
+    if (i < kXBursts) issue_x(g, i * kBurst, (i + 1) * kBurst < kXLoads ? (i + 1) * kBurst : kXLoads);
+    else if (i < kBursts) issue_w(g + 1, w_slot, (i - kXBursts) * kBurst, (i - kXBursts + 1) * kBurst);
   };
   auto step = [&](int g, auto tail, auto next_tail, auto has_next) {
 #pragma unroll
@@ -477,6 +477,7 @@ int64_t fp8_tile_workspace_bytes(int64_t rows, int64_t N, int64_t K) {
 hipError_t launch_fp8_tile(const Fp8Args& a, hipStream_t s) {
   if (a.q_out != nullptr) {
     if (a.N % (2 * kFp8Block) != 0 || static_cast<uint64_t>(a.N) * a.w_pitch >= 0xffffffffull) return hipErrorNotSupported;
+    if (a.rows <= 64 * a.experts) return launch_tile<4, 2, 4, 2, true, true>(a, Plan{}, s);
     return launch_tile<4, 2, 4, 4, true, true>(a, Plan{}, s);
   }
   if (a.precise) return launch_tile<4, 2, 4, 4, true, false>(a, Plan{}, s);
