@@ -79,13 +79,18 @@ gq::Fp8RowsArgs few_rows(const gq::Fp8Args& a) {
   return r;
 }
 
-// rows (of a segment on average) up to which the kernel that streams the weights past sixteen rows of x is the faster
-constexpr int64_t kFewRows = 16, kFewRowsEach = 10;
+// Where the kernel that streams the weights past up to sixteen rows of x is faster than the tiles.  Each of its workgroups brings all
+// of x to LDS: 0.4 us a row of 2048, 2 us a row of 14336.  In a graph, against the tiles with the quantiser that they need: 4096 x 4096
+// of 8 rows 12.1 / 14.6 us, of 12 13.8 / 14.4, of 16 16.2 / 15.1; 10240 x 8192 of 4 rows 26.4 / 25.6, of 6 28.6 / 25.7; 4096 x 14336
+// of 2 18.9 / 23.6, of 6 27.0 / 23.9.  With segments: rows of one on average.
+bool few_rows_dense(int64_t rows, int64_t K) { return rows == 1 || (rows <= 12 && rows * K < 49152); }
+constexpr int64_t kFewRowsEach = 10;
 
 hipError_t product(const gq::Fp8Args& a, hipStream_t s) {
   const int64_t segments = a.indptr ? (a.rows < a.experts ? a.rows : a.experts) : 1;
-  if (a.rows <= (a.indptr ? kFewRowsEach * segments : kFewRows)) {
-    const hipError_t e = gq::launch_fp8_rows(few_rows(a), s);
+  if (a.indptr ? a.rows <= kFewRowsEach * segments : few_rows_dense(a.rows, a.K)) {
+    hipError_t e = a.rows == 1 && !a.indptr ? gq::launch_fp8_gemv(few_rows(a), s) : hipErrorNotSupported;
+    if (e == hipErrorNotSupported) e = gq::launch_fp8_rows(few_rows(a), s);
     if (e != hipErrorNotSupported) return e;
   }
   return gq::launch_fp8_tile(a, s);
@@ -104,7 +109,7 @@ LinearWorkspace linear_workspace(int64_t M, int64_t N, int64_t K, bool x_quantiz
     w.q = c.take<uint8_t>(M * up16(K));
     w.scale = c.take<float>(M * groups_of(K));
   }
-  w.split_bytes = M > kFewRows ? gq::fp8_tile_workspace_bytes(M, N, K) : 0;
+  w.split_bytes = !few_rows_dense(M, K) || K % 16 != 0 ? gq::fp8_tile_workspace_bytes(M, N, K) : 0;
   w.split = c.take<char>(w.split_bytes);
   w.bytes = c.used;
   return w;
@@ -219,11 +224,12 @@ int mi355gq_fp8_linear(const void* x, int64_t x_pitch, const void* x_scale, cons
   a.precise = precise != 0;
   a.workspace = ws.split;
   a.workspace_bytes = ws.split_bytes;
-  if (x_scale == nullptr && M <= kFewRows && aligned16(x)) {  // the kernel quantises x itself
+  if (x_scale == nullptr && few_rows_dense(M, K) && aligned16(x)) {  // the kernel quantises x itself
     gq::Fp8RowsArgs r = few_rows(a);
     r.x = x;
     r.x_kind = model_dtype;
-    const hipError_t e = gq::launch_fp8_rows(r, as_stream(stream));
+    hipError_t e = M == 1 ? gq::launch_fp8_gemv(r, as_stream(stream)) : hipErrorNotSupported;
+    if (e == hipErrorNotSupported) e = gq::launch_fp8_rows(r, as_stream(stream));
     if (e != hipErrorNotSupported) return hip_result(e, "fp8_linear launch");
   }
   if (x_scale == nullptr) {
@@ -359,7 +365,7 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
     r.silu = 1;
     r.out_dtype = MI355GQ_F32;
     r.y_aligned = 1;
-    e = gq::launch_fp8_rows(r, s);
+    e = gq::launch_fp8_gemv(r, s);
     if (e == hipSuccess) {
       r.x = ws.both;
       r.x_rows = slots;
@@ -369,14 +375,11 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
       r.w_pitch = w2_pitch;
       r.N = hidden;
       r.K = inter;
-      r.y = ws.y;
+      r.y = out;
       r.x_div = 1;
       r.silu = 0;
       r.out_dtype = model_dtype;
-      e = gq::launch_fp8_rows(r, s);
-      if (e == hipSuccess)
-        e = gq::launch_moe_weighted_sum(ws.y, nullptr, static_cast<const int32_t*>(ids), static_cast<int>(num_experts),
-                                        static_cast<const float*>(weights), T, static_cast<int>(top_k), hidden, model_dtype, out, s);
+      e = gq::launch_fp8_gemv_sum(r, static_cast<const float*>(weights), static_cast<int>(top_k), s);
     }
     if (e != hipErrorNotSupported) return hip_result(e, "fp8_moe launch");
   }

@@ -130,6 +130,10 @@ struct Fp8RowsArgs {
 };
 // Sixteen rows of a segment at a time; hipErrorNotSupported where the kernel does not apply.
 hipError_t launch_fp8_rows(const Fp8RowsArgs& a, hipStream_t s);
+// One row, or (ids) one row of each expert; hipErrorNotSupported as above.  _sum: the rows' products with their experts' W, weighted
+// and added up, y [1, N]; x float32 [top_k, K].
+hipError_t launch_fp8_gemv(const Fp8RowsArgs& a, hipStream_t s);
+hipError_t launch_fp8_gemv_sum(const Fp8RowsArgs& a, const float* weights, int top_k, hipStream_t s);
 
 // Tiles, on the 8-bit matrix instruction or (precise) in float32 sums; K split over workgroups where the scratch for it is there.
 // silu: x [rows, K] times gate and up rows of w (N = 2 I), silu(gate) * up quantised into q_out [rows, I] and its scales
@@ -180,6 +184,21 @@ __device__ __forceinline__ void fp8_store(const Args& a, int64_t r, int n, int N
         if (v < count) y[v] = static_cast<uint16_t>(h[v]);
     }
   }
+}
+
+// one result, likewise
+template <class Args>
+__device__ __forceinline__ void fp8_store_one(const Args& a, int64_t r, int n, int N, float o) {
+  const int64_t at = r * N + n;
+  auto load = [&](const void* q, int64_t i) {
+    return a.model_dtype == MODEL_F32    ? static_cast<const float*>(q)[i]
+           : a.model_dtype == MODEL_BF16 ? bf2f(static_cast<const uint16_t*>(q)[i])
+                                         : h2f(static_cast<const uint16_t*>(q)[i]);
+  };
+  if (a.bias) o += load(a.bias, n);
+  if (a.residual) o += load(a.residual, at);
+  if (a.out_dtype == MODEL_F32) static_cast<float*>(a.y)[at] = o;
+  else static_cast<uint16_t*>(a.y)[at] = a.out_dtype == MODEL_BF16 ? f2bf(o) : f2h(o);
 }
 
 // eight e4m3 numbers as an operand of the bfloat16 matrix instruction (a bfloat16 holds them exactly)
