@@ -22,6 +22,9 @@ int64_t dtype_bytes(int d) { return d == MI355GQ_F32 ? 4 : 2; }
 bool dtype_aligned(const void* p, int d) { return (reinterpret_cast<uintptr_t>(p) & (dtype_bytes(d) - 1)) == 0; }
 bool dim_ok(int64_t d) { return d >= 0 && d < kMaxDim; }
 bool pitch_ok(int64_t pitch, int64_t k) { return pitch % 16 == 0 && pitch >= k && pitch < kMaxDim; }
+// rows of an operand of a product: 256 of them are to end below what is left of 2^32 at any block of K
+constexpr int64_t kMaxRow = (int64_t(1) << 24) - 256;
+bool rows_ok(int64_t pitch) { return pitch < kMaxRow; }
 int64_t groups_of(int64_t k) { return (k + gq::kFp8Block - 1) / gq::kFp8Block; }
 int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
 
@@ -199,6 +202,8 @@ int mi355gq_fp8_linear(const void* x, int64_t x_pitch, const void* x_scale, cons
               "fp8_linear: x_pitch=%lld, w_pitch=%lld for K=%lld: multiples of 16, at least K", (long long)x_pitch, (long long)w_pitch,
               (long long)K);
   if (M == 0 || N == 0) return MI355GQ_OK;
+  if (!rows_ok(w_pitch) || (x_scale && !rows_ok(x_pitch)) || K >= kMaxRow)
+    return set_error(MI355GQ_ERR_UNSUPPORTED, "fp8_linear: rows of %lld bytes (below 2^24)", (long long)(w_pitch > x_pitch ? w_pitch : x_pitch));
   FP8_REQUIRE(x && w && w_scale && y, "fp8_linear: null pointer");
   FP8_REQUIRE(aligned16(w) && aligned4(w_scale) && aligned4(x_scale) && (x_scale ? aligned16(x) : dtype_aligned(x, model_dtype)) &&
                   dtype_aligned(bias, model_dtype) && dtype_aligned(residual, model_dtype) && dtype_aligned(y, out_dtype),
@@ -257,6 +262,8 @@ int mi355gq_fp8_group_gemm(const void* x, int64_t x_pitch, const void* x_scale, 
   FP8_REQUIRE(pitch_ok(x_pitch, K) && pitch_ok(w_pitch, K), "fp8_group_gemm: x_pitch=%lld, w_pitch=%lld for K=%lld: multiples of 16, at least K",
               (long long)x_pitch, (long long)w_pitch, (long long)K);
   if (rows == 0 || N == 0) return MI355GQ_OK;
+  if (!rows_ok(w_pitch) || !rows_ok(x_pitch))
+    return set_error(MI355GQ_ERR_UNSUPPORTED, "fp8_group_gemm: rows of %lld bytes (below 2^24)", (long long)(w_pitch > x_pitch ? w_pitch : x_pitch));
   FP8_REQUIRE(x_row_index || x_rows == rows, "fp8_group_gemm: %lld rows of x for %lld rows without an index", (long long)x_rows, (long long)rows);
   FP8_REQUIRE(x_rows > 0 && x && x_scale && w && w_scale && indptr && y, "fp8_group_gemm: null pointer");
   FP8_REQUIRE(aligned16(x) && aligned16(w) && aligned4(x_scale) && aligned4(w_scale) && aligned4(indptr) && aligned4(x_row_index) &&
@@ -316,7 +323,7 @@ int mi355gq_moe_plan(const void* ids, int64_t T, int64_t top_k, int64_t num_expe
 }
 
 static bool moe_sizes_ok(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t top_k) {
-  return dim_ok(T) && T * hidden < (int64_t(1) << 32) && hidden > 0 && hidden % 16 == 0 && hidden < (1 << 24) && inter > 0 && inter % 16 == 0 && inter < (1 << 24) &&
+  return dim_ok(T) && T * hidden < (int64_t(1) << 32) && hidden > 0 && hidden % 16 == 0 && hidden < kMaxRow && inter > 0 && inter % 16 == 0 && inter < kMaxRow &&
          experts > 0 && experts <= 512 && top_k > 0 && top_k <= 32 && T * top_k / 64 + experts <= kMaxTiles;
 }
 
@@ -333,7 +340,7 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
   FP8_REQUIRE(moe_sizes_ok(T, hidden, inter, num_experts, top_k),
               "fp8_moe: T=%lld, hidden=%lld and inter=%lld (multiples of 16), num_experts=%lld (1..512), top_k=%lld (1..32)", (long long)T,
               (long long)hidden, (long long)inter, (long long)num_experts, (long long)top_k);
-  FP8_REQUIRE(pitch_ok(w13_pitch, hidden) && pitch_ok(w2_pitch, inter), "fp8_moe: w13_pitch=%lld, w2_pitch=%lld: multiples of 16, at least a row",
+  FP8_REQUIRE(pitch_ok(w13_pitch, hidden) && pitch_ok(w2_pitch, inter) && rows_ok(w13_pitch) && rows_ok(w2_pitch), "fp8_moe: w13_pitch=%lld, w2_pitch=%lld: multiples of 16, at least a row",
               (long long)w13_pitch, (long long)w2_pitch);
   if (T == 0) return MI355GQ_OK;
   FP8_REQUIRE(x && weights && ids && w13 && w13_scale && w2 && w2_scale && out, "fp8_moe: null pointer");

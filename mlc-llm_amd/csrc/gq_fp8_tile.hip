@@ -22,14 +22,15 @@ typedef __amdgpu_buffer_rsrc_t rsrc_t;
 
 // 16 bytes per lane from global memory into LDS at lds + 16 * lane, past the registers.  The compiler does not wait for them: the
 // loop below does (vmcnt), in front of the barrier that hands the stage over.
-__device__ __forceinline__ void load_to_lds(rsrc_t rsrc, uint32_t voff, uint32_t soff, uint8_t* lds) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)lds, 16, voff, soff, 0, 0);
+__device__ __forceinline__ void load_to_lds(rsrc_t rsrc, uint32_t off, uint8_t* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)lds, 16, off, 0, 0, 0);
 }
 
-__device__ __forceinline__ rsrc_t buffer_of(const void* base, int64_t bytes) {
-  const uint32_t n = bytes < 0 ? 0u : bytes > 0xffffffffll ? 0xffffffffu : static_cast<uint32_t>(bytes);
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(n), 0x00027000);
+__device__ __forceinline__ rsrc_t buffer_of(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(bytes), 0x00027000);
 }
+// bytes that a tile may reach: rows are below 2^24 bytes, so that a tile's 256 end below what is left of 2^32 at any block of K
+__device__ __forceinline__ uint32_t reach(int64_t bytes) { return bytes > 0xffffffffll ? 0xffffffffu : static_cast<uint32_t>(bytes); }
 
 // the bytes of a chunk of 16 at k that lie below K
 __device__ __forceinline__ int4_t mask_chunk(int4_t v, int left) {
@@ -45,8 +46,8 @@ __device__ __forceinline__ int4_t mask_chunk(int4_t v, int left) {
 
 // WN x WM waves, each TN x TM results of 16 x 16: a tile of BN = 16 WN TN rows of W by BM = 16 WM TM rows of x.
 // SILU: half of a wave's rows of W are gate rows and half the up rows that belong to them.
-template <int WN, int WM, int TN, int TM, bool PRECISE, bool SILU>
-__global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, int n_tiles, int m_tiles, int per_split) {
+template <int WN, int WM, int TN, int TM, int WS, bool PRECISE, bool SILU>
+__global__ __launch_bounds__(64 * WN * WM, WS == 2 ? 4 : 2) void fp8_tile_kernel(Fp8Args p, int n_tiles, int m_tiles, int per_split) {
   constexpr int kWaves = WN * WM, BN = 16 * WN * TN, BM = 16 * WM * TM;
   constexpr int kWLoads = BN / 8 / kWaves, kXLoads = BM / 8 / kWaves;  // of 1 KiB, eight rows, a wave and block of K
   constexpr int P = SILU ? 2 : 1, kPart = 16 * TN / P;  // parts of a wave's rows of W
@@ -87,11 +88,12 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
 
   const uint8_t* w0 = p.w + (static_cast<int64_t>(e) * N + n0) * p.w_pitch;
   const int k16 = (K + 15) & ~15;
-  // (every address below lies inside its matrix: rows past the end are read from the last one)
-  const rsrc_t w_rsrc = buffer_of(w0, static_cast<int64_t>(N - n0 - 1) * p.w_pitch + k16);
+  // Rows past the end are read from the last one.  A block's loads see the matrix from that block on, and nothing past its end: the last
+  // row's bytes past K are zeros, another row's are what lies there, and the last block is masked where it is used.
+  const uint32_t w_bytes = reach(static_cast<int64_t>(N - n0 - 1) * p.w_pitch + k16);
   const bool gather = p.x_row_index != nullptr;
   const uint8_t* x0 = p.x + (gather ? 0 : static_cast<int64_t>(r0) * p.x_pitch);
-  const rsrc_t x_rsrc = buffer_of(x0, (p.x_rows - 1 - (gather ? 0 : r0)) * p.x_pitch + k16);
+  const uint32_t x_bytes = reach((p.x_rows - 1 - (gather ? 0 : r0)) * p.x_pitch + k16);
   auto source = [&](int r) {  // row of x behind row r of the result, within x
     int j = r < r_end ? r : r_end - 1;
     if (gather) j = p.x_row_index[j];
@@ -119,34 +121,32 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
     x_off[i] = static_cast<uint32_t>(source(r0 + (i * kWaves + wave) * 8 + (lane >> 3)) - (gather ? 0 : r0)) * x_pitch + my_chunk;
     asm volatile("" : "+v"(x_off[i]));
   }
-  // Loads [from, to) of block g; past the last block, that one's again (nobody reads them).  A chunk past the row's end is
-  // read from its start, and masked where it is used.  No branches: the loop below is to stay one run of instructions.
-  auto shift_of = [&](int g) {
-    const int k = (g < last ? g : last) * 128;
-    return k + my_chunk < k16 ? k : -my_chunk;
-  };
+  // Loads [from, to) of block g; past the last block, that one's again (nobody reads them).  No branches: the loop below is to
+  // stay one run of instructions, and the vector unit's, which has a multiply-add to issue beside the matrix instructions nine times in ten,
+  // has none for addresses.
   auto issue_w = [&](int g, int slot, int from, int to) {
-    const int shift = shift_of(g);
+    const uint32_t k = (g < last ? g : last) * 128u;
+    const rsrc_t rsrc = buffer_of(w0 + k, w_bytes - k);
 #pragma unroll
-    for (int i = from; i < to; ++i) load_to_lds(w_rsrc, w_off[i] + shift, 0, smem + slot + (i * kWaves + wave) * 1024);
+    for (int i = from; i < to; ++i) load_to_lds(rsrc, w_off[i], smem + slot + (i * kWaves + wave) * 1024);
   };
   auto issue_x = [&](int g, int from, int to) {
-    const int shift = shift_of(g);
+    const uint32_t k = (g < last ? g : last) * 128u;
+    const rsrc_t rsrc = buffer_of(x0 + k, x_bytes - k);
 #pragma unroll
-    for (int i = from; i < to; ++i)
-      load_to_lds(x_rsrc, x_off[i] + shift, 0, smem + 3 * kWStage + (g & 1) * kXStage + (i * kWaves + wave) * 1024);
+    for (int i = from; i < to; ++i) load_to_lds(rsrc, x_off[i], smem + WS * kWStage + (g & 1) * kXStage + (i * kWaves + wave) * 1024);
   };
 
   const int wn = (wave % WN) * 16 * TN, wm = (wave / WN) * 16 * TM, frow = lane & 15, fquad = lane >> 4;
-  uint32_t xrow[TM];
+  const float* const xs0 = p.xs + (gather ? 0 : r0);
+  uint32_t xs_off[TM];  // (rows by an index: x ends below 4 GiB)
 #pragma unroll
-  for (int j = 0; j < TM; ++j) xrow[j] = source(r0 + wm + 16 * j + frow);
-  typedef const __attribute__((address_space(4))) float* scalar_floats;  // read through the scalar cache
-  scalar_floats ws[P];
+  for (int j = 0; j < TM; ++j) xs_off[j] = static_cast<uint32_t>(source(r0 + wm + 16 * j + frow) - (gather ? 0 : r0)) * 4u;
+  const float* ws[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const int b = (n0 + (wave % WN) * kPart + i * half) / kFp8Block;
-    ws[i] = (scalar_floats)(p.ws + (static_cast<int64_t>(e) * n_blocks + (b < n_blocks ? b : n_blocks - 1)) * groups);
+    ws[i] = p.ws + (static_cast<int64_t>(e) * n_blocks + (b < n_blocks ? b : n_blocks - 1)) * groups;
   }
 
   float4_t acc[TN][TM];
@@ -155,14 +155,17 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
 #pragma unroll
     for (int j = 0; j < TM; ++j) acc[i][j] = float4_t{};
 
-  // Scales are two blocks ahead, and asked for in front of a stage's loads: the wait for a load takes all before it as well.
+  // Scales are a block ahead.  Vector loads, also for W's: a scalar load counts with the reads of LDS and comes back in any order, so
+  // that a wait for one is a wait for all.  kCounted (volatile): hand_over counts these loads, none may be dropped or moved.
+  constexpr int kCounted = static_cast<int>(0x80000000u);
   float sx_next[TM], sw_next[P];
   auto scales = [&](int g) {
     g = g < last ? g : last;
+    const rsrc_t xs_rsrc = buffer_of(xs0 + g * p.x_rows, 0xffffffffu);
 #pragma unroll
-    for (int j = 0; j < TM; ++j) sx_next[j] = (p.xs + g * p.x_rows)[xrow[j]];
+    for (int j = 0; j < TM; ++j) sx_next[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(xs_rsrc, xs_off[j], 0, kCounted));
 #pragma unroll
-    for (int i = 0; i < P; ++i) sw_next[i] = ws[i][g];
+    for (int i = 0; i < P; ++i) sw_next[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer_of(ws[i] + g, 4), 0, 0, kCounted));
   };
   struct Operand {
     int4_t a, b;  // chunks q and q + 4 of a row
@@ -185,26 +188,18 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
     return Wide{{fp8_widen(o.a[0], o.a[1]), fp8_widen(o.a[2], o.a[3]), fp8_widen(o.b[0], o.b[1]), fp8_widen(o.b[2], o.b[3])}};
   };
   float4_t part[TM];                                   // a row of results of one block, unscaled
-  float sc[P][TM], sc_old[P][TM], sc_next[P][TM];  // scales of this block, the one before and the one behind it
+  float sc[P][TM];                                     // scales of its block
   Operand fx[TM], fw[2];
   Wide wx[PRECISE ? TM : 1];
   int w_now = 0, w_then = kWStage, w_last = 2 * kWStage;  // stages of W of this block, the next and the one behind it
   auto frag_w = [&](int g, int slot, int i, auto tail) { return frag(smem + slot, g, wn + 16 * i + frow, tail); };
-  auto frag_x = [&](int g, int j, auto tail) { return frag(smem + 3 * kWStage + (g & 1) * kXStage, g, wm + 16 * j + frow, tail); };
-  // Waits for block g's stages and hands them over.  Loads come back in order, and the last ones asked for are those of W for
-  // block g + 1, which may still be on their way: W comes from memory and is two blocks ahead, x from the L2 and one.  Every wave has
-  // read block g - 1 by then, whose stages take x of block g + 1 and W of block g + 2.
-  auto hand_over = [&](int g) {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kWLoads) : "memory");
+  auto frag_x = [&](int g, int j, auto tail) { return frag(smem + WS * kWStage + (g & 1) * kXStage, g, wm + 16 * j + frow, tail); };
+  // Waits for block g's stages and hands them over.  Loads come back in order, and the last ones asked for are the scales of block g
+  // and W of block g + 1, which may still be on their way: W comes from memory and is two blocks ahead, x from the L2 and one.  Every wave
+  // has read block g - 1 by then, whose stages take x of block g + 1 and W of block g + 2.
+  auto hand_over = [&](auto scale_loads) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(WS == 2 ? 0 : kWLoads + decltype(scale_loads)::value) : "memory");
     __builtin_amdgcn_s_barrier();
-#pragma unroll
-    for (int i = 0; i < P; ++i)
-#pragma unroll
-      for (int j = 0; j < TM; ++j) {
-        sc_next[i][j] = sw_next[i] * sx_next[j];
-        asm volatile("" : "+v"(sc_next[i][j]));  // here, not behind the loads below
-      }
-    scales(g + 1);
   };
   // One block.  The multiply-adds of a result run beside the matrix instructions of the row of results behind it, and the last
   // row's beside the next block's first; the next stage is handed over in front of the last row, so that its first operands
@@ -215,7 +210,13 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
   static_assert(kWLoads % kBurst == 0 && kBursts <= TN, "every burst has a row");
   auto burst = [&](int i, int g, int w_slot) {  // burst i of x of block g and W of block g + 1
     if (i < kXBursts) issue_x(g, i * kBurst, (i + 1) * kBurst < kXLoads ? (i + 1) * kBurst : kXLoads);
-    else if (i < kBursts) issue_w(g + 1, w_slot, (i - kXBursts) * kBurst, (i - kXBursts + 1) * kBurst);
+    else if (i < kBursts) issue_w(g + WS - 2, w_slot, (i - kXBursts) * kBurst, (i - kXBursts + 1) * kBurst);
+  };
+  auto next_stage = [&] {
+    const int freed = w_now;
+    w_now = w_then;
+    w_then = WS == 2 ? freed : w_last;
+    w_last = freed;
   };
   auto step = [&](int g, auto tail, auto next_tail, auto has_next) {
 #pragma unroll
@@ -223,17 +224,19 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
       if (i + 1 < TN) {
         fw[(i + 1) & 1] = frag_w(g, w_now, i + 1, tail);
       } else if (decltype(has_next)::value) {
-        hand_over(g + 1);
+        hand_over(std::integral_constant<int, TM + P>{});
         fw[0] = frag_w(g + 1, w_then, 0, next_tail);
         burst(0, g + 2, w_now);
       }
-      if (decltype(has_next)::value && i + 1 < TN) burst(i + 1, g + 1, w_last);
+      if (decltype(has_next)::value && i + 1 < TN) burst(i + 1, g + 1, WS == 2 ? w_then : w_last);
+      __builtin_amdgcn_sched_barrier(0);  // (loads first: they have the row's time)
       Wide ww;
       if constexpr (PRECISE) ww = wide(fw[i & 1]);
+      __builtin_amdgcn_s_setprio(1);  // (a wave with its operands goes before one that asks for them)
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
         const int prev = i == 0 ? TN - 1 : i - 1;
-        const float s = i == 0 ? sc_old[prev * P / TN][j] : sc[prev * P / TN][j];
+        const float s = sc[prev * P / TN][j];  // (the block before's while i is 0)
         float4_t& to = acc[prev][j];
 #pragma unroll
         for (int v = 0; v < 4; ++v) to[v] = __builtin_fmaf(part[j][v], s, to[v]);
@@ -252,53 +255,63 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(Fp8Args p, in
           __builtin_amdgcn_sched_barrier(0);  // (at once, not behind the row's other instructions)
         }
       }
+      if (i == 0) {  // nobody needs the scales of the block before any more
+#pragma unroll
+        for (int t = 0; t < P; ++t)
+#pragma unroll
+          for (int j = 0; j < TM; ++j) {
+            sc[t][j] = sw_next[t] * sx_next[j];
+            asm volatile("" : "+v"(sc[t][j]));  // here, in front of the loads
+          }
+        if (decltype(has_next)::value) scales(g + 1);
+      }
+      __builtin_amdgcn_s_setprio(0);
       __builtin_amdgcn_sched_barrier(0);  // rows in this order: operands of all rows at once would not fit the registers
     }
-    const int freed = w_now;
-    w_now = w_then;
-    w_then = w_last;
-    w_last = freed;
-#pragma unroll
-    for (int i = 0; i < P; ++i)
-#pragma unroll
-      for (int j = 0; j < TM; ++j) {
-        sc_old[i][j] = sc[i][j];
-        sc[i][j] = sc_next[i][j];
-      }
+    next_stage();
   };
   constexpr std::true_type yes{};
   constexpr std::false_type no{};
-  scales(first);
   issue_w(first, w_now, 0, kWLoads);
   issue_x(first, 0, kXLoads);
   asm volatile("" ::: "memory");  // (in this order)
-  issue_w(first + 1, w_then, 0, kWLoads);
-  hand_over(first);
+  scales(first);
+  asm volatile("" ::: "memory");
+  if (WS == 3) issue_w(first + 1, w_then, 0, kWLoads);
+  hand_over(std::integral_constant<int, TM + P>{});
   burst(0, first + 1, w_last);
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
     part[j] = float4_t{};
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      sc_old[i][j] = 0.f;
-      sc[i][j] = sc_next[i][j];
+    for (int i = 0; i < P; ++i) sc[i][j] = 0.f;
+  }
+  if (r0 + wm < r_end) {
+    auto begin = [&](auto tail) {
+      fw[0] = frag_w(first, w_now, 0, tail);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) fx[j] = frag_x(first, j, tail);
+    };
+    // the last block is masked, whether K ends inside it or not: one form of it, once a tile
+    if (first == last) begin(yes);
+    else begin(no);
+    for (int g = first; g < last - 1; ++g) step(g, no, no, yes);
+    if (first < last) step(last - 1, no, yes, yes);
+    step(last, yes, no, no);
+#pragma unroll
+    for (int j = 0; j < TM; ++j)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) acc[TN - 1][j][v] = __builtin_fmaf(part[j][v], sc[P - 1][j], acc[TN - 1][j][v]);
+  } else {
+    // none of this wave's rows of x exist: it only brings its part of the stages
+    for (int g = first; g < last; ++g) {
+#pragma unroll
+      for (int i = 1; i < kBursts; ++i) burst(i, g + 1, WS == 2 ? w_then : w_last);
+      hand_over(std::integral_constant<int, 0>{});
+      burst(0, g + 2, w_now);
+      next_stage();
     }
   }
-  auto begin = [&](auto tail) {
-    fw[0] = frag_w(first, w_now, 0, tail);
-#pragma unroll
-    for (int j = 0; j < TM; ++j) fx[j] = frag_x(first, j, tail);
-  };
-  // the last block is masked, whether K ends inside it or not: one form of it, once a tile
-  if (first == last) begin(yes);
-  else begin(no);
-  for (int g = first; g < last - 1; ++g) step(g, no, no, yes);
-  if (first < last) step(last - 1, no, yes, yes);
-  step(last, yes, no, no);
-#pragma unroll
-  for (int j = 0; j < TM; ++j)
-#pragma unroll
-    for (int v = 0; v < 4; ++v) acc[TN - 1][j][v] = __builtin_fmaf(part[j][v], sc_old[P - 1][j], acc[TN - 1][j][v]);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads that nobody reads may still land in the stages
   __syncthreads();  // (and the last stage has been read)
 
@@ -442,10 +455,10 @@ Plan plan_of(int64_t rows, int64_t N, int64_t K) {
   return best;
 }
 
-template <int WN, int WM, int TN, int TM, bool PRECISE, bool SILU>
+template <int WN, int WM, int TN, int TM, int WS, bool PRECISE, bool SILU>
 hipError_t launch_tile(const Fp8Args& a, const Plan& plan, hipStream_t s) {
   constexpr int BN = 16 * WN * TN, BM = 16 * WM * TM;
-  constexpr size_t stages = size_t(3 * BN + 2 * BM) * 128, results = SILU ? size_t(BM) * (4 * WN + kFp8Block + 16) : size_t(WN * WM) * 16 * (16 * TN + 4) * 4;
+  constexpr size_t stages = size_t(WS * BN + 2 * BM) * 128, results = SILU ? size_t(BM) * (4 * WN + kFp8Block + 16) : size_t(WN * WM) * 16 * (16 * TN + 4) * 4;
   constexpr size_t lds = stages > results ? stages : results;
   const int64_t groups = (a.K + kFp8Block - 1) / kFp8Block;
   const int64_t m_tiles = a.indptr ? a.rows / BM + a.experts : (a.rows + BM - 1) / BM, n_tiles = (a.N + BN - 1) / BN;
@@ -454,7 +467,7 @@ hipError_t launch_tile(const Fp8Args& a, const Plan& plan, hipStream_t s) {
     splits = plan.splits;
     per_split = plan.per_split;
   }
-  auto* kern = fp8_tile_kernel<WN, WM, TN, TM, PRECISE, SILU>;
+  auto* kern = fp8_tile_kernel<WN, WM, TN, TM, WS, PRECISE, SILU>;
   if (lds > 65536) {
     const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kern));
     if (e != hipSuccess) return e;
@@ -477,18 +490,18 @@ int64_t fp8_tile_workspace_bytes(int64_t rows, int64_t N, int64_t K) {
 hipError_t launch_fp8_tile(const Fp8Args& a, hipStream_t s) {
   if (a.q_out != nullptr) {
     if (a.N % (2 * kFp8Block) != 0 || static_cast<uint64_t>(a.N) * a.w_pitch >= 0xffffffffull) return hipErrorNotSupported;
-    if (a.rows <= 64 * a.experts) return launch_tile<4, 2, 4, 2, true, true>(a, Plan{}, s);
-    return launch_tile<4, 2, 4, 4, true, true>(a, Plan{}, s);
+    if (a.rows <= 64 * a.experts) return launch_tile<4, 2, 4, 2, 2, true, true>(a, Plan{}, s);
+    return launch_tile<4, 2, 4, 4, 3, true, true>(a, Plan{}, s);
   }
-  if (a.precise) return launch_tile<4, 2, 4, 4, true, false>(a, Plan{}, s);
+  if (a.precise) return launch_tile<4, 2, 4, 4, 3, true, false>(a, Plan{}, s);
   Plan plan;
   if (!a.indptr) plan = plan_of(a.rows, a.N, a.K);
   else plan.form = a.rows > 192 * a.experts ? 0 : a.rows > 64 * a.experts ? 1 : 3;
   switch (plan.form) {
-    case 0: return launch_tile<2, 4, 8, 4, false, false>(a, plan, s);
-    case 1: return launch_tile<4, 2, 4, 4, false, false>(a, plan, s);
-    case 2: return launch_tile<2, 2, 4, 4, false, false>(a, plan, s);
-    default: return launch_tile<2, 2, 4, 2, false, false>(a, plan, s);
+    case 0: return launch_tile<2, 4, 8, 4, 3, false, false>(a, plan, s);
+    case 1: return launch_tile<4, 2, 4, 4, 3, false, false>(a, plan, s);
+    case 2: return launch_tile<2, 2, 4, 4, 3, false, false>(a, plan, s);
+    default: return launch_tile<2, 2, 4, 2, 2, false, false>(a, plan, s);
   }
 }
 
