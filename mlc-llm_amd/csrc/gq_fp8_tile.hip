@@ -47,12 +47,12 @@ __device__ __forceinline__ int4_t mask_chunk(int4_t v, int left) {
 // WN x WM waves, each TN x TM results of 16 x 16: a tile of BN = 16 WN TN rows of W by BM = 16 WM TM rows of x.
 // SILU: half of a wave's rows of W are gate rows and half the up rows that belong to them.
 template <int WN, int WM, int TN, int TM, int WS, bool PRECISE, bool SILU>
-__global__ __launch_bounds__(64 * WN * WM, WS == 2 ? 4 : 2) void fp8_tile_kernel(Fp8Args p, int n_tiles, int m_tiles, int per_split) {
+__global__ __launch_bounds__(64 * WN * WM, WS == 2 ? 4 : 2) void fp8_tile_kernel(Fp8Args p, int n_first, int n_tiles, int m_tiles, int per_split) {
   constexpr int kWaves = WN * WM, BN = 16 * WN * TN, BM = 16 * WM * TM;
-  constexpr int kWLoads = BN / 8 / kWaves, kXLoads = BM / 8 / kWaves;  // of 1 KiB, eight rows, a wave and block of K
+  constexpr int kWLoads = BN / 8 / kWaves, kXLoads = (BM / 8 + kWaves - 1) / kWaves;  // of 1 KiB, eight rows, a wave and block of K
   constexpr int P = SILU ? 2 : 1, kPart = 16 * TN / P;  // parts of a wave's rows of W
-  constexpr int kWStage = BN * 128, kXStage = BM * 128;  // three stages of W and two of x in LDS
-  static_assert(BM / 8 % kWaves == 0 && BN / 8 % kWaves == 0, "whole loads");
+  constexpr int kWStage = BN * 128, kXStage = kXLoads * kWaves * 1024;  // three stages of W and two of x in LDS
+  static_assert(BN / 8 % kWaves == 0, "whole loads");
   static_assert(TN % 2 == 0, "the first row of a block uses fw[0]");
   static_assert(kPart <= kFp8Block && kFp8Block % kPart == 0, "a part lies in one block of W");
   static_assert(!SILU || BN == 2 * kFp8Block, "a tile holds one group of the activation");
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(64 * WN * WM, WS == 2 ? 4 : 2) void fp8_tile_kernel
   // shares rows of W and of x in its L2.
   const int tiles = n_tiles * m_tiles, per = (tiles + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if ((blockIdx.x >> 3) >= per || id >= tiles) return;
-  const int nt = id / m_tiles, mt = id - nt * m_tiles, n0 = nt * (BN / P);
+  const int nt = id / m_tiles, mt = id - nt * m_tiles, n0 = n_first + nt * (BN / P);
   int e = 0, r0 = mt * BM, r_end = static_cast<int>(p.rows);
   if (p.indptr != nullptr) {
     // tiles of segment e are numbered from indptr[e] / BM + e on: no two segments share a number, and some numbers have no tile
@@ -156,16 +156,15 @@ __global__ __launch_bounds__(64 * WN * WM, WS == 2 ? 4 : 2) void fp8_tile_kernel
     for (int j = 0; j < TM; ++j) acc[i][j] = float4_t{};
 
   // Scales are a block ahead.  Vector loads, also for W's: a scalar load counts with the reads of LDS and comes back in any order, so
-  // that a wait for one is a wait for all.  kCounted (volatile): hand_over counts these loads, none may be dropped or moved.
-  constexpr int kCounted = static_cast<int>(0x80000000u);
+  // that a wait for one is a wait for all.
   float sx_next[TM], sw_next[P];
   auto scales = [&](int g) {
     g = g < last ? g : last;
     const rsrc_t xs_rsrc = buffer_of(xs0 + g * p.x_rows, 0xffffffffu);
 #pragma unroll
-    for (int j = 0; j < TM; ++j) sx_next[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(xs_rsrc, xs_off[j], 0, kCounted));
+    for (int j = 0; j < TM; ++j) sx_next[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(xs_rsrc, xs_off[j], 0, 0));
 #pragma unroll
-    for (int i = 0; i < P; ++i) sw_next[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer_of(ws[i] + g, 4), 0, 0, kCounted));
+    for (int i = 0; i < P; ++i) sw_next[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer_of(ws[i] + g, 4), 0, 0, 0));
   };
   struct Operand {
     int4_t a, b;  // chunks q and q + 4 of a row
@@ -348,7 +347,7 @@ __global__ __launch_bounds__(64 * WN * WM, WS == 2 ? 4 : 2) void fp8_tile_kernel
         *reinterpret_cast<uint32_t*>(bytes + row * kBytes + (wave % WN) * kPart + 16 * i + 4 * fquad) =
             fp8_quad(acc[i][j][0] * inv, acc[i][j][1] * inv, acc[i][j][2] * inv, acc[i][j][3] * inv);
       if (wave % WN == 0 && fquad == 0 && r0 + row < r_end)
-        p.scale_out[static_cast<int64_t>(nt) * p.rows + r0 + row] = __builtin_bit_cast(float, bits);
+        p.scale_out[static_cast<int64_t>(n0 / kFp8Block) * p.rows + r0 + row] = __builtin_bit_cast(float, bits);
     }
     __syncthreads();
     for (int c = tid; c < BM * 8; c += 64 * kWaves) {
@@ -422,46 +421,90 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(Fp8Args p, int splits) {
 
 namespace {
 
-// A tile form and the shares of K of a dense product.
+// A tile form and the shares of K of a dense product; from column n_rest on, another form without shares.
 struct Plan {
   int form = 0, splits = 1, per_split = 0;
+  int64_t n_rest = 0;
+  int form_rest = 0;
+  float ns = 0.f;
 };
-// per block of K and round of workgroups, in ns (measured); workgroups that run at a time
+// Tiles, workgroups that run at a time, and what a block of K of a round of them takes in ns: alone_ns where few run, full_ns where all
+// of them do (L2 and clocks are shared).  Fitted to 5500 timings of 112 shapes, 18 to 2048 rows, all forms, 1 to 12 shares: the choice takes 1.7 %
+// longer than the best one on average, 15 % at most.
 struct Form {
   int bn, bm, at_a_time;
-  float block_ns;
+  float alone_ns, full_ns;
 };
-constexpr Form kForms[] = {{256, 256, 256, 2050.f}, {256, 128, 256, 1250.f}, {128, 128, 512, 1300.f}, {128, 64, 512, 900.f}};
-Plan plan_of(int64_t rows, int64_t N, int64_t K) {
+constexpr Form kForms[] = {{256, 256, 256, 875.f, 1687.f}, {256, 192, 256, 752.f, 1412.f}, {256, 160, 256, 822.f, 1203.f}, {256, 128, 256, 619.f, 927.f},
+                           {128, 128, 512, 436.f, 1046.f}, {128, 64, 768, 358.f, 970.f}};
+constexpr float kRoundNs = 1140.f, kJoinNs = 460.f, kShareNs = 1.42e-3f;  // a round's ends, the launch that joins, an element of a share
+constexpr int kFormCount = sizeof(kForms) / sizeof(kForms[0]);
+float ns_of(const Form& f, int64_t tiles, int64_t blocks) {
+  const int64_t full = tiles / f.at_a_time, rest = tiles - full * f.at_a_time;
+  float ns = full * (blocks * f.full_ns + kRoundNs);
+  if (rest > 0) ns += blocks * (f.alone_ns + (f.full_ns - f.alone_ns) * rest / f.at_a_time) + kRoundNs;
+  return ns;
+}
+bool may_take(int form) { return options().gemm_variant < 0 || options().gemm_variant >= kFormCount || options().gemm_variant == form; }
+Plan plan_of(int64_t rows, int64_t N, int64_t K, bool only_whole = false) {
   const int64_t groups = (K + kFp8Block - 1) / kFp8Block;
   Plan best;
-  float best_ns = 0.f;
-  for (int f = 0; f < 4; ++f) {
-    if (options().gemm_variant >= 0 && options().gemm_variant < 4 && options().gemm_variant != f) continue;
-    const int64_t tiles = ((rows + kForms[f].bm - 1) / kForms[f].bm) * ((N + kForms[f].bn - 1) / kForms[f].bn);
-    for (int64_t want = 1; want <= 16 && want <= (groups < 4 ? 1 : groups / 4); ++want) {
+  for (int f = 0; f < kFormCount; ++f) {
+    if (!may_take(f)) continue;
+    const int64_t m_tiles = (rows + kForms[f].bm - 1) / kForms[f].bm, n_tiles = (N + kForms[f].bn - 1) / kForms[f].bn, tiles = m_tiles * n_tiles;
+    for (int64_t want = 1; want <= 16 && want <= (only_whole || groups < 4 ? 1 : groups / 4); ++want) {
       if (options().gemm_split_k > 0 && options().gemm_split_k != want) continue;
       const int64_t per = (groups + want - 1) / want, splits = (groups + per - 1) / per;
-      const int64_t rounds = (tiles * splits + kForms[f].at_a_time - 1) / kForms[f].at_a_time;
-      const float ns = rounds * (per * kForms[f].block_ns + 4000.f) + (splits > 1 ? 2500.f + splits * rows * N * 8 / 4000.f : 0.f);
-      if (best.per_split == 0 || ns < best_ns) {
-        best_ns = ns;
+      const float ns = ns_of(kForms[f], tiles * splits, per) + (splits > 1 ? kJoinNs + splits * rows * N * kShareNs : 0.f);
+      if (best.per_split == 0 || ns < best.ns) {
+        best = Plan{};
         best.form = f;
         best.splits = static_cast<int>(splits);
         best.per_split = static_cast<int>(per);
+        best.ns = ns;
       }
+    }
+    // whole rounds of this form, and what is left of the last in a form that fills a round of its own
+    const int64_t whole = tiles / kForms[f].at_a_time * kForms[f].at_a_time / m_tiles;
+    if (!only_whole && options().gemm_split_k <= 1 && whole > 0 && whole < n_tiles) {
+      const Plan rest = plan_of(rows, N - whole * kForms[f].bn, K, true);
+      const float ns = ns_of(kForms[f], whole * m_tiles, groups) + rest.ns + 2000.f;
+      if (ns < best.ns) {
+        best = Plan{};
+        best.form = f;
+        best.per_split = static_cast<int>(groups);
+        best.n_rest = whole * kForms[f].bn;
+        best.form_rest = rest.form;
+        best.ns = ns;
+      }
+    }
+  }
+  return best;
+}
+// With segments a tile in two, about, of each is short.  No shares of K.
+int form_of(int64_t rows, int64_t experts, int64_t N, int64_t K) {
+  int best = 0;
+  float best_ns = 0.f;
+  for (int f = 0; f < kFormCount; ++f) {
+    if (!may_take(f)) continue;
+    const int64_t tiles = (rows / kForms[f].bm + (experts + 1) / 2) * ((N + kForms[f].bn - 1) / kForms[f].bn);
+    const float ns = ns_of(kForms[f], tiles, (K + kFp8Block - 1) / kFp8Block);
+    if (best_ns == 0.f || ns < best_ns) {
+      best_ns = ns;
+      best = f;
     }
   }
   return best;
 }
 
 template <int WN, int WM, int TN, int TM, int WS, bool PRECISE, bool SILU>
-hipError_t launch_tile(const Fp8Args& a, const Plan& plan, hipStream_t s) {
+hipError_t launch_tile(const Fp8Args& a, const Plan& plan, int part, hipStream_t s) {
   constexpr int BN = 16 * WN * TN, BM = 16 * WM * TM;
-  constexpr size_t stages = size_t(WS * BN + 2 * BM) * 128, results = SILU ? size_t(BM) * (4 * WN + kFp8Block + 16) : size_t(WN * WM) * 16 * (16 * TN + 4) * 4;
+  constexpr size_t stages = size_t(WS * BN) * 128 + 2 * ((BM / 8 + WN * WM - 1) / (WN * WM) * WN * WM * 1024), results = SILU ? size_t(BM) * (4 * WN + kFp8Block + 16) : size_t(WN * WM) * 16 * (16 * TN + 4) * 4;
   constexpr size_t lds = stages > results ? stages : results;
   const int64_t groups = (a.K + kFp8Block - 1) / kFp8Block;
-  const int64_t m_tiles = a.indptr ? a.rows / BM + a.experts : (a.rows + BM - 1) / BM, n_tiles = (a.N + BN - 1) / BN;
+  const int64_t m_tiles = a.indptr ? a.rows / BM + a.experts : (a.rows + BM - 1) / BM;
+  const int64_t n_first = part == 0 ? 0 : plan.n_rest, n_end = part == 0 && plan.n_rest > 0 ? plan.n_rest : a.N, n_tiles = (n_end - n_first + BN - 1) / BN;
   int splits = 1, per_split = static_cast<int>(groups);
   if (plan.splits > 1 && a.workspace != nullptr && a.workspace_bytes >= plan.splits * a.rows * a.N * 4) {
     splits = plan.splits;
@@ -474,10 +517,21 @@ hipError_t launch_tile(const Fp8Args& a, const Plan& plan, hipStream_t s) {
   }
   note_kernel("fp8_tile %dx%d%s, %d shares of K", BN, BM, PRECISE ? " float32 sums" : "", splits);
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((n_tiles * m_tiles + 7) / 8 * 8), splits), dim3(64 * WN * WM), lds, s, a,
-                     static_cast<int>(n_tiles), static_cast<int>(m_tiles), per_split);
+                     static_cast<int>(n_first), static_cast<int>(n_tiles), static_cast<int>(m_tiles), per_split);
   if (splits > 1)
     hipLaunchKernelGGL(fp8_join_kernel, dim3(static_cast<unsigned>((a.rows * ((a.N + 7) / 8) + 255) / 256)), dim3(256), 0, s, a, splits);
   return hipGetLastError();
+}
+
+hipError_t launch_part(const Fp8Args& a, const Plan& plan, int part, hipStream_t s) {
+  switch (part == 0 ? plan.form : plan.form_rest) {
+    case 0: return launch_tile<2, 4, 8, 4, 3, false, false>(a, plan, part, s);
+    case 1: return launch_tile<4, 2, 4, 6, 3, false, false>(a, plan, part, s);
+    case 2: return launch_tile<4, 2, 4, 5, 3, false, false>(a, plan, part, s);
+    case 3: return launch_tile<4, 2, 4, 4, 3, false, false>(a, plan, part, s);
+    case 4: return launch_tile<2, 2, 4, 4, 3, false, false>(a, plan, part, s);
+    default: return launch_tile<2, 2, 4, 2, 2, false, false>(a, plan, part, s);
+  }
 }
 
 }  // namespace
@@ -490,19 +544,15 @@ int64_t fp8_tile_workspace_bytes(int64_t rows, int64_t N, int64_t K) {
 hipError_t launch_fp8_tile(const Fp8Args& a, hipStream_t s) {
   if (a.q_out != nullptr) {
     if (a.N % (2 * kFp8Block) != 0 || static_cast<uint64_t>(a.N) * a.w_pitch >= 0xffffffffull) return hipErrorNotSupported;
-    if (a.rows <= 64 * a.experts) return launch_tile<4, 2, 4, 2, 2, true, true>(a, Plan{}, s);
-    return launch_tile<4, 2, 4, 4, 3, true, true>(a, Plan{}, s);
+    if (a.rows <= 64 * a.experts) return launch_tile<4, 2, 4, 2, 2, true, true>(a, Plan{}, 0, s);
+    return launch_tile<4, 2, 4, 4, 3, true, true>(a, Plan{}, 0, s);
   }
-  if (a.precise) return launch_tile<4, 2, 4, 4, 3, true, false>(a, Plan{}, s);
+  if (a.precise) return launch_tile<4, 2, 4, 4, 3, true, false>(a, Plan{}, 0, s);
   Plan plan;
   if (!a.indptr) plan = plan_of(a.rows, a.N, a.K);
-  else plan.form = a.rows > 192 * a.experts ? 0 : a.rows > 64 * a.experts ? 1 : 3;
-  switch (plan.form) {
-    case 0: return launch_tile<2, 4, 8, 4, 3, false, false>(a, plan, s);
-    case 1: return launch_tile<4, 2, 4, 4, 3, false, false>(a, plan, s);
-    case 2: return launch_tile<2, 2, 4, 4, 3, false, false>(a, plan, s);
-    default: return launch_tile<2, 2, 4, 2, 2, false, false>(a, plan, s);
-  }
+  else plan.form = form_of(a.rows, a.experts, a.N, a.K);
+  const hipError_t e = launch_part(a, plan, 0, s);
+  return e != hipSuccess || plan.n_rest == 0 ? e : launch_part(a, plan, 1, s);
 }
 
 }  // namespace gq
