@@ -446,7 +446,7 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
   a.out_dtype = model_dtype;
   if (e == hipSuccess) e = product(a, s);
   if (e == hipSuccess)
-    e = gq::launch_moe_weighted_sum(ws.y, ws.slot_row, nullptr, 0, static_cast<const float*>(weights), T, static_cast<int>(top_k), hidden,
+    e = gq::launch_moe_weighted_sum(ws.y, ws.slot_row, static_cast<const float*>(weights), T, static_cast<int>(top_k), hidden,
                                     model_dtype, out, s);
   return hip_result(e, "fp8_moe launch");
 }
