@@ -414,7 +414,6 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
     hipError_t done;
     if (by_rows) {
       gq::Fp8RowsArgs r = few_rows(a);
-      r.silu = 1;
       r.q_out = ws.hq;
       r.scale_out = ws.hs;
       done = gq::launch_fp8_rows(r, s);

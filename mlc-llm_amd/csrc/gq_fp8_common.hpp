@@ -117,16 +117,17 @@ struct Fp8RowsArgs {
   int64_t w_pitch = 0, N = 0, K = 0, experts = 1;
   const void* bias = nullptr;
   const void* residual = nullptr;
-  void* y = nullptr;  // [rows, N] (silu: [rows, N / 2] = silu(first half) * second half)
+  void* y = nullptr;  // [rows, N]
   int64_t rows = 0;
-  const int32_t* indptr = nullptr;       // segments as in Fp8Args, or
+  const int32_t* indptr = nullptr;       // (launch_fp8_rows) segments as in Fp8Args
   const int32_t* x_row_index = nullptr;
-  const int32_t* ids = nullptr;          // [rows] the expert of each row, segments of one row; row r reads row r / x_div of x
+  const int32_t* ids = nullptr;          // (launch_fp8_gemv) [rows] the expert of each row, which reads row r / x_div of x
   int x_div = 1;
-  int silu = 0, model_dtype = 0, out_dtype = 0;
+  int silu = 0;                          // (launch_fp8_gemv with ids) y [rows, N / 2] = silu(first half) * second half
+  int model_dtype = 0, out_dtype = 0;
   int y_aligned = 0;  // y starts at 16 bytes
-  uint8_t* q_out = nullptr;  // silu: the activation quantised, [rows, N / 2] and its scales [N / 256, rows], instead of y; N / 2 a
-  float* scale_out = nullptr;  // multiple of 128
+  uint8_t* q_out = nullptr;  // (launch_fp8_rows on quantised x) silu(first half) * second half quantised, [rows, N / 2] and its scales
+  float* scale_out = nullptr;  // [N / 256, rows], instead of y; N / 2 a multiple of 128
 };
 // Sixteen rows of a segment at a time; hipErrorNotSupported where the kernel does not apply.
 hipError_t launch_fp8_rows(const Fp8RowsArgs& a, hipStream_t s);

@@ -26,18 +26,10 @@ constexpr int kRowDepth = 4;       // blocks of 16 x 128 that a wave has in flig
 constexpr int kRowHead = 256;      // bytes of LDS in front of x
 constexpr int kRowLds = 152 * 1024;  // of a workgroup: x and the sums
 
-// Four neighbouring results (SILU: of the gate and of the up rows) of row r.
-template <bool SILU>
-__device__ __forceinline__ void store_rows(const Fp8RowsArgs& p, int64_t r, int n, int N, const float4_t* v) {
-  float o[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = SILU ? silu_mul_f32(v[0][i], v[SILU ? 1 : 0][i]) : v[0][i];
-  if (n < N) fp8_store<4>(p, r, n, N, N % 4 == 0 && p.y_aligned, o);
-}
-
 }  // namespace
 
-// Sixteen rows of W a step (SILU: sixteen gate rows and their sixteen up rows), sixteen rows of x a pass.
+// Sixteen rows of W a step, sixteen rows of x a pass.  SILU: sixteen gate rows and their sixteen up rows a step, the activation
+// quantised in the epilogue; a workgroup's eight steps are one group of it, so that its waves share no K.
 // nbw: blocks of K a wave and phase, a multiple of D; phase_blocks = KW nbw blocks of x lie in LDS at a time.
 template <int X, bool SILU>
 __global__ __launch_bounds__(64 * kRowWaves, 4) void fp8_rows_kernel(Fp8RowsArgs p, int kw_log2, int nbw, int steps, int phases) {
@@ -53,13 +45,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void fp8_rows_kernel(Fp8RowsArgs
 
   // the segment: expert e, `rows` rows from row r0 on
   int e = 0, rows = static_cast<int>(p.rows), r0 = 0;
-  if (p.ids != nullptr) {  // one token: its slots are the segments
-    e = p.ids[blockIdx.y];
-    if (e < 0 || e >= p.experts) return;
-    e = __builtin_amdgcn_readfirstlane(e);
-    rows = 1;
-    r0 = blockIdx.y;
-  } else if (p.indptr != nullptr) {
+  if (p.indptr != nullptr) {
     int before = 0;
     e = -1;
     for (int i0 = 0; i0 < p.experts && e < 0; i0 += 64) {  // the segment that is the blockIdx.y-th with any rows
@@ -124,7 +110,6 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void fp8_rows_kernel(Fp8RowsArgs
     auto y_row = [&](int m) -> int64_t { return r0 + pass + m; };  // row of y behind row m of the pass
     auto x_row = [&](int m) -> int64_t {
       int64_t r = y_row(m);
-      if (p.ids != nullptr) return r / p.x_div;
       if (p.x_row_index != nullptr) r = p.x_row_index[r];
       return r < 0 ? 0 : r < p.x_rows ? r : p.x_rows - 1;
     };
@@ -177,7 +162,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void fp8_rows_kernel(Fp8RowsArgs
       }
     };
     const int x_at = col < here ? col : here - 1;  // this lane's row of x in LDS
-    float4_t* const sums = reinterpret_cast<float4_t*>(x_lds + 16 * (x_pitch + phase_blocks * 4));  // [2][waves][NR][64]
+    float4_t* const sums = reinterpret_cast<float4_t*>(x_lds + 16 * (x_pitch + phase_blocks * 4));  // [2][waves][64]
     if (phases == 1) {
       stage_x(0);
       __syncthreads();
@@ -208,18 +193,6 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void fp8_rows_kernel(Fp8RowsArgs
           load_scales(s_next, ph_next, b_next);
 #pragma unroll
           for (int b = 0; b < D; ++b) {
-            bf16x8_t a[NR][4];
-            float w_scale[NR];
-#pragma unroll
-            for (int i = 0; i < NR; ++i) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                a[i][2 * h] = fp8_widen(wq[i][b][h][0], wq[i][b][h][1]);
-                a[i][2 * h + 1] = fp8_widen(wq[i][b][h][2], wq[i][b][h][3]);
-              }
-              load_w(at[i], ph_next, i, b_next + b, b);
-              w_scale[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale_now[i]), b));
-            }
             const int xb = kw * nbw + b0 + b;
             const uint8_t* const x = x_lds + x_at * x_pitch + xb * kFp8Block;
             const int4_t x0 = *reinterpret_cast<const int4_t*>(x + ((quad ^ (x_at & 7)) << 4));
@@ -228,32 +201,41 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void fp8_rows_kernel(Fp8RowsArgs
             const bf16x8_t xw[4] = {fp8_widen(x0[0], x0[1]), fp8_widen(x0[2], x0[3]), fp8_widen(x1[0], x1[1]), fp8_widen(x1[2], x1[3])};
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
+              bf16x8_t a[4];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                a[2 * h] = fp8_widen(wq[i][b][h][0], wq[i][b][h][1]);
+                a[2 * h + 1] = fp8_widen(wq[i][b][h][2], wq[i][b][h][3]);
+              }
+              load_w(at[i], ph_next, i, b_next + b, b);
+              const float scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale_now[i]), b)) * x_scale;
               float4_t part = {};
 #pragma unroll
-              for (int h = 0; h < 4; ++h) part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][h], xw[h], part, 0, 0, 0);
-              const float scale = w_scale[i] * x_scale;
+              for (int h = 0; h < 4; ++h) part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[h], xw[h], part, 0, 0, 0);
 #pragma unroll
               for (int v = 0; v < 4; ++v) acc[i][v] = __builtin_fmaf(part[v], scale, acc[i][v]);
             }
+            __builtin_amdgcn_sched_barrier(0);  // a block after the other: operands of two would not fit the registers
           }
         }
       }
+      const int n = 16 * s + 4 * quad;
+      const bool there = col < here && s < steps && n < N, vec = N % 4 == 0 && p.y_aligned;
+      auto store = [&](const float4_t& v) {
+        float o[4] = {v[0], v[1], v[2], v[3]};
+        fp8_store<4>(p, r0 + pass + col, n, N, vec, o);
+      };
       // the KW waves of a step add up, in LDS that the rounds take in turn: one barrier a round
-      if (KW > 1) {
-        float4_t* const buf = sums + (round & 1) * kRowWaves * NR * 64;
-#pragma unroll
-        for (int i = 0; i < NR; ++i) buf[(wave * NR + i) * 64 + lane] = acc[i];
+      if (!SILU && KW > 1) {
+        float4_t* const buf = sums + (round & 1) * kRowWaves * 64;
+        buf[wave * 64 + lane] = acc[0];
         __syncthreads();
         if (kw == 0) {
-          float4_t v[NR];
-#pragma unroll
-          for (int i = 0; i < NR; ++i) {
-            v[i] = acc[i];
-            for (int w = 1; w < KW; ++w) v[i] += buf[((wave + w) * NR + i) * 64 + lane];
-          }
-          if (col < here && s < steps) store_rows<SILU>(p, r0 + pass + col, 16 * s + 4 * quad, SILU ? half : N, v);
+          float4_t v = acc[0];
+          for (int w = 1; w < KW; ++w) v += buf[(wave + w) * 64 + lane];
+          if (there) store(v);
         }
-      } else if (SILU && p.q_out != nullptr) {
+      } else if (SILU) {
         // the workgroup's eight steps are one group of the activation: its top goes from wave to wave through LDS
         float* const tops = reinterpret_cast<float*>(sums);  // [waves][16]
         float h[4], top = 0.f;
@@ -277,7 +259,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void fp8_rows_kernel(Fp8RowsArgs
         }
         __syncthreads();
       } else {
-        if (col < here && s < steps) store_rows<SILU>(p, r0 + pass + col, 16 * s + 4 * quad, SILU ? half : N, acc);
+        if (there) store(acc[0]);
       }
     }
     if (pass + 16 < rows) __syncthreads();  // (x, the slots and the sums of this pass have been read)
@@ -292,22 +274,22 @@ static hipError_t launch_rows(const Fp8RowsArgs& a, hipStream_t s) {
   constexpr int NR = SILU ? 2 : 1, D = kRowDepth / NR;
   const int64_t groups = (a.K + kFp8Block - 1) / kFp8Block;
   const int steps = static_cast<int>(((SILU ? a.N / 2 : a.N) + 15) / 16);
-  const int64_t segments = a.ids ? a.rows : a.indptr ? (a.rows < a.experts ? a.rows : a.experts) : 1;
+  const int64_t segments = a.indptr ? (a.rows < a.experts ? a.rows : a.experts) : 1;
   constexpr int64_t kBlockBytes = 16 * (kFp8Block + 4);
   static_assert(kRowLds / kBlockBytes >= D, "a wave's blocks fit");
   // blocks a wave and phase, as many as fit beside the sums
   const auto fit = [](int log2) {
-    const int sums = log2 > 0 ? 2 * kRowWaves * NR * 1024 : 0;
+    const int sums = log2 > 0 ? 2 * kRowWaves * 1024 : 0;
     return ((kRowLds - sums) / kBlockBytes >> log2) / D * D;
   };
   const auto share = [&](int log2) { return (((groups + (1 << log2) - 1) >> log2) + D - 1) / D * D; };
   int kw_log2 = 0;
-  while (a.q_out == nullptr && kw_log2 < 3 && (steps * segments << kw_log2) < kRowTarget && (groups >> (kw_log2 + 1)) * 2 > D && fit(kw_log2 + 1) > 0 &&
+  while (!SILU && kw_log2 < 3 && (steps * segments << kw_log2) < kRowTarget && (groups >> (kw_log2 + 1)) * 2 > D && fit(kw_log2 + 1) > 0 &&
          (fit(kw_log2 + 1) >= share(kw_log2 + 1) || fit(kw_log2) < share(kw_log2)))
     ++kw_log2;
   const int64_t phases = (share(kw_log2) + fit(kw_log2) - 1) / fit(kw_log2);
   const int64_t nbw = ((share(kw_log2) + phases - 1) / phases + D - 1) / D * D;
-  const size_t lds = kRowHead + kBlockBytes * (nbw << kw_log2) + (kw_log2 > 0 ? 2 * kRowWaves * NR * 1024 : kRowWaves * 16 * 4);
+  const size_t lds = kRowHead + kBlockBytes * (nbw << kw_log2) + (kw_log2 > 0 ? 2 * kRowWaves * 1024 : kRowWaves * 16 * 4);
   const int64_t at_a_time = (segments > 1 ? 1024 : 256) * (lds <= 78 * 1024 ? 2 : 1);
   const int nw = kRowWaves >> kw_log2, sets = (steps + nw - 1) / nw;
   const int64_t want = (at_a_time + segments - 1) / segments, rounds = (sets + want - 1) / want;
@@ -323,13 +305,9 @@ static hipError_t launch_rows(const Fp8RowsArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_fp8_rows(const Fp8RowsArgs& a, hipStream_t s) {
-  if (a.K % 16 != 0 || (a.silu && a.N % 32 != 0) || (a.q_out != nullptr && a.N % (2 * kFp8Block) != 0) || static_cast<uint64_t>(a.N) * a.w_pitch >= 0xffffffffull) return hipErrorNotSupported;
-  if (a.silu) {
-    if (a.x_kind == kXFp8) return launch_rows<kXFp8, true>(a, s);
-    if (a.x_kind == MODEL_BF16) return launch_rows<MODEL_BF16, true>(a, s);
-    if (a.x_kind == MODEL_F16) return launch_rows<MODEL_F16, true>(a, s);
-    return launch_rows<MODEL_F32, true>(a, s);
-  }
+  if (a.K % 16 != 0 || (a.q_out != nullptr && a.N % (2 * kFp8Block) != 0) || static_cast<uint64_t>(a.N) * a.w_pitch >= 0xffffffffull)
+    return hipErrorNotSupported;
+  if (a.q_out != nullptr) return launch_rows<kXFp8, true>(a, s);
   if (a.x_kind == kXFp8) return launch_rows<kXFp8, false>(a, s);
   if (a.x_kind == MODEL_BF16) return launch_rows<MODEL_BF16, false>(a, s);
   if (a.x_kind == MODEL_F16) return launch_rows<MODEL_F16, false>(a, s);
