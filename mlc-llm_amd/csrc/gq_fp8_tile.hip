@@ -391,32 +391,29 @@ __global__ __launch_bounds__(64 * WN * WM, WS == 2 ? 4 : 2) void fp8_tile_kernel
   }
 }
 
-// the sums of the shares of K, in their order; bias, residual and the one rounding
+// the sums of the shares of K, in their order; bias, residual and the one rounding.  Four columns a thread, so that a wave's read of a
+// share is 1 KiB in one piece.
 __global__ __launch_bounds__(256) void fp8_join_kernel(Fp8Args p, int splits) {
-  const int N = static_cast<int>(p.N), runs = (N + 7) / 8;
+  const int N = static_cast<int>(p.N), runs = (N + 3) / 4;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= p.rows * runs) return;
   const int64_t r = i / runs;
-  const int n = static_cast<int>(i - r * runs) * 8;
+  const int n = static_cast<int>(i - r * runs) * 4;
   const float* from = static_cast<const float*>(p.workspace) + r * N + n;
-  float o[8];
-  if (N % 8 == 0) {
-    float4_t a = {}, b = {};
-    for (int s = 0; s < splits; ++s, from += p.rows * N) {
-      a += *reinterpret_cast<const float4_t*>(from);
-      b += *reinterpret_cast<const float4_t*>(from + 4);
-    }
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  const bool vec = N % 4 == 0;
+  for (int s = 0; s < splits; ++s, from += p.rows * N) {
+    if (vec) {
+      const float4_t a = *reinterpret_cast<const float4_t*>(from);
 #pragma unroll
-    for (int v = 0; v < 4; ++v) o[v] = a[v], o[v + 4] = b[v];
-  } else {
+      for (int v = 0; v < 4; ++v) o[v] += a[v];
+    } else {
 #pragma unroll
-    for (int v = 0; v < 8; ++v) o[v] = 0.f;
-    for (int s = 0; s < splits; ++s, from += p.rows * N)
-#pragma unroll
-      for (int v = 0; v < 8; ++v)
+      for (int v = 0; v < 4; ++v)
         if (n + v < N) o[v] += from[v];
+    }
   }
-  fp8_store<8>(p, r, n, N, N % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0, o);
+  fp8_store<4>(p, r, n, N, vec && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0, o);
 }
 
 namespace {
@@ -519,7 +516,7 @@ hipError_t launch_tile(const Fp8Args& a, const Plan& plan, int part, hipStream_t
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((n_tiles * m_tiles + 7) / 8 * 8), splits), dim3(64 * WN * WM), lds, s, a,
                      static_cast<int>(n_first), static_cast<int>(n_tiles), static_cast<int>(m_tiles), per_split);
   if (splits > 1)
-    hipLaunchKernelGGL(fp8_join_kernel, dim3(static_cast<unsigned>((a.rows * ((a.N + 7) / 8) + 255) / 256)), dim3(256), 0, s, a, splits);
+    hipLaunchKernelGGL(fp8_join_kernel, dim3(static_cast<unsigned>((a.rows * ((a.N + 3) / 4) + 255) / 256)), dim3(256), 0, s, a, splits);
   return hipGetLastError();
 }
 
