@@ -450,7 +450,7 @@ MI355GQ_API int mi355gq_moe_combine_dt(const void* y, const void* slot_positions
  *   activations q [rows, K], rows q_pitch bytes apart, scale float32 [ceil(K / 128), rows] (a group's scales lie side by side);
  *   weights     q [N, K], rows w_pitch bytes apart, scale float32 [ceil(N / 128), ceil(K / 128)]; stacks of experts [experts, ...].
  * The value of a number is q * scale.  Pitches are multiples of 16 and at least K; bases are 16-byte aligned.  What a row
- * holds between K and its pitch is never used.
+ * holds between K and its pitch is never used.  Products take rows below 2^24 - 256 bytes (MI355GQ_ERR_UNSUPPORTED beyond).
  *
  * mi355gq_fp8_quantize: x [rows, K] in model_dtype, dense -> q, scale.  A group's scale is the smallest power of two s
  * with max|x| <= 448 s (at least 2^-126, and 1 for a group of zeros), q = x / s rounded to nearest, ties to even: one
@@ -529,7 +529,7 @@ MI355GQ_API int mi355gq_moe_plan(const void* ids, int64_t T, int64_t top_k, int6
  * q() quantises as mi355gq_fp8_quantize does; w13 [num_experts, 2 inter, hidden] (gate rows, then up rows), w2 [num_experts,
  * hidden, inter], with their scales; weights float32 [T, top_k], ids int32 [T, top_k] (an id outside the experts adds nothing).
  * The first product is precise (its results are rounded to e4m3 again), the second as with precise 0 above, all other sums are in
- * float32; an expert's output is rounded to model_dtype before it is weighted.  hidden and inter: multiples of 16.
+ * float32 and rounded to model_dtype once.  hidden and inter: multiples of 16.
  * workspace: mi355gq_fp8_moe_workspace_bytes() bytes, 16-byte aligned.
  */
 MI355GQ_API int64_t mi355gq_fp8_moe_workspace_bytes(int64_t T, int64_t hidden, int64_t inter, int64_t num_experts,

@@ -240,9 +240,9 @@ hipError_t launch_moe_plan(const int32_t* ids, int64_t slots, int k, int E, int3
 hipError_t launch_moe_plan_quantize(const int32_t* ids, int64_t slots, int k, int E, int32_t* row_token, int32_t* slot_row,
                                     int32_t* indptr, const void* x, int64_t rows, int64_t cols, int model_dtype, uint8_t* q, float* scale,
                                     hipStream_t s);
-// out[t] = sum over j of weights[t, j] y[slot_row[t k + j]] in float32 (a negative row: nothing); y and out in model_dtype, float16 or
+// out[t] = sum over j of weights[t, j] y[slot_row[t k + j]] in float32 (a negative row: nothing); out in model_dtype, float16 or
 // bfloat16, H % 8 == 0
-hipError_t launch_moe_weighted_sum(const void* y, const int32_t* slot_row, const float* weights, int64_t T, int k, int64_t H, int model_dtype,
+hipError_t launch_moe_weighted_sum(const float* y, const int32_t* slot_row, const float* weights, int64_t T, int k, int64_t H, int model_dtype,
                                    void* out, hipStream_t s);
 
 }  // namespace gq

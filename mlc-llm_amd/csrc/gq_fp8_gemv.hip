@@ -191,7 +191,7 @@ __global__ __launch_bounds__(64 * kGemvWaves, 2) void fp8_gemv_kernel(Fp8RowsArg
 }
 
 // One token's second expert product and the weighted sum over its experts: a wave an expert, R rows of every W, out [N] in
-// out_dtype.  An expert's result is rounded to out_dtype before it is weighted, as it would be on its way through memory.
+// out_dtype.
 template <int NI, int R>
 __global__ __launch_bounds__(512) void fp8_gemv_sum_kernel(Fp8RowsArgs p, const float* __restrict__ weights, int top_k) {
   __shared__ float part[32][R];
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(512) void fp8_gemv_sum_kernel(Fp8RowsArgs p, const 
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const float sum = wave_sum_last(row_dot<NI>(w[r], x, scale));
-      if (lane == 63) part[j][r] = known ? weight * (p.out_dtype == MODEL_BF16 ? bf2f(f2bf(sum)) : h2f(f2h(sum))) : 0.f;
+      if (lane == 63) part[j][r] = known ? weight * sum : 0.f;
     }
   }
   __syncthreads();

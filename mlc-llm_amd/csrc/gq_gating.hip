@@ -319,11 +319,11 @@ hipError_t launch_moe_plan_quantize(const int32_t* ids, int64_t slots, int k, in
                                    : launch_plan<MODEL_F16>(ids, slots, k, E, row_token, slot_row, indptr, x, rows, cols, q, scale, s);
 }
 
-// One thread eight neighbouring columns of a token; float32 throughout, one rounding at the end.  Four experts at a time, rows and then
+// One thread eight neighbouring columns of a token; y and the sum in float32, one rounding at the end.  Four experts at a time, rows and then
 // values asked for together: one after the other, 16 tokens of 8 experts and 2048 columns took 6.2 us.  A slot without an expert reads row 0 and
 // adds nothing.
 template <int DT>
-__global__ __launch_bounds__(256) void moe_weighted_sum_kernel(const void* __restrict__ y, const int32_t* __restrict__ slot_row,
+__global__ __launch_bounds__(256) void moe_weighted_sum_kernel(const float* __restrict__ y, const int32_t* __restrict__ slot_row,
                                                                const float* __restrict__ weights, int64_t T, int k, int64_t H,
                                                                void* __restrict__ out) {
   const int64_t per_row = H / 8, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(256) void moe_weighted_sum_kernel(const void* __res
       if (j0 + u >= k) at[u] = -1;
     }
 #pragma unroll
-    for (int u = 0; u < kAtATime; ++u) fp8_load8<DT>(y, (at[u] < 0 ? 0 : at[u]) * H + h, f[u]);
+    for (int u = 0; u < kAtATime; ++u) fp8_load8<MODEL_F32>(y, (at[u] < 0 ? 0 : at[u]) * H + h, f[u]);
 #pragma unroll
     for (int u = 0; u < kAtATime; ++u)
 #pragma unroll
@@ -352,7 +352,7 @@ __global__ __launch_bounds__(256) void moe_weighted_sum_kernel(const void* __res
   for (int v = 0; v < 8; ++v) Elem<DT>::store(out, t * H + h + v, acc[v]);
 }
 
-hipError_t launch_moe_weighted_sum(const void* y, const int32_t* slot_row, const float* weights, int64_t T, int k, int64_t H, int model_dtype,
+hipError_t launch_moe_weighted_sum(const float* y, const int32_t* slot_row, const float* weights, int64_t T, int k, int64_t H, int model_dtype,
                                    void* out, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>((T * (H / 8) + 255) / 256));
   if (model_dtype == MODEL_BF16)
