@@ -85,9 +85,10 @@ gq::Fp8RowsArgs few_rows(const gq::Fp8Args& a) {
 // Where the kernel that streams the weights past up to sixteen rows of x is faster than the tiles.  Each of its workgroups brings all
 // of x to LDS: 0.4 us a row of 2048, 2 us a row of 14336.  In a graph, against the tiles with the quantiser that they need: 4096 x 4096
 // of 8 rows 12.1 / 14.6 us, of 12 13.8 / 14.4, of 16 16.2 / 15.1; 10240 x 8192 of 4 rows 26.4 / 25.6, of 6 28.6 / 25.7; 4096 x 14336
-// of 2 18.9 / 23.6, of 6 27.0 / 23.9.  With segments: rows of one on average.
+// of 2 18.9 / 23.6, of 6 27.0 / 23.9.  With segments, rows of one on average: expert layers of 128 x 2048 x 768 at 4 rows 128 / 139 us, at
+// 8 138 / 143, at 10 159 / 145; of 8 x 4096 x 14336 at 5 rows 289 / 292, at 10 314 / 305.
 bool few_rows_dense(int64_t rows, int64_t K) { return rows == 1 || (rows <= 12 && rows * K < 49152); }
-constexpr int64_t kFewRowsEach = 10;
+constexpr int64_t kFewRowsEach = 8;
 
 hipError_t product(const gq::Fp8Args& a, hipStream_t s) {
   const int64_t segments = a.indptr ? (a.rows < a.experts ? a.rows : a.experts) : 1;

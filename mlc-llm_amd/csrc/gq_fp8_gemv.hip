@@ -7,6 +7,11 @@
 // chunk; it is quantised there by every wave, the group's maximum three DPP steps away, so that nothing but the row's sum ever
 // leaves a lane: no LDS, no barrier.  Rows go through v_dot2_f32_bf16 (float32 sums), each chunk is scaled, and the lanes add up.
 // x is asked for before W: loads come back in order, and x has to be converted while W is on its way.
+//
+// Measured: 4096 x 4096 6.1 us a call among others (16.8 MB, of which 3.2 us at a large copy's rate; an empty launch takes 1.9),
+// 28672 x 4096 25.2 us = 4.7 TB/s.  The few-row kernel, which brings x through LDS and shares K between waves, took 8.7 us for the first.
+// Longer K than 8192 stays with it: 16 chunks of x a lane leave too few registers for W (4096 x 14336 18.2 us there).
+// One token of six experts of 2048 x 1408: 19 us, in two launches here and the router's (52 MB; 10 us at the copy's rate).
 #include "gq_fp8_common.hpp"
 #include "gq_topk.hpp"
 
