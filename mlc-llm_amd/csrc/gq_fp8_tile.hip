@@ -441,24 +441,32 @@ struct Form {
 constexpr Form kForms[] = {{256, 256, 256, 875.f, 1687.f}, {256, 192, 256, 752.f, 1412.f}, {256, 160, 256, 822.f, 1203.f}, {256, 128, 256, 619.f, 927.f},
                            {128, 128, 512, 436.f, 1046.f}, {128, 64, 768, 358.f, 970.f}};
 constexpr float kRoundNs = 1140.f, kJoinNs = 460.f, kShareNs = 1.42e-3f;  // a round's ends, the launch that joins, an element of a share
-constexpr int kFormCount = sizeof(kForms) / sizeof(kForms[0]);
+// float32 sums: widening, and four instructions for one.  64 rows of 4096 x 14336 29 us in 16 shares, 119 in one; 300 of 4096 x 4096 29 and 52.
+constexpr Form kPreciseForms[] = {{256, 128, 256, 1060.f, 2200.f}, {256, 64, 512, 1000.f, 2600.f}};
+struct Forms {
+  const Form* form;
+  int count;
+};
+Forms forms_of(bool precise) { return precise ? Forms{kPreciseForms, 2} : Forms{kForms, 6}; }
 float ns_of(const Form& f, int64_t tiles, int64_t blocks) {
   const int64_t full = tiles / f.at_a_time, rest = tiles - full * f.at_a_time;
   float ns = full * (blocks * f.full_ns + kRoundNs);
   if (rest > 0) ns += blocks * (f.alone_ns + (f.full_ns - f.alone_ns) * rest / f.at_a_time) + kRoundNs;
   return ns;
 }
-bool may_take(int form) { return options().gemm_variant < 0 || options().gemm_variant >= kFormCount || options().gemm_variant == form; }
-Plan plan_of(int64_t rows, int64_t N, int64_t K, bool only_whole = false) {
+bool may_take(const Forms& forms, int form) {
+  return options().gemm_variant < 0 || options().gemm_variant >= forms.count || options().gemm_variant == form;
+}
+Plan plan_of(const Forms& forms, int64_t rows, int64_t N, int64_t K, bool only_whole = false) {
   const int64_t groups = (K + kFp8Block - 1) / kFp8Block;
   Plan best;
-  for (int f = 0; f < kFormCount; ++f) {
-    if (!may_take(f)) continue;
-    const int64_t m_tiles = (rows + kForms[f].bm - 1) / kForms[f].bm, n_tiles = (N + kForms[f].bn - 1) / kForms[f].bn, tiles = m_tiles * n_tiles;
+  for (int f = 0; f < forms.count; ++f) {
+    if (!may_take(forms, f)) continue;
+    const int64_t m_tiles = (rows + forms.form[f].bm - 1) / forms.form[f].bm, n_tiles = (N + forms.form[f].bn - 1) / forms.form[f].bn, tiles = m_tiles * n_tiles;
     for (int64_t want = 1; want <= 16 && want <= (only_whole || groups < 4 ? 1 : groups / 4); ++want) {
       if (options().gemm_split_k > 0 && options().gemm_split_k != want) continue;
       const int64_t per = (groups + want - 1) / want, splits = (groups + per - 1) / per;
-      const float ns = ns_of(kForms[f], tiles * splits, per) + (splits > 1 ? kJoinNs + splits * rows * N * kShareNs : 0.f);
+      const float ns = ns_of(forms.form[f], tiles * splits, per) + (splits > 1 ? kJoinNs + splits * rows * N * kShareNs : 0.f);
       if (best.per_split == 0 || ns < best.ns) {
         best = Plan{};
         best.form = f;
@@ -468,15 +476,15 @@ Plan plan_of(int64_t rows, int64_t N, int64_t K, bool only_whole = false) {
       }
     }
     // whole rounds of this form, and what is left of the last in a form that fills a round of its own
-    const int64_t whole = tiles / kForms[f].at_a_time * kForms[f].at_a_time / m_tiles;
+    const int64_t whole = tiles / forms.form[f].at_a_time * forms.form[f].at_a_time / m_tiles;
     if (!only_whole && options().gemm_split_k <= 1 && whole > 0 && whole < n_tiles) {
-      const Plan rest = plan_of(rows, N - whole * kForms[f].bn, K, true);
-      const float ns = ns_of(kForms[f], whole * m_tiles, groups) + rest.ns + 2000.f;
+      const Plan rest = plan_of(forms, rows, N - whole * forms.form[f].bn, K, true);
+      const float ns = ns_of(forms.form[f], whole * m_tiles, groups) + rest.ns + 2000.f;
       if (ns < best.ns) {
         best = Plan{};
         best.form = f;
         best.per_split = static_cast<int>(groups);
-        best.n_rest = whole * kForms[f].bn;
+        best.n_rest = whole * forms.form[f].bn;
         best.form_rest = rest.form;
         best.ns = ns;
       }
@@ -485,13 +493,13 @@ Plan plan_of(int64_t rows, int64_t N, int64_t K, bool only_whole = false) {
   return best;
 }
 // With segments a tile in two, about, of each is short.  No shares of K.
-int form_of(int64_t rows, int64_t experts, int64_t N, int64_t K) {
+int form_of(const Forms& forms, int64_t rows, int64_t experts, int64_t N, int64_t K) {
   int best = 0;
   float best_ns = 0.f;
-  for (int f = 0; f < kFormCount; ++f) {
-    if (!may_take(f)) continue;
-    const int64_t tiles = (rows / kForms[f].bm + (experts + 1) / 2) * ((N + kForms[f].bn - 1) / kForms[f].bn);
-    const float ns = ns_of(kForms[f], tiles, (K + kFp8Block - 1) / kFp8Block);
+  for (int f = 0; f < forms.count; ++f) {
+    if (!may_take(forms, f)) continue;
+    const int64_t tiles = (rows / forms.form[f].bm + (experts + 1) / 2) * ((N + forms.form[f].bn - 1) / forms.form[f].bn);
+    const float ns = ns_of(forms.form[f], tiles, (K + kFp8Block - 1) / kFp8Block);
     if (best_ns == 0.f || ns < best_ns) {
       best_ns = ns;
       best = f;
@@ -527,7 +535,10 @@ hipError_t launch_tile(const Fp8Args& a, const Plan& plan, int part, hipStream_t
 }
 
 hipError_t launch_part(const Fp8Args& a, const Plan& plan, int part, hipStream_t s) {
-  switch (part == 0 ? plan.form : plan.form_rest) {
+  const int form = part == 0 ? plan.form : plan.form_rest;
+  if (a.precise)
+    return form == 0 ? launch_tile<4, 2, 4, 4, 3, true, false>(a, plan, part, s) : launch_tile<4, 2, 4, 2, 2, true, false>(a, plan, part, s);
+  switch (form) {
     case 0: return launch_tile<2, 4, 8, 4, 3, false, false>(a, plan, part, s);
     case 1: return launch_tile<4, 2, 4, 6, 3, false, false>(a, plan, part, s);
     case 2: return launch_tile<4, 2, 4, 5, 3, false, false>(a, plan, part, s);
@@ -540,8 +551,12 @@ hipError_t launch_part(const Fp8Args& a, const Plan& plan, int part, hipStream_t
 }  // namespace
 
 int64_t fp8_tile_workspace_bytes(int64_t rows, int64_t N, int64_t K) {
-  const Plan p = plan_of(rows, N, K);
-  return p.splits > 1 ? p.splits * rows * N * 4 : 0;
+  int64_t bytes = 0;
+  for (const bool precise : {false, true}) {
+    const Plan p = plan_of(forms_of(precise), rows, N, K);
+    if (p.splits > 1 && p.splits * rows * N * 4 > bytes) bytes = p.splits * rows * N * 4;
+  }
+  return bytes;
 }
 
 hipError_t launch_fp8_tile(const Fp8Args& a, hipStream_t s) {
@@ -552,10 +567,9 @@ hipError_t launch_fp8_tile(const Fp8Args& a, hipStream_t s) {
     if (a.rows < 96 * a.experts) return launch_tile<4, 2, 4, 2, 2, true, true>(a, Plan{}, 0, s);
     return launch_tile<4, 2, 4, 4, 3, true, true>(a, Plan{}, 0, s);
   }
-  if (a.precise) return launch_tile<4, 2, 4, 4, 3, true, false>(a, Plan{}, 0, s);
   Plan plan;
-  if (!a.indptr) plan = plan_of(a.rows, a.N, a.K);
-  else plan.form = form_of(a.rows, a.experts, a.N, a.K);
+  if (!a.indptr) plan = plan_of(forms_of(a.precise), a.rows, a.N, a.K);
+  else plan.form = form_of(forms_of(a.precise), a.rows, a.experts, a.N, a.K);
   const hipError_t e = launch_part(a, plan, 0, s);
   return e != hipSuccess || plan.n_rest == 0 ? e : launch_part(a, plan, 1, s);
 }

@@ -50,6 +50,25 @@ def test_tile_forms_and_shares(options, form, m, n, k):
         assert torch.equal(y, ops.fp8_linear(x, wd, wsd, bias=bias))
 
 
+@pytest.mark.parametrize("form", range(2))
+@pytest.mark.parametrize("m,n,k", [(18, 136, 528), (70, 260, 1040), (200, 392, 1536), (300, 520, 2064)])
+def test_precise_forms_and_shares(options, form, m, n, k):
+    x = torch.randn(m, k, generator=_gen(m + n))
+    w, ws = _weights(n, k, 3)
+    residual = torch.randn(m, n, generator=_gen(m))
+    wd, wsd = w.cuda()[:, :k], ws.cuda()
+    xv, wv = quantized(x.double())[2].cuda(), block_values(w[:, :k].float().nan_to_num(), ws).cuda()
+    exact = xv @ wv.t() + residual.cuda().double()
+    for shares in (1, 2, 3, 4):
+        if shares > 1 and -(-k // 128) < 4 * shares:
+            continue
+        options(form, shares)
+        y = ops.fp8_linear(x.cuda(), wd, wsd, residual=residual.cuda())
+        assert "float32 sums, %d shares" % shares in _lib.last_kernel()
+        bound = _linear_bound(xv, wv, exact, torch.float32) + (exact.abs() + residual.cuda().double().abs()) * 2.0**-22
+        assert ((y.double() - exact).abs() <= bound).all()
+
+
 def test_last_round_in_a_form_of_its_own(options):
     m, n, k = 1024, 16500, 1024
     x = torch.randn(m, k, generator=_gen(1)).to(torch.bfloat16).cuda()
