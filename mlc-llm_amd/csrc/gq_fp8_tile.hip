@@ -441,13 +441,13 @@ struct Form {
 constexpr Form kForms[] = {{256, 256, 256, 875.f, 1687.f}, {256, 192, 256, 752.f, 1412.f}, {256, 160, 256, 822.f, 1203.f}, {256, 128, 256, 619.f, 927.f},
                            {128, 128, 512, 436.f, 1046.f}, {128, 64, 768, 358.f, 970.f}};
 constexpr float kRoundNs = 1140.f, kJoinNs = 460.f, kShareNs = 1.42e-3f;  // a round's ends, the launch that joins, an element of a share
-// float32 sums: widening, and four instructions for one.  64 rows of 4096 x 14336 29 us in 16 shares, 119 in one; 300 of 4096 x 4096 29 and 52.
-constexpr Form kPreciseForms[] = {{256, 128, 256, 1060.f, 2200.f}, {256, 64, 512, 1000.f, 2600.f}};
+// float32 sums: widening, and four instructions for one.  Fitted alike (36 shapes: 1.4 % on average).  64 rows of 4096 x 14336 29 us in 16 shares, 119 in one; 300 of 4096 x 4096 29 and 52.
+constexpr Form kPreciseForms[] = {{256, 192, 256, 1493.f, 2287.f}, {256, 128, 256, 962.f, 1765.f}, {256, 64, 512, 582.f, 2050.f}};
 struct Forms {
   const Form* form;
   int count;
 };
-Forms forms_of(bool precise) { return precise ? Forms{kPreciseForms, 2} : Forms{kForms, 6}; }
+Forms forms_of(bool precise) { return precise ? Forms{kPreciseForms, 3} : Forms{kForms, 6}; }
 float ns_of(const Form& f, int64_t tiles, int64_t blocks) {
   const int64_t full = tiles / f.at_a_time, rest = tiles - full * f.at_a_time;
   float ns = full * (blocks * f.full_ns + kRoundNs);
@@ -536,8 +536,11 @@ hipError_t launch_tile(const Fp8Args& a, const Plan& plan, int part, hipStream_t
 
 hipError_t launch_part(const Fp8Args& a, const Plan& plan, int part, hipStream_t s) {
   const int form = part == 0 ? plan.form : plan.form_rest;
-  if (a.precise)
-    return form == 0 ? launch_tile<4, 2, 4, 4, 3, true, false>(a, plan, part, s) : launch_tile<4, 2, 4, 2, 2, true, false>(a, plan, part, s);
+  if (a.precise) {
+    if (form == 0) return launch_tile<2, 4, 8, 3, 3, true, false>(a, plan, part, s);
+    if (form == 1) return launch_tile<4, 2, 4, 4, 3, true, false>(a, plan, part, s);
+    return launch_tile<4, 2, 4, 2, 2, true, false>(a, plan, part, s);
+  }
   switch (form) {
     case 0: return launch_tile<2, 4, 8, 4, 3, false, false>(a, plan, part, s);
     case 1: return launch_tile<4, 2, 4, 6, 3, false, false>(a, plan, part, s);
@@ -562,10 +565,11 @@ int64_t fp8_tile_workspace_bytes(int64_t rows, int64_t N, int64_t K) {
 hipError_t launch_fp8_tile(const Fp8Args& a, hipStream_t s) {
   if (a.q_out != nullptr) {
     if (a.N % (2 * kFp8Block) != 0 || static_cast<uint64_t>(a.N) * a.w_pitch >= 0xffffffffull) return hipErrorNotSupported;
-    // 64 rows in two workgroups a unit, or 128 in one: expert layers of 128 x 2048 x 768 at 32 rows an expert 166 / 189 us, at 64 228 / 238, at
-    // 96 268 / 278; of 8 x 4096 x 14336 at 64 rows 395 / 449, at 96 479 / 473
-    if (a.rows < 96 * a.experts) return launch_tile<4, 2, 4, 2, 2, true, true>(a, Plan{}, 0, s);
-    return launch_tile<4, 2, 4, 4, 3, true, true>(a, Plan{}, 0, s);
+    // 64 rows in two workgroups a unit, or 192 in one: expert layers of 128 x 2048 x 768 at 64 rows an expert 227 / 246 us, at 128 312 / 327, at
+    // 256 499 / 517; of 8 x 4096 x 14336 at 64 rows 387 / 396, at 192 689 / 727, at 256 852 / 822, at 384 1177 / 1125.  (A form of 128 rows,
+    // whose waves widen a third more operands than 192's for a result, was behind one of them at all of these.)
+    if (a.rows < 256 * a.experts) return launch_tile<4, 2, 4, 2, 2, true, true>(a, Plan{}, 0, s);
+    return launch_tile<2, 4, 8, 3, 3, true, true>(a, Plan{}, 0, s);
   }
   Plan plan;
   if (!a.indptr) plan = plan_of(forms_of(a.precise), a.rows, a.N, a.K);

@@ -50,7 +50,7 @@ def test_tile_forms_and_shares(options, form, m, n, k):
         assert torch.equal(y, ops.fp8_linear(x, wd, wsd, bias=bias))
 
 
-@pytest.mark.parametrize("form", range(2))
+@pytest.mark.parametrize("form", range(3))
 @pytest.mark.parametrize("m,n,k", [(18, 136, 528), (70, 260, 1040), (200, 392, 1536), (300, 520, 2064)])
 def test_precise_forms_and_shares(options, form, m, n, k):
     x = torch.randn(m, k, generator=_gen(m + n))
@@ -196,3 +196,23 @@ def test_layers_run_the_operators():
         y = moe(x, gate)
         weights, ids = ops.moe_gating(gate, 4, "sigmoid", moe.score_bias, 4, 2, True, 2.5)
         assert y.shape == x.shape and torch.equal(y.view(-1, 256), ops.fp8_moe_experts(x.view(-1, 256), weights, ids, w13, s13, w2, s2))
+
+
+@pytest.mark.parametrize("t,ne,k", [(1100, 3, 2), (600, 2, 1), (300, 2, 2), (770, 3, 3)])
+def test_layers_of_many_rows_an_expert(t, ne, k):
+    # the gate/up product in both of its forms, tiles that end in every row of waves, against the two steps on their own
+    hidden, inter = 400, 256
+    x = torch.randn(t, hidden, generator=_gen(t)).to(torch.float16).cuda()
+    logits = torch.randn(t, ne, generator=_gen(t + 1)).cuda()
+    w13, s13 = (v.cuda() for v in _weights(2 * inter, hidden, 2, ne))
+    w2, s2 = (v.cuda() for v in _weights(hidden, inter, 3, ne))
+    weights, ids = ops.moe_gating(logits, k)
+    row_token, slot_row, indptr = ops.moe_plan(ids, ne)
+    q, s = ops.fp8_quantize(x)
+    both = ops.fp8_group_gemm(q, s, row_token, w13, s13, indptr, torch.float32, True)
+    h, hs = ops.fp8_silu_mul_quantize(both)
+    y = ops.fp8_group_gemm(h, hs, None, w2, s2, indptr, torch.float32, False).double()
+    want = (y[slot_row.view(t, k).long()] * weights.double()[..., None]).sum(1)
+    got = ops.fp8_moe_experts(x, weights, ids, w13, s13, w2, s2)
+    size = (y[slot_row.view(t, k).long()].abs() * weights.double()[..., None]).sum(1)
+    assert ((got.double() - want).abs() <= 2.0**-11 * want.abs() + size * (k + 2) * 2.0**-23 + 2.0**-24).all()
