@@ -216,3 +216,32 @@ def test_layers_of_many_rows_an_expert(t, ne, k):
     got = ops.fp8_moe_experts(x, weights, ids, w13, s13, w2, s2)
     size = (y[slot_row.view(t, k).long()].abs() * weights.double()[..., None]).sum(1)
     assert ((got.double() - want).abs() <= 2.0**-11 * want.abs() + size * (k + 2) * 2.0**-23 + 2.0**-24).all()
+
+
+def test_weights_beyond_four_gib():
+    n, k = 262144 + 4096, 16384
+    w = torch.randint(0, 0x78, (n, k), dtype=torch.uint8, device="cuda")  # no NaN
+    w[:, ::3] |= 0x80
+    w = w.view(torch.float8_e4m3fn)
+    ws = 2e-4 * (0.5 + torch.rand(-(-n // 128), k // 128, device="cuda"))
+    assert w.numel() > 2**32
+    for m in (1, 8, 20):
+        x = torch.randn(m, k, generator=_gen(m)).to(torch.bfloat16).cuda()
+        y = ops.fp8_linear(x, w, ws, out_dtype=torch.float32)
+        xv = quantized(x.cpu().double())[2].cuda()
+        for part in (slice(0, 256), slice(131072, 131072 + 256), slice(n - 256, n)):
+            wv = block_values(w[part].float(), ws[part.start // 128 : part.stop // 128])
+            exact = xv @ wv.t()
+            assert ((y[:, part].double() - exact).abs() <= _linear_bound(xv, wv, exact, torch.float32)).all()
+    # the same bytes as a stack of experts, a few rows and many rows each
+    experts = 65
+    stack, scales = w.view(experts, n // experts, k), ws.view(experts, n // experts // 128, k // 128)
+    for each in (3, 40):
+        indptr = torch.arange(experts + 1, dtype=torch.int32).cuda() * each
+        x = torch.randn(experts * each, k, generator=_gen(each)).to(torch.bfloat16).cuda()
+        y = ops.fp8_group_gemm(*ops.fp8_quantize(x), None, stack, scales, indptr, torch.float32)
+        for e in (0, 64):
+            xv = quantized(x[e * each : e * each + each].cpu().double())[2].cuda()
+            wv = block_values(stack[e, :256].float(), scales[e, :2])
+            exact = xv @ wv.t()
+            assert ((y[e * each : e * each + each, :256].double() - exact).abs() <= _linear_bound(xv, wv, exact, torch.float32)).all()
