@@ -48,7 +48,7 @@ struct Carver {
 int quantize(const void* x, int64_t rows, int64_t K, int model_dtype, bool silu, void* q, int64_t q_pitch, void* scale,
              mi355gq_stream_t stream, const char* what) {
   FP8_REQUIRE(dtype_ok(model_dtype), "%s: model_dtype=%d (MI355GQ_F16, MI355GQ_F32 or MI355GQ_BF16)", what, model_dtype);
-  FP8_REQUIRE(dim_ok(rows) && dim_ok(K), "%s: bad shape [%lld, %lld]", what, (long long)rows, (long long)K);
+  FP8_REQUIRE(dim_ok(rows) && dim_ok(K) && (K + 511) / 512 <= kMaxTiles, "%s: bad shape [%lld, %lld]", what, (long long)rows, (long long)K);
   FP8_REQUIRE(pitch_ok(q_pitch, K), "%s: q_pitch=%lld for K=%lld: a multiple of 16, at least K", what, (long long)q_pitch, (long long)K);
   if (rows == 0 || K == 0) return MI355GQ_OK;
   FP8_REQUIRE(x && q && scale, "%s: null pointer", what);
@@ -176,7 +176,7 @@ int mi355gq_fp8_dequantize(const void* q, int64_t q_pitch, const void* scale, in
   FP8_REQUIRE(dtype_ok(out_dtype), "fp8_dequantize: out_dtype=%d", out_dtype);
   FP8_REQUIRE(row_groups == 0 || (row_groups == 1 && mats == 1), "fp8_dequantize: row_groups=%d with %lld matrices", row_groups,
               (long long)mats);
-  FP8_REQUIRE(dim_ok(mats) && dim_ok(rows) && dim_ok(K) && (rows == 0 || mats < kMaxDim / rows), "fp8_dequantize: bad shape [%lld, %lld, %lld]",
+  FP8_REQUIRE(dim_ok(mats) && dim_ok(rows) && dim_ok(K) && (K + 511) / 512 <= kMaxTiles && (rows == 0 || mats < kMaxDim / rows), "fp8_dequantize: bad shape [%lld, %lld, %lld]",
               (long long)mats, (long long)rows, (long long)K);
   FP8_REQUIRE(pitch_ok(q_pitch, K), "fp8_dequantize: q_pitch=%lld for K=%lld: a multiple of 16, at least K", (long long)q_pitch, (long long)K);
   if (mats == 0 || rows == 0 || K == 0) return MI355GQ_OK;

@@ -23,7 +23,6 @@ __device__ __forceinline__ uint32_t fp8_scale_bits(float top) {
   const int e = static_cast<int>(u >> 23) - ((u & 0x7fffffu) <= 0x600000u ? 8 : 7);
   return top > 0.f ? static_cast<uint32_t>(e < 1 ? 1 : e) << 23 : 0x3f800000u;
 }
-__device__ __forceinline__ float fp8_scale(float top) { return __builtin_bit_cast(float, fp8_scale_bits(top)); }
 // 1 / s of such a scale, exact (s lies in 2^-126 .. 2^120)
 __device__ __forceinline__ float fp8_inverse(uint32_t scale_bits) {
   return __builtin_bit_cast(float, (254u << 23) - scale_bits);

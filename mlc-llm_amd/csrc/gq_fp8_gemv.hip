@@ -13,7 +13,6 @@
 // Longer K than 8192 stays with it: 16 chunks of x a lane leave too few registers for W (4096 x 14336 18.2 us there).
 // One token of six experts of 2048 x 1408: 19 us, in two launches here and the router's (52 MB; 10 us at the copy's rate).
 #include "gq_fp8_common.hpp"
-#include "gq_topk.hpp"
 
 namespace gq {
 

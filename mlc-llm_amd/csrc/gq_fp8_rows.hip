@@ -15,7 +15,6 @@
 // Measured: 4096 x 4096 of 2 / 8 rows 8.8 / 11.8 us, 28672 x 4096 of 8 rows 28.7 us (4.1 TB/s; bound by HBM, and by the x that each of
 // its workgroups quantises).  16 tokens over 128 experts of 2048 x 768: gate/up 44 us, down 27 us (about 390 MB, 5.5 TB/s).
 #include "gq_fp8_common.hpp"
-#include "gq_topk.hpp"
 
 namespace gq {
 

@@ -18,7 +18,6 @@
 // Precise products sum in float32 throughout: the operands are widened to bfloat16 (which holds them exactly) on their way from
 // LDS, four instructions of 16 x 16 x 32 to a block, at half the rate.  So do products that are rounded to e4m3 again.
 #include "gq_fp8_common.hpp"
-#include "gq_topk.hpp"
 
 namespace gq {
 

@@ -34,6 +34,7 @@ def test_quantisers_check_their_arguments():
         _refused(fn(X, 4, 128, 9, Y, 128, WS, None), "model_dtype")
         _refused(fn(X, -1, 128, f16, Y, 128, WS, None), "shape")
         _refused(fn(X, 4, 1 << 40, f16, Y, 1 << 40, WS, None), "shape")
+        _refused(fn(X, 4, 1 << 25, f16, Y, 1 << 25, WS, None), "shape")
         _refused(fn(X, 4, 130, f16, Y, 130, WS, None), "multiple of 16")
         _refused(fn(X, 4, 130, f16, Y, 128, WS, None), "multiple of 16")
         _refused(fn(None, 4, 128, f16, Y, 128, WS, None), "null")
