@@ -7,17 +7,20 @@ namespace gq {
 
 namespace {
 
-// over the 16 lanes of a token
+// over the 32 lanes of a token, two rows of 16: rotations within a row, then each row with its neighbour
 template <class Op>
-__device__ __forceinline__ uint32_t row_reduce16(uint32_t v, Op op) {
+__device__ __forceinline__ uint32_t reduce32(uint32_t v, Op op) {
   v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x128, 0xf, 0xf, false)));  // row_ror:8
   v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x124, 0xf, 0xf, false)));
   v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x122, 0xf, 0xf, false)));
-  return op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x121, 0xf, 0xf, false)));
+  v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x121, 0xf, 0xf, false)));
+  const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return op(both[0], both[1]);
 }
-__device__ __forceinline__ float row_sum16(float v) {
-  return __builtin_bit_cast(float, row_reduce16(__builtin_bit_cast(uint32_t, v), [](uint32_t a, uint32_t b) {
-    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+template <class Op>
+__device__ __forceinline__ float reduce32_f(float v, Op op) {
+  return __builtin_bit_cast(float, reduce32(__builtin_bit_cast(uint32_t, v), [op](uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, op(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
   }));
 }
 // bits in the order of the numbers; 0 stands behind all of them
@@ -28,27 +31,28 @@ __device__ __forceinline__ uint32_t in_order(float v) {
 
 }  // namespace
 
-// Four tokens a wave: lane r of a token's 16 holds experts NC r to NC r + NC - 1.  With logits x:
+// Two tokens a wave: lane r of a token's 32 holds experts NC r to NC r + NC - 1.  With logits x:
 //   score = softmax(x) or 1 / (1 + exp(-x)) in float32, with the division and the exponential of the C library;
 //   key   = score + bias.
 // With groups, a group's standing is its best key, or the sum of its best two where there is a bias, and only the experts
 // of the top_groups best are looked at.  Then k rounds pick the largest key left, and of equal ones (as of equal groups) the one of the
-// lowest index: the largest of a lane's keys, then of the row's 16 by rotations, then the lowest expert that has it.
+// lowest index: the largest of a lane's keys, then of the 32 lanes', then the lowest expert that has it.
 // A NaN logit has score 0 and stands behind every other expert (as one of a NaN key does); +inf counts as the largest finite number, and a
 // softmax over nothing but -inf has scores 0.  Weights whose sum is 0 stay 0.
 //
-// Bound by instructions: a round is about 5 NC + 20 of them, for four tokens.  With a token a wave, four experts a lane and ballots for
-// the choice, 4096 tokens of 256 experts in 8 groups took 9.2 us, so 8.4 (6.4 beside the launch).
+// Bound by the length of one wave's chain of instructions: a round is about 5 NC + 20 of them.  4096
+// tokens of 256 experts in 8 groups 7.1 us in a graph, 1.9 of it the launch (a token a wave, and ballots for the choice: 9.2; four tokens a
+// wave: 8.4); one token of 64 experts 2.6.
 template <int NC, int DT>
 __global__ __launch_bounds__(64) void gating_kernel(const void* __restrict__ logits, const float* __restrict__ bias,
                                                     int64_t T, int E, int k, int sigmoid, int groups, int top_groups,
                                                     int group_inv, int renormalize, float scale, int vec,
                                                     float* __restrict__ weights, int32_t* __restrict__ ids) {
-  __shared__ __attribute__((aligned(16))) float scores[4][NC * 16];
-  __shared__ __attribute__((aligned(16))) float keys[4][NC * 16];
-  __shared__ float standings[4][64];
-  const int r = threadIdx.x & 15, token = threadIdx.x >> 4, e0 = r * NC;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + token;
+  __shared__ __attribute__((aligned(16))) float scores[2][NC * 32];
+  __shared__ __attribute__((aligned(16))) float keys[2][NC * 32];
+  __shared__ float standings[2][64];
+  const int r = threadIdx.x & 31, token = threadIdx.x >> 5, e0 = r * NC;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 2 + token;
   const bool there = at < T;
   const int64_t t = there ? at : T - 1;  // (a token past the end computes the last one's and writes nothing)
   constexpr float kBig = 3.402823466e38f;
@@ -80,14 +84,14 @@ __global__ __launch_bounds__(64) void gating_kernel(const void* __restrict__ log
     float m = score[0];
 #pragma unroll
     for (int c = 1; c < NC; ++c) m = fmaxf(m, score[c]);
-    m = row_max16(m);
+    m = reduce32_f(m, [](float a, float b) { return fmaxf(a, b); });
     float sum = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       score[c] = score[c] == -inf ? 0.f : expf(score[c] - m);
       sum += score[c];
     }
-    sum = row_sum16(sum);
+    sum = reduce32_f(sum, [](float a, float b) { return a + b; });
 #pragma unroll
     for (int c = 0; c < NC; ++c) score[c] = sum > 0.f ? score[c] / sum : 0.f;
   }
@@ -146,7 +150,7 @@ __global__ __launch_bounds__(64) void gating_kernel(const void* __restrict__ log
 #pragma unroll
       for (int c = 0; c < NC; ++c) keys[token][e0 + c] = key[c];
       written();
-      for (int g = r; g < groups; g += 16) {
+      for (int g = r; g < groups; g += 32) {
         float best = -inf, next = -inf;
 #pragma unroll 4
         for (int j = 0; j < size; ++j) join(best, next, keys[token][g * size + j], -inf);
@@ -154,11 +158,11 @@ __global__ __launch_bounds__(64) void gating_kernel(const void* __restrict__ log
       }
       written();
       uint64_t kept = 0;  // groups of this lane's, then of all lanes'
-      for (int g = r; g < groups; g += 16)
+      for (int g = r; g < groups; g += 32)
         if (groups_ahead(g, standings[token][g]) < top_groups) kept |= 1ull << g;
       auto either = [](uint32_t a, uint32_t b) { return a | b; };
-      kept = row_reduce16(static_cast<uint32_t>(kept), either) |
-             static_cast<uint64_t>(row_reduce16(static_cast<uint32_t>(kept >> 32), either)) << 32;
+      kept = reduce32(static_cast<uint32_t>(kept), either) |
+             static_cast<uint64_t>(reduce32(static_cast<uint32_t>(kept >> 32), either)) << 32;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const int g = ((e0 + c) * group_inv) >> 20;  // (e0 + c) / size
@@ -168,29 +172,26 @@ __global__ __launch_bounds__(64) void gating_kernel(const void* __restrict__ log
   }
   written();
   float sum = 0.f;
-  int my_id[2] = {0, 0};
+  int my_id = 0;
   for (int i = 0; i < k; ++i) {
     uint32_t m = order[0];
 #pragma unroll
     for (int c = 1; c < NC; ++c) m = m > order[c] ? m : order[c];
-    m = row_reduce16(m, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+    m = reduce32(m, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
     uint32_t first = 0x7fffffffu;
 #pragma unroll
     for (int c = NC - 1; c >= 0; --c) first = order[c] == m ? static_cast<uint32_t>(e0 + c) : first;
-    first = row_reduce16(first, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+    first = reduce32(first, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
 #pragma unroll
     for (int c = 0; c < NC; ++c) order[c] = static_cast<uint32_t>(e0 + c) == first ? 0u : order[c];
-    if (r == (i & 15)) my_id[i >> 4] = static_cast<int>(first);
+    if (r == i) my_id = static_cast<int>(first);
     sum += scores[token][first];
   }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = r + 16 * h;
-    if (i >= k || !there) continue;
-    float s = scores[token][my_id[h]];
-    if (renormalize) s = sum > 0.f ? s / sum : 0.f;
-    weights[t * k + i] = s * scale;
-    ids[t * k + i] = my_id[h];
+  if (r < k && there) {
+    float v = scores[token][my_id];
+    if (renormalize) v = sum > 0.f ? v / sum : 0.f;
+    weights[t * k + r] = v * scale;
+    ids[t * k + r] = my_id;
   }
 }
 
@@ -198,7 +199,7 @@ hipError_t launch_moe_gating(const GatingArgs& a, hipStream_t s) {
   const int size = a.E / a.groups;
   const int vec = a.E % 8 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0;
   auto go = [&](auto nc, auto dt) {
-    hipLaunchKernelGGL((gating_kernel<decltype(nc)::value, decltype(dt)::value>), dim3(static_cast<unsigned>((a.T + 3) / 4)), dim3(64), 0, s,
+    hipLaunchKernelGGL((gating_kernel<decltype(nc)::value, decltype(dt)::value>), dim3(static_cast<unsigned>((a.T + 1) / 2)), dim3(64), 0, s,
                        a.logits, a.bias, a.T, a.E, a.k, a.sigmoid, a.groups, a.top_groups, ((1 << 20) + size - 1) / size, a.renormalize,
                        a.scale, vec, a.weights, a.ids);
   };
@@ -207,10 +208,10 @@ hipError_t launch_moe_gating(const GatingArgs& a, hipStream_t s) {
     else if (a.model_dtype == MODEL_BF16) go(nc, std::integral_constant<int, MODEL_BF16>{});
     else go(nc, std::integral_constant<int, MODEL_F16>{});
   };
-  if (a.E <= 64) by_type(std::integral_constant<int, 4>{});
-  else if (a.E <= 128) by_type(std::integral_constant<int, 8>{});
-  else if (a.E <= 256) by_type(std::integral_constant<int, 16>{});
-  else by_type(std::integral_constant<int, 32>{});
+  if (a.E <= 64) by_type(std::integral_constant<int, 2>{});
+  else if (a.E <= 128) by_type(std::integral_constant<int, 4>{});
+  else if (a.E <= 256) by_type(std::integral_constant<int, 8>{});
+  else by_type(std::integral_constant<int, 16>{});
   return hipGetLastError();
 }
 
