@@ -130,6 +130,10 @@ struct Fp8RowsArgs {
 };
 // Sixteen rows of a segment at a time; hipErrorNotSupported where the kernel does not apply.
 hipError_t launch_fp8_rows(const Fp8RowsArgs& a, hipStream_t s);
+// What the kernels of one row take: a row of K in registers, offsets into W in 32 bits.
+inline bool fp8_gemv_takes(int64_t N, int64_t K, int64_t w_pitch) {
+  return K % 16 == 0 && K <= 8192 && static_cast<uint64_t>(N) * w_pitch < 0xffffffffull;
+}
 // One row, or (ids) one row of each expert; hipErrorNotSupported as above.  _sum: the rows' products with their experts' W, weighted
 // and added up, y [1, N]; x float32 [top_k, K].
 hipError_t launch_fp8_gemv(const Fp8RowsArgs& a, hipStream_t s);

@@ -271,8 +271,7 @@ hipError_t launch_gemv_by_k(const Fp8RowsArgs& a, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_fp8_gemv(const Fp8RowsArgs& a, hipStream_t s) {
-  if (a.K % 16 != 0 || a.K > 8192 || static_cast<uint64_t>(a.N) * a.w_pitch >= 0xffffffffull || (a.silu && a.N % 4 != 0))
-    return hipErrorNotSupported;
+  if (!fp8_gemv_takes(a.N, a.K, a.w_pitch) || (a.silu && a.N % 4 != 0)) return hipErrorNotSupported;
   if (a.silu) {
     if (a.x_kind == MODEL_BF16) return launch_gemv_by_k<MODEL_BF16, true>(a, s);
     return a.x_kind == MODEL_F16 ? launch_gemv_by_k<MODEL_F16, true>(a, s) : hipErrorNotSupported;
@@ -284,7 +283,7 @@ hipError_t launch_fp8_gemv(const Fp8RowsArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_fp8_gemv_sum(const Fp8RowsArgs& a, const float* weights, int top_k, hipStream_t s) {
-  if (a.K % 16 != 0 || a.K > 8192 || static_cast<uint64_t>(a.N) * a.w_pitch >= 0xffffffffull || top_k > 32) return hipErrorNotSupported;
+  if (!fp8_gemv_takes(a.N, a.K, a.w_pitch) || top_k > 32) return hipErrorNotSupported;
   const int waves = top_k < 8 ? top_k : 8;
   auto go = [&](auto ni, auto r) {
     constexpr int R = decltype(r)::value;

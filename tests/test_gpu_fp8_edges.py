@@ -1,0 +1,85 @@
+"""8-bit block-scaled operators where one form ends and another begins: one token beyond the one-row kernel, rows that lie in a wider
+buffer, segments of several passes, a layer whose every sum is known exactly, layers that are copied, moved and cast."""
+
+import copy
+
+import pytest
+import torch
+
+from mlc_llm_amd import _lib, nn as layers, ops
+from test_gpu_fp8 import DTYPES, E4M3, UNIT, _gen, _linear_bound, _step_bound, _weights, block_values, quantized
+
+pytestmark = pytest.mark.gpu
+
+
+class ExactLayer:
+    """An expert layer on whole numbers: gate and up sums below 2^24 are the same in any order, so the activation's bytes are known
+    and what remains is the second product, the weighted sum and one rounding."""
+
+    def __init__(self, t, hidden, inter, ne, ids, dtype, top=8):
+        g = torch.Generator(device="cuda").manual_seed(t + hidden + inter)
+
+        def whole(*shape):
+            return torch.randint(-top, top + 1, shape, generator=g, device="cuda", dtype=torch.int8).to(dtype).float()
+
+        assert top * top * hidden < 2**24
+        self.x, self.ids, self.dtype = whole(t, hidden).to(dtype), ids.int().cuda(), dtype
+        self.w13, self.w2 = (torch.stack([whole(n, k).to(E4M3) for _ in range(ne)]) for n, k in ((2 * inter, hidden), (hidden, inter)))
+        self.s13 = torch.full((ne, -(-2 * inter // 128), -(-hidden // 128)), 2.0**-9, device="cuda")
+        self.s2 = 2e-4 * (0.5 + torch.rand(ne, -(-hidden // 128), -(-inter // 128), generator=g, device="cuda"))
+        self.weights = 0.1 + torch.rand(ids.shape, generator=g, device="cuda")
+        self.hidden, self.inter, self.ne = hidden, inter, ne
+
+    def want(self):
+        """The layer in float64 and the sum of magnitudes behind each result; and the operands' step bound of the second product."""
+        out, size, step = (torch.zeros(self.x.shape, dtype=torch.float64, device="cuda") for _ in range(3))
+        for e in range(self.ne):
+            token, slot = torch.nonzero(self.ids == e, as_tuple=True)
+            if len(token) == 0:
+                continue
+            both = self.x[token].double() @ self.w13[e].double().t() * 2.0**-9
+            assert torch.equal(both.float().double(), both)
+            h, hs = ops.fp8_silu_mul_quantize(both.float())
+            hv = h.double() * hs.double().t().repeat_interleave(128, 1)[:, : self.inter]
+            down = self.w2[e].double() * self.s2[e].double().repeat_interleave(128, 0)[: self.hidden].repeat_interleave(128, 1)[:, : self.inter]
+            w = self.weights[token, slot].double()[:, None]
+            out.index_add_(0, token, w * (hv @ down.t()))
+            size.index_add_(0, token, w * (hv.abs() @ down.abs().t()))
+            step.index_add_(0, token, w * _step_bound(hv, down))
+        return out, size, step
+
+    def check(self, y, eight_bit=False):
+        out, size, step = self.want()
+        # float32 sums of the second product as in _linear_bound, the weights' products and their sum, one rounding to the type
+        terms = self.inter / 128 + 20 + self.ids.shape[1] + 2
+        bound = size * terms * 2.0**-23 + out.abs() * UNIT[self.dtype] + 2.0**-24 * (self.dtype == torch.float16)
+        err = (y.double() - out).abs()
+        assert (err <= bound + (step * (1 + 2.0**-20) if eight_bit else 0)).all(), (err / bound).max()
+
+    def run(self):
+        return ops.fp8_moe_experts(self.x, self.weights, self.ids, self.w13, self.s13, self.w2, self.s2)
+
+
+@pytest.mark.parametrize("hidden,inter", [(256, 8208), (4096, 14336), (512, 8320), (8208, 256), (8192, 8192), (9344, 384)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_one_token_beyond_the_one_row_kernel(hidden, inter, dtype):
+    ne, k = 3, 2
+    layer = ExactLayer(1, hidden, inter, ne, torch.tensor([[2, 0]]), dtype, top=8 if hidden < 8192 else 4)
+    layer.check(layer.run())
+    # the same through the C entry, in a workspace that shows what was written: no product is computed for another form to compute again
+    size = _lib.lib().mi355gq_fp8_moe_workspace_bytes(1, hidden, inter, ne, k)
+    space = torch.full((size,), 0xA5, dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(layer.x)
+    _lib.call("mi355gq_fp8_moe", layer.x.data_ptr(), 1, hidden, inter, ne, k, layer.weights.data_ptr(), layer.ids.data_ptr(), layer.w13.data_ptr(),
+              hidden, layer.s13.data_ptr(), layer.w2.data_ptr(), inter, layer.s2.data_ptr(), ops._MODEL_DTYPES[dtype], out.data_ptr(),
+              space.data_ptr(), size, ops._stream())
+    layer.check(out)
+    written = int((space != 0xA5).sum())
+    both = 4 * k * inter
+    rest = hidden + k * inter + 4 * (hidden // 128 + 1 + k * (inter // 128 + 1) + 2 * k + ne + 1) + 4 * k * hidden
+    if hidden <= 8192 and inter <= 8192:
+        assert "fp8_gemv_sum" in _lib.last_kernel() and written <= both
+    elif inter % 128 == 0:
+        assert "fp8_rows" in _lib.last_kernel() and written <= rest, (written, rest)
+    else:  # gate and up apart from the activation
+        assert "fp8_rows" in _lib.last_kernel() and written <= rest + 2 * both
