@@ -455,9 +455,9 @@ MI355GQ_API int mi355gq_moe_combine_dt(const void* y, const void* slot_positions
  * mi355gq_fp8_quantize: x [rows, K] in model_dtype, dense -> q, scale.  A group's scale is the smallest power of two s
  * with max|x| <= 448 s (at least 2^-126, and 1 for a group of zeros), q = x / s rounded to nearest, ties to even: one
  * rounding, the same on any machine.  An infinity or NaN becomes NaN and leaves the scale to the group's other numbers.
- * The bytes between K and the next multiple of 8 (at most the pitch) are written as zeros.
+ * The bytes between K and the next multiple of 8 are written as zeros, what lies between there and the next row is left as it is.
  * mi355gq_fp8_silu_mul_quantize: the same of silu(x1) * x2, x = [x1, x2] [rows, 2 K], computed in float32.
- * mi355gq_fp8_quantize_weight: w [mats, N, K] dense -> q, scale with one scale per block, chosen alike.
+ * mi355gq_fp8_quantize_weight: w [mats, N, K] dense -> q, scale with one scale per block, chosen and written alike.
  * mi355gq_fp8_dequantize: out [mats, rows, K] dense in out_dtype = q * scale; row_groups 1: the activations' scale (mats 1),
  * 0: the weights'.
  */

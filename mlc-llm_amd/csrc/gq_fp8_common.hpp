@@ -216,7 +216,7 @@ __device__ __forceinline__ bf16x8_t fp8_widen(uint32_t lo, uint32_t hi) {
 }
 
 // rows of x [rows, cols] (silu_mul: of x [rows, 2 cols], silu(first half) * second half) to e4m3 groups; the q bytes between
-// cols and pitch are written as zeros
+// cols and the next multiple of 8 are written as zeros, nothing behind them
 hipError_t launch_fp8_quantize(const void* x, int64_t rows, int64_t cols, int model_dtype, bool silu_mul, uint8_t* q,
                                int64_t q_pitch, float* scale, hipStream_t s);
 hipError_t launch_fp8_quantize_weight(const void* w, int64_t mats, int64_t N, int64_t K, int model_dtype, uint8_t* q,

@@ -46,10 +46,9 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const void* __restric
   }
   uint32_t bits;
   const uint2 out = fp8_group(f, &bits);
-  if (col < q_pitch) {  // pitch is a multiple of 16
-    *reinterpret_cast<uint2*>(q + row * q_pitch + col) = out;
-  }
-  if ((lane & 15) == 0 && col < cols) scale[static_cast<int64_t>(col / kFp8Block) * rows + row] = __builtin_bit_cast(float, bits);
+  if (col >= cols) return;  // (what a row holds from the next multiple of 8 on may be somebody's)
+  *reinterpret_cast<uint2*>(q + row * q_pitch + col) = out;
+  if ((lane & 15) == 0) scale[static_cast<int64_t>(col / kFp8Block) * rows + row] = __builtin_bit_cast(float, bits);
 }
 
 hipError_t launch_fp8_quantize(const void* x, int64_t rows, int64_t cols, int model_dtype, bool silu_mul, uint8_t* q,
@@ -105,7 +104,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_weight_kernel(const void* __
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int row = row0 + 16 * i;
-    if (row < N && col < q_pitch) {
+    if (row < N && col < K) {
       uint2 out;
       out.x = fp8_quad(f[i][0] * inv, f[i][1] * inv, f[i][2] * inv, f[i][3] * inv);
       out.y = fp8_quad(f[i][4] * inv, f[i][5] * inv, f[i][6] * inv, f[i][7] * inv);

@@ -83,3 +83,24 @@ def test_one_token_beyond_the_one_row_kernel(hidden, inter, dtype):
         assert "fp8_rows" in _lib.last_kernel() and written <= rest, (written, rest)
     else:  # gate and up apart from the activation
         assert "fp8_rows" in _lib.last_kernel() and written <= rest + 2 * both
+
+
+@pytest.mark.parametrize("rows,k,pitch", [(3, 128, 512), (5, 130, 400), (1, 1, 256), (4, 40, 48), (2, 600, 1600), (7, 136, 144)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantisers_write_their_own_bytes_alone(rows, k, pitch, dtype):
+    # rows in a wider buffer, whose other bytes belong to somebody: [K, the next multiple of 8) becomes zeros, the rest stays
+    x = torch.randn(rows, k, generator=_gen(k)).to(dtype).cuda()
+    both = torch.randn(rows, 2 * k, generator=_gen(k)).to(dtype).cuda()
+    up8 = -(-k // 8) * 8
+    scale = torch.empty(-(-k // 128) * max(rows, 128), device="cuda")
+    code, stream = ops._MODEL_DTYPES[dtype], ops._stream()
+    calls = {"mi355gq_fp8_quantize": lambda q: (x.data_ptr(), rows, k, code, q, pitch, scale.data_ptr(), stream),
+             "mi355gq_fp8_silu_mul_quantize": lambda q: (both.data_ptr(), rows, k, code, q, pitch, scale.data_ptr(), stream),
+             "mi355gq_fp8_quantize_weight": lambda q: (x.data_ptr(), 1, rows, k, code, q, pitch, scale.data_ptr(), stream)}
+    want = {"mi355gq_fp8_quantize": lambda: ops.fp8_quantize(x)[0], "mi355gq_fp8_silu_mul_quantize": lambda: ops.fp8_silu_mul_quantize(both)[0],
+            "mi355gq_fp8_quantize_weight": lambda: ops.fp8_quantize_weight(x)[0]}
+    for name, args in calls.items():
+        buf = torch.full((rows + 1, pitch), 0xA5, dtype=torch.uint8, device="cuda")
+        _lib.call(name, *args(buf.data_ptr()))
+        assert torch.equal(buf[:rows, :k], want[name]().view(torch.uint8)[:, :k]), name
+        assert (buf[:rows, k:up8] == 0).all() and (buf[:rows, up8:] == 0xA5).all() and (buf[rows] == 0xA5).all(), name
