@@ -21,22 +21,52 @@ def _weight(*shape, device=None) -> nn.Parameter:
     return nn.Parameter(torch.empty((*shape[:-1], -(-k // 16) * 16), dtype=torch.float8_e4m3fn, device=device)[..., :k], requires_grad=False)
 
 
+def _rows_apart(t: torch.Tensor) -> torch.Tensor:
+    """t, or where its rows are e4m3 and do not lie as _weight's do a copy that does."""
+    k = t.shape[-1] if t.dim() > 1 else 0
+    if t.dtype != torch.float8_e4m3fn or k % 16 == 0:
+        return t
+    like = _weight(*t.shape, device="meta")
+    if t.stride() == like.stride() and t.untyped_storage().nbytes() - t.storage_offset() >= like.untyped_storage().nbytes():
+        return t
+    return _weight(*t.shape, device=t.device).data.copy_(t)
+
+
 def _scale(*shape, device=None) -> nn.Parameter:
     blocks = (*shape[:-2], -(-shape[-2] // ops.FP8_BLOCK), -(-shape[-1] // ops.FP8_BLOCK))
     return nn.Parameter(torch.empty(blocks, dtype=torch.float32, device=device), requires_grad=False)
 
 
-class Fp8Linear(nn.Module):
+class _Fp8Weight(nn.Module):
+    """q_weight and q_scale of a linear or a stack of experts.  A row that is no multiple of 16 bytes long stands in a wider one, as a view that torch
+    makes dense where it copies or moves a module; the rows are put apart again there."""
+
+    def __init__(self, *shape, device=None):
+        super().__init__()
+        self.q_weight = _weight(*shape, device=device)
+        self.q_scale = _scale(*shape, device=device)
+
+    def _apply(self, fn, recurse=True):  # .to, .cuda, .to_empty, ...
+        return super()._apply(lambda t: _rows_apart(fn(t)), recurse)
+
+    def __setstate__(self, state):  # copy.deepcopy, pickle
+        super().__setstate__(state)
+        self.q_weight.data = _rows_apart(self.q_weight.data)
+
+    def _load_from_state_dict(self, *args, **kwargs):  # (assign=True takes the given tensors)
+        super()._load_from_state_dict(*args, **kwargs)
+        self.q_weight.data = _rows_apart(self.q_weight.data)
+
+
+class Fp8Linear(_Fp8Weight):
     """y = x . W^T (+ bias) (+ residual) with W in e4m3; out_dtype as in ops.fp8_linear."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, dtype: torch.dtype = torch.float16,
                  out_dtype: Optional[torch.dtype] = None, device=None):
-        super().__init__()
+        super().__init__(out_features, in_features, device=device)
         self.in_features = in_features
         self.out_features = out_features
         self.out_dtype = out_dtype
-        self.q_weight = _weight(out_features, in_features, device=device)
-        self.q_scale = _scale(out_features, in_features, device=device)
         self.bias = nn.Parameter(torch.empty((out_features,), dtype=dtype, device=device), requires_grad=False) if bias else None
 
     @staticmethod
@@ -68,11 +98,8 @@ class Fp8MoE(nn.Module):
         self.num_local_experts = num_local_experts
         self.routing = {"scoring": scoring, "num_groups": num_groups, "top_groups": top_groups, "renormalize": renormalize,
                         "scale": routed_scale}
-        for name, n, k in (("e1_e3", 2 * intermediate_size, hidden_size), ("e2", hidden_size, intermediate_size)):
-            stack = nn.Module()
-            stack.q_weight = _weight(num_local_experts, n, k, device=device)
-            stack.q_scale = _scale(num_local_experts, n, k, device=device)
-            setattr(self, name, stack)
+        self.e1_e3 = _Fp8Weight(num_local_experts, 2 * intermediate_size, hidden_size, device=device)
+        self.e2 = _Fp8Weight(num_local_experts, hidden_size, intermediate_size, device=device)
         self.score_bias = nn.Parameter(torch.zeros((num_local_experts,), dtype=torch.float32, device=device), requires_grad=False) \
             if score_bias else None
 

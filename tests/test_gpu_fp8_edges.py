@@ -104,3 +104,21 @@ def test_quantisers_write_their_own_bytes_alone(rows, k, pitch, dtype):
         _lib.call(name, *args(buf.data_ptr()))
         assert torch.equal(buf[:rows, :k], want[name]().view(torch.uint8)[:, :k]), name
         assert (buf[:rows, k:up8] == 0).all() and (buf[:rows, up8:] == 0xA5).all() and (buf[rows] == 0xA5).all(), name
+
+
+def test_layers_run_after_a_copy_and_a_move(tmp_path):
+    n, k = 72, 200  # rows of 200 bytes in 208
+    torch.manual_seed(0)
+    src = torch.nn.Linear(k, n, dtype=torch.float16, device="cuda")
+    linear = layers.Fp8Linear.from_linear(src)
+    x = torch.randn(3, k, device="cuda", dtype=torch.float16)
+    want = linear(x)
+    on_cpu = copy.deepcopy(linear).cpu()
+    fresh = layers.Fp8Linear(k, n, dtype=torch.float16)
+    fresh.load_state_dict(on_cpu.state_dict())
+    assigned = layers.Fp8Linear(k, n, dtype=torch.float16, device="cuda")
+    assigned.load_state_dict({name: v.clone() for name, v in linear.state_dict().items()}, assign=True)
+    torch.save(on_cpu, tmp_path / "layer.pt")
+    loaded = torch.load(tmp_path / "layer.pt", weights_only=False)  # (written above)
+    for other in (copy.deepcopy(linear), on_cpu.cuda(), fresh.cuda(), assigned, loaded.to("cuda")):
+        assert torch.equal(other(x), want)
