@@ -37,9 +37,19 @@ def _scale(*shape, device=None) -> nn.Parameter:
     return nn.Parameter(torch.empty(blocks, dtype=torch.float32, device=device), requires_grad=False)
 
 
+def _kept(fn, *fixed):
+    """fn of a module's _apply, which moves tensors and casts them: the `fixed` ones move and keep their type, which the kernels go by."""
+
+    def apply(t):
+        y = fn(t)
+        return _rows_apart(t.to(y.device) if y.dtype != t.dtype and any(t is f for f in fixed) else y)
+
+    return apply
+
+
 class _Fp8Weight(nn.Module):
-    """q_weight and q_scale of a linear or a stack of experts.  A row that is no multiple of 16 bytes long stands in a wider one, as a view that torch
-    makes dense where it copies or moves a module; the rows are put apart again there."""
+    """q_weight and q_scale of a linear or a stack of experts, whose types no cast of a model (.half(), .to(dtype)) changes.  A row that is no multiple
+    of 16 bytes long stands in a wider one, as a view that torch makes dense where it copies or moves a module; the rows are put apart again there."""
 
     def __init__(self, *shape, device=None):
         super().__init__()
@@ -47,7 +57,7 @@ class _Fp8Weight(nn.Module):
         self.q_scale = _scale(*shape, device=device)
 
     def _apply(self, fn, recurse=True):  # .to, .cuda, .to_empty, ...
-        return super()._apply(lambda t: _rows_apart(fn(t)), recurse)
+        return super()._apply(_kept(fn, self.q_weight, self.q_scale), recurse)
 
     def __setstate__(self, state):  # copy.deepcopy, pickle
         super().__setstate__(state)
@@ -102,6 +112,9 @@ class Fp8MoE(nn.Module):
         self.e2 = _Fp8Weight(num_local_experts, hidden_size, intermediate_size, device=device)
         self.score_bias = nn.Parameter(torch.zeros((num_local_experts,), dtype=torch.float32, device=device), requires_grad=False) \
             if score_bias else None
+
+    def _apply(self, fn, recurse=True):
+        return super()._apply(_kept(fn, self.score_bias), recurse)
 
     def load_experts(self, e1_e3: torch.Tensor, e2: torch.Tensor) -> None:
         """Quantise e1_e3 [experts, 2 inter, hidden] and e2 [experts, hidden, inter] (float16, bfloat16 or float32) into the layer."""

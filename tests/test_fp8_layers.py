@@ -68,3 +68,24 @@ def test_rows_of_a_layer_on_another_device():
     moe = copy.deepcopy(layers.Fp8MoE(250, 144, 3, 2))
     assert moe.e1_e3.q_weight.stride() == (288 * 256, 256, 1) and moe.e2.q_weight.stride() == (250 * 144, 144, 1)
     assert moe.to("meta").e1_e3.q_weight.stride() == (288 * 256, 256, 1)
+
+
+CASTS = {"half": lambda m: m.half(), "bfloat16": lambda m: m.to(torch.bfloat16), "float": lambda m: m.float(), "double": lambda m: m.double(),
+         "device and type": lambda m: m.to("cpu", torch.bfloat16), "type": lambda m: m.type(torch.float16), "meta": lambda m: m.to("meta", torch.float16),
+         "inside": lambda m: torch.nn.Sequential(torch.nn.Linear(3, 3), m).half()[1]}
+
+
+@pytest.mark.parametrize("cast", sorted(CASTS))
+def test_a_cast_leaves_weights_scales_and_the_choice_bias(cast):
+    linear, moe = _linear(), layers.Fp8MoE(256, 144, 3, 2, scoring="sigmoid", score_bias=True)
+    for p in moe.parameters():
+        _filled(p.data)
+    before = [{name: v.clone() for name, v in m.state_dict().items()} for m in (linear, moe)]
+    other = CASTS[cast](linear), CASTS[cast](moe)
+    assert other[0].q_weight.stride() == (208, 1)
+    bias_type = {"bfloat16": torch.bfloat16, "device and type": torch.bfloat16, "float": torch.float32, "double": torch.float64}.get(cast, torch.float16)
+    assert other[0].bias.dtype == bias_type  # this one has the model's type
+    for m, was in zip(other, before):
+        for name, v in m.state_dict().items():
+            if name != "bias":
+                assert v.dtype == was[name].dtype and (v.is_meta or _same(v, was[name]))

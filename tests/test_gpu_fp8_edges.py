@@ -122,3 +122,20 @@ def test_layers_run_after_a_copy_and_a_move(tmp_path):
     loaded = torch.load(tmp_path / "layer.pt", weights_only=False)  # (written above)
     for other in (copy.deepcopy(linear), on_cpu.cuda(), fresh.cuda(), assigned, loaded.to("cuda")):
         assert torch.equal(other(x), want)
+
+
+def test_layers_run_after_a_cast():
+    n, k = 72, 200
+    torch.manual_seed(0)
+    linear = layers.Fp8Linear.from_linear(torch.nn.Linear(k, n, dtype=torch.float16, device="cuda"))
+    x = torch.randn(3, k, device="cuda", dtype=torch.float16)
+    assert torch.equal(copy.deepcopy(linear).half()(x), linear(x))
+    both = copy.deepcopy(linear).to(torch.bfloat16)
+    assert both.bias.dtype == torch.bfloat16 and both(x.bfloat16()).dtype == torch.bfloat16
+    assert torch.equal(both(x.bfloat16()), ops.fp8_linear(x.bfloat16(), linear.q_weight, linear.q_scale, bias=linear.bias.bfloat16()))
+    moe = layers.Fp8MoE(256, 144, 4, 2, scoring="sigmoid", score_bias=True)
+    moe = moe.to("cuda", torch.float16)
+    moe.load_experts(torch.randn(4, 288, 256, device="cuda") * 0.05, torch.randn(4, 256, 144, device="cuda") * 0.05)
+    x, gate = torch.randn(5, 256, device="cuda", dtype=torch.float16), torch.randn(5, 4, device="cuda", dtype=torch.float16)
+    want = moe(x, gate)
+    assert torch.equal(copy.deepcopy(moe).half()(x, gate), want) and torch.equal(torch.nn.Sequential(moe).half()[0](x, gate), want)
