@@ -126,7 +126,9 @@ struct MoeWorkspace {
   float* y;
   int64_t bytes;
 };
-MoeWorkspace moe_workspace(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t top_k, void* base) {
+// `both`, gate and up in float32, is the largest piece by far: it is there only where no kernel quantises the activation as it comes up
+// (one token's is small; its first product leaves silu(gate) * up there).
+MoeWorkspace moe_workspace(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t top_k, int64_t w13_pitch, void* base) {
   const int64_t slots = T * top_k;
   Carver c{static_cast<char*>(base)};
   MoeWorkspace w;
@@ -135,7 +137,7 @@ MoeWorkspace moe_workspace(int64_t T, int64_t hidden, int64_t inter, int64_t exp
   w.row_token = c.take<int32_t>(slots);
   w.slot_row = c.take<int32_t>(slots);
   w.indptr = c.take<int32_t>(experts + 1);
-  w.both = c.take<float>(slots * 2 * inter);
+  w.both = c.take<float>(T == 1 || !gq::fp8_silu_takes(2 * inter, w13_pitch) ? slots * 2 * inter : 0);
   w.hq = c.take<uint8_t>(slots * inter);
   w.hs = c.take<float>(slots * groups_of(inter));
   w.y = c.take<float>(slots * hidden);
@@ -330,7 +332,7 @@ static bool moe_sizes_ok(int64_t T, int64_t hidden, int64_t inter, int64_t exper
 
 int64_t mi355gq_fp8_moe_workspace_bytes(int64_t T, int64_t hidden, int64_t inter, int64_t num_experts, int64_t top_k) {
   if (!moe_sizes_ok(T, hidden, inter, num_experts, top_k) || T == 0) return 0;
-  return moe_workspace(T, hidden, inter, num_experts, top_k, nullptr).bytes;
+  return moe_workspace(T, hidden, inter, num_experts, top_k, hidden, nullptr).bytes;
 }
 
 int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int64_t num_experts, int64_t top_k, const void* weights,
@@ -347,7 +349,7 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
   FP8_REQUIRE(x && weights && ids && w13 && w13_scale && w2 && w2_scale && out, "fp8_moe: null pointer");
   FP8_REQUIRE(aligned16(x) && aligned16(out) && aligned16(w13) && aligned16(w2) && aligned4(weights) && aligned4(ids) && aligned4(w13_scale) &&
                   aligned4(w2_scale), "fp8_moe: misaligned pointer (x, out and e4m3 tensors: 16 bytes)");
-  const MoeWorkspace ws = moe_workspace(T, hidden, inter, num_experts, top_k, workspace);
+  const MoeWorkspace ws = moe_workspace(T, hidden, inter, num_experts, top_k, w13_pitch, workspace);
   FP8_REQUIRE(workspace == nullptr || aligned16(workspace), "fp8_moe: workspace must be 16-byte aligned");
   if (workspace == nullptr || workspace_bytes < ws.bytes)
     return set_error(MI355GQ_ERR_WORKSPACE, "fp8_moe: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)ws.bytes);
@@ -414,24 +416,21 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
   a.precise = true;  // sums that are rounded to e4m3 again: an error of 1e-5 would move one in thousands by a sixteenth
   const bool by_rows = slots <= kFewRowsEach * segments;
   if (e == hipSuccess) {
-    hipError_t done;
-    if (by_rows) {
+    if (!gq::fp8_silu_takes(a.N, a.w_pitch)) {  // inter is no multiple of 128, mostly: product and activation apart
+      e = product(a, s);
+      if (e == hipSuccess) e = gq::launch_fp8_quantize(ws.both, slots, inter, MI355GQ_F32, true, ws.hq, inter, ws.hs, s);
+    } else if (by_rows) {
       gq::Fp8RowsArgs r = few_rows(a);
       r.q_out = ws.hq;
       r.scale_out = ws.hs;
-      done = gq::launch_fp8_rows(r, s);
+      e = gq::launch_fp8_rows(r, s);
     } else {
       a.q_out = ws.hq;
       a.scale_out = ws.hs;
-      done = gq::launch_fp8_tile(a, s);
+      e = gq::launch_fp8_tile(a, s);
       a.q_out = nullptr;
       a.scale_out = nullptr;
     }
-    if (done == hipErrorNotSupported) {  // inter is no multiple of 128: product and activation apart
-      done = product(a, s);
-      if (done == hipSuccess) done = gq::launch_fp8_quantize(ws.both, slots, inter, MI355GQ_F32, true, ws.hq, inter, ws.hs, s);
-    }
-    e = done;
   }
   a.precise = false;  // (the layer's output has 16 bits)
   a.x = ws.hq;

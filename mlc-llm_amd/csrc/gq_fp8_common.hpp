@@ -128,6 +128,11 @@ struct Fp8RowsArgs {
   uint8_t* q_out = nullptr;  // (launch_fp8_rows on quantised x) silu(first half) * second half quantised, [rows, N / 2] and its scales
   float* scale_out = nullptr;  // [N / 256, rows], instead of y; N / 2 a multiple of 128
 };
+// What the products take that quantise silu(first half) * second half in their epilogue (q_out), few rows and tiles: whole groups of the
+// activation, offsets into W in 32 bits.
+inline bool fp8_silu_takes(int64_t N, int64_t w_pitch) {
+  return N % (2 * kFp8Block) == 0 && static_cast<uint64_t>(N) * w_pitch < 0xffffffffull;
+}
 // Sixteen rows of a segment at a time; hipErrorNotSupported where the kernel does not apply.
 hipError_t launch_fp8_rows(const Fp8RowsArgs& a, hipStream_t s);
 // What the kernels of one row take: a row of K in registers, offsets into W in 32 bits.

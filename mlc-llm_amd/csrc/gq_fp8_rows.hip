@@ -307,7 +307,7 @@ static hipError_t launch_rows(const Fp8RowsArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_fp8_rows(const Fp8RowsArgs& a, hipStream_t s) {
-  if (a.K % 16 != 0 || (a.q_out != nullptr && a.N % (2 * kFp8Block) != 0) || static_cast<uint64_t>(a.N) * a.w_pitch >= 0xffffffffull)
+  if (a.K % 16 != 0 || static_cast<uint64_t>(a.N) * a.w_pitch >= 0xffffffffull || (a.q_out != nullptr && !fp8_silu_takes(a.N, a.w_pitch)))
     return hipErrorNotSupported;
   if (a.q_out != nullptr) return launch_rows<kXFp8, true>(a, s);
   if (a.x_kind == kXFp8) return launch_rows<kXFp8, false>(a, s);

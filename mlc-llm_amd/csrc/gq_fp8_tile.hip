@@ -566,7 +566,7 @@ int64_t fp8_tile_workspace_bytes(int64_t rows, int64_t N, int64_t K) {
 
 hipError_t launch_fp8_tile(const Fp8Args& a, hipStream_t s) {
   if (a.q_out != nullptr) {
-    if (a.N % (2 * kFp8Block) != 0 || static_cast<uint64_t>(a.N) * a.w_pitch >= 0xffffffffull) return hipErrorNotSupported;
+    if (!fp8_silu_takes(a.N, a.w_pitch)) return hipErrorNotSupported;
     // 64 rows in two workgroups a unit, or 192 in one: expert layers of 128 x 2048 x 768 at 64 rows an expert 227 / 246 us, at 128 312 / 327, at
     // 256 499 / 517; of 8 x 4096 x 14336 at 64 rows 387 / 396, at 192 689 / 727, at 256 852 / 822, at 384 1177 / 1125.  (A form of 128 rows,
     // whose waves widen a third more operands than 192's for a result, was behind one of them at all of these.)

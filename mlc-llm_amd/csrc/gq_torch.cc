@@ -371,7 +371,8 @@ PyObject* fp8_moe(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     rc = run_gating(g, &weights, &ids);
     if (rc == MI355GQ_OK) {
       out = at::empty(x->sizes(), x->options());
-      const int64_t bytes = mi355gq_fp8_moe_workspace_bytes(t, hidden, inter, experts, g.k);
+      int64_t bytes = mi355gq_fp8_moe_workspace_bytes(t, hidden, inter, experts, g.k);
+      if (2 * inter * p13 >= 0xffffffffll) bytes += 8 * t * g.k * inter + 256;
       Scratch scratch(*x, bytes);
       rc = mi355gq_fp8_moe(x->const_data_ptr(), t, hidden, inter, experts, g.k, weights.const_data_ptr(), ids.const_data_ptr(),
                            w13->const_data_ptr(), p13, s13->const_data_ptr(), w2->const_data_ptr(), p2, s2->const_data_ptr(), code,

@@ -901,6 +901,8 @@ def fp8_moe_experts(x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, w
     k = ids.shape[1]
     out = torch.empty_like(x)
     ws_bytes = _lib.lib().mi355gq_fp8_moe_workspace_bytes(t, hidden, inter, ne, k)
+    if ws_bytes and 2 * inter * pitch13 >= 2**32 - 1:
+        ws_bytes += 8 * t * k * inter + 256
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
     _lib.call("mi355gq_fp8_moe", x.data_ptr(), t, hidden, inter, ne, k, weights.data_ptr(), ids.data_ptr(), w13.data_ptr(), pitch13,
               w13_scale.data_ptr(), w2.data_ptr(), pitch2, w2_scale.data_ptr(), _MODEL_DTYPES[x.dtype], out.data_ptr(),

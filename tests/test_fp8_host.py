@@ -157,3 +157,25 @@ def test_layers_hold_weights_of_padded_rows():
     assert not any(p.requires_grad for p in moe.parameters())
     with pytest.raises(ValueError, match="expected"):
         moe.load_experts(torch.zeros(5, 544, 128), torch.zeros(5, 256, 272))
+
+
+def test_layer_workspace_holds_what_the_call_uses():
+    lib = _lib.lib()
+    size = lib.mi355gq_fp8_moe_workspace_bytes
+
+    def pieces(t, hidden, inter, experts, k):
+        """x and the activation in e4m3 with their scales, the plan, the second product in float32; nine pieces of multiples of 256."""
+        slots = t * k
+        return (t * hidden + slots * inter + 4 * (t * -(-hidden // 128) + slots * -(-inter // 128) + 2 * slots + experts + 1 + slots * hidden) + 9 * 256)
+
+    # gate and up in float32, the largest piece by far, where the activation is not quantised as it comes up: 8 slots * inter bytes
+    for case in ((2048, 4096, 14336, 8, 2), (2048, 2048, 768, 128, 8), (16, 2048, 768, 128, 8), (2, 256, 128, 4, 1)):
+        assert 0 < size(*case) <= pieces(*case)
+    for case in ((2048, 4096, 14320, 8, 2), (16, 2048, 144, 64, 6), (1, 2048, 1408, 64, 6), (2, 16384, 131072, 1, 1)):
+        assert pieces(*case) - 9 * 256 <= size(*case) - 8 * case[0] * case[4] * case[2] <= pieces(*case)
+    # rows of gate and up so far apart that an expert's reach 4 GiB
+    f16 = _codes()[0]
+    need = size(40, 256, 256, 2, 1)
+    pitch = (1 << 23) + 16
+    for given in (need, need + 8 * 40 * 256 - 1):
+        assert lib.mi355gq_fp8_moe(X, 40, 256, 256, 2, 1, XS, Y, W, pitch, WS, W, 256, WS, f16, Y, Z, given, None) == _lib.ERR_WORKSPACE

@@ -139,3 +139,23 @@ def test_layers_run_after_a_cast():
     x, gate = torch.randn(5, 256, device="cuda", dtype=torch.float16), torch.randn(5, 4, device="cuda", dtype=torch.float16)
     want = moe(x, gate)
     assert torch.equal(copy.deepcopy(moe).half()(x, gate), want) and torch.equal(torch.nn.Sequential(moe).half()[0](x, gate), want)
+
+
+def test_layer_whose_expert_spans_four_gib_by_its_pitch():
+    # rows of gate and up far apart: neither fused form reaches them, product and activation go apart and need the scratch for it
+    t, hidden, inter, pitch = 40, 256, 256, (1 << 23) + 16
+    layer = ExactLayer(t, hidden, inter, 1, torch.zeros(t, 1), torch.float16)
+    wide = torch.empty(2 * inter * pitch, dtype=torch.uint8, device="cuda").view(E4M3).as_strided((1, 2 * inter, hidden), (2 * inter * pitch, pitch, 1))
+    assert 2 * inter * pitch > 2**32
+    wide.copy_(layer.w13)
+    want = layer.run()
+    layer.w13 = wide
+    got = layer.run()
+    assert torch.equal(got, want)
+    layer.check(got, eight_bit=True)
+    # the router and the layer in one call
+    logits = torch.zeros(t, 1, device="cuda")
+    assert torch.equal(ops.fp8_moe(layer.x, logits, wide, layer.s13, layer.w2, layer.s2, 1),
+                       ops.fp8_moe_experts(layer.x, torch.ones(t, 1, device="cuda"), layer.ids, wide, layer.s13, layer.w2, layer.s2))
+    layer.x, layer.ids, layer.weights = layer.x[:1], layer.ids[:1], layer.weights[:1]  # one token
+    layer.check(layer.run())
