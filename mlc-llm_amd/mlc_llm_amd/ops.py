@@ -671,15 +671,19 @@ def _chk_fp8(t: torch.Tensor, name: str, dims: int) -> int:
         raise TypeError(f"{name}: dtype {t.dtype}, expected {_E4M3}")
     if t.dim() != dims:
         raise ValueError(f"{name}: {t.dim()} dimensions, expected {dims}")
-    k = t.shape[-1]
-    pitch = t.stride(-2) if t.shape[-2] > 1 else max(t.stride(-2), -(-k // 16) * 16)
+    n, k = t.shape[-2:]
+    row = -(-k // 16) * 16  # what the kernels' loads touch of one
+    if n > 1:
+        pitch = t.stride(-2)
+    else:  # (of a single row the stride says nothing)
+        pitch = t.stride(0) if dims == 3 and t.shape[0] > 1 else row
     if t.numel() and ((k > 1 and t.stride(-1) != 1) or pitch < k or pitch % 16
-                      or (dims == 3 and t.shape[0] > 1 and t.stride(0) != t.shape[1] * pitch)):
+                      or (dims == 3 and t.shape[0] > 1 and t.stride(0) != n * pitch)):
         raise ValueError(f"{name}: rows must be contiguous and lie a multiple of 16 bytes apart (strides {t.stride()}); "
                          "fp8_quantize_weight makes such a tensor, torch.nn.functional.pad one of a checkpoint's")
-    if t.numel() and t.shape[-2] == 1 and k % 16 and t.untyped_storage().nbytes() - t.storage_offset() < pitch:
-        raise ValueError(f"{name}: a row of {k} bytes needs {pitch} of storage")
-    return max(pitch, -(-k // 16) * 16)
+    if t.numel() and t.untyped_storage().nbytes() - t.storage_offset() < (t.numel() // k - 1) * pitch + row:
+        raise ValueError(f"{name}: the last row of {k} bytes needs {row} of storage")
+    return max(pitch, row)
 
 
 def _chk_scale(t: torch.Tensor, shape, name: str) -> torch.Tensor:

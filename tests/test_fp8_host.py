@@ -179,3 +179,30 @@ def test_layer_workspace_holds_what_the_call_uses():
     pitch = (1 << 23) + 16
     for given in (need, need + 8 * 40 * 256 - 1):
         assert lib.mi355gq_fp8_moe(X, 40, 256, 256, 2, 1, XS, Y, W, pitch, WS, W, 256, WS, f16, Y, Z, given, None) == _lib.ERR_WORKSPACE
+
+
+class _OnGpu(torch.Tensor):
+    """A CPU tensor that passes for one on the GPU, for checks that look at strides alone."""
+
+    is_cuda = True
+
+
+def _strided(nbytes, shape, strides, offset=0):
+    return torch.zeros(nbytes, dtype=torch.uint8).view(torch.float8_e4m3fn).as_strided(shape, strides, offset).as_subclass(_OnGpu)
+
+
+@pytest.mark.parametrize("nbytes,shape,strides,offset,pitch", [
+    (5 * 208, (5, 200), (208, 1), 0, 208), (4 * 208 + 200, (5, 200), (208, 1), 0, None), (4 * 208 + 207, (5, 200), (208, 1), 0, None),
+    (5 * 208 + 16, (5, 200), (208, 1), 16, 208), (5 * 208 + 15, (5, 200), (208, 1), 16, None), (4 * 208 + 192, (5, 192), (208, 1), 0, 208),
+    (200, (1, 200), (208, 1), 0, None), (208, (1, 200), (208, 1), 0, 208), (208, (1, 200), (200, 1), 0, 208),
+    # the last row of a wider matrix, some of its columns: what lies behind them in the pitch is not theirs and is not needed
+    (4 * 4096, (1, 88), (4096, 1), 3 * 4096 + 4000, 96), (4 * 130, (1, 128), (130, 1), 0, 128),
+    (3 * 208, (3, 1, 200), (208, 208, 1), 0, 208), (2 * 208 + 200, (3, 1, 200), (208, 208, 1), 0, None), (3 * 512, (3, 1, 128), (512, 7, 1), 0, 512),
+    (6 * 112, (3, 2, 100), (224, 112, 1), 0, 112), (6 * 112 - 1, (3, 2, 100), (224, 112, 1), 0, None), (3 * 240, (3, 2, 100), (240, 112, 1), 0, None),
+    (5 * 200, (5, 200), (200, 1), 0, None), (5 * 208, (5, 200), (208, 0), 0, None), (208, (5, 200), (0, 1), 0, None), (0, (0, 200), (200, 1), 0, 208)])
+def test_rows_of_e4m3_lie_in_their_storage(nbytes, shape, strides, offset, pitch):
+    if pitch is None:
+        with pytest.raises(ValueError, match="of storage|multiple of 16 bytes apart"):
+            ops._chk_fp8(_strided(nbytes, shape, strides, offset), "q", len(shape))
+    else:
+        assert ops._chk_fp8(_strided(nbytes, shape, strides, offset), "q", len(shape)) == pitch

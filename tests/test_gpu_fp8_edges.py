@@ -159,3 +159,17 @@ def test_layer_whose_expert_spans_four_gib_by_its_pitch():
                        ops.fp8_moe_experts(layer.x, torch.ones(t, 1, device="cuda"), layer.ids, wide, layer.s13, layer.w2, layer.s2))
     layer.x, layer.ids, layer.weights = layer.x[:1], layer.ids[:1], layer.weights[:1]  # one token
     layer.check(layer.run())
+
+
+def test_linear_on_one_row_of_a_wider_matrix():
+    # a single row's stride says nothing: columns of a matrix's last row, whose pitch the row's own bytes do not fill
+    x = torch.randn(7, 256, generator=_gen(2)).half().cuda()
+    q, s = ops.fp8_quantize(x)
+    wide = torch.zeros(7, 4096, dtype=torch.uint8, device="cuda").view(E4M3)
+    wide[:, 3840:] = q
+    w, ws = (v.cuda() for v in _weights(64, 256, 1))
+    want = ops.fp8_linear((q, s), w, ws)
+    last = ops.fp8_linear((wide[6:7, 3840:], s[:, 6:7].contiguous()), w, ws)
+    assert torch.equal(last, ops.fp8_linear((q[6:7].contiguous(), s[:, 6:7].contiguous()), w, ws))
+    assert ((last - want[6:7]).abs() <= 2.0**-9 * want[6:7].abs() + 2.0**-10).all()
+    assert torch.equal(ops.fp8_dequantize(wide[6:7, 3840:], s[:, 6:7].contiguous(), row_groups=True), ops.fp8_dequantize(q, s, row_groups=True)[6:7])
