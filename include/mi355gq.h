@@ -518,7 +518,7 @@ MI355GQ_API int mi355gq_moe_gating(const void* logits, const void* bias, int64_t
 /*
  * ids int32 [T, top_k] -> the slots t * top_k + j in the order of their expert, slot order within one: row_token int32 [T * top_k]
  * (the token of each row), slot_row int32 [T * top_k] (the row of each slot; -1 for an id outside the experts, which has
- * none), indptr int32 [num_experts + 1].
+ * none), indptr int32 [num_experts + 1].  T * top_k <= 2^31 - 2304.
  */
 MI355GQ_API int mi355gq_moe_plan(const void* ids, int64_t T, int64_t top_k, int64_t num_experts, void* row_token,
                      void* slot_row, void* indptr, mi355gq_stream_t stream);

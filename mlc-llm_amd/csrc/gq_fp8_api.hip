@@ -14,6 +14,7 @@ using gq::set_error;
 
 constexpr int64_t kMaxDim = (int64_t(1) << 31) - 256;
 constexpr int64_t kMaxTiles = 65535;
+constexpr int64_t kMaxSlots = kMaxDim - 2048;  // (moe_plan_kernel's waves count up to 1342 past the last slot, in 32 bits)
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
@@ -316,7 +317,7 @@ int mi355gq_moe_gating(const void* logits, const void* bias, int64_t T, int64_t 
 
 int mi355gq_moe_plan(const void* ids, int64_t T, int64_t top_k, int64_t num_experts, void* row_token, void* slot_row, void* indptr,
                      mi355gq_stream_t stream) {
-  FP8_REQUIRE(dim_ok(T) && top_k > 0 && top_k <= 512 && T <= kMaxDim / top_k && num_experts > 0 && num_experts <= 512,
+  FP8_REQUIRE(dim_ok(T) && top_k > 0 && top_k <= 512 && T <= kMaxSlots / top_k && num_experts > 0 && num_experts <= 512,
               "moe_plan: T=%lld, top_k=%lld, num_experts=%lld (1..512)", (long long)T, (long long)top_k, (long long)num_experts);
   FP8_REQUIRE(indptr && (T == 0 || (ids && row_token && slot_row)), "moe_plan: null pointer");
   FP8_REQUIRE(aligned4(ids) && aligned4(row_token) && aligned4(slot_row) && aligned4(indptr), "moe_plan: misaligned pointer");

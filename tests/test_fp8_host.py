@@ -206,3 +206,18 @@ def test_rows_of_e4m3_lie_in_their_storage(nbytes, shape, strides, offset, pitch
             ops._chk_fp8(_strided(nbytes, shape, strides, offset), "q", len(shape))
     else:
         assert ops._chk_fp8(_strided(nbytes, shape, strides, offset), "q", len(shape)) == pitch
+
+
+@pytest.mark.parametrize("t,k", [((1 << 31) - 300, 1), ((1 << 31) - 1500, 1), ((1 << 30) - 600, 2)])
+def test_plan_refuses_slots_that_its_waves_cannot_count(t, k):
+    # a wave's run is a multiple of 64 slots, and the last ones end behind the slots: past 2^31 there a wave would see none of its own
+    _refused(_lib.lib().mi355gq_moe_plan(X, t, k, 8, Y, Z, W, None), "moe_plan")
+
+
+def test_plan_counts_in_32_bits():
+    largest = (1 << 31) - 256 - 2048
+    for slots in (largest, largest - 1, largest // 2):
+        waves = 16
+        per_wave = ((slots + waves - 1) // waves + 63) // 64 * 64
+        begin, end = (waves - 1) * per_wave, min(waves * per_wave, slots)
+        assert waves * per_wave < 2**31 and begin + 4 * 64 < 2**31 and end + 64 + 63 < 2**31
