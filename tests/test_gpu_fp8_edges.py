@@ -173,3 +173,66 @@ def test_linear_on_one_row_of_a_wider_matrix():
     assert torch.equal(last, ops.fp8_linear((q[6:7].contiguous(), s[:, 6:7].contiguous()), w, ws))
     assert ((last - want[6:7]).abs() <= 2.0**-9 * want[6:7].abs() + 2.0**-10).all()
     assert torch.equal(ops.fp8_dequantize(wide[6:7, 3840:], s[:, 6:7].contiguous(), row_groups=True), ops.fp8_dequantize(q, s, row_groups=True)[6:7])
+
+
+@pytest.mark.parametrize("counts,n,k,form", [([40, 0, 0, 0, 0, 0], 64, 2048, "4 blocks x 4 waves, 1 phases"), ([0, 17, 1, 0, 0, 0, 33, 0], 200, 272, None),
+                                             ([0, 17, 1, 0, 0, 0, 33, 0], 130, 14336, "2 phases"), ([0] * 15 + [90], 1032, 1040, None),
+                                             ([48, 0, 0, 0, 0, 0], 136, 20480, "phases"), ([16, 32, 0, 0, 0, 0, 0, 1], 36, 16, None)])
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("out", DTYPES)
+def test_segments_of_several_passes(counts, n, k, form, gather, out):
+    rows, experts = sum(counts), len(counts)
+    w, ws = _weights(n, k, 13, experts)
+    indptr = torch.tensor([0] + counts).cumsum(0).to(torch.int32)
+    source = max(rows // 3, 1) if gather else rows
+    x = torch.randn(source, k, generator=_gen(rows + k)).to(torch.bfloat16)
+    index = torch.randint(0, source, (rows,), generator=_gen(1), dtype=torch.int32) if gather else None
+    q, s = ops.fp8_quantize(x.cuda())
+    y = ops.fp8_group_gemm(q, s, index.cuda() if gather else None, w.cuda()[..., :k], ws.cuda(), indptr.cuda(), out).cpu().double()
+    assert "fp8_rows" in _lib.last_kernel()
+    if form == "phases":
+        assert "1 phases" not in _lib.last_kernel()
+    elif form:
+        assert form in _lib.last_kernel()
+    xv = quantized(x.double())[2]
+    xv = xv[index.long()] if gather else xv
+    for e in range(experts):
+        part = slice(int(indptr[e]), int(indptr[e + 1]))
+        wv = block_values(w[e, :, :k].float().nan_to_num(), ws[e])
+        exact = xv[part] @ wv.t()
+        assert ((y[part] - exact).abs() <= _linear_bound(xv[part], wv, exact, out)).all()
+
+
+def _skewed(t, ne, k, first):
+    """Expert `first` for every token, the others spread."""
+    others = [e for e in range(ne) if e != first]
+    return torch.tensor([[first] + [others[(i * (k - 1) + j) % len(others)] for j in range(k - 1)] for i in range(t)])
+
+
+@pytest.mark.parametrize("t,hidden,inter,ne,ids,few", [
+    (1, 512, 256, 8, _skewed(1, 8, 3, 5), True), (4, 512, 256, 8, _skewed(4, 8, 2, 0), True), (16, 256, 384, 64, _skewed(16, 64, 4, 63), True),
+    (40, 256, 128, 64, _skewed(40, 64, 1, 7), True), (50, 384, 256, 96, _skewed(50, 96, 2, 3), True), (36, 9344, 128, 40, _skewed(36, 40, 1, 9), True),
+    (40, 272, 144, 64, _skewed(40, 64, 1, 7), True), (70, 256, 128, 6, _skewed(70, 6, 2, 2), False), (300, 512, 256, 4, _skewed(300, 4, 1, 1), False),
+    (130, 272, 144, 5, _skewed(130, 5, 2, 4), False)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_layer_rounds_once(t, hidden, inter, ne, ids, few, dtype):
+    # skewed routing: one expert has all tokens, several passes of the few-row kernel (9344: x of a pass in two phases) or many tiles
+    layer = ExactLayer(t, hidden, inter, ne, ids, dtype, top=8 if hidden < 8192 else 4)
+    layer.check(layer.run(), eight_bit=not few)
+
+
+@pytest.mark.parametrize("m", [2, 3, 7, 12])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [torch.inf, -torch.inf, torch.nan])
+def test_few_rows_keep_what_is_not_finite_in_its_row(m, dtype, bad):
+    for n, k in ((256, 512), (1000, 1040)):
+        w, ws = (v.cuda() for v in _weights(n, k, 5))
+        x = torch.randn(m, k, generator=_gen(6)).to(dtype)
+        clean = ops.fp8_linear(x.cuda(), w, ws)
+        assert "fp8_rows" in _lib.last_kernel()
+        for row, at in ((0, 300), (m - 1, k - 1)):
+            dirty = x.clone()
+            dirty[row, at] = bad
+            for y in (ops.fp8_linear(dirty.cuda(), w, ws), ops.fp8_linear(ops.fp8_quantize(dirty.cuda()), w, ws, out_dtype=dtype)):
+                rest = [r for r in range(m) if r != row]
+                assert y[row].isnan().all() and torch.equal(y[rest], clean[rest])
