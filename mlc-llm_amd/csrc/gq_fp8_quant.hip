@@ -25,13 +25,17 @@ __device__ __forceinline__ void load8_row(const void* p, int64_t row0, int col, 
 
 }  // namespace
 
+// A launch of 2^32 or more work items loses all but the rest of that division, without an error: the row kernels, four rows a workgroup of 256,
+// take this many at most.
+constexpr int64_t kRowsALaunch = int64_t(1) << 25;
+
 // A wave takes four groups of a row at a time: 16 lanes a group, eight numbers a lane, the group's maximum by four DPP steps.
 template <int DT, bool SILU, bool ALIGNED>
-__global__ __launch_bounds__(256) void fp8_quantize_kernel(const void* __restrict__ x, int64_t rows, int cols,
+__global__ __launch_bounds__(256) void fp8_quantize_kernel(const void* __restrict__ x, int64_t row0, int64_t rows, int cols,
                                                            uint8_t* __restrict__ q, int64_t q_pitch,
                                                            float* __restrict__ scale) {
   const int lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t row = row0 + static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
   const int col = blockIdx.y * 512 + lane * 8;
   float f[8];
@@ -54,10 +58,13 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const void* __restric
 hipError_t launch_fp8_quantize(const void* x, int64_t rows, int64_t cols, int model_dtype, bool silu_mul, uint8_t* q,
                                int64_t q_pitch, float* scale, hipStream_t s) {
   const bool aligned = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
-  const dim3 grid(static_cast<unsigned>((rows + 3) / 4), static_cast<unsigned>((cols + 511) / 512));
   auto go = [&](auto dt, auto silu, auto al) {
-    hipLaunchKernelGGL((fp8_quantize_kernel<decltype(dt)::value, decltype(silu)::value, decltype(al)::value>), grid, dim3(256),
-                       0, s, x, rows, static_cast<int>(cols), q, q_pitch, scale);
+    for (int64_t row0 = 0; row0 < rows; row0 += kRowsALaunch) {
+      const int64_t here = rows - row0 < kRowsALaunch ? rows - row0 : kRowsALaunch;
+      const dim3 grid(static_cast<unsigned>((here + 3) / 4), static_cast<unsigned>((cols + 511) / 512));
+      hipLaunchKernelGGL((fp8_quantize_kernel<decltype(dt)::value, decltype(silu)::value, decltype(al)::value>), grid, dim3(256),
+                         0, s, x, row0, rows, static_cast<int>(cols), q, q_pitch, scale);
+    }
   };
   auto by_form = [&](auto dt) {
     if (silu_mul) {
@@ -147,9 +154,9 @@ hipError_t launch_fp8_quantize_weight(const void* w, int64_t mats, int64_t N, in
 // [mats, ceil(rows / 128), ceil(cols / 128)] (weights).
 template <int DT, bool ROWS>
 __global__ __launch_bounds__(256) void fp8_dequantize_kernel(const uint8_t* __restrict__ q, int64_t q_pitch,
-                                                             const float* __restrict__ scale, int64_t rows_all, int64_t rows,
-                                                             int cols, void* __restrict__ out) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+                                                             const float* __restrict__ scale, int64_t row0, int64_t rows_all,
+                                                             int64_t rows, int cols, void* __restrict__ out) {
+  const int64_t row = row0 + static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int col = blockIdx.y * 512 + (threadIdx.x & 63) * 8;
   if (row >= rows_all || col >= cols) return;
   const int64_t mat = ROWS ? 0 : row / rows;
@@ -173,10 +180,13 @@ __global__ __launch_bounds__(256) void fp8_dequantize_kernel(const uint8_t* __re
 
 hipError_t launch_fp8_dequantize(const uint8_t* q, int64_t q_pitch, const float* scale, int64_t mats, int64_t rows,
                                  int64_t cols, bool row_groups, int out_dtype, void* out, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>((mats * rows + 3) / 4), static_cast<unsigned>((cols + 511) / 512));
   auto go = [&](auto dt, auto by_row) {
-    hipLaunchKernelGGL((fp8_dequantize_kernel<decltype(dt)::value, decltype(by_row)::value>), grid, dim3(256), 0, s, q, q_pitch,
-                       scale, mats * rows, rows, static_cast<int>(cols), out);
+    for (int64_t row0 = 0; row0 < mats * rows; row0 += kRowsALaunch) {
+      const int64_t here = mats * rows - row0 < kRowsALaunch ? mats * rows - row0 : kRowsALaunch;
+      const dim3 grid(static_cast<unsigned>((here + 3) / 4), static_cast<unsigned>((cols + 511) / 512));
+      hipLaunchKernelGGL((fp8_dequantize_kernel<decltype(dt)::value, decltype(by_row)::value>), grid, dim3(256), 0, s, q, q_pitch,
+                         scale, row0, mats * rows, rows, static_cast<int>(cols), out);
+    }
   };
   auto by_form = [&](auto dt) {
     if (row_groups) go(dt, std::true_type{});

@@ -236,3 +236,28 @@ def test_few_rows_keep_what_is_not_finite_in_its_row(m, dtype, bad):
             for y in (ops.fp8_linear(dirty.cuda(), w, ws), ops.fp8_linear(ops.fp8_quantize(dirty.cuda()), w, ws, out_dtype=dtype)):
                 rest = [r for r in range(m) if r != row]
                 assert y[row].isnan().all() and torch.equal(y[rest], clean[rest])
+
+
+def test_more_rows_than_a_grid_holds():
+    # four rows a workgroup of 256: from 2^26 rows on a launch's grid would leave 32 bits
+    rows, k = (1 << 26) + 5, 16
+    assert (rows + 3) // 4 * 256 > 2**32
+    x = torch.randn(rows, k, device="cuda", dtype=torch.bfloat16)
+    q, s = ops.fp8_quantize(x)
+    back = ops.fp8_dequantize(q, s, torch.bfloat16, row_groups=True)
+    for part in (slice(0, 300), slice(rows // 2 - 100, rows // 2 + 100), slice(rows - 300, rows)):
+        want_q, want_s, want_v = quantized(x[part].cpu().double())
+        assert torch.equal(s[0, part].cpu().double(), want_s[:, 0]) and torch.equal(q[part].cpu().double(), want_q)
+        assert torch.equal(back[part].cpu(), want_v.float().bfloat16())
+    # everything, by the definition of the scale: within half a step of the value, and no smaller scale would do
+    for part in torch.arange(0, rows, 1 << 23).tolist():
+        end = min(part + (1 << 23), rows)
+        v, top, sc = x[part:end].float(), x[part:end].float().abs().amax(1), s[0, part:end]
+        assert ((top <= 448 * sc) & ((top > 224 * sc) | (top == 0))).all()
+        assert ((back[part:end].float() - v).abs() <= v.abs() * (2.0**-4 + 2.0**-8) + sc[:, None] * 2.0**-9).all()
+    del x, back
+    both = torch.randn(rows, 2 * k, device="cuda", dtype=torch.float16)
+    q, s = ops.fp8_silu_mul_quantize(both)
+    part = slice(rows - 300, rows)
+    q2, s2 = ops.fp8_silu_mul_quantize(both[part].contiguous())
+    assert torch.equal(q[part].view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s[:, part], s2)
