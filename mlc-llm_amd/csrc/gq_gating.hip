@@ -198,10 +198,14 @@ __global__ __launch_bounds__(64) void gating_kernel(const void* __restrict__ log
 hipError_t launch_moe_gating(const GatingArgs& a, hipStream_t s) {
   const int size = a.E / a.groups;
   const int vec = a.E % 8 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0;
+  constexpr int64_t kTokensALaunch = int64_t(1) << 26;  // (32 work items each; 2^32 of them would wrap, without an error)
   auto go = [&](auto nc, auto dt) {
-    hipLaunchKernelGGL((gating_kernel<decltype(nc)::value, decltype(dt)::value>), dim3(static_cast<unsigned>((a.T + 1) / 2)), dim3(64), 0, s,
-                       a.logits, a.bias, a.T, a.E, a.k, a.sigmoid, a.groups, a.top_groups, ((1 << 20) + size - 1) / size, a.renormalize,
-                       a.scale, vec, a.weights, a.ids);
+    for (int64_t t0 = 0; t0 < a.T; t0 += kTokensALaunch) {
+      const int64_t here = a.T - t0 < kTokensALaunch ? a.T - t0 : kTokensALaunch;
+      hipLaunchKernelGGL((gating_kernel<decltype(nc)::value, decltype(dt)::value>), dim3(static_cast<unsigned>((here + 1) / 2)), dim3(64), 0, s,
+                         static_cast<const char*>(a.logits) + t0 * a.E * (a.model_dtype == MODEL_F32 ? 4 : 2), a.bias, here, a.E, a.k, a.sigmoid,
+                         a.groups, a.top_groups, ((1 << 20) + size - 1) / size, a.renormalize, a.scale, vec, a.weights + t0 * a.k, a.ids + t0 * a.k);
+    }
   };
   auto by_type = [&](auto nc) {
     if (a.model_dtype == MODEL_F32) go(nc, std::integral_constant<int, MODEL_F32>{});

@@ -261,3 +261,14 @@ def test_more_rows_than_a_grid_holds():
     part = slice(rows - 300, rows)
     q2, s2 = ops.fp8_silu_mul_quantize(both[part].contiguous())
     assert torch.equal(q[part].view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s[:, part], s2)
+
+
+def test_more_tokens_than_a_grid_holds():
+    # 32 work items a token: from 2^27 tokens on a launch's grid would leave 32 bits
+    t = (1 << 27) + 5
+    logits = torch.randint(-3, 4, (t, 2), device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    weights, ids = ops.moe_gating(logits, 1, "sigmoid", renormalize=False)
+    for part in torch.arange(0, t, 1 << 24).tolist():
+        a, b = logits[part : part + (1 << 24)].float().unbind(1)
+        assert torch.equal(ids[part : part + (1 << 24), 0], (b > a).int())  # ties keep the lower index
+        assert ((weights[part : part + (1 << 24), 0] - torch.sigmoid(torch.maximum(a, b))).abs() <= 2.0**-21).all()
