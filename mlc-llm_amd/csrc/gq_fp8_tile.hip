@@ -519,7 +519,8 @@ hipError_t launch_tile(const Fp8Args& a, const Plan& plan, int part, hipStream_t
   const int64_t m_tiles = a.indptr ? a.rows / BM + a.experts : (a.rows + BM - 1) / BM;
   const int64_t n_first = part == 0 ? 0 : plan.n_rest, n_end = part == 0 && plan.n_rest > 0 ? plan.n_rest : a.N, n_tiles = (n_end - n_first + BN - 1) / BN;
   int splits = 1, per_split = static_cast<int>(groups);
-  if (plan.splits > 1 && a.workspace != nullptr && a.workspace_bytes >= plan.splits * a.rows * a.N * 4) {
+  const int64_t joined = a.rows * ((a.N + 3) / 4);  // work items of the join; 2^32 or more in a launch would wrap, without an error
+  if (plan.splits > 1 && a.workspace != nullptr && a.workspace_bytes >= plan.splits * a.rows * a.N * 4 && joined < 0xffffff00ll) {
     splits = plan.splits;
     per_split = plan.per_split;
   }
@@ -529,10 +530,13 @@ hipError_t launch_tile(const Fp8Args& a, const Plan& plan, int part, hipStream_t
     if (e != hipSuccess) return e;
   }
   note_kernel("fp8_tile %dx%d%s, %d shares of K", BN, BM, PRECISE ? " float32 sums" : "", splits);
-  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((n_tiles * m_tiles + 7) / 8 * 8), splits), dim3(64 * WN * WM), lds, s, a,
-                     static_cast<int>(n_first), static_cast<int>(n_tiles), static_cast<int>(m_tiles), per_split);
-  if (splits > 1)
-    hipLaunchKernelGGL(fp8_join_kernel, dim3(static_cast<unsigned>((a.rows * ((a.N + 3) / 4) + 255) / 256)), dim3(256), 0, s, a, splits);
+  const int64_t most = (0xffffffffll / (64 * WN * WM) - 8) / m_tiles;  // columns of tiles a launch, likewise (m_tiles is 65535 at most)
+  for (int64_t t0 = 0; t0 < n_tiles; t0 += most) {
+    const int64_t here = n_tiles - t0 < most ? n_tiles - t0 : most;
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((here * m_tiles + 7) / 8 * 8), splits), dim3(64 * WN * WM), lds, s, a,
+                       static_cast<int>(n_first + t0 * (SILU ? BN / 2 : BN)), static_cast<int>(here), static_cast<int>(m_tiles), per_split);
+  }
+  if (splits > 1) hipLaunchKernelGGL(fp8_join_kernel, dim3(static_cast<unsigned>((joined + 255) / 256)), dim3(256), 0, s, a, splits);
   return hipGetLastError();
 }
 

@@ -272,3 +272,23 @@ def test_more_tokens_than_a_grid_holds():
         a, b = logits[part : part + (1 << 24)].float().unbind(1)
         assert torch.equal(ids[part : part + (1 << 24), 0], (b > a).int())  # ties keep the lower index
         assert ((weights[part : part + (1 << 24), 0] - torch.sigmoid(torch.maximum(a, b))).abs() <= 2.0**-21).all()
+
+
+def test_more_tiles_than_a_grid_holds():
+    # 512 experts, all but the first without rows, and so many columns that 512 tiles a column of 128 are 2^32 work items and more.  K = 8 is the
+    # tiles', whatever the number of rows.  Only the first expert's weights are there: nothing reads the others'.
+    rows, n, k, experts = 3, 4300000, 8, 512
+    assert -(-n // 128) * experts * 256 > 2**32
+    x = torch.randint(-8, 9, (rows, k), device="cuda").half()
+    q, s = ops.fp8_quantize(x)
+    w = torch.zeros(n, 16, dtype=torch.uint8, device="cuda").view(E4M3)
+    w[:, :k] = torch.randint(-8, 9, (n, k), device="cuda", dtype=torch.int8).half().to(E4M3)
+    ws = torch.full((-(-n // 128), 1), 0.5, device="cuda")
+    indptr = torch.full((experts + 1,), rows, dtype=torch.int32, device="cuda")
+    indptr[0] = 0
+    want = (x.float() @ w[:, :k].float().t().contiguous()) * 0.5  # whole numbers: exact in any order
+    for precise in (0, 1):
+        y = torch.full((rows, n), -1e9, device="cuda")
+        _lib.call("mi355gq_fp8_group_gemm", q.data_ptr(), 16, s.data_ptr(), rows, None, rows, w.data_ptr(), 16, ws.data_ptr(), indptr.data_ptr(), experts,
+                  n, k, ops._MODEL_DTYPES[torch.float32], precise, y.data_ptr(), ops._stream())
+        assert "fp8_tile" in _lib.last_kernel() and torch.equal(y, want)
