@@ -292,3 +292,19 @@ def test_more_tiles_than_a_grid_holds():
         _lib.call("mi355gq_fp8_group_gemm", q.data_ptr(), 16, s.data_ptr(), rows, None, rows, w.data_ptr(), 16, ws.data_ptr(), indptr.data_ptr(), experts,
                   n, k, ops._MODEL_DTYPES[torch.float32], precise, y.data_ptr(), ops._stream())
         assert "fp8_tile" in _lib.last_kernel() and torch.equal(y, want)
+
+
+@pytest.mark.parametrize("spread,documented", [(0.0, 1.5e-5), (0.7, 2.7e-5), (2.0, 7.7e-5)])
+@pytest.mark.parametrize("m,n,k", [(24, 1024, 4096), (300, 1024, 14336), (512, 1024, 768)])
+def test_what_the_8_bit_instruction_drops(m, n, k, spread, documented):
+    # the documented error of a whole result, normal weights and x's channels spread by exp(spread N), which other seeds move little
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x = torch.randn(m, k, generator=g, device="cuda") * torch.exp(spread * torch.randn(k, generator=g, device="cuda"))
+    w = (100 * torch.randn(n, k, generator=g, device="cuda")).clamp(-448, 448).to(E4M3)
+    ws = 2e-4 * (0.5 + torch.rand(-(-n // 128), k // 128, generator=g, device="cuda"))
+    q, s = ops.fp8_quantize(x)
+    wv = w.double() * ws.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)
+    exact = torch.matmul(q.double() * s.double().t().repeat_interleave(128, 1), wv.t().contiguous())
+    for precise, most in ((False, 2 * documented), (True, 4e-7)):
+        y = ops.fp8_linear((q, s), w, ws, out_dtype=torch.float32, precise=precise).double()
+        assert (y - exact).norm() <= most * exact.norm()
