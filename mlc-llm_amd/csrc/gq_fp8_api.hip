@@ -414,7 +414,7 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
   a.K = hidden;
   a.y = ws.both;
   a.out_dtype = MI355GQ_F32;
-  a.precise = true;  // sums that are rounded to e4m3 again: an error of 1e-5 would move one in thousands by a sixteenth
+  a.precise = true;  // sums that are rounded to e4m3 again: an error of 2e-5 would move one in thousands by a sixteenth
   const bool by_rows = slots <= kFewRowsEach * segments;
   if (e == hipSuccess) {
     if (!gq::fp8_silu_takes(a.N, a.w_pitch)) {  // inter is no multiple of 128, mostly: product and activation apart
@@ -433,7 +433,7 @@ int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_t inter, int
       a.scale_out = nullptr;
     }
   }
-  a.precise = false;  // (the layer's output has 16 bits)
+  a.precise = false;  // the layer's output has 16 bits: as a linear's (4096 rows of 8 x 4096 x 14336 297 us, with float32 sums throughout 466)
   a.x = ws.hq;
   a.xs = ws.hs;
   a.x_pitch = inter;

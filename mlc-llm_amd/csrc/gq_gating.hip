@@ -41,8 +41,8 @@ __device__ __forceinline__ uint32_t in_order(float v) {
 // softmax over nothing but -inf has scores 0.  Weights whose sum is 0 stay 0.
 //
 // Bound by the length of one wave's chain of instructions: a round is about 5 NC + 20 of them.  4096
-// tokens of 256 experts in 8 groups 7.1 us in a graph, 1.9 of it the launch (a token a wave, and ballots for the choice: 9.2; four tokens a
-// wave: 8.4); one token of 64 experts 2.6.
+// tokens of 256 experts in 8 groups 7.1 to 7.3 us in a graph of them, 1.9 of it the launch, and 6.6 a call among others (a token a wave, and ballots
+// for the choice: 9.2 in a graph; four tokens a wave: 8.4); one token of 64 experts 2.6.
 template <int NC, int DT>
 __global__ __launch_bounds__(64) void gating_kernel(const void* __restrict__ logits, const float* __restrict__ bias,
                                                     int64_t T, int E, int k, int sigmoid, int groups, int top_groups,

@@ -22,7 +22,7 @@ struct Options {
   int gemv_ksplit = -1;         // -1: heuristic, 0: never, 1: wherever it applies (register GEMV: two waves share a row's K)
   int quad_ksplit = -1;         // -1: heuristic, 0 | 1 | 2: log2 of the waves that share a quad set's K range
   int gemv_variant = -1;        // -1: heuristic, 0: LDS GEMV, 1: register GEMV, 2..5 skinny forms, 6..8 quad-row forms (x in LDS), 9: quad-row with x in registers
-  int gemm_variant = -1;
+  int gemm_variant = -1;        // (8-bit products: the tile form; gemm_split_k the shares of K)
   int gemv_waves = -1;          // total waves of a persistent GEMV / quad-row / skinny grid
   int gemm_split_k = -1;        // wanted workgroups of the few-row GEMM's split along K
 };

@@ -762,8 +762,9 @@ def fp8_linear(x, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Option
     type (of a pair: the output's, float16 by default), the output out_dtype, or that type.
 
     precise: blocks of 128 are summed in float32.  Without it they may be summed by the 8-bit matrix instructions, which of eight
-    neighbouring products drop what lies more than 13 bits below the largest: 1e-5 of a typical result.  None: a float32 output is
-    precise, a 16-bit one, whose rounding is far larger, is not.  Blocks join one another in float32 either way."""
+    neighbouring products drop what lies more than 13 bits below the largest: 1.5e-5 of a whole result's norm for normal x and weights, 8e-5
+    where channels of x differ by factors of seven; more of a single result that is far below its products.  None: a float32 output is
+    precise, a 16-bit one (whose rounding is 2e-4 in float16, 1.7e-3 in bfloat16) is not.  Blocks join one another in float32 either way."""
     native = _lib.native()
     done = native.fp8_linear(x, weight, weight_scale, bias, out_dtype, residual, precise) if native is not None else None
     if isinstance(done, torch.Tensor):
@@ -889,7 +890,10 @@ def fp8_moe_experts(x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, w
                     w2: torch.Tensor, w2_scale: torch.Tensor) -> torch.Tensor:
     """One expert layer on routed tokens: x [T, hidden] float16 or bfloat16, weights float32 [T, k] and ids int32 [T, k] as
     moe_gating gives them, w13 e4m3 [experts, 2 inter, hidden] (gate rows, then up rows), w2 e4m3 [experts, hidden, inter].
-    An id outside the experts adds nothing."""
+    An id outside the experts adds nothing.  A block of w13's scales that holds both gate and up rows, where inter is no multiple of 128, is of both.
+
+    Gate and up are summed in float32, the second product as fp8_linear does for a 16-bit output; moe_plan, fp8_quantize, fp8_group_gemm
+    with precise and fp8_silu_mul_quantize are the same layer in steps, in float32 throughout."""
     _chk(x, (torch.float16, torch.bfloat16), "x")
     _chk(ids, torch.int32, "ids")
     pitch13, pitch2 = _chk_fp8(w13, "w13", 3), _chk_fp8(w2, "w2", 3)
