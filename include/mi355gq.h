@@ -530,7 +530,7 @@ MI355GQ_API int mi355gq_moe_plan(const void* ids, int64_t T, int64_t top_k, int6
  * q() quantises as mi355gq_fp8_quantize does; w13 [num_experts, 2 inter, hidden] (gate rows, then up rows), w2 [num_experts,
  * hidden, inter], with their scales; weights float32 [T, top_k], ids int32 [T, top_k] (an id outside the experts adds nothing).
  * The first product is precise (its results are rounded to e4m3 again), the second as with precise 0 above, all other sums are in
- * float32 and rounded to model_dtype once.  hidden and inter: multiples of 16.
+ * float32 and rounded to model_dtype once.  hidden and inter: multiples of 16.  x and out start at 16 bytes; out may be x.
  * workspace: mi355gq_fp8_moe_workspace_bytes() bytes, 16-byte aligned; 8 T top_k inter + 256 more where w13_pitch is not hidden and
  * 2 inter w13_pitch, the reach of an expert's rows, is 2^32 - 1 or beyond.  MI355GQ_ERR_WORKSPACE where it is smaller.
  */

@@ -907,6 +907,8 @@ def fp8_moe_experts(x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, w
     _chk_scale(w13_scale, (ne, -(-2 * inter // FP8_BLOCK), -(-hidden // FP8_BLOCK)), "w13_scale")
     _chk_scale(w2_scale, (ne, -(-hidden // FP8_BLOCK), -(-inter // FP8_BLOCK)), "w2_scale")
     k = ids.shape[1]
+    if x.data_ptr() % 16:  # the quantiser's loads
+        x = x.clone()
     out = torch.empty_like(x)
     ws_bytes = _lib.lib().mi355gq_fp8_moe_workspace_bytes(t, hidden, inter, ne, k)
     if ws_bytes and 2 * inter * pitch13 >= 2**32 - 1:

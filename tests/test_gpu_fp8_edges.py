@@ -308,3 +308,31 @@ def test_what_the_8_bit_instruction_drops(m, n, k, spread, documented):
     for precise, most in ((False, 2 * documented), (True, 4e-7)):
         y = ops.fp8_linear((q, s), w, ws, out_dtype=torch.float32, precise=precise).double()
         assert (y - exact).norm() <= most * exact.norm()
+
+
+@pytest.mark.parametrize("t", [1, 5, 40])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_layer_on_x_at_an_odd_offset(t, dtype):
+    layer = ExactLayer(t, 256, 128, 8, _skewed(t, 8, 2, 3), dtype)
+    want = layer.run()
+    flat = torch.empty(layer.x.numel() + 1, dtype=dtype, device="cuda")
+    flat[1:] = layer.x.flatten()
+    odd = flat[1:].view(t, 256)
+    assert odd.data_ptr() % 16 and odd.is_contiguous()
+    logits = torch.randn(t, 8, generator=_gen(t)).cuda()
+    args = (logits, layer.w13, layer.s13, layer.w2, layer.s2, 2)
+    assert torch.equal(ops.fp8_moe(odd, *args), ops.fp8_moe(layer.x, *args))
+    layer.x = odd
+    assert torch.equal(layer.run(), want)
+
+
+@pytest.mark.parametrize("t", [1, 5, 40])
+def test_layer_in_place(t):
+    layer = ExactLayer(t, 256, 128, 8, _skewed(t, 8, 2, 3), torch.float16)
+    want, x = layer.run(), layer.x.clone()
+    size = _lib.lib().mi355gq_fp8_moe_workspace_bytes(t, 256, 128, 8, 2)
+    space = torch.empty(size, dtype=torch.uint8, device="cuda")
+    _lib.call("mi355gq_fp8_moe", x.data_ptr(), t, 256, 128, 8, 2, layer.weights.data_ptr(), layer.ids.data_ptr(), layer.w13.data_ptr(), 256,
+              layer.s13.data_ptr(), layer.w2.data_ptr(), 128, layer.s2.data_ptr(), ops._MODEL_DTYPES[torch.float16], x.data_ptr(), space.data_ptr(), size,
+              ops._stream())
+    assert torch.equal(x, want)
