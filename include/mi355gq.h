@@ -541,6 +541,34 @@ MI355GQ_API int mi355gq_fp8_moe(const void* x, int64_t T, int64_t hidden, int64_
                     const void* w2, int64_t w2_pitch, const void* w2_scale, int model_dtype, void* out, void* workspace,
                     int64_t workspace_bytes, mi355gq_stream_t stream);
 
+/* ---- 16-bit weights: the layers that a quantised model leaves as they are, and models that are not quantised ---- */
+
+/*
+ * mi355gq_dense_linear:       y[M, N] = act(x[M, K] . w[N, K]^T (+ bias[N])) (+ residual[M, N])
+ * mi355gq_dense_linear_gated: y[M, inter] = act(g) * u,  [g, u] = x[M, K] . w[2 inter, K]^T (+ bias[2 inter]): gate rows, then up rows
+ * x, w, bias and residual in model_dtype (MI355GQ_F16 or MI355GQ_BF16), y in it or in float32; dense, at their natural alignment.  Sums and
+ * epilogue are in float32 and rounded once.  act(v), with infinities and NaN as these formulas give them:
+ *   MI355GQ_ACT_NONE v   MI355GQ_ACT_RELU max(v, 0)   MI355GQ_ACT_SILU v / (1 + exp(-v))   MI355GQ_ACT_GELU v Phi(v), Phi the normal
+ *   distribution   MI355GQ_ACT_GELU_TANH v / 2 (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3)))
+ * to 1e-6 of their value (far out on the negative side, where they vanish, to 2^-21 times the exponent).  residual may be y itself where their types agree.  K below 2^23 - 128 (MI355GQ_ERR_UNSUPPORTED beyond).  x and w at 16
+ * bytes with K a multiple of 8 take the fast kernels, anything else a slow one.
+ * workspace: mi355gq_dense_linear_workspace_bytes(M, N, K, gated) bytes of device scratch (N columns of y), 16-byte aligned, for
+ * sums of shares of K; NULL or too small is not an error: K is not shared then, which is slower.  Undefined afterwards; calls that share one
+ * must be stream-ordered.
+ */
+#define MI355GQ_ACT_NONE 0
+#define MI355GQ_ACT_RELU 1
+#define MI355GQ_ACT_SILU 2
+#define MI355GQ_ACT_GELU 3
+#define MI355GQ_ACT_GELU_TANH 4
+MI355GQ_API int64_t mi355gq_dense_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated);
+MI355GQ_API int mi355gq_dense_linear(const void* x, const void* w, const void* bias, const void* residual, int64_t M, int64_t N,
+                         int64_t K, int activation, int model_dtype, int out_dtype, void* y, void* workspace,
+                         int64_t workspace_bytes, mi355gq_stream_t stream);
+MI355GQ_API int mi355gq_dense_linear_gated(const void* x, const void* w, const void* bias, int64_t M, int64_t inter, int64_t K,
+                               int activation, int model_dtype, int out_dtype, void* y, void* workspace,
+                               int64_t workspace_bytes, mi355gq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,165 @@
+// Shared pieces of the operators on 16-bit weights (float16 or bfloat16, x, W, bias and residual alike): the epilogue that every
+// kernel of them ends in, and the matrix instruction by type.
+#pragma once
+
+#include "gq_common.hpp"
+#include "gq_internal.hpp"
+
+namespace gq {
+
+typedef int int4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+
+// values of the public enum MI355GQ_ACT_*
+constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4;
+
+// y = act(x W^T + bias) + residual, or (gated, W = gate rows then up rows) y = act(gate + bias) * (up + bias).
+struct DenseArgs {
+  const uint16_t* x = nullptr;  // [rows, K]
+  const uint16_t* w = nullptr;  // [N, K]
+  const uint16_t* bias = nullptr;      // [N] or null
+  const uint16_t* residual = nullptr;  // [rows, N] or null (not gated)
+  void* y = nullptr;            // [rows, N], gated [rows, N / 2]
+  int64_t rows = 0, N = 0, K = 0;
+  int act = 0, gated = 0, bf16 = 0, out_f32 = 0;
+  int vec = 0;      // columns of y a multiple of 8 and y, bias and residual at 16 bytes: whole runs of columns are loaded and stored
+  void* workspace = nullptr;
+  int64_t workspace_bytes = 0;
+};
+
+// Any sizes and alignments; the kernel of the calls that the others do not take.
+hipError_t launch_dense_simple(const DenseArgs& a, hipStream_t s);
+
+__device__ __forceinline__ float dense_load(const uint16_t* p, int64_t i, int bf16) { return bf16 ? bf2f(p[i]) : h2f(p[i]); }
+
+// a 16 x 16 tile of float32 sums, W as operand A and x as operand B: lane l holds row l % 16 of x and rows 4 (l / 16) .. + 3 of W
+template <bool BF>
+__device__ __forceinline__ float4_t dense_mfma(int4_t w, int4_t x, float4_t acc) {
+  if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w), __builtin_bit_cast(bf16x8_t, x), acc, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, w), __builtin_bit_cast(half8_t, x), acc, 0, 0, 0);
+}
+
+// 1 / (1 + exp(-v)) by the hardware's exp2 and reciprocal, 1 ulp each: 16-bit results round 2^12 times coarser, float32 ones are
+// the sums of products of 16-bit numbers
+__device__ __forceinline__ float dense_sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896341f));
+}
+
+// v Phi(v).  Phi(-a) = exp(-a^2 / 2) t P(t), t = 1 / (1 + 0.3 a), for a >= 0: the factor behind the exponential is smooth in t, and P is the
+// Chebyshev interpolation of degree 7 of it over 0 <= a <= 14, beyond which Phi(-a) is 0 in float32.  Relative error 5e-7 of Phi(-a), so
+// also far out on the negative side.  (The C library's erfc takes three times the instructions; the epilogue of 2048 x 14336 results of
+// a large product is otherwise idle time of its matrix cores.)
+__device__ __forceinline__ float dense_gelu(float v) {
+  const float a = __builtin_fabsf(v), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3f, a, 1.0f));
+  float p = 0.03622337058186531f;
+  p = __builtin_fmaf(p, t, -0.1593545526266098f);
+  p = __builtin_fmaf(p, t, 0.20981964468955994f);
+  p = __builtin_fmaf(p, t, -0.05664501339197159f);
+  p = __builtin_fmaf(p, t, 0.13000500202178955f);
+  p = __builtin_fmaf(p, t, 0.09951350837945938f);
+  p = __builtin_fmaf(p, t, 0.12081217765808105f);
+  p = __builtin_fmaf(p, t, 0.11962586641311646f);
+  const float tail = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f) * (t * p);
+  return v * (v > 0.f ? 1.0f - tail : tail);
+}
+
+__device__ __forceinline__ float dense_act(float v, int act) {
+  switch (act) {  // (the same for the whole launch)
+    case ACT_RELU: return v > 0.f ? v : v != v ? v : 0.f;
+    case ACT_SILU: return v * dense_sigmoid(v);
+    case ACT_GELU: return dense_gelu(v);
+    // v / 2 (1 + tanh(u)) = v / (1 + exp(-2 u)), u = sqrt(2 / pi) (v + 0.044715 v^3)
+    case ACT_GELU_TANH: return v * dense_sigmoid(1.5957691216057308f * v * __builtin_fmaf(0.044715f * v, v, 1.0f));
+    default: return v;
+  }
+}
+
+// CNT (a multiple of 4) neighbouring 16-bit numbers as float32
+template <int CNT>
+__device__ __forceinline__ void dense_load_run(const uint16_t* p, int bf16, float (&f)[CNT]) {
+#pragma unroll
+  for (int v = 0; v < CNT; v += 4) {
+    const uint2 q = *reinterpret_cast<const uint2*>(p + v);
+    const uint32_t u[2] = {q.x, q.y};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f[v + 2 * i] = bf16 ? bf2f(u[i] & 0xffffu) : h2f(u[i] & 0xffffu);
+      f[v + 2 * i + 1] = bf16 ? bf2f(u[i] >> 16) : h2f(u[i] >> 16);
+    }
+  }
+}
+
+// The epilogue, in float32 with one rounding at its end: CNT (4 or 8) sums o of row r from column n on; gated: u are the up sums of the same columns.
+template <int CNT, bool GATED>
+__device__ __forceinline__ void dense_store(const DenseArgs& a, int64_t r, int n, float (&o)[CNT], float (&u)[CNT]) {
+  const int cols = static_cast<int>(GATED ? a.N / 2 : a.N), count = cols - n < CNT ? cols - n : CNT;
+  const int64_t at = r * cols + n;
+  if (a.vec) {
+    float f[CNT];
+    if (a.bias) {
+      dense_load_run<CNT>(a.bias + n, a.bf16, f);
+#pragma unroll
+      for (int v = 0; v < CNT; ++v) o[v] += f[v];
+      if constexpr (GATED) {
+        dense_load_run<CNT>(a.bias + cols + n, a.bf16, f);
+#pragma unroll
+        for (int v = 0; v < CNT; ++v) u[v] += f[v];
+      }
+    }
+  } else if (a.bias) {
+#pragma unroll
+    for (int v = 0; v < CNT; ++v)
+      if (v < count) {
+        o[v] += dense_load(a.bias, n + v, a.bf16);
+        if constexpr (GATED) u[v] += dense_load(a.bias, cols + n + v, a.bf16);
+      }
+  }
+  if (a.act != ACT_NONE) {
+#pragma unroll
+    for (int v = 0; v < CNT; ++v) o[v] = dense_act(o[v], a.act);
+  }
+  if constexpr (GATED) {
+#pragma unroll
+    for (int v = 0; v < CNT; ++v) o[v] *= u[v];
+  } else if (a.residual) {
+    if (a.vec) {
+      float f[CNT];
+      dense_load_run<CNT>(a.residual + at, a.bf16, f);
+#pragma unroll
+      for (int v = 0; v < CNT; ++v) o[v] += f[v];
+    } else {
+#pragma unroll
+      for (int v = 0; v < CNT; ++v)
+        if (v < count) o[v] += dense_load(a.residual, at + v, a.bf16);
+    }
+  }
+  if (a.out_f32) {
+    float* y = static_cast<float*>(a.y) + at;
+    if (a.vec) {
+#pragma unroll
+      for (int v = 0; v < CNT; v += 4) *reinterpret_cast<float4_t*>(y + v) = float4_t{o[v], o[v + 1], o[v + 2], o[v + 3]};
+    } else {
+#pragma unroll
+      for (int v = 0; v < CNT; ++v)
+        if (v < count) y[v] = o[v];
+    }
+  } else {
+    uint32_t h[CNT];
+#pragma unroll
+    for (int v = 0; v < CNT; ++v) h[v] = a.bf16 ? f2bf(o[v]) : f2h(o[v]);
+    uint16_t* y = static_cast<uint16_t*>(a.y) + at;
+    if (a.vec) {
+      uint32_t q[CNT / 2];
+#pragma unroll
+      for (int v = 0; v < CNT / 2; ++v) q[v] = h[2 * v] | h[2 * v + 1] << 16;
+      if constexpr (CNT == 8) *reinterpret_cast<uint4*>(y) = uint4{q[0], q[1], q[2], q[3]};
+      else *reinterpret_cast<uint2*>(y) = uint2{q[0], q[1]};
+    } else {
+#pragma unroll
+      for (int v = 0; v < CNT; ++v)
+        if (v < count) y[v] = static_cast<uint16_t>(h[v]);
+    }
+  }
+}
+
+}  // namespace gq

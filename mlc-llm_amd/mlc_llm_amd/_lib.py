@@ -28,6 +28,7 @@ ROUND_HALF_AWAY, ROUND_HALF_EVEN = 0, 1
 I32, I64 = 0, 1
 EPILOGUE_NONE, EPILOGUE_SILU_MUL = 0, 1
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = range(5)
 
 _P, _I, _L, _F = c_void_p, c_int, c_int64, c_float
 
@@ -101,6 +102,9 @@ SIGNATURES = {
     "mi355gq_moe_plan": (_I, [_P, _L, _L, _L, _P, _P, _P, _P]),
     "mi355gq_fp8_moe_workspace_bytes": (_L, [_L, _L, _L, _L, _L]),
     "mi355gq_fp8_moe": (_I, [_P, _L, _L, _L, _L, _L, _P, _P, _P, _L, _P, _P, _L, _P, _I, _P, _P, _L, _P]),
+    "mi355gq_dense_linear_workspace_bytes": (_L, [_L, _L, _L, _I]),
+    "mi355gq_dense_linear": (_I, [_P, _P, _P, _P, _L, _L, _L, _I, _I, _I, _P, _P, _L, _P]),
+    "mi355gq_dense_linear_gated": (_I, [_P, _P, _P, _L, _L, _L, _I, _I, _I, _P, _P, _L, _P]),
 }
 
 

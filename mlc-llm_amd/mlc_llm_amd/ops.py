@@ -932,3 +932,95 @@ def fp8_moe(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w13_scale:
         return done
     weights, ids = moe_gating(logits, top_k, scoring, bias, num_groups, top_groups, renormalize, scale)
     return fp8_moe_experts(x, weights, ids, w13, w13_scale, w2, w2_scale)
+
+
+# ---- 16-bit weights ----
+#
+# x, weights, bias and residual are all float16 or all bfloat16, dense, on one GPU; the call runs there, on its current stream.
+
+_HALVES = (torch.float16, torch.bfloat16)
+_ACTIVATIONS = {None: _lib.ACT_NONE, "relu": _lib.ACT_RELU, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH}
+
+
+def _chk_here(x: torch.Tensor, t: torch.Tensor, dtype, shape, name: str) -> torch.Tensor:
+    """t of this type and shape, on x's GPU."""
+    _chk(t, dtype, name)
+    if t.device != x.device:
+        raise ValueError(f"{name}: on {t.device}, x on {x.device}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return t
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two dense tensors of a GPU have bytes in common."""
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    return a0 < b0 + b.numel() * b.element_size() and b0 < a0 + a.numel() * a.element_size()
+
+
+def _activation(name) -> int:
+    if not isinstance(name, (str, type(None))) or name not in _ACTIVATIONS:
+        raise ValueError(f"activation {name!r}, expected one of {[a for a in _ACTIVATIONS]}")
+    return _ACTIVATIONS[name]
+
+
+def _dense_args(x, weight, bias, out_dtype, gated: bool):
+    """The checks that both products share: (rows, columns of y, K, out_dtype)."""
+    _chk(x, _HALVES, "x")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError("weight must be a [N, K] tensor")
+    n, k = weight.shape
+    if x.dim() < 1 or x.shape[-1] != k or k == 0:
+        raise ValueError(f"x {tuple(x.shape)} for a weight of {tuple(weight.shape)}")
+    _chk_here(x, weight, x.dtype, weight.shape, "weight")
+    if bias is not None:
+        _chk_here(x, bias, x.dtype, (n,), "bias")
+    if gated and n % 2:
+        raise ValueError(f"dense_linear_gated: {n} rows cannot be split into gate and up halves")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"out_dtype {out_dtype} for a {x.dtype} model")
+    return x.numel() // k, n // 2 if gated else n, k, out_dtype
+
+
+def dense_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+                 residual: Optional[torch.Tensor] = None, out_dtype=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y[..., N] = act(x[..., K] . weight[N, K]^T (+ bias)) (+ residual[..., N]) on float16 or bfloat16 weights.
+
+    activation: None, "relu", "silu", "gelu" (v Phi(v)) or "gelu_tanh".  Sums and epilogue are float32 with one rounding, to out_dtype: x's
+    type (the default) or float32.  residual has x's type and y's shape; as `out` too it is updated in place."""
+    m, n, k, out_dtype = _dense_args(x, weight, bias, out_dtype, False)
+    act = _activation(activation)
+    shape = (*x.shape[:-1], n)
+    if residual is not None:
+        _chk_here(x, residual, x.dtype, shape, "residual")
+    if out is not None:
+        _chk_here(x, out, out_dtype, shape, "out")
+        if any(t is not None and _overlap(out, t) for t in (x, weight, bias)) or (
+                residual is not None and _overlap(out, residual) and (out.data_ptr() != residual.data_ptr() or out.dtype != residual.dtype)):
+            raise ValueError("out: shares memory with an input (it may be the residual itself)")
+    with torch.cuda.device(x.device):
+        if out is None:
+            out = torch.empty(shape, dtype=out_dtype, device=x.device)
+        ws_bytes = _lib.lib().mi355gq_dense_linear_workspace_bytes(m, n, k, 0)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+        _lib.call("mi355gq_dense_linear", x.data_ptr(), weight.data_ptr(), bias.data_ptr() if bias is not None else None,
+                  residual.data_ptr() if residual is not None else None, m, n, k, act, _MODEL_DTYPES[x.dtype], _MODEL_DTYPES[out_dtype],
+                  out.data_ptr(), ws.data_ptr() if ws is not None else None, ws_bytes, _stream())
+    return out
+
+
+def dense_linear_gated(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = "silu",
+                       out_dtype=None) -> torch.Tensor:
+    """act(gate) * up with gate, up = split(x . weight^T (+ bias), 2, axis=-1): the gate_up projection of an MLP with its activation, weight
+    [2 inter, K] as gate rows, then up rows.  Types and activations as in dense_linear; one rounding, of the product."""
+    m, inter, k, out_dtype = _dense_args(x, weight, bias, out_dtype, True)
+    act = _activation(activation)
+    with torch.cuda.device(x.device):
+        out = torch.empty((*x.shape[:-1], inter), dtype=out_dtype, device=x.device)
+        ws_bytes = _lib.lib().mi355gq_dense_linear_workspace_bytes(m, inter, k, 1)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+        _lib.call("mi355gq_dense_linear_gated", x.data_ptr(), weight.data_ptr(), bias.data_ptr() if bias is not None else None, m, inter, k, act,
+                  _MODEL_DTYPES[x.dtype], _MODEL_DTYPES[out_dtype], out.data_ptr(), ws.data_ptr() if ws is not None else None, ws_bytes,
+                  _stream())
+    return out

@@ -1,0 +1,264 @@
+"""Operators on 16-bit weights against their definitions in float64, within bounds that follow from their roundings.
+
+A sum of K products in float32, in any order, is off by at most K 2^-23 of the sum of their magnitudes (K - 1 additions of 2^-24 each,
+and as much again for a matrix unit that truncates).  Behind it an activation passes an error on at most 1.13 times (the steepest slope
+of gelu and silu) and is itself good to 1e-6 of its value; a rounding is off by half a step."""
+
+import math
+
+import pytest
+import torch
+
+import mlc_llm_amd as gq
+from mlc_llm_amd import ops
+
+HALVES = [torch.float16, torch.bfloat16]
+UNIT = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8, torch.float32: 2.0**-24}
+TINY = {torch.float16: 2.0**-25, torch.bfloat16: 2.0**-134, torch.float32: 2.0**-149}  # half a step of the smallest numbers
+ACTS = [None, "relu", "silu", "gelu", "gelu_tanh"]
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _normal(g, dtype, *shape, scale=1.0):
+    return (scale * torch.randn(*shape, generator=g)).to(dtype).cuda()
+
+
+def act_of(v, name):
+    if name == "relu":
+        return v.clamp(min=0)
+    if name == "silu":
+        return v * torch.sigmoid(v)
+    if name == "gelu":
+        return 0.5 * v * torch.erfc(-(0.5**0.5) * v)  # = v Phi(v), with all digits of its tail
+    if name == "gelu_tanh":
+        return v * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v**3))  # = v / 2 (1 + tanh(half of that))
+    return v
+
+
+def product(x, w, bias=None):
+    """(y, error bound) of x w^T + bias in float32."""
+    x, w = x.double(), w.double()
+    y, size = x @ w.t(), x.abs() @ w.abs().t()
+    if bias is not None:
+        y, size = y + bias.double(), size + bias.double().abs()
+    return y, (x.shape[1] + 2) * 2.0**-23 * size
+
+
+def rounded(err, y, dtype):
+    return err + UNIT[dtype] * (y.abs() + err) + TINY[dtype]
+
+
+def linear_ref(x, w, bias, act, residual, out_dtype):
+    v, err = product(x, w, bias)
+    y = act_of(v, act)
+    if act:
+        err = 1.13 * err + 1e-6 * y.abs() + 1e-37
+    if residual is not None:
+        y = y + residual.double()
+        err = err + 2.0**-23 * (y.abs() + residual.double().abs())
+    return y, rounded(err, y, out_dtype)
+
+
+def gated_ref(x, w, bias, act, out_dtype):
+    v, err = product(x, w, bias)
+    (g, u), (eg, eu) = v.chunk(2, 1), err.chunk(2, 1)
+    a = act_of(g, act)
+    if act:
+        eg = 1.13 * eg + 1e-6 * a.abs() + 1e-37
+    y = a * u
+    err = eg * u.abs() + a.abs() * eu + eg * eu + 2.0**-23 * y.abs()
+    return y, rounded(err, y, out_dtype)
+
+
+def close(got, want):
+    y, bound = want
+    assert got.shape == y.shape
+    worst = ((got.double() - y).abs() / bound).max().item() if y.numel() else 0.0
+    assert worst <= 1.0, f"{worst} of the bound ({gq._lib.last_kernel()})"
+
+
+# (rows, columns, K): one of everything, tiles that end inside, every kernel's range of rows
+SIZES = [(1, 1, 1), (1, 16, 8), (2, 17, 40), (3, 5, 33), (1, 4096, 4096), (5, 8, 14336), (7, 515, 136), (16, 128, 2048), (17, 130, 264),
+         (33, 64, 72), (48, 512, 1408), (63, 1000, 8), (64, 96, 4096), (65, 257, 1000), (129, 515, 136), (200, 72, 2056), (257, 128, 64),
+         (300, 1000, 520), (513, 769, 392), (1030, 264, 328)]
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_linear(m, n, k, dtype):
+    g = _gen(m * 7 + n * 3 + k)
+    x, w = _normal(g, dtype, m, k), _normal(g, dtype, n, k, scale=k**-0.5)
+    bias, residual = _normal(g, dtype, n), _normal(g, dtype, m, n)
+    close(ops.dense_linear(x, w), linear_ref(x, w, None, None, None, dtype))
+    for i, act in enumerate(ACTS):
+        out_dtype = torch.float32 if i % 2 else dtype
+        b, r = (bias if i != 2 else None), (residual if i != 3 else None)
+        got = ops.dense_linear(x, w, bias=b, activation=act, residual=r, out_dtype=out_dtype)
+        assert got.dtype == out_dtype
+        close(got, linear_ref(x, w, b, act, r, out_dtype))
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_gated(m, n, k, dtype):
+    g = _gen(m * 5 + n * 11 + k)
+    x, w, bias = _normal(g, dtype, m, k), _normal(g, dtype, 2 * n, k, scale=k**-0.5), _normal(g, dtype, 2 * n)
+    close(ops.dense_linear_gated(x, w), gated_ref(x, w, None, "silu", dtype))
+    for i, act in enumerate(ACTS):
+        out_dtype = torch.float32 if i % 2 else dtype
+        b = bias if i != 2 else None
+        close(ops.dense_linear_gated(x, w, bias=b, activation=act, out_dtype=out_dtype), gated_ref(x, w, b, act, out_dtype))
+
+
+@pytest.mark.parametrize("m", [1, 6, 20, 40, 130])
+def test_unaligned_pointers_and_leading_dimensions(m):
+    """Tensors in the middle of others, at 2 bytes, and x of more than two dimensions."""
+    g = _gen(m)
+    dtype = torch.bfloat16
+    k, n = 264, 136
+
+    def inside(*shape):
+        size = math.prod(shape)
+        return _normal(g, dtype, size + 9)[1 : 1 + size].view(shape)
+
+    x, w, b, r = inside(m, k), inside(n, k), inside(n), inside(m, n)
+    for xx in (x, x.clone()):
+        for ww in (w, w.clone()):
+            for bb, rr in ((b, r), (b.clone(), r.clone()), (None, r)):
+                close(ops.dense_linear(xx, ww, bias=bb, activation="silu", residual=rr), linear_ref(xx, ww, bb, "silu", rr, dtype))
+            close(ops.dense_linear_gated(xx, ww, bias=b, activation="gelu"), gated_ref(xx, ww, b, "gelu", dtype))
+    out = torch.full((m * n + 9,), 7.0, dtype=dtype, device="cuda")
+    ops.dense_linear(x, w, out=out[3 : 3 + m * n].view(m, n))
+    close(out[3 : 3 + m * n].view(m, n), linear_ref(x, w, None, None, None, dtype))
+    assert (out[:3] == 7).all() and (out[3 + m * n :] == 7).all()
+    y = ops.dense_linear(x.view(m, 1, 1, k), w)
+    assert y.shape == (m, 1, 1, n) and torch.equal(y.view(m, n), ops.dense_linear(x, w))
+    one = ops.dense_linear(x[0].clone(), w)
+    assert one.shape == (n,)
+
+
+@pytest.mark.parametrize("m", [1, 9, 33, 150])
+def test_in_place_residual_and_neighbours(m):
+    g = _gen(m + 50)
+    n, k = 520, 1032
+    x, w = _normal(g, torch.float16, m, k), _normal(g, torch.float16, n, k, scale=k**-0.5)
+    wide = torch.full((m + 2, n), -3.0, dtype=torch.float16, device="cuda")
+    hidden = wide[1 : m + 1]
+    hidden.copy_(_normal(g, torch.float16, m, n))
+    want = linear_ref(x, w, None, "gelu_tanh", hidden.clone(), torch.float16)
+    assert ops.dense_linear(x, w, activation="gelu_tanh", residual=hidden, out=hidden) is hidden
+    close(hidden, want)
+    assert (wide[0] == -3).all() and (wide[m + 1] == -3).all()
+
+
+@pytest.mark.parametrize("m", [1, 20, 100])
+def test_empty(m):
+    w = torch.zeros(0, 64, dtype=torch.float16, device="cuda")
+    assert ops.dense_linear(torch.ones(m, 64, dtype=torch.float16, device="cuda"), w).shape == (m, 0)
+    assert ops.dense_linear_gated(torch.ones(m, 64, dtype=torch.float16, device="cuda"), w).shape == (m, 0)
+    w = torch.zeros(m, 64, dtype=torch.float16, device="cuda")
+    assert ops.dense_linear(torch.ones(0, 64, dtype=torch.float16, device="cuda"), w).shape == (0, m)
+    assert ops.dense_linear_gated(torch.ones(2, 0, 64, dtype=torch.float16, device="cuda"), torch.cat([w, w])).shape == (2, 0, m)
+
+
+def test_activations_over_their_range():
+    """W = 1, x = v: the activation of every float16 number, in float32."""
+    v = torch.arange(-(2**15), 2**15, dtype=torch.int32).to(torch.int16).view(torch.float16).cuda()
+    v = v[v.isfinite()]
+    x = torch.zeros(len(v), 8, dtype=torch.float16, device="cuda")
+    x[:, 0] = v
+    w = torch.ones(8, 8, dtype=torch.float16, device="cuda")
+    for act in ACTS[1:]:
+        want = act_of(v.double(), act)
+        # (an activation far out on the negative side may end below float32's smallest number, and its factors do a little before)
+        bound = 2e-6 * want.abs() + 1e-36 * v.double().abs() + 1e-37
+        if act == "gelu":  # exp(-v^2 / 2) from v^2 in float32
+            bound = bound + want.abs() * v.double() ** 2 * 2.0**-23
+        if act in ("gelu_tanh", "silu"):  # the exponent in float32, likewise
+            e = v.double().abs() if act == "silu" else 1.6 * (v.double().abs() + 0.044715 * v.double().abs() ** 3)
+            bound = bound + want.abs() * e * 2.0**-21
+        got = ops.dense_linear(x, w, activation=act, out_dtype=torch.float32)[:, 0].double()
+        assert ((got - want).abs() <= bound).all(), act
+
+
+def test_not_finite():
+    inf, nan = math.inf, math.nan
+    for m in (2, 20, 100):
+        x = torch.ones(m, 64, dtype=torch.float16, device="cuda")
+        w = torch.zeros(24, 64, dtype=torch.float16, device="cuda")
+        w[:, 0] = 1
+        w[3, 5], w[4, 5], w[5, 5] = inf, -inf, nan
+        y = ops.dense_linear(x, w)
+        assert (y[:, 3] == inf).all() and (y[:, 4] == -inf).all() and y[:, 5].isnan().all()
+        assert y[:, [i for i in range(24) if i not in (3, 4, 5)]].eq(1).all()
+        for act in ACTS[1:]:
+            y = ops.dense_linear(x, w, activation=act)
+            assert (y[:, 3] == inf).all() and y[:, 5].isnan().all(), act
+            assert (y[:, 4] == 0).all() if act == "relu" else y[:, 4].isnan().all(), act
+        x[1, 7] = nan  # one token's trouble is its own
+        y = ops.dense_linear(x, w)
+        assert y[1].isnan().all() and y[0, 0] == 1
+
+
+@pytest.mark.parametrize("m", [3, 40])
+def test_weights_beyond_4_gib(m):
+    n, k = 270000, 8192
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.empty(n, k, dtype=torch.bfloat16, device="cuda")
+    for part in w.split(30000):
+        part.copy_(torch.randn(part.shape, generator=g, device="cuda") / 90)
+    x = torch.randn(m, k, generator=g, device="cuda").to(torch.bfloat16)
+    rows = torch.tensor([0, 1, 131071, 131072, 131073, 262143, 262144, 262145, n // 2 - 1, n // 2, n - 17, n - 1], device="cuda")
+    y = ops.dense_linear(x, w)
+    close(y[:, rows], linear_ref(x, w[rows], None, None, None, torch.bfloat16))
+    y = ops.dense_linear_gated(x, w)
+    rows = torch.tensor([0, 1, 17, 65535, 65536, 131071, 131072, 134999], device="cuda")
+    close(y[:, rows], gated_ref(x, torch.cat([w[rows], w[rows + n // 2]]), None, "silu", torch.bfloat16))
+
+
+def test_results_beyond_2_to_the_31():
+    m, n, k = 70001, 32776, 64
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x, w = (torch.randn(r, k, generator=g, device="cuda").to(torch.float16) for r in (m, n))
+    y = ops.dense_linear(x, w, activation="relu")
+    rows = torch.tensor([0, 1, 255, 256, 65535, 65536, 65537, m - 2, m - 1], device="cuda")
+    close(y[rows], linear_ref(x[rows], w, None, "relu", None, torch.float16))
+
+
+@pytest.mark.parametrize("m", [1, 12, 40, 300])
+def test_graph_replays(m):
+    g = _gen(m)
+    k, n = 1024, 520
+    x, w, r = _normal(g, torch.bfloat16, m, k), _normal(g, torch.bfloat16, n, k, scale=k**-0.5), _normal(g, torch.bfloat16, m, n)
+    ops.dense_linear(x, w, residual=r), ops.dense_linear_gated(x, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, b = ops.dense_linear(x, w, activation="silu", residual=r), ops.dense_linear_gated(x, w, activation="gelu")
+    for i in range(4):
+        x.copy_(_normal(g, torch.bfloat16, m, k))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, ops.dense_linear(x, w, activation="silu", residual=r))
+        assert torch.equal(b, ops.dense_linear_gated(x, w, activation="gelu"))
+
+
+def test_other_stream():
+    g = _gen(3)
+    w = _normal(g, torch.float16, 2048, 2048, scale=2048**-0.5)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        x = torch.ones(64, 2048, dtype=torch.float16, device="cuda")
+        for _ in range(20):
+            x = ops.dense_linear(x, w, activation="silu")
+        y = x * 2
+    side.synchronize()
+    z = torch.ones(64, 2048, dtype=torch.float16, device="cuda")
+    for _ in range(20):
+        z = ops.dense_linear(z, w, activation="silu")
+    assert torch.equal(y, z * 2)
