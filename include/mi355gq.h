@@ -569,6 +569,23 @@ MI355GQ_API int mi355gq_dense_linear_gated(const void* x, const void* w, const v
                                int activation, int model_dtype, int out_dtype, void* y, void* workspace,
                                int64_t workspace_bytes, mi355gq_stream_t stream);
 
+/*
+ * One expert layer on up to 64 tokens, in two kernels; x and out [T, hidden] in model_dtype (MI355GQ_F16 or MI355GQ_BF16):
+ *   out[t] = sum over j of weights[t, j] * w2[e] . (act(g) * u),  [g, u] = w13[e] . x[t],  e = ids[t, j]
+ * weights and ids are mi355gq_moe_gating's of logits [T, num_experts] in logits_dtype (score_bias is its bias); w13 [num_experts,
+ * 2 inter, hidden] (gate rows, then up rows) and w2 [num_experts, hidden, inter] in model_dtype, dense.  All sums are in float32;
+ * weights * act(g) * u is held as the sum of two numbers of model_dtype (an infinity beyond its range), the output rounded once.  An expert touches no token
+ * that did not choose it, whatever its weights hold.  hidden and inter: multiples of 8.  x, w13, w2 and out start at 16 bytes; out may be x.
+ * workspace: mi355gq_dense_moe_workspace_bytes() bytes, 16-byte aligned; MI355GQ_ERR_WORKSPACE where it is smaller.  Undefined afterwards; calls
+ * that share one must be stream-ordered.  More than 64 tokens, or 2 T top_k inter of 2^32 - 16 and more: MI355GQ_ERR_UNSUPPORTED.
+ */
+MI355GQ_API int64_t mi355gq_dense_moe_workspace_bytes(int64_t T, int64_t hidden, int64_t inter, int64_t num_experts,
+                                          int64_t top_k);
+MI355GQ_API int mi355gq_dense_moe(const void* x, const void* logits, const void* score_bias, int64_t T, int64_t hidden, int64_t inter,
+                      int64_t num_experts, int64_t top_k, int scoring, int64_t num_groups, int64_t top_groups,
+                      int renormalize, float scale, int logits_dtype, const void* w13, const void* w2, int activation,
+                      int model_dtype, void* out, void* workspace, int64_t workspace_bytes, mi355gq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

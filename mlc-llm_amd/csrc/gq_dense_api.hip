@@ -56,8 +56,18 @@ int product(const char* what, const void* x, const void* w, const void* bias, co
     a.workspace = workspace;
     a.workspace_bytes = workspace_bytes;
   }
-  return hip_result(gq::launch_dense_simple(a, as_stream(stream)), what);
+  const hipStream_t s = as_stream(stream);
+  hipError_t e = gq::dense_aligned(a) ? gq::launch_dense_rows(a, s) : hipErrorNotSupported;
+  if (e == hipErrorNotSupported) e = gq::launch_dense_simple(a, s);
+  return hip_result(e, what);
 }
+
+bool moe_sizes_ok(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t top_k) {
+  return T >= 0 && T < kMaxDim && hidden > 0 && hidden % 8 == 0 && hidden < kMaxRow && inter > 0 && inter % 8 == 0 && inter < kMaxRow && experts > 0 &&
+         experts <= 512 && top_k > 0 && top_k <= 32 && top_k <= experts;
+}
+// the rows of the workspace are reached by 32-bit offsets
+bool moe_takes(int64_t T, int64_t inter, int64_t top_k) { return T <= gq::kMoeTokens && T * top_k * inter * 2 < 0xfffffff0ll; }
 
 }  // namespace
 
@@ -78,6 +88,61 @@ int mi355gq_dense_linear_gated(const void* x, const void* w, const void* bias, i
                                int out_dtype, void* y, void* workspace, int64_t workspace_bytes, mi355gq_stream_t stream) {
   return product("dense_linear_gated", x, w, bias, nullptr, M, inter, K, true, activation, model_dtype, out_dtype, y, workspace, workspace_bytes,
                  stream);
+}
+
+int64_t mi355gq_dense_moe_workspace_bytes(int64_t T, int64_t hidden, int64_t inter, int64_t num_experts, int64_t top_k) {
+  if (!moe_sizes_ok(T, hidden, inter, num_experts, top_k) || T == 0 || !moe_takes(T, inter, top_k)) return 0;
+  return gq::dense_moe_workspace_bytes(T, hidden, inter, num_experts, top_k);
+}
+
+int mi355gq_dense_moe(const void* x, const void* logits, const void* score_bias, int64_t T, int64_t hidden, int64_t inter, int64_t num_experts,
+                      int64_t top_k, int scoring, int64_t num_groups, int64_t top_groups, int renormalize, float scale, int logits_dtype,
+                      const void* w13, const void* w2, int activation, int model_dtype, void* out, void* workspace, int64_t workspace_bytes,
+                      mi355gq_stream_t stream) {
+  DENSE_REQUIRE(model_dtype == MI355GQ_F16 || model_dtype == MI355GQ_BF16, "dense_moe: model_dtype=%d (MI355GQ_F16 or MI355GQ_BF16)", model_dtype);
+  DENSE_REQUIRE(logits_dtype == MI355GQ_F16 || logits_dtype == MI355GQ_F32 || logits_dtype == MI355GQ_BF16, "dense_moe: logits_dtype=%d", logits_dtype);
+  DENSE_REQUIRE(act_ok(activation), "dense_moe: activation=%d", activation);
+  DENSE_REQUIRE(scoring == MI355GQ_SCORE_SOFTMAX || scoring == MI355GQ_SCORE_SIGMOID, "dense_moe: scoring=%d", scoring);
+  DENSE_REQUIRE(moe_sizes_ok(T, hidden, inter, num_experts, top_k),
+                "dense_moe: T=%lld, hidden=%lld and inter=%lld (multiples of 8 below 2^23 - 128), num_experts=%lld (1..512), top_k=%lld (1..32)", (long long)T,
+                (long long)hidden, (long long)inter, (long long)num_experts, (long long)top_k);
+  DENSE_REQUIRE(num_groups > 0 && num_groups <= 64 && num_experts % num_groups == 0 && top_groups > 0 && top_groups <= num_groups &&
+                    top_groups * (num_experts / num_groups) >= top_k,
+                "dense_moe: the %lld best of %lld groups of %lld experts cannot give %lld", (long long)top_groups, (long long)num_groups,
+                (long long)num_experts, (long long)top_k);
+  if (T == 0) return MI355GQ_OK;
+  if (!moe_takes(T, inter, top_k))
+    return set_error(MI355GQ_ERR_UNSUPPORTED, "dense_moe: %lld tokens of %lld experts of %lld (%d tokens at most, and 4 GiB of activations)", (long long)T,
+                     (long long)top_k, (long long)inter, gq::kMoeTokens);
+  DENSE_REQUIRE(x && logits && w13 && w2 && out, "dense_moe: null pointer");
+  DENSE_REQUIRE(aligned(x, 16) && aligned(w13, 16) && aligned(w2, 16) && aligned(out, 16) && aligned(score_bias, 4) &&
+                    aligned(logits, logits_dtype == MI355GQ_F32 ? 4 : 2), "dense_moe: misaligned pointer (x, out and weights: 16 bytes)");
+  DENSE_REQUIRE(aligned(workspace, 16), "dense_moe: workspace must be 16-byte aligned");
+  const int64_t need = gq::dense_moe_workspace_bytes(T, hidden, inter, num_experts, top_k);
+  if (workspace == nullptr || workspace_bytes < need)
+    return set_error(MI355GQ_ERR_WORKSPACE, "dense_moe: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  gq::DenseMoeArgs a;
+  a.x = static_cast<const uint16_t*>(x);
+  a.w13 = static_cast<const uint16_t*>(w13);
+  a.w2 = static_cast<const uint16_t*>(w2);
+  a.out = static_cast<uint16_t*>(out);
+  a.logits = logits;
+  a.score_bias = static_cast<const float*>(score_bias);
+  a.T = static_cast<int>(T);
+  a.experts = static_cast<int>(num_experts);
+  a.k = static_cast<int>(top_k);
+  a.hidden = static_cast<int>(hidden);
+  a.inter = static_cast<int>(inter);
+  a.act = activation;
+  a.bf16 = model_dtype == MI355GQ_BF16;
+  a.sigmoid = scoring == MI355GQ_SCORE_SIGMOID;
+  a.groups = static_cast<int>(num_groups);
+  a.top_groups = static_cast<int>(top_groups);
+  a.renormalize = renormalize != 0;
+  a.logits_dtype = logits_dtype;
+  a.scale = scale;
+  a.workspace = workspace;
+  return hip_result(gq::launch_dense_moe(a, as_stream(stream)), "dense_moe launch");
 }
 
 }  // extern "C"

@@ -27,6 +27,31 @@ struct DenseArgs {
   int64_t workspace_bytes = 0;
 };
 
+// x and w at 16 bytes and K a multiple of 8, for the kernels that load eight numbers at a time.
+inline bool dense_aligned(const DenseArgs& a) {
+  return a.K % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w)) & 15u) == 0;
+}
+
+// Up to 32 rows of aligned operands; hipErrorNotSupported beyond.
+hipError_t launch_dense_rows(const DenseArgs& a, hipStream_t s);
+
+// One expert layer on up to kMoeTokens tokens, see mi355gq_dense_moe.
+constexpr int kMoeTokens = 64;
+struct DenseMoeArgs {
+  const uint16_t* x = nullptr;    // [T, hidden]
+  const uint16_t* w13 = nullptr;  // [experts, 2 inter, hidden]
+  const uint16_t* w2 = nullptr;   // [experts, hidden, inter]
+  uint16_t* out = nullptr;        // [T, hidden]
+  const void* logits = nullptr;   // [T, experts] in logits_dtype
+  const float* score_bias = nullptr;
+  int T = 0, experts = 0, k = 0, hidden = 0, inter = 0, act = 0, bf16 = 0;
+  int sigmoid = 0, groups = 1, top_groups = 1, renormalize = 1, logits_dtype = 0;
+  float scale = 1.f;
+  void* workspace = nullptr;
+};
+int64_t dense_moe_workspace_bytes(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k);
+hipError_t launch_dense_moe(const DenseMoeArgs& a, hipStream_t s);
+
 // Any sizes and alignments; the kernel of the calls that the others do not take.
 hipError_t launch_dense_simple(const DenseArgs& a, hipStream_t s);
 

@@ -105,6 +105,8 @@ SIGNATURES = {
     "mi355gq_dense_linear_workspace_bytes": (_L, [_L, _L, _L, _I]),
     "mi355gq_dense_linear": (_I, [_P, _P, _P, _P, _L, _L, _L, _I, _I, _I, _P, _P, _L, _P]),
     "mi355gq_dense_linear_gated": (_I, [_P, _P, _P, _L, _L, _L, _I, _I, _I, _P, _P, _L, _P]),
+    "mi355gq_dense_moe_workspace_bytes": (_L, [_L, _L, _L, _L, _L]),
+    "mi355gq_dense_moe": (_I, [_P, _P, _P, _L, _L, _L, _L, _L, _I, _L, _L, _I, _F, _I, _P, _P, _I, _I, _P, _P, _L, _P]),
 }
 
 

@@ -1024,3 +1024,43 @@ def dense_linear_gated(x: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
                   _MODEL_DTYPES[x.dtype], _MODEL_DTYPES[out_dtype], out.data_ptr(), ws.data_ptr() if ws is not None else None, ws_bytes,
                   _stream())
     return out
+
+
+DENSE_MOE_TOKENS = 64
+
+
+def dense_moe(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, top_k: int, activation: Optional[str] = "silu",
+              scoring: str = "softmax", bias: Optional[torch.Tensor] = None, num_groups: int = 1, top_groups: int = 1,
+              renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """One expert layer on up to DENSE_MOE_TOKENS tokens, in two kernels: x [T, hidden] float16 or bfloat16, logits [T, experts] (any of the
+    model dtypes) routed as moe_gating does with the same arguments, w13 [experts, 2 inter, hidden] (gate rows, then up rows) and w2
+    [experts, hidden, inter] in x's type.  y[t] = sum over the chosen experts of their weight times w2 . (act(gate) * up), in float32
+    sums with one rounding."""
+    _chk(x, _HALVES, "x")
+    for t, name in ((w13, "w13"), (w2, "w2")):
+        _chk(t, x.dtype, name)
+        if t.dim() != 3:
+            raise ValueError(f"{name}: {t.dim()} dimensions, expected 3")
+    ne, hidden, inter = w2.shape
+    if tuple(w13.shape) != (ne, 2 * inter, hidden) or x.dim() != 2 or x.shape[1] != hidden:
+        raise ValueError(f"dense_moe: x {tuple(x.shape)}, w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} do not belong together")
+    t = x.shape[0]
+    _chk_here(x, w13, x.dtype, w13.shape, "w13")
+    _chk_here(x, w2, x.dtype, w2.shape, "w2")
+    _chk_here(x, logits, _FLOATS, (t, ne), "logits")
+    if bias is not None:
+        _chk_here(x, bias, torch.float32, (ne,), "bias")
+    act = _activation(activation)
+    if scoring not in _SCORING:
+        raise ValueError(f"dense_moe: scoring {scoring!r}, expected one of {sorted(_SCORING)}")
+    with torch.cuda.device(x.device):
+        if x.data_ptr() % 16:  # the kernels' loads
+            x = x.clone()
+        out = torch.empty_like(x)
+        ws_bytes = _lib.lib().mi355gq_dense_moe_workspace_bytes(t, hidden, inter, ne, top_k)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+        _lib.call("mi355gq_dense_moe", x.data_ptr(), logits.data_ptr(), bias.data_ptr() if bias is not None else None, t, hidden, inter, ne,
+                  top_k, _SCORING[scoring], num_groups, top_groups, 1 if renormalize else 0, float(scale), _MODEL_DTYPES[logits.dtype],
+                  w13.data_ptr(), w2.data_ptr(), act, _MODEL_DTYPES[x.dtype], out.data_ptr(), ws.data_ptr() if ws is not None else None,
+                  ws_bytes, _stream())
+    return out

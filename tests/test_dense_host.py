@@ -54,6 +54,38 @@ def test_products_check_their_arguments():
     assert all(size(m, n, k, g) >= 0 for m in (1, 40, 5000) for n in (1, 4096) for k in (8, 4096) for g in (0, 1))
 
 
+def test_expert_layer_checks_its_arguments():
+    need = _lib.lib().mi355gq_dense_moe_workspace_bytes(4, 64, 32, 8, 2)
+    assert need >= 2 * 4 * 2 * 32 * 2
+
+    def moe(x=X, lg=B, sb=None, t=4, h=64, i=32, e=8, k=2, sc=0, g=1, tg=1, ldt=F32, w13=W, w2=R, act=2, dt=F16, out=Y, ws=S, size=need):
+        return _lib.lib().mi355gq_dense_moe(x, lg, sb, t, h, i, e, k, sc, g, tg, 1, 1.0, ldt, w13, w2, act, dt, out, ws, size, None)
+
+    _refused(moe(dt=F32), "model_dtype")
+    _refused(moe(ldt=5), "logits_dtype")
+    _refused(moe(act=9), "activation")
+    _refused(moe(sc=2), "scoring")
+    for bad in ({"t": -1}, {"h": 60}, {"h": 0}, {"i": 12}, {"e": 0}, {"e": 513}, {"k": 0}, {"k": 9}, {"k": 33, "e": 64}, {"h": 1 << 23}, {"i": 1 << 23}):
+        _refused(moe(**bad), "multiples of 8")
+    _refused(moe(g=3), "groups")
+    _refused(moe(g=4, tg=5), "groups")
+    _refused(moe(g=8, tg=1), "cannot give 2")
+    _refused(moe(t=65), "64 tokens at most", _lib.ERR_UNSUPPORTED)
+    _refused(moe(t=64, i=(1 << 23) - 256, e=64, k=32), "4 GiB", _lib.ERR_UNSUPPORTED)
+    for name in ("x", "lg", "w13", "w2", "out"):
+        _refused(moe(**{name: None}), "null")
+    for name in ("x", "w13", "w2", "out"):
+        _refused(moe(**{name: P(0x10008)}), "misaligned")
+    _refused(moe(lg=P(0x10002)), "misaligned")
+    _refused(moe(sb=P(0x10002)), "misaligned")
+    _refused(moe(ws=P(0x10008)), "workspace")
+    _refused(moe(size=need - 1), "needed", _lib.ERR_WORKSPACE)
+    _refused(moe(ws=None), "needed", _lib.ERR_WORKSPACE)
+    assert moe(t=0, x=None, ws=None) == 0
+    size = _lib.lib().mi355gq_dense_moe_workspace_bytes
+    assert size(0, 64, 32, 8, 2) == size(65, 64, 32, 8, 2) == size(4, 60, 32, 8, 2) == 0
+
+
 def test_python_refusals():
     x, w = torch.zeros(4, 64, dtype=torch.float16), torch.zeros(32, 64, dtype=torch.float16)
     with pytest.raises(ValueError, match="must live on the GPU"):
@@ -112,5 +144,19 @@ def test_python_refusals_of_tensors():
         with pytest.raises(ValueError, match="out: shares memory"):
             ops.dense_linear(x, square, out=out)
     pair = t(8, 32)
+    w13, w2, logits = t(8, 64, 64), t(8, 64, 32), t(4, 8, dtype=torch.float32)
+    ops.dense_moe(x, logits, w13, w2, 2)
+    for bad, err, text in (((x.float(), logits, w13, w2), TypeError, "x: dtype"), ((x, logits.double(), w13, w2), TypeError, "logits: dtype"),
+                           ((x, logits, w13.bfloat16(), w2), TypeError, "w13: dtype"), ((x, logits, w13[0], w2), ValueError, "dimensions"),
+                           ((x, logits, w13[:7], w2), ValueError, "do not belong together"), ((x, logits[:3], w13, w2), ValueError, "logits shape"),
+                           ((t(4, 72), logits, w13, w2), ValueError, "do not belong together")):
+        with pytest.raises(err, match=text):
+            ops.dense_moe(*bad, 2)
+    with pytest.raises(ValueError, match="bias shape"):
+        ops.dense_moe(x, logits, w13, w2, 2, bias=t(7, dtype=torch.float32))
+    with pytest.raises(ValueError, match="scoring"):
+        ops.dense_moe(x, logits, w13, w2, 2, scoring="relu")
+    with pytest.raises(ValueError, match="activation"):
+        ops.dense_moe(x, logits, w13, w2, 2, activation="swish")
     with pytest.raises(ValueError, match="out: shares memory"):
         ops.dense_linear(x, w, residual=pair[:4], out=pair[1:5])

@@ -262,3 +262,157 @@ def test_other_stream():
     for _ in range(20):
         z = ops.dense_linear(z, w, activation="silu")
     assert torch.equal(y, z * 2)
+
+
+# ---- the expert layer ----
+
+
+def moe_ref(x, weights, ids, w13, w2, act, dtype):
+    """(y, bound) of a layer on routed tokens, in float64 from the very weights and ids of moe_gating."""
+    y = torch.zeros(x.shape, dtype=torch.float64, device=x.device)
+    err = torch.zeros_like(y)
+    for e in ids.unique().tolist():
+        token, slot = torch.nonzero(ids == e, as_tuple=True)
+        v, ev = product(x[token], w13[e])
+        (g, u), (eg, eu) = v.chunk(2, 1), ev.chunk(2, 1)
+        a = act_of(g, act)
+        if act:
+            eg = 1.13 * eg + 1e-6 * a.abs() + 1e-37
+        w = weights[token, slot].double()[:, None]
+        h = w * a * u
+        # the float32 product; held as two numbers, half a step of a half step, or of the smallest numbers
+        eh = w.abs() * (eg * u.abs() + a.abs() * eu + eg * eu) + (2.0**-23 + UNIT[dtype] ** 2) * h.abs() + 2 * TINY[dtype]
+        d, ed = product(h, w2[e])
+        y[token] += d
+        # a sum over twice as many products, and over the token's experts
+        err[token] += 2 * ed + eh @ w2[e].double().abs().t() + ids.shape[1] * 2.0**-23 * (h.abs() @ w2[e].double().abs().t())
+    return y, rounded(err, y, dtype)
+
+
+def _layer(g, dtype, t, hidden, inter, experts, logits_dtype=torch.float32):
+    return (_normal(g, dtype, t, hidden), _normal(g, logits_dtype, t, experts, scale=1.5), _normal(g, dtype, experts, 2 * inter, hidden, scale=hidden**-0.5),
+            _normal(g, dtype, experts, hidden, inter, scale=inter**-0.5))
+
+
+# (tokens, hidden, inter, experts, top_k): each number of experts a lane holds, shares of the second product, sizes that end inside a block
+LAYERS = [(1, 256, 128, 8, 2), (1, 2048, 1408, 64, 6), (2, 64, 8, 4, 4), (3, 72, 200, 5, 1), (4, 512, 1032, 8, 2), (7, 8, 8, 1, 1), (15, 520, 136, 60, 8),
+          (16, 2048, 768, 128, 8), (17, 264, 328, 24, 3), (31, 136, 264, 160, 6), (32, 1024, 512, 16, 4), (33, 104, 64, 300, 32), (50, 256, 96, 512, 8),
+          (64, 512, 264, 8, 2), (64, 136, 72, 2, 2), (64, 64, 64, 64, 32)]
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t,hidden,inter,experts,k", LAYERS)
+def test_moe(t, hidden, inter, experts, k, dtype):
+    g = _gen(t * 31 + hidden + inter + experts)
+    for i, (scoring, act, logits_dtype) in enumerate([("softmax", "silu", torch.float32), ("sigmoid", "gelu_tanh", dtype), ("softmax", "gelu", torch.float32)]):
+        x, logits, w13, w2 = _layer(g, dtype, t, hidden, inter, experts, logits_dtype)
+        how = {"scoring": scoring, "renormalize": i != 1, "scale": 2.5 if i == 1 else 1.0}
+        if i == 1:
+            how["bias"] = _normal(g, torch.float32, experts, scale=0.1)
+        if i and experts % 4 == 0 and experts // 2 >= k:
+            how.update(num_groups=4, top_groups=2)
+        weights, ids = ops.moe_gating(logits, k, **how)
+        got = ops.dense_moe(x, logits, w13, w2, k, activation=act, **how)
+        assert got.dtype == dtype
+        close(got, moe_ref(x, weights, ids, w13, w2, act, dtype))
+        assert torch.equal(got, ops.dense_moe(x, logits, w13, w2, k, activation=act, **how))
+
+
+@pytest.mark.parametrize("t", [5, 20, 64])
+def test_moe_skewed_routing(t):
+    """Every token to the same experts, and one expert of many for all."""
+    g = _gen(t)
+    x, logits, w13, w2 = _layer(g, torch.bfloat16, t, 256, 200, 40)
+    logits[:, 7] = 9.0
+    logits[:, 39] = 8.0
+    for k in (1, 2, 3):
+        weights, ids = ops.moe_gating(logits, k)
+        close(ops.dense_moe(x, logits, w13, w2, k), moe_ref(x, weights, ids, w13, w2, "silu", torch.bfloat16))
+    logits[:] = 0  # ties: the lowest experts
+    weights, ids = ops.moe_gating(logits, 4)
+    assert (ids == torch.arange(4, device="cuda")).all()
+    close(ops.dense_moe(x, logits, w13, w2, 4), moe_ref(x, weights, ids, w13, w2, "silu", torch.bfloat16))
+
+
+@pytest.mark.parametrize("t", [2, 40])
+def test_moe_troubles_stay_where_they_are(t):
+    """Experts that nobody chose, and those that others chose, may hold anything; a token's NaN is its own."""
+    g = _gen(t)
+    x, logits, w13, w2 = _layer(g, torch.float16, t, 128, 64, 8)
+    logits[:, 3] = -50.0
+    logits[0, 5], logits[1:, 5] = 20.0, -40.0  # expert 5: token 0 alone
+    weights, ids = ops.moe_gating(logits, 2)
+    assert (ids[0] == 5).any() and not (ids[1:] == 5).any() and not (ids == 3).any()
+    w13[3], w2[3] = math.nan, math.inf
+    w13[5, 0], w2[5, 1] = math.inf, math.nan
+    got = ops.dense_moe(x, logits, w13, w2, 2)
+    assert got[0, 1].isnan()
+    y, bound = moe_ref(x[1:], weights[1:], ids[1:], w13, w2, "silu", torch.float16)
+    close(got[1:], (y, bound))
+    x[1, 3] = math.nan
+    again = ops.dense_moe(x, logits, w13, w2, 2)
+    assert again[1].isnan().all() and torch.equal(again[2:], got[2:])
+
+
+def test_moe_weights_beyond_4_gib():
+    t, hidden, inter, experts, k = 12, 4096, 8200, 40, 3
+    g = torch.Generator(device="cuda").manual_seed(5)
+    w13 = torch.empty(experts, 2 * inter, hidden, dtype=torch.bfloat16, device="cuda")
+    w2 = torch.empty(experts, hidden, inter, dtype=torch.bfloat16, device="cuda")
+    for w in (w13, w2):
+        for part in w:
+            part.copy_(torch.randn(part.shape, generator=g, device="cuda") / 80)
+    x = torch.randn(t, hidden, generator=g, device="cuda").to(torch.bfloat16)
+    logits = torch.randn(t, experts, generator=g, device="cuda")
+    logits[0, 39] = logits[1, 0] = 20.0
+    weights, ids = ops.moe_gating(logits, k)
+    close(ops.dense_moe(x, logits, w13, w2, k), moe_ref(x, weights, ids, w13, w2, "silu", torch.bfloat16))
+
+
+@pytest.mark.parametrize("t", [1, 16, 40])
+def test_moe_graph_replays(t):
+    """Two captured layers that take their scratch from one pool, replayed in turn with other work between."""
+    g = _gen(t)
+    x, logits, w13, w2 = _layer(g, torch.bfloat16, t, 512, 264, 24)
+    ops.dense_moe(x, logits, w13, w2, 3)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for k in (3, 6):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            outs.append(ops.dense_moe(x, logits, w13, w2, k))
+        graphs.append(graph)
+    for i in range(4):
+        x.copy_(_normal(g, torch.bfloat16, *x.shape))
+        logits.copy_(_normal(g, torch.float32, *logits.shape))
+        for k, graph, out in zip((3, 6), graphs, outs):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, ops.dense_moe(x, logits, w13, w2, k))
+
+
+def test_router_layer_and_residual_together():
+    """As a decoder layer runs them: router logits in float32, experts, a shared gated MLP whose down projection adds the rest up."""
+    g = _gen(9)
+    dtype, t, hidden, inter, experts, k = torch.bfloat16, 11, 512, 264, 24, 3
+    x, _, w13, w2 = _layer(g, dtype, t, hidden, inter, experts)
+    router = _normal(g, dtype, experts, hidden, scale=hidden**-0.5)
+    up, down = _normal(g, dtype, 2 * inter, hidden, scale=hidden**-0.5), _normal(g, dtype, hidden, inter, scale=inter**-0.5)
+    logits = ops.dense_linear(x, router, out_dtype=torch.float32)
+    close(logits, linear_ref(x, router, None, None, None, torch.float32))
+    routed = ops.dense_moe(x, logits, w13, w2, k)
+    weights, ids = ops.moe_gating(logits, k)
+    close(routed, moe_ref(x, weights, ids, w13, w2, "silu", dtype))
+    shared = ops.dense_linear_gated(x, up, activation="gelu_tanh")
+    close(shared, gated_ref(x, up, None, "gelu_tanh", dtype))
+    y = ops.dense_linear(shared, down, residual=routed, out=routed)
+    assert y is routed
+    close(y, linear_ref(shared, down, None, None, ops.dense_moe(x, logits, w13, w2, k), dtype))
+
+
+def test_moe_refuses_more_tokens():
+    x, logits, w13, w2 = _layer(_gen(1), torch.float16, 65, 64, 32, 4)
+    with pytest.raises(gq._lib.Mi355gqError) as err:
+        ops.dense_moe(x, logits, w13, w2, 2)
+    assert err.value.code == gq._lib.ERR_UNSUPPORTED and "64 tokens at most" in err.value.message
+    assert ops.dense_moe(x[:0], logits[:0], w13, w2, 2).shape == (0, 64)
