@@ -577,7 +577,7 @@ MI355GQ_API int mi355gq_dense_linear_gated(const void* x, const void* w, const v
  * weights * act(g) * u is held as the sum of two numbers of model_dtype (an infinity beyond its range), the output rounded once.  An expert touches no token
  * that did not choose it, whatever its weights hold.  hidden and inter: multiples of 8.  x, w13, w2 and out start at 16 bytes; out may be x.
  * workspace: mi355gq_dense_moe_workspace_bytes() bytes, 16-byte aligned; MI355GQ_ERR_WORKSPACE where it is smaller.  Undefined afterwards; calls
- * that share one must be stream-ordered.  More than 64 tokens, or 2 T top_k inter of 2^32 - 16 and more: MI355GQ_ERR_UNSUPPORTED.
+ * that share one must be stream-ordered.  More than 64 tokens, or 2 T top_k inter of 3 * 2^30 and more: MI355GQ_ERR_UNSUPPORTED.
  */
 MI355GQ_API int64_t mi355gq_dense_moe_workspace_bytes(int64_t T, int64_t hidden, int64_t inter, int64_t num_experts,
                                           int64_t top_k);

@@ -32,7 +32,7 @@ inline bool dense_aligned(const DenseArgs& a) {
   return a.K % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w)) & 15u) == 0;
 }
 
-// Up to 32 rows of aligned operands; hipErrorNotSupported beyond.
+// Up to 16 rows of aligned operands; hipErrorNotSupported beyond.
 hipError_t launch_dense_rows(const DenseArgs& a, hipStream_t s);
 
 // One expert layer on up to kMoeTokens tokens, see mi355gq_dense_moe.

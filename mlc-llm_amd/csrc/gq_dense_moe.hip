@@ -6,8 +6,8 @@
 // are three) and streams the gate and up rows of the experts that some token chose past these experts' tokens.  A row of w h, the
 // weighted activation of one token and expert, goes to the workspace as two 16-bit numbers, the rounded value and what the rounding
 // left, so that the second product loses nothing to it.
-// The second streams the down rows.  Its columns of x are the tokens, for every expert: a token that did not choose an expert reads zeros there
-// (and its sums of that expert's part are dropped, whatever W holds), so that the sum over a token's experts is the accumulator's.
+// The second streams the down rows past the same rows of w h; what comes out of an expert joins the sums of its tokens, which lie in LDS.  An
+// expert meets the tokens that chose it alone, whatever W or the other tokens hold.
 #include "gq_dense_stream.hpp"
 #include "gq_gating.hpp"
 
@@ -15,24 +15,24 @@ namespace gq {
 
 namespace {
 
-constexpr int kWaves = 8, kThreads = 64 * kWaves;
-constexpr double kTarget = 3000;
+constexpr int kWaves = kStreamWaves, kThreads = 64 * kWaves;
 
-struct MoeExpert {
-  int e, row0;    // the expert and the first of its rows of h
-  uint64_t mask;  // its tokens
+// Up to 8 XG rows of one expert, the columns of x of both products.
+struct MoeSegment {
+  int e, row0, rows;
 };
-// The workspace: what the first kernel leaves for the second.
+// The workspace: what the first kernel leaves for the second.  Offsets; at 0 the number of segments.
 struct MoeLayout {
-  int64_t count = 0, experts, tickets, shares, h, bytes;  // offsets; h: [2][T k][inter]
+  int64_t segs, row_token, tickets, shares, h, bytes;  // h: [2][T k][inter]
 };
-__host__ __device__ inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 inline int moe_shares(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k);
 inline MoeLayout moe_layout(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k) {
   const int64_t slots = T * k, tiles = (hidden + 15) / 16;
   MoeLayout l;
-  l.experts = 256;
-  l.tickets = l.experts + up256((experts < slots ? experts : slots) * static_cast<int64_t>(sizeof(MoeExpert)));
+  l.segs = 256;
+  l.row_token = l.segs + up256(slots * static_cast<int64_t>(sizeof(MoeSegment)));
+  l.tickets = l.row_token + up256(slots * 4);
   l.shares = l.tickets + up256(tiles * 4);
   const int shares = moe_shares(T, hidden, inter, experts, k);
   l.h = l.shares + (shares > 1 ? up256(static_cast<int64_t>(shares) * tiles * T * 64) : 0);
@@ -45,46 +45,48 @@ inline double experts_chosen(int64_t T, int64_t experts, int64_t k) {
   for (int64_t t = 0; t < T; ++t) none *= 1 - static_cast<double>(k) / static_cast<double>(experts);
   return static_cast<double>(experts) * (1 - none);
 }
-// Workgroups that share the K (all chosen experts' inter) of sixteen columns in the second kernel: about two a unit.
+// eights of rows of a segment: sixteen rows where experts have more than four on average
+inline int moe_eights(int64_t T, int64_t experts, int64_t k) { return T > 8 && T * k > 4 * experts ? 2 : 1; }
+// Workgroups that share the K (all chosen experts' inter) of sixteen columns in the second kernel: two a unit.
 inline int moe_shares(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k) {
   const int64_t tiles = (hidden + 15) / 16;
   const double blocks = experts_chosen(T, experts, k) * static_cast<double>((inter + kStreamBlock - 1) / kStreamBlock);
   int s = 1;
-  while (s < 8 && tiles * s < 400 && blocks / (2 * s) >= 4 * kWaves) s *= 2;
+  while (s < 8 && tiles * s < 400 && blocks / (2 * s) >= 2 * kStreamDepth * kWaves) s *= 2;
   return s;
 }
 
 struct MoeTables {  // in LDS, in front of the rest
   uint64_t* mask;      // [experts] tokens of each
+  MoeSegment* segs;    // [T k at most]
   int* slot_id;        // [T k]
   float* slot_w;       // [T k]
   int* row_token;      // [T k] in the order of the experts
   float* row_w;        // [T k]
-  int2* segs;          // [T k at most] up to 16 TT rows of one expert: (expert, first row | rows << 16)
-  int* totals;         // [32]
+  uint64_t* totals;    // [waves]
 };
-__host__ __device__ inline size_t moe_tables_bytes(int experts, int slots) { return (static_cast<size_t>(experts) * 8 + static_cast<size_t>(slots) * 24 + 256 + 15) / 16 * 16; }
+inline size_t moe_tables_bytes(int experts, int slots) { return (64 + static_cast<size_t>(experts) * 8 + static_cast<size_t>(slots) * (16 + sizeof(MoeSegment)) + 15) / 16 * 16; }
 
 }  // namespace
 
-// NC: experts a lane in the routing.  TT: 16 TT tokens of an expert at a time.
-template <bool BF, int NC, int TT>
-__global__ __launch_bounds__(kThreads, 4) void dense_moe_up_kernel(DenseMoeArgs a, MoeLayout layout, int group_inv, int logits_vec, int kw_log2, int nb) {
+// NC: experts a lane in the routing.  XG: eights of rows of a segment.
+template <bool BF, int NC, int XG>
+__global__ __launch_bounds__(kThreads, 4) void dense_moe_up_kernel(DenseMoeArgs a, MoeLayout layout, int group_inv, int logits_vec, int kw_log2, int nb,
+                                                                  int tables_bytes) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  constexpr int NR = 2, D = 2, kTiles = NR * TT;
+  constexpr int TT = (XG + 1) / 2, kSegRows = 8 * XG;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int slots = a.T * a.k, E = a.experts, K = a.hidden, I = a.inter;
   MoeTables tab;
-  tab.mask = reinterpret_cast<uint64_t*>(smem);
+  tab.totals = reinterpret_cast<uint64_t*>(smem);
+  tab.mask = tab.totals + 8;
   tab.slot_id = reinterpret_cast<int*>(tab.mask + E);
   tab.slot_w = reinterpret_cast<float*>(tab.slot_id + slots);
   tab.row_token = reinterpret_cast<int*>(tab.slot_w + slots);
   tab.row_w = reinterpret_cast<float*>(tab.row_token + slots);
-  tab.segs = reinterpret_cast<int2*>(tab.row_w + slots);
-  tab.totals = reinterpret_cast<int*>(tab.segs + slots);
-  uint8_t* const rest = smem + moe_tables_bytes(E, slots);
+  tab.segs = reinterpret_cast<MoeSegment*>(tab.row_w + slots);
+  uint8_t* const rest = smem + tables_bytes;
   GateScratch<NC>& gate = reinterpret_cast<GateScratch<NC>*>(rest)[wave];
-  float4_t* const sums = reinterpret_cast<float4_t*>(rest);  // [2][waves][kTiles][64]
 
   // ---- routing ----
   if (tid < E) tab.mask[tid] = 0;
@@ -108,31 +110,31 @@ __global__ __launch_bounds__(kThreads, 4) void dense_moe_up_kernel(DenseMoeArgs 
     __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
-  // Rows, segments and chosen experts in front of each expert: three sums in one number of 16 bits each.
+  // Rows and segments in front of each expert: two sums in one number.
   const uint64_t mine = tid < E ? tab.mask[tid] : 0;
-  const int n_rows = __popcll(mine), n_segs = (n_rows + 16 * TT - 1) / (16 * TT);
-  const uint64_t own = static_cast<uint64_t>(n_rows) | static_cast<uint64_t>(n_segs) << 16 | static_cast<uint64_t>(mine != 0) << 32;
-  uint64_t upto = own;
+  const int n_rows = __popcll(mine), n_segs = (n_rows + kSegRows - 1) / kSegRows;
+  const uint32_t own = static_cast<uint32_t>(n_rows) | static_cast<uint32_t>(n_segs) << 16;
+  uint32_t upto = own;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const uint64_t other = __shfl_up(upto, d);
+    const uint32_t other = __shfl_up(upto, d);
     if (lane >= d) upto += other;
   }
-  uint64_t* const wave_sums = reinterpret_cast<uint64_t*>(tab.totals);  // [8]
-  if (lane == 63) wave_sums[wave] = upto;
+  if (lane == 63) tab.totals[wave] = upto;
   __syncthreads();
-  uint64_t before = upto - own, all = 0;
+  uint32_t before = upto - own, all = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    const uint64_t v = wave_sums[w];
+    const uint32_t v = static_cast<uint32_t>(tab.totals[w]);
     if (w < wave) before += v;
     all += v;
   }
-  const int row0 = static_cast<int>(before & 0xffff), segs_all = static_cast<int>(all >> 16 & 0xffff);
+  const int row0 = before & 0xffff, segs_all = __builtin_amdgcn_readfirstlane(all >> 16);
   for (int s = 0; s < n_segs; ++s) {
-    const int n = n_rows - 16 * TT * s < 16 * TT ? n_rows - 16 * TT * s : 16 * TT;
-    tab.segs[static_cast<int>(before >> 16 & 0xffff) + s] = int2{tid, (row0 + 16 * TT * s) | n << 16};
+    const int left = n_rows - kSegRows * s;
+    tab.segs[(before >> 16) + s] = MoeSegment{tid, row0 + kSegRows * s, left < kSegRows ? left : kSegRows};
   }
+  // this expert's rows: its tokens in order, and their weights
   {
     uint64_t left = mine;
     for (int i = 0; i < n_rows; ++i) {
@@ -143,17 +145,18 @@ __global__ __launch_bounds__(kThreads, 4) void dense_moe_up_kernel(DenseMoeArgs 
         if (tab.slot_id[t * a.k + j] == tid) tab.row_w[row0 + i] = tab.slot_w[t * a.k + j];
     }
   }
+  __syncthreads();
   char* const ws = static_cast<char*>(a.workspace);
   if (blockIdx.x == 0) {
-    if (mine != 0) reinterpret_cast<MoeExpert*>(ws + layout.experts)[before >> 32 & 0xffff] = MoeExpert{tid, row0, mine};
-    if (tid == 0) *reinterpret_cast<int*>(ws) = static_cast<int>(all >> 32 & 0xffff);
+    for (int i = tid; i < segs_all; i += kThreads) reinterpret_cast<MoeSegment*>(ws + layout.segs)[i] = tab.segs[i];
+    for (int i = tid; i < slots; i += kThreads) reinterpret_cast<int*>(ws + layout.row_token)[i] = tab.row_token[i];
     for (int i = tid; i < (K + 15) / 16; i += kThreads) reinterpret_cast<int*>(ws + layout.tickets)[i] = 0;
+    if (tid == 0) *reinterpret_cast<int*>(ws) = segs_all;
   }
-  __syncthreads();
 
-  // ---- the product: items of 16 gate rows and their up rows of one segment ----
-  const int KW = 1 << kw_log2, kw = wave & (KW - 1), nw = wave >> kw_log2, NW = kWaves >> kw_log2, stride = gridDim.x * NW;
-  const int n_tiles = (I + 15) / 16, items = segs_all * n_tiles, first = blockIdx.x * NW + nw;
+  // ---- the product: items of 8 gate rows and their up rows of one segment ----
+  const int KW = 1 << kw_log2, kw = wave & (KW - 1), nw = wave >> kw_log2, stride = gridDim.x * (kWaves >> kw_log2);
+  const int n_tiles = (I + 7) / 8, items = segs_all * n_tiles, first = blockIdx.x * (kWaves >> kw_log2) + nw;
   const int rounds = (items + stride - 1) / stride;
   const int64_t pitch = static_cast<int64_t>(K) * 2;
   struct Item {
@@ -165,43 +168,34 @@ __global__ __launch_bounds__(kThreads, 4) void dense_moe_up_kernel(DenseMoeArgs 
     Item it;
     it.there = round < rounds && i < items;
     const int s = it.there ? i / n_tiles : 0;
-    const int2 seg = tab.segs[s];
-    it.e = __builtin_amdgcn_readfirstlane(seg.x);
-    const int v = __builtin_amdgcn_readfirstlane(seg.y);
-    it.row0 = v & 0xffff;
-    it.rows = v >> 16;
-    it.n0 = it.there ? (i - s * n_tiles) * 16 : 0;
+    const MoeSegment seg = tab.segs[s];
+    it.e = __builtin_amdgcn_readfirstlane(seg.e);
+    it.row0 = __builtin_amdgcn_readfirstlane(seg.row0);
+    it.rows = __builtin_amdgcn_readfirstlane(seg.rows);
+    it.n0 = it.there ? (i - s * n_tiles) * 8 : 0;
     return it;
   };
+  const rsrc_t x = dense_buffer(a.x, a.T * pitch);
   auto place_of = [&](int round) {
     const Item it = item_of(round);
-    StreamPlace<NR, TT> p;
+    StreamPlace<XG, 1> p;
+    p.k = kw * kStreamBlock;
     p.end = it.there ? K : 0;
-    const int64_t left = I - it.n0 < 16 ? I - it.n0 : 16;
 #pragma unroll
-    for (int i = 0; i < NR; ++i)
-      p.w[i] = dense_buffer(reinterpret_cast<const char*>(a.w13) + (static_cast<int64_t>(it.e) * 2 * I + static_cast<int64_t>(i) * I + it.n0) * pitch, left * pitch);
+    for (int i = 0; i < 2; ++i)  // (inter is a multiple of 8)
+      p.w[i] = dense_buffer(reinterpret_cast<const char*>(a.w13) + ((static_cast<int64_t>(it.e) * 2 + i) * I + it.n0) * pitch, 8 * pitch);
+    p.x[0] = x;
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      const int c = 16 * t + (lane & 15);
-      p.x_at[t] = static_cast<uint32_t>(tab.row_token[it.row0 + (c < it.rows ? c : it.rows - 1)]) * static_cast<uint32_t>(pitch);
+    for (int g = 0; g < XG; ++g) {
+      const int c = 8 * g + (lane >> 3);
+      p.x_at[g] = c < it.rows ? static_cast<uint32_t>(tab.row_token[it.row0 + c]) * static_cast<uint32_t>(pitch) : kNowhere;
     }
     return p;
   };
-  auto done = [&](int round, float4_t (&acc)[NR][TT]) {
-    if (KW > 1) {
-      float4_t* const buf = sums + (round & 1) * kWaves * kTiles * 64;
-#pragma unroll
-      for (int i = 0; i < NR; ++i)
-#pragma unroll
-        for (int t = 0; t < TT; ++t) buf[(wave * kTiles + i * TT + t) * 64 + lane] = acc[i][t];
-      __syncthreads();
+  auto done = [&](int round, float4_t (&acc)[TT]) {
+    if (KW > 1) {  // (two buffers in turn: one barrier a round)
+      stream_join(reinterpret_cast<float4_t*>(rest + kWaves * stream_ring<XG, 1>()) + (round & 1) * kWaves * TT * 64, wave, KW, acc);
       if (kw != 0) return;
-      for (int w = 1; w < KW; ++w)
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-          for (int t = 0; t < TT; ++t) acc[i][t] += buf[((wave + w) * kTiles + i * TT + t) * 64 + lane];
     }
     const Item it = item_of(round);
     const int n = it.n0 + 4 * (lane >> 4);
@@ -209,48 +203,62 @@ __global__ __launch_bounds__(kThreads, 4) void dense_moe_up_kernel(DenseMoeArgs 
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
       const int c = 16 * t + (lane & 15);
-      if (!it.there || c >= it.rows || n >= I) continue;
-      const int64_t row = it.row0 + c, at = row * I + n;
+      const float4_t g = acc[t], up = stream_up(g);
+      if (!it.there || c >= it.rows || lane >= 32) continue;
+      const int row = it.row0 + c;
+      const int64_t at = static_cast<int64_t>(row) * I + n;
       const float w = tab.row_w[row];
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        const float f = w * (dense_act(acc[0][t][v], a.act) * acc[1][t][v]);
+        const float f = w * (dense_act(g[v], a.act) * up[v]);
         hi[v] = BF ? f2bf(f) : f2h(f);
-        const float rounded = BF ? bf2f(hi[v]) : h2f(hi[v]), rest = f - rounded;
-        lo[v] = __builtin_fabsf(rounded) <= 3.402823466e38f ? (BF ? f2bf(rest) : f2h(rest)) : 0u;  // (nothing is left of an infinity)
+        const float rounded = BF ? bf2f(hi[v]) : h2f(hi[v]), left = f - rounded;
+        lo[v] = __builtin_fabsf(rounded) <= 3.402823466e38f ? (BF ? f2bf(left) : f2h(left)) : 0u;  // (nothing is left of an infinity)
       }
       *reinterpret_cast<uint2*>(h + at) = uint2{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16};
       *reinterpret_cast<uint2*>(h + static_cast<int64_t>(slots) * I + at) = uint2{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16};
     }
   };
-  dense_stream<BF, NR, TT, D>(K, kw, KW, nb, rounds, dense_buffer(a.x, a.T * pitch), place_of, done);
+  __syncthreads();  // (the routing's part of LDS is the rings' now)
+  dense_stream<BF, XG>(rest + wave * stream_ring<XG, 1>(), static_cast<uint32_t>(pitch), KW * kStreamBlock, nb, rounds, place_of, done);
 }
 
-// Sixteen columns of the output and all tokens a workgroup, 16 TT of them at most; gridDim.y workgroups share the chosen experts' K.
-template <bool BF, int TT>
-__global__ __launch_bounds__(kThreads, TT == 1 ? 4 : 2) void dense_moe_down_kernel(DenseMoeArgs a, MoeLayout layout) {
-  constexpr int D = 2;
-  __shared__ MoeExpert experts[512];
-  __shared__ __attribute__((aligned(16))) float4_t sums[kWaves][TT][64];
-  __shared__ int last_one;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
-  char* const ws = static_cast<char*>(a.workspace);
-  const int chosen = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(ws));
-  for (int i = tid; i < chosen; i += kThreads) experts[i] = reinterpret_cast<const MoeExpert*>(ws + layout.experts)[i];
-  __syncthreads();
-  const int H = a.hidden, I = a.inter, n0 = blockIdx.x * 16, per = (I + kStreamBlock - 1) / kStreamBlock;  // blocks an expert
-  const int64_t blocks = static_cast<int64_t>(chosen) * per;
-  const int64_t begin = blocks * blockIdx.y / gridDim.y, end = blocks * (blockIdx.y + 1) / gridDim.y;
-  const int64_t pitch = static_cast<int64_t>(I) * 2, plane = static_cast<int64_t>(a.T) * a.k * pitch;
-  const rsrc_t h_hi = dense_buffer(ws + layout.h, plane), h_lo = dense_buffer(ws + layout.h + plane, plane);
-  const int64_t w_bytes = (H - n0 < 16 ? H - n0 : 16) * pitch;
-  const uint32_t w_at = static_cast<uint32_t>(lane & 15) * static_cast<uint32_t>(pitch);
+template <bool BF>
+__device__ __forceinline__ void moe_store(uint16_t* to, const float4_t& v) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = BF ? f2bf(v[i]) : f2h(v[i]);
+  *reinterpret_cast<uint2*>(to) = uint2{u[0] | u[1] << 16, u[2] | u[3] << 16};
+}
 
-  // this wave's blocks: every kWaves-th; (expert, block of it) of the next one to load, and of the one to compute
+// Sixteen columns of the output for all tokens a workgroup; gridDim.y workgroups share the K, which is all segments' inter.
+template <bool BF, int XG>
+__global__ __launch_bounds__(kThreads, XG == 1 ? 4 : 2) void dense_moe_down_kernel(DenseMoeArgs a, MoeLayout layout) {
+  constexpr int D = kStreamDepth, TT = (XG + 1) / 2, kStage = stream_stage<XG, 2>();
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
+  const int slots = a.T * a.k;
+  char* const ws = static_cast<char*>(a.workspace);
+  uint8_t* const ring = smem + wave * stream_ring<XG, 2>();
+  float4_t* const sums = reinterpret_cast<float4_t*>(smem + kWaves * stream_ring<XG, 2>());  // [waves][T][4]
+  int* const row_token = reinterpret_cast<int*>(sums + kWaves * a.T * 4);                     // [T k]
+  MoeSegment* const segs = reinterpret_cast<MoeSegment*>(row_token + slots);                  // [T k at most]
+  const int n_segs = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(ws));
+  for (int i = tid; i < slots; i += kThreads) row_token[i] = reinterpret_cast<const int*>(ws + layout.row_token)[i];
+  for (int i = tid; i < n_segs; i += kThreads) segs[i] = reinterpret_cast<const MoeSegment*>(ws + layout.segs)[i];
+  for (int i = tid; i < kWaves * a.T * 4; i += kThreads) sums[i] = float4_t{};
+  __syncthreads();
+  const int H = a.hidden, I = a.inter, n0 = blockIdx.x * 16, per = (I + kStreamBlock - 1) / kStreamBlock;  // blocks a segment
+  const int blocks = n_segs * per;
+  const int begin = static_cast<int>(static_cast<int64_t>(blocks) * blockIdx.y / gridDim.y);
+  const int end = static_cast<int>(static_cast<int64_t>(blocks) * (blockIdx.y + 1) / gridDim.y);
+  const int64_t pitch = static_cast<int64_t>(I) * 2, plane = slots * pitch;
+  const rsrc_t h_hi = dense_buffer(ws + layout.h, plane), h_lo = dense_buffer(ws + layout.h + plane, plane);
+
+  // this wave's blocks: every kWaves-th; (segment, block of it) of the next one to load, and of the one to compute
   struct At {
-    int64_t b;
-    int i, kb;
+    int b, i, kb;
   };
   auto next = [&](At& at) {
     at.b += kWaves;
@@ -260,44 +268,38 @@ __global__ __launch_bounds__(kThreads, TT == 1 ? 4 : 2) void dense_moe_down_kern
       ++at.i;
     }
   };
-  At load_at{begin + wave, static_cast<int>((begin + wave) / per), static_cast<int>((begin + wave) % per)}, now = load_at;
-  int4_t wq[D][2], hq[D][TT][2], lq[D][TT][2];
+  At ahead{begin + wave, (begin + wave) / per, (begin + wave) % per}, now = ahead;
   auto load = [&](int s) {
-    const bool there = load_at.b < end;
-    const MoeExpert ex = experts[there ? load_at.i : 0];
-    const int e = __builtin_amdgcn_readfirstlane(ex.e);
-    const rsrc_t w = dense_buffer(reinterpret_cast<const char*>(a.w2) + (static_cast<int64_t>(e) * H + n0) * pitch, there ? w_bytes : 0);
-    uint32_t row_at[TT];
+    const bool there = ahead.b < end;
+    const MoeSegment seg = segs[there ? ahead.i : 0];
+    const int64_t e = __builtin_amdgcn_readfirstlane(seg.e);
+    StreamPlace<XG, 2> p;
+    p.end = there ? I : 0;
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      const int token = 16 * t + (lane & 15);
-      row_at[t] = there && (ex.mask >> token & 1) ? static_cast<uint32_t>(ex.row0 + __popcll(ex.mask & ((1ull << token) - 1))) * static_cast<uint32_t>(pitch) : kNowhere;
+    for (int i = 0; i < 2; ++i) {
+      const int64_t left = H - n0 - 8 * i;
+      p.w[i] = dense_buffer(reinterpret_cast<const char*>(a.w2) + (e * H + n0 + 8 * i) * pitch, left > 0 ? 8 * pitch : 0);  // (hidden is a multiple of 8)
     }
+    p.x[0] = h_hi;
+    p.x[1] = h_lo;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = load_at.kb * kStreamBlock + 32 * h + 8 * quad;
-      const bool in = k < I;
-      wq[s][h] = dense_chunk(w, in ? w_at + 2u * k : kNowhere);
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        const uint32_t at = in && row_at[t] != kNowhere ? row_at[t] + 2u * k : kNowhere;
-        hq[s][t][h] = dense_chunk(h_hi, at);
-        lq[s][t][h] = dense_chunk(h_lo, at);
-      }
+    for (int g = 0; g < XG; ++g) {
+      const int c = 8 * g + (lane >> 3);
+      p.x_at[g] = c < seg.rows ? static_cast<uint32_t>(seg.row0 + c) * static_cast<uint32_t>(pitch) : kNowhere;
     }
-    next(load_at);
+    stream_load(p, ahead.kb * kStreamBlock, static_cast<uint32_t>(pitch), ring + s * kStage);
+    next(ahead);
   };
-  float4_t acc[TT], part[TT];
+  float4_t acc[TT];
 #pragma unroll
-  for (int t = 0; t < TT; ++t) acc[t] = part[t] = float4_t{};
-  auto join = [&](int i) {  // the sums of expert i go to the tokens that chose it
-    const uint64_t mask = experts[i].mask;
+  for (int t = 0; t < TT; ++t) acc[t] = float4_t{};
+  auto join = [&](int i) {  // a segment's sums go to its tokens'
+    const MoeSegment seg = segs[i];
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      const bool mine = mask >> (16 * t + (lane & 15)) & 1;
-#pragma unroll
-      for (int v = 0; v < 4; ++v) acc[t][v] += mine ? part[t][v] : 0.f;
-      part[t] = float4_t{};
+      const int c = 16 * t + (lane & 15);
+      if (c < seg.rows) sums[(wave * a.T + row_token[seg.row0 + c]) * 4 + quad] += acc[t];
+      acc[t] = float4_t{};
     }
   };
 #pragma unroll
@@ -310,101 +312,98 @@ __global__ __launch_bounds__(kThreads, TT == 1 ? 4 : 2) void dense_moe_down_kern
         join(current);
         current = now.i;
       }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-          part[t] = dense_mfma<BF>(wq[s][h], hq[s][t][h], part[t]);
-          part[t] = dense_mfma<BF>(wq[s][h], lq[s][t][h], part[t]);
-        }
+      stream_wait<XG, 2>();
+      stream_block<BF, XG, 2>(ring + s * kStage, acc);  // (past the end: zeros)
       next(now);
       load(s);
-      __builtin_amdgcn_sched_barrier(0);
     }
   }
   if (begin + wave < end) join(current);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
 
-#pragma unroll
-  for (int t = 0; t < TT; ++t) sums[wave][t][lane] = acc[t];
-  __syncthreads();
-  // The waves' sums in their order: thread (token, four columns).
-  const int token = 16 * (tid >> 6) + (lane & 15), n = n0 + 4 * quad;
-  const bool mine = tid < 64 * TT && token < a.T && n < H;
-  float4_t v = {};
-  if (mine) {
-    for (int w = 0; w < kWaves; ++w) v += sums[w][tid >> 6][lane];
+  // The waves' sums in their order: a thread four columns of a token.
+  for (int i = tid; i < a.T * 4; i += kThreads) {
+    const int n = n0 + 4 * (i & 3);
+    float4_t v = sums[i];
+    for (int w = 1; w < kWaves; ++w) v += sums[w * a.T * 4 + i];
+    sums[i] = v;
+    if (gridDim.y == 1 && n < H) moe_store<BF>(a.out + static_cast<int64_t>(i >> 2) * H + n, v);
   }
-  auto store = [&](const float4_t& o) {
-    uint32_t u[4];
+  if (gridDim.y == 1) return;
+  // Shares of several workgroups: the one that comes last adds them all, in their order.  They go past the L2 of a die (agent-scope stores
+  // and loads) and are there before the ticket is drawn; a fence would write back the die's whole L2 instead, which took 100 us.
+  float* const shares = reinterpret_cast<float*>(ws + layout.shares);  // [shares][tiles][T][16]
+  auto share_of = [&](int s) { return shares + (static_cast<int64_t>(s) * gridDim.x + blockIdx.x) * a.T * 16; };
+  for (int i = tid; i < a.T * 4; i += kThreads)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = BF ? f2bf(o[i]) : f2h(o[i]);
-    *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(token) * H + n) = uint2{u[0] | u[1] << 16, u[2] | u[3] << 16};
-  };
-  if (gridDim.y == 1) {
-    if (mine) store(v);
-    return;
-  }
-  // Shares of several workgroups: the one that comes last adds them all, in their order.
-  float4_t* const shares = reinterpret_cast<float4_t*>(ws + layout.shares);  // [shares][tiles][T][4]
-  auto place = [&](int s) { return ((static_cast<int64_t>(s) * gridDim.x + blockIdx.x) * a.T + token) * 4 + quad; };
-  if (mine) shares[place(blockIdx.y)] = v;
-  __threadfence();
+    for (int v = 0; v < 4; ++v) __hip_atomic_store(share_of(blockIdx.y) + 4 * i + v, sums[i][v], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (tid == 0) last_one = atomicAdd(reinterpret_cast<int*>(ws + layout.tickets) + blockIdx.x, 1) == static_cast<int>(gridDim.y) - 1;
+  int* const last_one = reinterpret_cast<int*>(smem);  // (the rings are done with)
+  if (tid == 0)
+    *last_one = __hip_atomic_fetch_add(reinterpret_cast<int*>(ws + layout.tickets) + blockIdx.x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+               static_cast<int>(gridDim.y) - 1;
   __syncthreads();
-  if (!last_one) return;
-  __threadfence();
-  if (mine) {
-    v = float4_t{};
-    for (int s = 0; s < static_cast<int>(gridDim.y); ++s) v += shares[place(s)];
-    store(v);
+  if (!*last_one) return;
+  for (int i = tid; i < a.T * 4; i += kThreads) {
+    float4_t v = {};
+    for (int s = 0; s < static_cast<int>(gridDim.y); ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += __hip_atomic_load(share_of(s) + 4 * i + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int n = n0 + 4 * (i & 3);
+    if (n < H) moe_store<BF>(a.out + static_cast<int64_t>(i >> 2) * H + n, v);
   }
 }
 
 int64_t dense_moe_workspace_bytes(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k) { return moe_layout(T, hidden, inter, experts, k).bytes; }
 
-template <bool BF, int NC, int TT>
+template <class Kernel>
+static hipError_t may_use(Kernel* kern, size_t lds) {
+  return lds > 65536 ? allow_large_lds(reinterpret_cast<const void*>(kern)) : hipSuccess;
+}
+
+template <bool BF, int NC, int XG>
 static hipError_t launch_up(const DenseMoeArgs& a, const MoeLayout& layout, hipStream_t s) {
-  const int slots = a.T * a.k, n_tiles = (a.inter + 15) / 16;
-  const StreamPlan plan = stream_plan(experts_chosen(a.T, a.experts, a.k) * n_tiles, a.hidden, 2, kTarget);
-  const int64_t most = static_cast<int64_t>(slots < a.experts ? slots : a.experts + slots / (16 * TT)) * n_tiles;  // items
+  const int slots = a.T * a.k, n_tiles = a.inter / 8;
+  const StreamPlan plan = stream_plan(a.hidden);
+  const int64_t most = static_cast<int64_t>(slots < a.experts ? slots : a.experts + slots / (8 * XG)) * n_tiles;  // items
   const int nw = kWaves >> plan.kw_log2;
   const int64_t sets = (most + nw - 1) / nw;
-  const size_t sums = plan.kw_log2 > 0 ? 2 * kWaves * 2 * TT * 1024 : 0, gate = kWaves * sizeof(GateScratch<NC>);
-  const size_t lds = moe_tables_bytes(a.experts, slots) + (sums > gate ? sums : gate);
-  auto* kern = dense_moe_up_kernel<BF, NC, TT>;
-  if (lds > 65536) {
-    const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kern));
-    if (e != hipSuccess) return e;
-  }
+  const size_t tables = moe_tables_bytes(a.experts, slots), gate = kWaves * sizeof(GateScratch<NC>);
+  const size_t rings = kWaves * (stream_ring<XG, 1>() + (plan.kw_log2 > 0 ? 2 * ((XG + 1) / 2) * 1024 : 0)), lds = tables + (rings > gate ? rings : gate);
+  auto* kern = dense_moe_up_kernel<BF, NC, XG>;
+  const hipError_t e = may_use(kern, lds);
+  if (e != hipSuccess) return e;
   const int vec = a.experts % 8 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0;
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(sets < 512 ? sets : 512)), dim3(kThreads), lds, s, a, layout, gate_group_inv(a.experts, a.groups),
-                     vec, plan.kw_log2, plan.nb);
+                     vec, plan.kw_log2, plan.nb, static_cast<int>(tables));
   return hipGetLastError();
 }
 
-template <bool BF>
+template <bool BF, int XG>
 static hipError_t launch(const DenseMoeArgs& a, hipStream_t s) {
   const MoeLayout layout = moe_layout(a.T, a.hidden, a.inter, a.experts, a.k);
-  auto up = [&](auto nc) {
-    constexpr int NC = decltype(nc)::value;
-    return a.T <= 16 ? launch_up<BF, NC, 1>(a, layout, s) : launch_up<BF, NC, 2>(a, layout, s);
-  };
-  hipError_t e = a.experts <= 64    ? up(std::integral_constant<int, 2>{})
-                 : a.experts <= 128 ? up(std::integral_constant<int, 4>{})
-                 : a.experts <= 256 ? up(std::integral_constant<int, 8>{})
-                                    : up(std::integral_constant<int, 16>{});
+  const hipError_t e = a.experts <= 64    ? launch_up<BF, 2, XG>(a, layout, s)
+                       : a.experts <= 128 ? launch_up<BF, 4, XG>(a, layout, s)
+                       : a.experts <= 256 ? launch_up<BF, 8, XG>(a, layout, s)
+                                          : launch_up<BF, 16, XG>(a, layout, s);
   if (e != hipSuccess) return e;
   const int shares = moe_shares(a.T, a.hidden, a.inter, a.experts, a.k);
   const dim3 grid(static_cast<unsigned>((a.hidden + 15) / 16), static_cast<unsigned>(shares));
-  note_kernel("dense_moe, %d shares", shares);
-  auto down = [&](auto* kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, s, a, layout); };
-  if (a.T <= 16) down(dense_moe_down_kernel<BF, 1>);
-  else if (a.T <= 32) down(dense_moe_down_kernel<BF, 2>);
-  else down(dense_moe_down_kernel<BF, 4>);
+  note_kernel("dense_moe up to %d rows, %d shares", 8 * XG, shares);
+  const size_t lds = kWaves * (stream_ring<XG, 2>() + a.T * 64) + static_cast<size_t>(a.T) * a.k * (4 + sizeof(MoeSegment));
+  auto* kern = dense_moe_down_kernel<BF, XG>;
+  const hipError_t d = may_use(kern, lds);
+  if (d != hipSuccess) return d;
+  hipLaunchKernelGGL(kern, grid, dim3(kThreads), lds, s, a, layout);
   return hipGetLastError();
 }
 
-hipError_t launch_dense_moe(const DenseMoeArgs& a, hipStream_t s) { return a.bf16 ? launch<true>(a, s) : launch<false>(a, s); }
+hipError_t launch_dense_moe(const DenseMoeArgs& a, hipStream_t s) {
+  const int eights = moe_eights(a.T, a.experts, a.k);
+  if (a.bf16) return eights == 1 ? launch<true, 1>(a, s) : launch<true, 2>(a, s);
+  return eights == 1 ? launch<false, 1>(a, s) : launch<false, 2>(a, s);
+}
 
 }  // namespace gq

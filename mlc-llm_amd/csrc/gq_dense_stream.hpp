@@ -1,8 +1,11 @@
-// The core of the products of few rows: weights stream from memory into registers and through the matrix instruction once.
+// The core of the products of few rows: weights stream from memory through LDS and the matrix instruction once, bound by HBM.
 //
-// An operand of v_mfma_f32_16x16x32 is 16 rows by 32 numbers of K, 8 of them a lane.  A wave takes 16 rows of W (operand A) times 16
-// rows of x (operand B) in blocks of 64 of K: two loads of 16 rows x 64 bytes, which are the two halves of the same 128-byte lines.  x comes
-// from the caches in the same form.  D blocks are in flight while one is computed, also from one tile to the next: bound by HBM.
+// A block is 16 rows of W by 64 numbers of K, 128 bytes of a row, and the same part of 8 XG rows of x.  Loads go past the registers into
+// the wave's own ring in LDS, eight rows of whole 128-byte lines an instruction, D blocks ahead of their use, without a barrier: the wave waits
+// for its own loads alone.  From there v_mfma_f32_16x16x32 takes W as operand A and x as operand B.
+// Measured on the way here, 128256 x 4096 of 5 rows: operands loaded straight into registers, 64 bytes of 16 rows an instruction, 175 us; the same
+// with `nt` loads (of lines that are read once), which then come for every half of a line, 196; whole lines through LDS 170, with `nt` 156, and x
+// on the same way 153 = 6.85 TB/s, what a large copy's reads reach.  16 rows of 4096 x 14336 in these forms: 31, 36, 27, 26 and 23.6 us.
 #pragma once
 
 #include "gq_dense_common.hpp"
@@ -10,91 +13,139 @@
 namespace gq {
 
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
-constexpr uint32_t kNowhere = 0xffffffffu;  // past any buffer's end: reads as zeros, and asks the memory for nothing
+constexpr uint32_t kNowhere = 0xc0000000u;  // past the end of any buffer here, also with an offset into a row behind it: reads as zeros
+constexpr int64_t kReach = 0xc0000000ll;    // bytes of a buffer, below
 constexpr int kStreamBlock = 64;            // numbers of K in a block
+constexpr int kStreamWaves = 8;             // of a workgroup
+constexpr int kStreamDepth = 2;             // blocks in flight, D
 
 __device__ __forceinline__ rsrc_t dense_buffer(const void* base, int64_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(bytes > 0xfffffff0ll ? 0xfffffff0u : static_cast<uint32_t>(bytes)),
-                                           0x00027000);
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(bytes < kReach ? static_cast<uint32_t>(bytes) : kNowhere), 0x00027000);
 }
-__device__ __forceinline__ int4_t dense_chunk(rsrc_t r, uint32_t at) {
-  return __builtin_bit_cast(int4_t, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+// 16 bytes a lane into LDS at lds + 16 * lane.  ONCE: weights, which no other load will ask for (`nt`).
+template <bool ONCE>
+__device__ __forceinline__ void dense_to_lds(rsrc_t r, uint32_t at, uint8_t* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, at, 0, 0, ONCE ? 2 : 0);
 }
 
-// What a wave works on: NR times 16 rows of W, each from the start of its buffer (which ends behind the last row that is there: the
-// others read as zeros), and TT times 16 rows of x.  end: K, or 0 for nothing.
-template <int NR, int TT>
+// What a wave works on: twice eight rows of W, each from the start of its buffer (which ends behind the last row that is there: the
+// others read as zeros), and XG times eight rows of x, in PX planes whose products add up.
+template <int XG, int PX>
 struct StreamPlace {
-  rsrc_t w[NR];
-  uint32_t x_at[TT];  // byte offset of this lane's row of x
-  int end;
+  rsrc_t w[2];
+  rsrc_t x[PX];
+  uint32_t x_at[XG];  // byte offset of this lane's row of x, row lane / 8 of eight
+  int k, end;         // this wave's first number of K and the end of K in a row (0: nothing to do)
 };
 
-// `rounds` places one after the other.  This wave takes every KW-th block of K from block kw on, nb blocks of each place (a multiple of D; past
-// K they are zeros).  place_of(round) gives a place, done(round, sums) takes its sums: the lane holds row lane % 16 of x, rows
-// 4 (lane / 16) .. + 3 of W.
-template <bool BF, int NR, int TT, int D, class PlaceOf, class Done>
-__device__ __forceinline__ void dense_stream(int K, int kw, int KW, int nb, int rounds, rsrc_t x, PlaceOf place_of, Done done) {
-  const int lane = threadIdx.x & 63, quad = lane >> 4;
-  const uint32_t w_at = static_cast<uint32_t>(lane & 15) * static_cast<uint32_t>(K) * 2u;
-  int4_t wq[D][NR][2], xq[D][TT][2];
-  auto load = [&](const StreamPlace<NR, TT>& p, int j, int s) {
+template <int XG, int PX>
+constexpr int stream_stage() { return 2048 + PX * XG * 1024; }
+template <int XG, int PX>
+constexpr int stream_ring() { return kStreamDepth * stream_stage<XG, PX>(); }
+
+// One block from number k of the rows on, into a stage.  Chunk c of 16 bytes of a row lies at place c ^ (row & 7), so that the 16 lanes that LDS
+// serves at a time meet all its banks.
+template <int XG, int PX>
+__device__ __forceinline__ void stream_load(const StreamPlace<XG, PX>& p, int k, uint32_t w_pitch, uint8_t* stage) {
+  const int lane = threadIdx.x & 63, kc = k + 8 * ((lane & 7) ^ (lane >> 3));  // a chunk of 8; K is a multiple of 8
+  const bool in = kc < p.end;
+  const uint32_t w_at = in ? static_cast<uint32_t>(lane >> 3) * w_pitch + 2u * kc : kNowhere;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = (j * KW + kw) * kStreamBlock + 32 * h + 8 * quad;  // a chunk of 8; K is a multiple of 8
-      const bool in = k < p.end;
+  for (int i = 0; i < 2; ++i) dense_to_lds<true>(p.w[i], w_at, stage + 1024 * i);
 #pragma unroll
-      for (int i = 0; i < NR; ++i) wq[s][i][h] = dense_chunk(p.w[i], in ? w_at + 2u * k : kNowhere);
+  for (int g = 0; g < XG; ++g) {
+    const uint32_t at = in ? p.x_at[g] + 2u * kc : kNowhere;
 #pragma unroll
-      for (int t = 0; t < TT; ++t) xq[s][t][h] = dense_chunk(x, in ? p.x_at[t] + 2u * k : kNowhere);
+    for (int i = 0; i < PX; ++i) dense_to_lds<false>(p.x[i], at, stage + 2048 + (i * XG + g) * 1024);
+  }
+}
+// Waits until all but the newest `newer` blocks have landed.
+template <int XG, int PX>
+__device__ __forceinline__ void stream_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStreamDepth - 1) * (2 + PX * XG)) : "memory");
+}
+// sums += the block in a stage; the lane holds row 16 t + lane % 16 of x and rows 4 (lane / 16) .. + 3 of W.
+template <bool BF, int XG, int PX>
+__device__ __forceinline__ void stream_block(const uint8_t* stage, float4_t (&acc)[(XG + 1) / 2]) {
+  constexpr int TT = (XG + 1) / 2;
+  const int lane = threadIdx.x & 63, quad = lane >> 4, row = lane & 15;
+  const int c0 = (quad ^ (row & 7)) << 4, c1 = ((quad + 4) ^ (row & 7)) << 4;
+  const int4_t w0 = *reinterpret_cast<const int4_t*>(stage + row * 128 + c0), w1 = *reinterpret_cast<const int4_t*>(stage + row * 128 + c1);
+#pragma unroll
+  for (int i = 0; i < PX; ++i)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      // (eight rows of x: rows 8 to 15 of the operand are those again, and their sums nobody's)
+      const uint8_t* const x = stage + 2048 + i * XG * 1024 + (XG == 1 ? row & 7 : 16 * t + row) * 128;
+      acc[t] = dense_mfma<BF>(w0, *reinterpret_cast<const int4_t*>(x + c0), acc[t]);
+      acc[t] = dense_mfma<BF>(w1, *reinterpret_cast<const int4_t*>(x + c1), acc[t]);
     }
-  };
-  StreamPlace<NR, TT> here = place_of(0);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read, before the stage is loaded again)
+}
+
+// `rounds` places one after the other, of each nb blocks (a multiple of D), `step` numbers of K apart; past K they are zeros.  place_of(round)
+// gives a place, done(round, sums) takes its sums.
+template <bool BF, int XG, class PlaceOf, class Done>
+__device__ __forceinline__ void dense_stream(uint8_t* ring, uint32_t w_pitch, int step, int nb, int rounds, PlaceOf place_of, Done done) {
+  constexpr int D = kStreamDepth, TT = (XG + 1) / 2, kStage = stream_stage<XG, 1>();
+  StreamPlace<XG, 1> here = place_of(0);
 #pragma unroll
-  for (int s = 0; s < D; ++s) load(here, s, s);
+  for (int s = 0; s < D; ++s) stream_load(here, here.k + s * step, w_pitch, ring + s * kStage);
   for (int round = 0; round < rounds; ++round) {
-    float4_t acc[NR][TT];
+    float4_t acc[TT];
 #pragma unroll
-    for (int i = 0; i < NR; ++i)
-#pragma unroll
-      for (int t = 0; t < TT; ++t) acc[i][t] = float4_t{};
-    auto compute = [&](int s) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-          for (int t = 0; t < TT; ++t) acc[i][t] = dense_mfma<BF>(wq[s][i][h], xq[s][t][h], acc[i][t]);
-    };
+    for (int t = 0; t < TT; ++t) acc[t] = float4_t{};
     for (int j = D; j < nb; j += D) {
 #pragma unroll
       for (int s = 0; s < D; ++s) {
-        compute(s);
-        load(here, j + s, s);
-        __builtin_amdgcn_sched_barrier(0);  // a block after the other: operands of all would not fit the registers twice
+        stream_wait<XG, 1>();
+        stream_block<BF, XG, 1>(ring + s * kStage, acc);
+        stream_load(here, here.k + (j + s) * step, w_pitch, ring + s * kStage);
       }
     }
     here = place_of(round + 1);
 #pragma unroll
     for (int s = 0; s < D; ++s) {
-      compute(s);
-      load(here, s, s);
-      __builtin_amdgcn_sched_barrier(0);
+      stream_wait<XG, 1>();
+      stream_block<BF, XG, 1>(ring + s * kStage, acc);
+      stream_load(here, here.k + s * step, w_pitch, ring + s * kStage);
     }
     done(round, acc);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (loads of nothing may still land in the ring)
 }
 
-// How a launch shares work: KW of a workgroup's eight waves take a share of K each, the fewest that keep the memory busy.
+// The sums of the KW waves that share an item, in the first one's acc; buf: kStreamWaves TT KiB, no use of it may be left.
+template <int TT>
+__device__ __forceinline__ void stream_join(float4_t* buf, int wave, int KW, float4_t (&acc)[TT]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int t = 0; t < TT; ++t) buf[(wave * TT + t) * 64 + lane] = acc[t];
+  __syncthreads();
+  if ((wave & (KW - 1)) != 0) return;
+  for (int w = 1; w < KW; ++w)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[t] += buf[((wave + w) * TT + t) * 64 + lane];
+}
+
+// Gated: rows 0 to 7 of a block are gates and rows 8 to 15 their up rows, two quarters of the wave apart.
+__device__ __forceinline__ float4_t stream_up(float4_t v) {
+  float4_t u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = __shfl_down(v[i], 32);
+  return u;
+}
+
+// KW of a workgroup's eight waves share the K of an item, as many as have D blocks each: the rows that a workgroup reads are long then.
 struct StreamPlan {
   int kw_log2, nb;
 };
-inline StreamPlan stream_plan(double items, int64_t K, int D, double target) {
+inline StreamPlan stream_plan(int64_t K) {
   const int64_t blocks = (K + kStreamBlock - 1) / kStreamBlock;
   int log2 = 0;
-  while (log2 < 3 && items * (1 << log2) < target && (blocks >> (log2 + 1)) * 2 > D) ++log2;
+  while (log2 < 3 && (blocks >> (log2 + 1)) >= kStreamDepth) ++log2;
   const int64_t each = (blocks + (1 << log2) - 1) >> log2;
-  return {log2, static_cast<int>((each + D - 1) / D * D)};
+  return {log2, static_cast<int>((each + kStreamDepth - 1) / kStreamDepth * kStreamDepth)};
 }
 
 }  // namespace gq

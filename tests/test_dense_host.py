@@ -71,7 +71,7 @@ def test_expert_layer_checks_its_arguments():
     _refused(moe(g=4, tg=5), "groups")
     _refused(moe(g=8, tg=1), "cannot give 2")
     _refused(moe(t=65), "64 tokens at most", _lib.ERR_UNSUPPORTED)
-    _refused(moe(t=64, i=(1 << 23) - 256, e=64, k=32), "4 GiB", _lib.ERR_UNSUPPORTED)
+    _refused(moe(t=64, i=(1 << 23) - 256, e=64, k=32), "3 GiB", _lib.ERR_UNSUPPORTED)
     for name in ("x", "lg", "w13", "w2", "out"):
         _refused(moe(**{name: None}), "null")
     for name in ("x", "w13", "w2", "out"):
