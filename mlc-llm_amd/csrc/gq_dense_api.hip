@@ -25,6 +25,8 @@ int hip_result(hipError_t e, const char* what) {
 }
 hipStream_t as_stream(mi355gq_stream_t s) { return static_cast<hipStream_t>(s); }
 
+bool few_rows(int64_t M) { return M <= 16; }
+
 // cols: of y
 int product(const char* what, const void* x, const void* w, const void* bias, const void* residual, int64_t M, int64_t cols, int64_t K,
             bool gated, int activation, int model_dtype, int out_dtype, void* y, void* workspace, int64_t workspace_bytes, mi355gq_stream_t stream) {
@@ -57,7 +59,11 @@ int product(const char* what, const void* x, const void* w, const void* bias, co
     a.workspace_bytes = workspace_bytes;
   }
   const hipStream_t s = as_stream(stream);
-  hipError_t e = gq::dense_aligned(a) ? gq::launch_dense_rows(a, s) : hipErrorNotSupported;
+  hipError_t e = hipErrorNotSupported;
+  if (gq::dense_aligned(a)) {
+    if (few_rows(M)) e = gq::launch_dense_rows(a, s);
+    if (e == hipErrorNotSupported) e = gq::launch_dense_tile(a, s);
+  }
   if (e == hipErrorNotSupported) e = gq::launch_dense_simple(a, s);
   return hip_result(e, what);
 }
@@ -74,9 +80,9 @@ bool moe_takes(int64_t T, int64_t inter, int64_t top_k) { return T <= gq::kMoeTo
 extern "C" {
 
 int64_t mi355gq_dense_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated) {
-  (void)gated;
-  if (!dim_ok(M) || !dim_ok(N) || !dim_ok(K) || M == 0 || N == 0 || K == 0) return 0;
-  return 0;
+  const int64_t rows_of_w = gated ? 2 * N : N;
+  if (!dim_ok(M) || !dim_ok(N) || !dim_ok(rows_of_w) || !dim_ok(K) || M == 0 || N == 0 || K == 0 || few_rows(M) || K % 8 != 0) return 0;
+  return gq::dense_tile_workspace_bytes(M, rows_of_w, K);
 }
 
 int mi355gq_dense_linear(const void* x, const void* w, const void* bias, const void* residual, int64_t M, int64_t N, int64_t K, int activation,

@@ -35,6 +35,10 @@ inline bool dense_aligned(const DenseArgs& a) {
 // Up to 16 rows of aligned operands; hipErrorNotSupported beyond.
 hipError_t launch_dense_rows(const DenseArgs& a, hipStream_t s);
 
+// Any number of aligned rows; K split over workgroups where the scratch for it is there.
+hipError_t launch_dense_tile(const DenseArgs& a, hipStream_t s);
+int64_t dense_tile_workspace_bytes(int64_t rows, int64_t N, int64_t K);
+
 // One expert layer on up to kMoeTokens tokens, see mi355gq_dense_moe.
 constexpr int kMoeTokens = 64;
 struct DenseMoeArgs {

@@ -114,6 +114,38 @@ def test_gated(m, n, k, dtype):
         close(ops.dense_linear_gated(x, w, bias=b, activation=act, out_dtype=out_dtype), gated_ref(x, w, b, act, out_dtype))
 
 
+@pytest.mark.parametrize("shares", [1, 3])
+@pytest.mark.parametrize("form", range(6))
+def test_tile_forms(form, shares):
+    """Every tile form, whole and in shares of K, on tiles that end inside in all directions."""
+    g = _gen(form * 10 + shares)
+    gq._lib.set_option("gemm_variant", form)
+    gq._lib.set_option("gemm_split_k", shares)
+    try:
+        for i, (m, n, k) in enumerate([(17, 40, 776), (33, 257, 1032), (200, 520, 776), (300, 129, 968), (521, 392, 1288)]):
+            dtype = HALVES[i % 2]
+            x, w, bias = _normal(g, dtype, m, k), _normal(g, dtype, n, k, scale=k**-0.5), _normal(g, dtype, n)
+            r = _normal(g, dtype, m, n)
+            got = ops.dense_linear(x, w, bias=bias, activation="gelu", residual=r)
+            assert f"{shares} shares" in gq._lib.last_kernel()
+            close(got, linear_ref(x, w, bias, "gelu", r, dtype))
+            x, w, bias = _normal(g, dtype, m, k), _normal(g, dtype, 2 * n, k, scale=k**-0.5), _normal(g, dtype, 2 * n)
+            close(ops.dense_linear_gated(x, w, bias=bias), gated_ref(x, w, bias, "silu", dtype))
+    finally:
+        gq._lib.set_option("gemm_variant", -1)
+        gq._lib.set_option("gemm_split_k", -1)
+
+
+@pytest.mark.parametrize("m,n,k", [(2048, 14500, 520), (300, 30000, 264)])
+def test_rest_of_the_last_round(m, n, k):
+    """More tiles than run at a time: columns in one form, the rest of them in another."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x = torch.randn(m, k, generator=g, device="cuda").to(torch.bfloat16)
+    w = (torch.randn(n, k, generator=g, device="cuda") / k**0.5).to(torch.bfloat16)
+    close(ops.dense_linear(x, w, activation="silu"), linear_ref(x, w, None, "silu", None, torch.bfloat16))
+    close(ops.dense_linear_gated(x, w), gated_ref(x, w, None, "silu", torch.bfloat16))
+
+
 @pytest.mark.parametrize("m", [1, 6, 20, 40, 130])
 def test_unaligned_pointers_and_leading_dimensions(m):
     """Tensors in the middle of others, at 2 bytes, and x of more than two dimensions."""
