@@ -1,5 +1,5 @@
 // The dense operators' way from a Python call to a kernel launch, in native code: argument checks, the output and scratch
-// allocation, the current stream and the C ABI call of linear / linear_silu_mul / embedding_take and of the 8-bit operators, one
+// allocation, the current stream and the C ABI call of linear / linear_silu_mul / embedding_take and of the operators on 8-bit and 16-bit weights, one
 // Python call each.
 //
 // What it replaces took 13 us of interpreter time per projection (a torch.cuda.Stream object, three Python checks per tensor, two
@@ -14,6 +14,7 @@
 
 #include <ATen/Functions.h>
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -384,6 +385,113 @@ PyObject* fp8_moe(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- operators on 16-bit weights: on x's GPU, whichever is current, and its current stream ----
+
+bool activation(PyObject* o, int* act) {
+  static const char* const names[] = {"relu", "silu", "gelu", "gelu_tanh"};
+  if (o == Py_None) {
+    *act = MI355GQ_ACT_NONE;
+    return true;
+  }
+  if (!PyUnicode_CheckExact(o)) return false;
+  for (int i = 0; i < 4; ++i)
+    if (PyUnicode_CompareWithASCIIString(o, names[i]) == 0) {
+      *act = MI355GQ_ACT_RELU + i;
+      return true;
+    }
+  return false;
+}
+
+bool half_code(ScalarType t, int* code) {
+  *code = model_code(t);
+  return *code == MI355GQ_F16 || *code == MI355GQ_BF16;
+}
+
+// a tensor of x's type and GPU with these sizes
+const Tensor* beside(PyObject* o, const Tensor& x, at::IntArrayRef sizes) {
+  const Tensor* t = plain(o);
+  return t && t->scalar_type() == x.scalar_type() && t->device() == x.device() && t->sizes() == sizes ? t : nullptr;
+}
+
+void* stream_of(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.device().index()).stream(); }
+
+// dense(x, weight, bias | None, activation | None, out_dtype | None, residual | None): GATED without the last
+template <bool GATED>
+PyObject* dense(PyObject* const* a, Py_ssize_t nargs) {
+  if (nargs != (GATED ? 5 : 6) || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+  const Tensor *x = plain(a[0]), *w = plain(a[1]), *bias = nullptr, *residual = nullptr;
+  int act = 0, code = 0;
+  if (!x || !w || x->dim() < 1 || w->dim() != 2 || !half_code(x->scalar_type(), &code) || w->scalar_type() != x->scalar_type() || w->device() != x->device() ||
+      !activation(a[3], &act))
+    Py_RETURN_NONE;
+  const int64_t k = x->size(-1), rows_of_w = w->size(0), n = GATED ? rows_of_w / 2 : rows_of_w, m = leading_rows(*x);
+  if (w->size(1) != k || k == 0 || m == 0 || n == 0 || (GATED && rows_of_w % 2)) Py_RETURN_NONE;
+  if (a[2] != Py_None && !(bias = beside(a[2], *x, {rows_of_w}))) Py_RETURN_NONE;
+  ScalarType out_dtype = x->scalar_type();
+  if (a[4] != Py_None) {
+    if (!THPDtype_Check(a[4])) Py_RETURN_NONE;
+    out_dtype = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
+    if (out_dtype != x->scalar_type() && out_dtype != ScalarType::Float) Py_RETURN_NONE;
+  }
+  const auto shape = with_last(*x, n);
+  if (!GATED && a[5] != Py_None && !(residual = beside(a[5], *x, shape))) Py_RETURN_NONE;
+  Tensor out;
+  int rc;
+  {
+    pybind11::gil_scoped_release release;
+    const c10::DeviceGuard guard(x->device());
+    out = at::empty(shape, x->options().dtype(out_dtype));
+    const int64_t bytes = mi355gq_dense_linear_workspace_bytes(m, n, k, GATED);
+    Scratch ws(*x, bytes);
+    const void *xp = x->const_data_ptr(), *wp = w->const_data_ptr(), *bp = bias ? bias->const_data_ptr() : nullptr;
+    if constexpr (GATED)
+      rc = mi355gq_dense_linear_gated(xp, wp, bp, m, n, k, act, code, model_code(out_dtype), out.mutable_data_ptr(), ws.ptr, bytes, stream_of(*x));
+    else
+      rc = mi355gq_dense_linear(xp, wp, bp, residual ? residual->const_data_ptr() : nullptr, m, n, k, act, code, model_code(out_dtype),
+                                out.mutable_data_ptr(), ws.ptr, bytes, stream_of(*x));
+  }
+  return result(rc, out);
+}
+PyObject* dense_linear(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  return dense<false>(a, nargs);
+  END_HANDLE_TH_ERRORS
+}
+PyObject* dense_linear_gated(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  return dense<true>(a, nargs);
+  END_HANDLE_TH_ERRORS
+}
+
+// dense_moe(x, w13, w2, activation | None, then moe_gating's arguments)
+PyObject* dense_moe(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Gating g;
+  int act = 0, code = 0;
+  if (nargs != 12 || at::impl::torch_function_mode_enabled() || !gating_args(a + 4, &g) || !activation(a[3], &act)) Py_RETURN_NONE;
+  const Tensor *x = plain(a[0]), *w2 = plain(a[2]);
+  if (!x || !w2 || x->dim() != 2 || w2->dim() != 3 || !half_code(x->scalar_type(), &code) || w2->scalar_type() != x->scalar_type()) Py_RETURN_NONE;
+  const int64_t t = x->size(0), experts = w2->size(0), hidden = w2->size(1), inter = w2->size(2);
+  const Tensor* w13 = beside(a[1], *x, {experts, 2 * inter, hidden});
+  if (!w13 || t == 0 || x->size(1) != hidden || w2->device() != x->device() || g.logits->device() != x->device() || g.logits->size(0) != t ||
+      g.logits->size(1) != experts || (g.bias && g.bias->device() != x->device()) || reinterpret_cast<uintptr_t>(x->const_data_ptr()) % 16)
+    Py_RETURN_NONE;
+  Tensor out;
+  int rc;
+  {
+    pybind11::gil_scoped_release release;
+    const c10::DeviceGuard guard(x->device());
+    out = at::empty(x->sizes(), x->options());
+    const int64_t bytes = mi355gq_dense_moe_workspace_bytes(t, hidden, inter, experts, g.k);
+    Scratch ws(*x, bytes);
+    rc = mi355gq_dense_moe(x->const_data_ptr(), g.logits->const_data_ptr(), g.bias ? g.bias->const_data_ptr() : nullptr, t, hidden, inter, experts, g.k,
+                           g.scoring, g.groups, g.top_groups, g.renormalize ? 1 : 0, g.scale, g.code, w13->const_data_ptr(), w2->const_data_ptr(), act,
+                           code, out.mutable_data_ptr(), ws.ptr, bytes, stream_of(*x));
+  }
+  return result(rc, out);
+  END_HANDLE_TH_ERRORS
+}
+
 // the current HIP stream of the current device, as a number
 PyObject* stream(PyObject*, PyObject*) {
   HANDLE_TH_ERRORS
@@ -400,6 +508,9 @@ PyMethodDef kMethods[] = {
     {"fp8_linear", GQ_FAST(fp8_linear), nullptr},
     {"moe_gating", GQ_FAST(moe_gating), nullptr},
     {"fp8_moe", GQ_FAST(fp8_moe), nullptr},
+    {"dense_linear", GQ_FAST(dense_linear), nullptr},
+    {"dense_linear_gated", GQ_FAST(dense_linear_gated), nullptr},
+    {"dense_moe", GQ_FAST(dense_moe), nullptr},
     {"stream", stream, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

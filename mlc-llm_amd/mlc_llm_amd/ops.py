@@ -989,6 +989,12 @@ def dense_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
 
     activation: None, "relu", "silu", "gelu" (v Phi(v)) or "gelu_tanh".  Sums and epilogue are float32 with one rounding, to out_dtype: x's
     type (the default) or float32.  residual has x's type and y's shape; as `out` too it is updated in place."""
+    native = _lib.native()
+    done = native.dense_linear(x, weight, bias, activation, out_dtype, residual) if native is not None and out is None else None
+    if isinstance(done, torch.Tensor):
+        return done
+    if done is not None:
+        raise _lib.failed("mi355gq_dense_linear", done)
     m, n, k, out_dtype = _dense_args(x, weight, bias, out_dtype, False)
     act = _activation(activation)
     shape = (*x.shape[:-1], n)
@@ -1014,6 +1020,12 @@ def dense_linear_gated(x: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
                        out_dtype=None) -> torch.Tensor:
     """act(gate) * up with gate, up = split(x . weight^T (+ bias), 2, axis=-1): the gate_up projection of an MLP with its activation, weight
     [2 inter, K] as gate rows, then up rows.  Types and activations as in dense_linear; one rounding, of the product."""
+    native = _lib.native()
+    done = native.dense_linear_gated(x, weight, bias, activation, out_dtype) if native is not None else None
+    if isinstance(done, torch.Tensor):
+        return done
+    if done is not None:
+        raise _lib.failed("mi355gq_dense_linear_gated", done)
     m, inter, k, out_dtype = _dense_args(x, weight, bias, out_dtype, True)
     act = _activation(activation)
     with torch.cuda.device(x.device):
@@ -1036,6 +1048,12 @@ def dense_moe(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w2: torc
     model dtypes) routed as moe_gating does with the same arguments, w13 [experts, 2 inter, hidden] (gate rows, then up rows) and w2
     [experts, hidden, inter] in x's type.  y[t] = sum over the chosen experts of their weight times w2 . (act(gate) * up), in float32
     sums with one rounding."""
+    native = _lib.native()
+    done = native.dense_moe(x, w13, w2, activation, logits, top_k, scoring, bias, num_groups, top_groups, renormalize, scale) if native is not None else None
+    if isinstance(done, torch.Tensor):
+        return done
+    if done is not None:
+        raise _lib.failed("mi355gq_dense_moe", done)
     _chk(x, _HALVES, "x")
     for t, name in ((w13, "w13"), (w2, "w2")):
         _chk(t, x.dtype, name)

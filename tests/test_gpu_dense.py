@@ -448,3 +448,33 @@ def test_moe_refuses_more_tokens():
         ops.dense_moe(x, logits, w13, w2, 2)
     assert err.value.code == gq._lib.ERR_UNSUPPORTED and "64 tokens at most" in err.value.message
     assert ops.dense_moe(x[:0], logits[:0], w13, w2, 2).shape == (0, 64)
+
+
+class Plain(torch.Tensor):
+    """A subclass: the native call path declines it, the Python route takes it."""
+
+
+@pytest.mark.parametrize("lead", [(1,), (2, 3), (40,), ()])
+def test_native_and_python_routes_agree(lead):
+    g, dtype, n, k = _gen(7), torch.bfloat16, 72, 136
+    x, w, b, r = _normal(g, dtype, *lead, k), _normal(g, dtype, n, k), _normal(g, dtype, n), _normal(g, dtype, *lead, n)
+    native = gq._lib.native()
+    for bias in (None, b):
+        for act in ACTS:
+            for out_dtype in (None, torch.float32):
+                for residual in (None, r):
+                    assert isinstance(native.dense_linear(x, w, bias, act, out_dtype, residual), torch.Tensor)
+                    got = ops.dense_linear(x, w, bias, act, residual, out_dtype)
+                    want = ops.dense_linear(x.as_subclass(Plain), w, bias, act, residual, out_dtype)
+                    assert got.dtype == want.dtype and got.shape == (*lead, n) and torch.equal(got, want.as_subclass(torch.Tensor))
+                    out = torch.empty_like(got)
+                    assert ops.dense_linear(x, w, bias, act, residual, out_dtype, out) is out and torch.equal(out, got)
+                assert isinstance(native.dense_linear_gated(x, w, bias, act, out_dtype), torch.Tensor)
+                got, want = ops.dense_linear_gated(x, w, bias, act, out_dtype), ops.dense_linear_gated(x.as_subclass(Plain), w, bias, act, out_dtype)
+                assert got.dtype == want.dtype and got.shape == (*lead, n // 2) and torch.equal(got, want.as_subclass(torch.Tensor))
+    x, logits, w13, w2 = _layer(g, dtype, 5, 128, 64, 8, torch.float16)
+    bias = torch.randn(8, device="cuda")
+    for how in ({}, {"scoring": "sigmoid", "bias": bias, "num_groups": 2, "top_groups": 1, "renormalize": False, "scale": 2.5, "activation": "gelu"}):
+        got, want = ops.dense_moe(x, logits, w13, w2, 2, **how), ops.dense_moe(x.as_subclass(Plain), logits, w13, w2, 2, **how)
+        assert torch.equal(got, want.as_subclass(torch.Tensor))
+    assert isinstance(native.dense_moe(x, w13, w2, "silu", logits, 2, "softmax", None, 1, 1, True, 1.0), torch.Tensor)
