@@ -115,7 +115,7 @@ def test_gated(m, n, k, dtype):
 
 
 @pytest.mark.parametrize("shares", [1, 3])
-@pytest.mark.parametrize("form", range(6))
+@pytest.mark.parametrize("form", range(9))
 def test_tile_forms(form, shares):
     """Every tile form, whole and in shares of K, on tiles that end inside in all directions."""
     g = _gen(form * 10 + shares)
