@@ -59,8 +59,6 @@ hipError_t launch_dense_moe(const DenseMoeArgs& a, hipStream_t s);
 // Any sizes and alignments; the kernel of the calls that the others do not take.
 hipError_t launch_dense_simple(const DenseArgs& a, hipStream_t s);
 
-__device__ __forceinline__ float dense_load(const uint16_t* p, int64_t i, int bf16) { return bf16 ? bf2f(p[i]) : h2f(p[i]); }
-
 // a 16 x 16 tile of float32 sums, W as operand A and x as operand B: lane l holds row l % 16 of x and rows 4 (l / 16) .. + 3 of W
 template <bool BF>
 __device__ __forceinline__ float4_t dense_mfma(int4_t w, int4_t x, float4_t acc) {
@@ -92,75 +90,84 @@ __device__ __forceinline__ float dense_gelu(float v) {
   return v * (v > 0.f ? 1.0f - tail : tail);
 }
 
-__device__ __forceinline__ float dense_act(float v, int act) {
-  switch (act) {  // (the same for the whole launch)
-    case ACT_RELU: return v > 0.f ? v : v != v ? v : 0.f;
-    case ACT_SILU: return v * dense_sigmoid(v);
-    case ACT_GELU: return dense_gelu(v);
-    // v / 2 (1 + tanh(u)) = v / (1 + exp(-2 u)), u = sqrt(2 / pi) (v + 0.044715 v^3)
-    case ACT_GELU_TANH: return v * dense_sigmoid(1.5957691216057308f * v * __builtin_fmaf(0.044715f * v, v, 1.0f));
-    default: return v;
+__device__ __forceinline__ float dense_gelu_tanh(float v) {
+  // v / 2 (1 + tanh(u)) = v / (1 + exp(-2 u)), u = sqrt(2 / pi) (v + 0.044715 v^3)
+  return v * dense_sigmoid(1.5957691216057308f * v * __builtin_fmaf(0.044715f * v, v, 1.0f));
+}
+__device__ __forceinline__ float dense_relu(float v) { return v > 0.f ? v : v != v ? v : 0.f; }
+// (one switch for all: `act` is the same for the whole launch)
+template <int CNT>
+__device__ __forceinline__ void dense_act(float (&o)[CNT], int act) {
+  auto all = [&](auto f) {
+#pragma unroll
+    for (int v = 0; v < CNT; ++v) o[v] = f(o[v]);
+  };
+  switch (act) {
+    case ACT_RELU: return all(dense_relu);
+    case ACT_SILU: return all([](float v) { return v * dense_sigmoid(v); });
+    case ACT_GELU: return all(dense_gelu);
+    case ACT_GELU_TANH: return all(dense_gelu_tanh);
+    default: return;
   }
 }
 
-// CNT (a multiple of 4) neighbouring 16-bit numbers as float32
-template <int CNT>
-__device__ __forceinline__ void dense_load_run(const uint16_t* p, int bf16, float (&f)[CNT]) {
+// one 16-bit number as float32, and two rounded ones side by side
+template <bool BF>
+__device__ __forceinline__ float dense_widen(uint32_t h) {
+  return BF ? bf2f(static_cast<uint16_t>(h)) : h2f(static_cast<uint16_t>(h));
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t dense_pair(float a, float b) {
+  typedef float float2_v __attribute__((ext_vector_type(2)));
+  if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_v{a, b}), bf16x2_dot_t));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_v{a, b}), half2_t));
+}
+
+// CNT (4 or 8) neighbouring 16-bit numbers, at 8 (16) bytes, as float32
+template <bool BF, int CNT>
+__device__ __forceinline__ void dense_load_run(const uint16_t* p, float (&f)[CNT]) {
+  uint32_t u[CNT / 2];
+  if constexpr (CNT == 8) {
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    u[0] = q.x, u[1] = q.y, u[2] = q.z, u[3] = q.w;
+  } else {
+    const uint2 q = *reinterpret_cast<const uint2*>(p);
+    u[0] = q.x, u[1] = q.y;
+  }
 #pragma unroll
-  for (int v = 0; v < CNT; v += 4) {
-    const uint2 q = *reinterpret_cast<const uint2*>(p + v);
-    const uint32_t u[2] = {q.x, q.y};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      f[v + 2 * i] = bf16 ? bf2f(u[i] & 0xffffu) : h2f(u[i] & 0xffffu);
-      f[v + 2 * i + 1] = bf16 ? bf2f(u[i] >> 16) : h2f(u[i] >> 16);
-    }
+  for (int i = 0; i < CNT / 2; ++i) {
+    f[2 * i] = dense_widen<BF>(u[i] & 0xffffu);
+    f[2 * i + 1] = dense_widen<BF>(u[i] >> 16);
   }
 }
 
 // The epilogue, in float32 with one rounding at its end: CNT (4 or 8) sums o of row r from column n on; gated: u are the up sums of the same columns.
-template <int CNT, bool GATED>
+template <bool BF, int CNT, bool GATED>
 __device__ __forceinline__ void dense_store(const DenseArgs& a, int64_t r, int n, float (&o)[CNT], float (&u)[CNT]) {
   const int cols = static_cast<int>(GATED ? a.N / 2 : a.N), count = cols - n < CNT ? cols - n : CNT;
   const int64_t at = r * cols + n;
-  if (a.vec) {
-    float f[CNT];
-    if (a.bias) {
-      dense_load_run<CNT>(a.bias + n, a.bf16, f);
+  auto add = [&](const uint16_t* from, float (&to)[CNT]) {
+    if (a.vec) {
+      float f[CNT];
+      dense_load_run<BF, CNT>(from, f);
 #pragma unroll
-      for (int v = 0; v < CNT; ++v) o[v] += f[v];
-      if constexpr (GATED) {
-        dense_load_run<CNT>(a.bias + cols + n, a.bf16, f);
+      for (int v = 0; v < CNT; ++v) to[v] += f[v];
+    } else {
 #pragma unroll
-        for (int v = 0; v < CNT; ++v) u[v] += f[v];
-      }
+      for (int v = 0; v < CNT; ++v)
+        if (v < count) to[v] += dense_widen<BF>(from[v]);
     }
-  } else if (a.bias) {
-#pragma unroll
-    for (int v = 0; v < CNT; ++v)
-      if (v < count) {
-        o[v] += dense_load(a.bias, n + v, a.bf16);
-        if constexpr (GATED) u[v] += dense_load(a.bias, cols + n + v, a.bf16);
-      }
+  };
+  if (a.bias) {
+    add(a.bias + n, o);
+    if constexpr (GATED) add(a.bias + cols + n, u);
   }
-  if (a.act != ACT_NONE) {
-#pragma unroll
-    for (int v = 0; v < CNT; ++v) o[v] = dense_act(o[v], a.act);
-  }
+  dense_act<CNT>(o, a.act);
   if constexpr (GATED) {
 #pragma unroll
     for (int v = 0; v < CNT; ++v) o[v] *= u[v];
   } else if (a.residual) {
-    if (a.vec) {
-      float f[CNT];
-      dense_load_run<CNT>(a.residual + at, a.bf16, f);
-#pragma unroll
-      for (int v = 0; v < CNT; ++v) o[v] += f[v];
-    } else {
-#pragma unroll
-      for (int v = 0; v < CNT; ++v)
-        if (v < count) o[v] += dense_load(a.residual, at + v, a.bf16);
-    }
+    add(a.residual + at, o);
   }
   if (a.out_f32) {
     float* y = static_cast<float*>(a.y) + at;
@@ -173,20 +180,17 @@ __device__ __forceinline__ void dense_store(const DenseArgs& a, int64_t r, int n
         if (v < count) y[v] = o[v];
     }
   } else {
-    uint32_t h[CNT];
+    uint32_t q[CNT / 2];
 #pragma unroll
-    for (int v = 0; v < CNT; ++v) h[v] = a.bf16 ? f2bf(o[v]) : f2h(o[v]);
+    for (int v = 0; v < CNT / 2; ++v) q[v] = dense_pair<BF>(o[2 * v], o[2 * v + 1]);
     uint16_t* y = static_cast<uint16_t*>(a.y) + at;
     if (a.vec) {
-      uint32_t q[CNT / 2];
-#pragma unroll
-      for (int v = 0; v < CNT / 2; ++v) q[v] = h[2 * v] | h[2 * v + 1] << 16;
       if constexpr (CNT == 8) *reinterpret_cast<uint4*>(y) = uint4{q[0], q[1], q[2], q[3]};
       else *reinterpret_cast<uint2*>(y) = uint2{q[0], q[1]};
     } else {
 #pragma unroll
       for (int v = 0; v < CNT; ++v)
-        if (v < count) y[v] = static_cast<uint16_t>(h[v]);
+        if (v < count) y[v] = static_cast<uint16_t>(v % 2 ? q[v / 2] >> 16 : q[v / 2]);
     }
   }
 }

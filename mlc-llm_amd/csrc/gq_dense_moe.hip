@@ -208,16 +208,19 @@ __global__ __launch_bounds__(kThreads, 4) void dense_moe_up_kernel(DenseMoeArgs 
       const int row = it.row0 + c;
       const int64_t at = static_cast<int64_t>(row) * I + n;
       const float w = tab.row_w[row];
-      uint32_t hi[4], lo[4];
+      float f[4] = {g[0], g[1], g[2], g[3]};
+      dense_act<4>(f, a.act);
+      uint32_t hi[2], lo[2];
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const float f = w * (dense_act(g[v], a.act) * up[v]);
-        hi[v] = BF ? f2bf(f) : f2h(f);
-        const float rounded = BF ? bf2f(hi[v]) : h2f(hi[v]), left = f - rounded;
-        lo[v] = __builtin_fabsf(rounded) <= 3.402823466e38f ? (BF ? f2bf(left) : f2h(left)) : 0u;  // (nothing is left of an infinity)
+      for (int v = 0; v < 2; ++v) {
+        const float f0 = w * (f[2 * v] * up[2 * v]), f1 = w * (f[2 * v + 1] * up[2 * v + 1]);
+        hi[v] = dense_pair<BF>(f0, f1);
+        const float r0 = dense_widen<BF>(hi[v] & 0xffffu), r1 = dense_widen<BF>(hi[v] >> 16);
+        auto left = [](float of, float rounded) { return __builtin_fabsf(rounded) <= 3.402823466e38f ? of - rounded : 0.f; };  // (nothing is left of an infinity)
+        lo[v] = dense_pair<BF>(left(f0, r0), left(f1, r1));
       }
-      *reinterpret_cast<uint2*>(h + at) = uint2{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16};
-      *reinterpret_cast<uint2*>(h + static_cast<int64_t>(slots) * I + at) = uint2{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16};
+      *reinterpret_cast<uint2*>(h + at) = uint2{hi[0], hi[1]};
+      *reinterpret_cast<uint2*>(h + static_cast<int64_t>(slots) * I + at) = uint2{lo[0], lo[1]};
     }
   };
   __syncthreads();  // (the routing's part of LDS is the rings' now)
@@ -226,10 +229,7 @@ __global__ __launch_bounds__(kThreads, 4) void dense_moe_up_kernel(DenseMoeArgs 
 
 template <bool BF>
 __device__ __forceinline__ void moe_store(uint16_t* to, const float4_t& v) {
-  uint32_t u[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) u[i] = BF ? f2bf(v[i]) : f2h(v[i]);
-  *reinterpret_cast<uint2*>(to) = uint2{u[0] | u[1] << 16, u[2] | u[3] << 16};
+  *reinterpret_cast<uint2*>(to) = uint2{dense_pair<BF>(v[0], v[1]), dense_pair<BF>(v[2], v[3])};
 }
 
 // Sixteen columns of the output for all tokens a workgroup; gridDim.y workgroups share the K, which is all segments' inter.

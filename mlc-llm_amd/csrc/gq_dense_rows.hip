@@ -41,7 +41,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, 4) void dense_rows_kernel(DenseA
       const int r = 16 * t + (lane & 15);
       const float4_t g = acc[t], up = GATED ? stream_up(g) : g;
       float o[4] = {g[0], g[1], g[2], g[3]}, u[4] = {up[0], up[1], up[2], up[3]};
-      if (r < rows && n < cols && (!GATED || lane < 32)) dense_store<4, GATED>(a, r, static_cast<int>(n), o, u);
+      if (r < rows && n < cols && (!GATED || lane < 32)) dense_store<BF, 4, GATED>(a, r, static_cast<int>(n), o, u);
     }
   };
   dense_stream<BF, XG>(ring, static_cast<uint32_t>(pitch), KW * kStreamBlock, nb, 1, place_of, done);

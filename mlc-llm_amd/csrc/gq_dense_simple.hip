@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256) void dense_simple_kernel(DenseArgs a, int64_t 
       if (r < a.rows && n < half) {
         const float4_t g = acc[i], up = acc[GATED ? i + 2 : i];
         float o[4] = {g[0], g[1], g[2], g[3]}, u[4] = {up[0], up[1], up[2], up[3]};
-        dense_store<4, GATED>(a, r, static_cast<int>(n), o, u);
+        dense_store<BF, 4, GATED>(a, r, static_cast<int>(n), o, u);
       }
     }
   }

@@ -4,7 +4,7 @@
 namespace gq {
 
 // the sums of the shares of K, in their order, and the epilogue.  Four columns a thread.
-template <bool GATED>
+template <bool BF, bool GATED>
 __global__ __launch_bounds__(256) void dense_join_kernel(DenseArgs p, int splits) {
   const int N = static_cast<int>(p.N), cols = GATED ? N / 2 : N, runs = (cols + 3) / 4;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -28,14 +28,15 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseArgs p, int splits
       }
     }
   }
-  dense_store<4, GATED>(p, r, n, o[0], o[GATED ? 1 : 0]);
+  dense_store<BF, 4, GATED>(p, r, n, o[0], o[GATED ? 1 : 0]);
 }
 
 hipError_t launch_dense_join(const DenseArgs& a, int splits, hipStream_t s) {
   const int64_t items = a.rows * (((a.gated ? a.N / 2 : a.N) + 3) / 4);
   const dim3 grid(static_cast<unsigned>((items + 255) / 256));
-  if (a.gated) hipLaunchKernelGGL(dense_join_kernel<true>, grid, dim3(256), 0, s, a, splits);
-  else hipLaunchKernelGGL(dense_join_kernel<false>, grid, dim3(256), 0, s, a, splits);
+  auto go = [&](auto* kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a, splits); };
+  if (a.bf16) a.gated ? go(dense_join_kernel<true, true>) : go(dense_join_kernel<true, false>);
+  else a.gated ? go(dense_join_kernel<false, true>) : go(dense_join_kernel<false, false>);
   return hipGetLastError();
 }
 

@@ -263,7 +263,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p
             for (int e = 0; e < 4; ++e) o[i][v + e] = a[e];
           }
         if (!share) {
-          dense_store<8, GATED>(p, r0 + r, n, o[0], o[P - 1]);
+          dense_store<BF, 8, GATED>(p, r0 + r, n, o[0], o[P - 1]);
         } else {  // a share of K: its sums go to the scratch as they are
           for (int i = 0; i < P; ++i) {
             float* const at = to + static_cast<int64_t>(r) * N + i * half + n;
