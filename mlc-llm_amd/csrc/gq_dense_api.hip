@@ -25,7 +25,10 @@ int hip_result(hipError_t e, const char* what) {
 }
 hipStream_t as_stream(mi355gq_stream_t s) { return static_cast<hipStream_t>(s); }
 
-bool few_rows(int64_t M) { return M <= 16; }
+// Where the kernel that streams the weights past up to sixteen rows of x is faster than the tiles; N rows of W.  us, it / the best tiles:
+// 4096 x 4096 of 2 rows 8.5 / 10.6, of 16 9.8 / 11.3; 28672 x 4096 of 2 rows 38.5 / 37.6, of 8 39.9 / 39.0, of 12 42.7 / 39.0; 5120 x 5120 of 2
+// rows 12.7 / 13.2, of 8 14.3 / 13.7, of 12 16.2 / 14.1; 11264 x 2048 of 8 rows 11.7 / 11.0, of 12 12.6 / 11.2; 8192 x 2048 of 12 9.9 / 9.9.
+bool few_rows(int64_t M, int64_t N, int64_t K) { return gq::options().gemm_variant < 0 && (M <= 8 || (M <= 16 && N * K < 20000000)); }
 
 // cols: of y
 int product(const char* what, const void* x, const void* w, const void* bias, const void* residual, int64_t M, int64_t cols, int64_t K,
@@ -61,7 +64,7 @@ int product(const char* what, const void* x, const void* w, const void* bias, co
   const hipStream_t s = as_stream(stream);
   hipError_t e = hipErrorNotSupported;
   if (gq::dense_aligned(a)) {
-    if (few_rows(M)) e = gq::launch_dense_rows(a, s);
+    if (few_rows(M, a.N, K)) e = gq::launch_dense_rows(a, s);
     if (e == hipErrorNotSupported) e = gq::launch_dense_tile(a, s);
   }
   if (e == hipErrorNotSupported) e = gq::launch_dense_simple(a, s);
@@ -81,7 +84,7 @@ extern "C" {
 
 int64_t mi355gq_dense_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated) {
   const int64_t rows_of_w = gated ? 2 * N : N;
-  if (!dim_ok(M) || !dim_ok(N) || !dim_ok(rows_of_w) || !dim_ok(K) || M == 0 || N == 0 || K == 0 || few_rows(M) || K % 8 != 0) return 0;
+  if (!dim_ok(M) || !dim_ok(N) || !dim_ok(rows_of_w) || !dim_ok(K) || M == 0 || N == 0 || K == 0 || few_rows(M, rows_of_w, K) || K % 8 != 0) return 0;
   return gq::dense_tile_workspace_bytes(M, rows_of_w, K);
 }
 

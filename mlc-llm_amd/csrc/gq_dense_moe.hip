@@ -47,31 +47,34 @@ inline double experts_chosen(int64_t T, int64_t experts, int64_t k) {
 }
 // eights of rows of a segment: sixteen rows where experts have more than four on average
 inline int moe_eights(int64_t T, int64_t experts, int64_t k) { return T > 8 && T * k > 4 * experts ? 2 : 1; }
-// Workgroups that share the K (all chosen experts' inter) of sixteen columns in the second kernel: two a unit.
+// Workgroups that share the K (all chosen experts' inter) of sixteen columns in the second kernel: about one a unit (sixteen tokens
+// of 128 experts, 128 tiles: 131 us with two shares, 159 with one and 136 with four; 224 tiles: 212 with one, 219 with two).
 inline int moe_shares(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k) {
+  if (options().gemm_split_k > 0) return options().gemm_split_k < 8 ? options().gemm_split_k : 8;
   const int64_t tiles = (hidden + 15) / 16;
   const double blocks = experts_chosen(T, experts, k) * static_cast<double>((inter + kStreamBlock - 1) / kStreamBlock);
   int s = 1;
-  while (s < 8 && tiles * s < 400 && blocks / (2 * s) >= 2 * kStreamDepth * kWaves) s *= 2;
+  while (s < 8 && tiles * s < 200 && blocks / (2 * s) >= 4 * kWaves) s *= 2;
   return s;
 }
 
 struct MoeTables {  // in LDS, in front of the rest
   uint64_t* mask;      // [experts] tokens of each
   MoeSegment* segs;    // [T k at most]
+  int* expert_row;     // [experts] the first row of each
   int* slot_id;        // [T k]
   float* slot_w;       // [T k]
   int* row_token;      // [T k] in the order of the experts
   float* row_w;        // [T k]
   uint64_t* totals;    // [waves]
 };
-inline size_t moe_tables_bytes(int experts, int slots) { return (64 + static_cast<size_t>(experts) * 8 + static_cast<size_t>(slots) * (16 + sizeof(MoeSegment)) + 15) / 16 * 16; }
+inline size_t moe_tables_bytes(int experts, int slots) { return (64 + static_cast<size_t>(experts) * 12 + static_cast<size_t>(slots) * (16 + sizeof(MoeSegment)) + 15) / 16 * 16; }
 
 }  // namespace
 
 // NC: experts a lane in the routing.  XG: eights of rows of a segment.
-template <bool BF, int NC, int XG>
-__global__ __launch_bounds__(kThreads, 4) void dense_moe_up_kernel(DenseMoeArgs a, MoeLayout layout, int group_inv, int logits_vec, int kw_log2, int nb,
+template <bool BF, int NC, int XG, int D>
+__global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(DenseMoeArgs a, MoeLayout layout, int group_inv, int logits_vec, int kw_log2, int nb,
                                                                   int tables_bytes) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   constexpr int TT = (XG + 1) / 2, kSegRows = 8 * XG;
@@ -80,7 +83,8 @@ __global__ __launch_bounds__(kThreads, 4) void dense_moe_up_kernel(DenseMoeArgs 
   MoeTables tab;
   tab.totals = reinterpret_cast<uint64_t*>(smem);
   tab.mask = tab.totals + 8;
-  tab.slot_id = reinterpret_cast<int*>(tab.mask + E);
+  tab.expert_row = reinterpret_cast<int*>(tab.mask + E);
+  tab.slot_id = tab.expert_row + E;
   tab.slot_w = reinterpret_cast<float*>(tab.slot_id + slots);
   tab.row_token = reinterpret_cast<int*>(tab.slot_w + slots);
   tab.row_w = reinterpret_cast<float*>(tab.row_token + slots);
@@ -134,16 +138,14 @@ __global__ __launch_bounds__(kThreads, 4) void dense_moe_up_kernel(DenseMoeArgs 
     const int left = n_rows - kSegRows * s;
     tab.segs[(before >> 16) + s] = MoeSegment{tid, row0 + kSegRows * s, left < kSegRows ? left : kSegRows};
   }
-  // this expert's rows: its tokens in order, and their weights
-  {
-    uint64_t left = mine;
-    for (int i = 0; i < n_rows; ++i) {
-      const int t = __builtin_ctzll(left);
-      left &= left - 1;
-      tab.row_token[row0 + i] = t;
-      for (int j = 0; j < a.k; ++j)
-        if (tab.slot_id[t * a.k + j] == tid) tab.row_w[row0 + i] = tab.slot_w[t * a.k + j];
-    }
+  if (tid < E) tab.expert_row[tid] = row0;
+  __syncthreads();
+  // a slot's row: behind its expert's tokens of lower numbers
+  for (int i = tid; i < slots; i += kThreads) {
+    const int e = tab.slot_id[i], t = i / a.k;
+    const int row = tab.expert_row[e] + __popcll(tab.mask[e] & ((1ull << t) - 1));
+    tab.row_token[row] = t;
+    tab.row_w[row] = tab.slot_w[i];
   }
   __syncthreads();
   char* const ws = static_cast<char*>(a.workspace);
@@ -194,7 +196,7 @@ __global__ __launch_bounds__(kThreads, 4) void dense_moe_up_kernel(DenseMoeArgs 
   };
   auto done = [&](int round, float4_t (&acc)[TT]) {
     if (KW > 1) {  // (two buffers in turn: one barrier a round)
-      stream_join(reinterpret_cast<float4_t*>(rest + kWaves * stream_ring<XG, 1>()) + (round & 1) * kWaves * TT * 64, wave, KW, acc);
+      stream_join(reinterpret_cast<float4_t*>(rest + kWaves * stream_ring<XG, 1, D>()) + (round & 1) * kWaves * TT * 64, wave, KW, acc);
       if (kw != 0) return;
     }
     const Item it = item_of(round);
@@ -224,7 +226,7 @@ __global__ __launch_bounds__(kThreads, 4) void dense_moe_up_kernel(DenseMoeArgs 
     }
   };
   __syncthreads();  // (the routing's part of LDS is the rings' now)
-  dense_stream<BF, XG>(rest + wave * stream_ring<XG, 1>(), static_cast<uint32_t>(pitch), KW * kStreamBlock, nb, rounds, place_of, done);
+  dense_stream<BF, XG, D>(rest + wave * stream_ring<XG, 1, D>(), static_cast<uint32_t>(pitch), KW * kStreamBlock, nb, rounds, place_of, done);
 }
 
 template <bool BF>
@@ -233,20 +235,22 @@ __device__ __forceinline__ void moe_store(uint16_t* to, const float4_t& v) {
 }
 
 // Sixteen columns of the output for all tokens a workgroup; gridDim.y workgroups share the K, which is all segments' inter.
-template <bool BF, int XG>
-__global__ __launch_bounds__(kThreads, XG == 1 ? 4 : 2) void dense_moe_down_kernel(DenseMoeArgs a, MoeLayout layout) {
-  constexpr int D = kStreamDepth, TT = (XG + 1) / 2, kStage = stream_stage<XG, 2>();
+template <bool BF, int XG, int D>
+__global__ __launch_bounds__(kThreads, XG == 1 && D == 2 ? 4 : 2) void dense_moe_down_kernel(DenseMoeArgs a, MoeLayout layout) {
+  constexpr int TT = (XG + 1) / 2, kStage = stream_stage<XG, 2>();
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
   const int slots = a.T * a.k;
   char* const ws = static_cast<char*>(a.workspace);
-  uint8_t* const ring = smem + wave * stream_ring<XG, 2>();
-  float4_t* const sums = reinterpret_cast<float4_t*>(smem + kWaves * stream_ring<XG, 2>());  // [waves][T][4]
+  uint8_t* const ring = smem + wave * stream_ring<XG, 2, D>();
+  float4_t* const sums = reinterpret_cast<float4_t*>(smem + kWaves * stream_ring<XG, 2, D>());  // [waves][T][4]
   int* const row_token = reinterpret_cast<int*>(sums + kWaves * a.T * 4);                     // [T k]
   MoeSegment* const segs = reinterpret_cast<MoeSegment*>(row_token + slots);                  // [T k at most]
   const int n_segs = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(ws));
-  for (int i = tid; i < slots; i += kThreads) row_token[i] = reinterpret_cast<const int*>(ws + layout.row_token)[i];
-  for (int i = tid; i < n_segs; i += kThreads) segs[i] = reinterpret_cast<const MoeSegment*>(ws + layout.segs)[i];
+  for (int i = tid; i < slots; i += kThreads) {  // (all that may be there, without a wait for their number)
+    row_token[i] = reinterpret_cast<const int*>(ws + layout.row_token)[i];
+    segs[i] = reinterpret_cast<const MoeSegment*>(ws + layout.segs)[i];
+  }
   for (int i = tid; i < kWaves * a.T * 4; i += kThreads) sums[i] = float4_t{};
   __syncthreads();
   const int H = a.hidden, I = a.inter, n0 = blockIdx.x * 16, per = (I + kStreamBlock - 1) / kStreamBlock;  // blocks a segment
@@ -312,7 +316,7 @@ __global__ __launch_bounds__(kThreads, XG == 1 ? 4 : 2) void dense_moe_down_kern
         join(current);
         current = now.i;
       }
-      stream_wait<XG, 2>();
+      stream_wait<XG, 2, D>();
       stream_block<BF, XG, 2>(ring + s * kStage, acc);  // (past the end: zeros)
       next(now);
       load(s);
@@ -363,41 +367,54 @@ static hipError_t may_use(Kernel* kern, size_t lds) {
   return lds > 65536 ? allow_large_lds(reinterpret_cast<const void*>(kern)) : hipSuccess;
 }
 
-template <bool BF, int NC, int XG>
+template <bool BF, int NC, int XG, int D>
 static hipError_t launch_up(const DenseMoeArgs& a, const MoeLayout& layout, hipStream_t s) {
   const int slots = a.T * a.k, n_tiles = a.inter / 8;
-  const StreamPlan plan = stream_plan(a.hidden);
+  const StreamPlan plan = stream_plan(experts_chosen(a.T, a.experts, a.k) * n_tiles, a.hidden, D);
   const int64_t most = static_cast<int64_t>(slots < a.experts ? slots : a.experts + slots / (8 * XG)) * n_tiles;  // items
   const int nw = kWaves >> plan.kw_log2;
   const int64_t sets = (most + nw - 1) / nw;
   const size_t tables = moe_tables_bytes(a.experts, slots), gate = kWaves * sizeof(GateScratch<NC>);
-  const size_t rings = kWaves * (stream_ring<XG, 1>() + (plan.kw_log2 > 0 ? 2 * ((XG + 1) / 2) * 1024 : 0)), lds = tables + (rings > gate ? rings : gate);
-  auto* kern = dense_moe_up_kernel<BF, NC, XG>;
+  const size_t rings = kWaves * (stream_ring<XG, 1, D>() + 2 * ((XG + 1) / 2) * 1024), lds = tables + (rings > gate ? rings : gate);
+  if (lds > 160 * 1024) return hipErrorNotSupported;
+  auto* kern = dense_moe_up_kernel<BF, NC, XG, D>;
   const hipError_t e = may_use(kern, lds);
   if (e != hipSuccess) return e;
   const int vec = a.experts % 8 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0;
-  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(sets < 512 ? sets : 512)), dim3(kThreads), lds, s, a, layout, gate_group_inv(a.experts, a.groups),
+  const int64_t at_a_time = kStreamUnits * (lds > 80 * 1024 ? 1 : 2);
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(sets < at_a_time ? sets : at_a_time)), dim3(kThreads), lds, s, a, layout, gate_group_inv(a.experts, a.groups),
                      vec, plan.kw_log2, plan.nb, static_cast<int>(tables));
+  return hipGetLastError();
+}
+
+template <bool BF, int XG, int D>
+static hipError_t launch_down(const DenseMoeArgs& a, const MoeLayout& layout, hipStream_t s) {
+  const int shares = moe_shares(a.T, a.hidden, a.inter, a.experts, a.k);
+  const dim3 grid(static_cast<unsigned>((a.hidden + 15) / 16), static_cast<unsigned>(shares));
+  note_kernel("dense_moe up to %d rows, %d shares", 8 * XG, shares);
+  const size_t lds = kWaves * (stream_ring<XG, 2, D>() + a.T * 64) + static_cast<size_t>(a.T) * a.k * (4 + sizeof(MoeSegment));
+  if (lds > 160 * 1024) return hipErrorNotSupported;
+  auto* kern = dense_moe_down_kernel<BF, XG, D>;
+  const hipError_t e = may_use(kern, lds);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(kern, grid, dim3(kThreads), lds, s, a, layout);
   return hipGetLastError();
 }
 
 template <bool BF, int XG>
 static hipError_t launch(const DenseMoeArgs& a, hipStream_t s) {
   const MoeLayout layout = moe_layout(a.T, a.hidden, a.inter, a.experts, a.k);
-  const hipError_t e = a.experts <= 64    ? launch_up<BF, 2, XG>(a, layout, s)
-                       : a.experts <= 128 ? launch_up<BF, 4, XG>(a, layout, s)
-                       : a.experts <= 256 ? launch_up<BF, 8, XG>(a, layout, s)
-                                          : launch_up<BF, 16, XG>(a, layout, s);
-  if (e != hipSuccess) return e;
-  const int shares = moe_shares(a.T, a.hidden, a.inter, a.experts, a.k);
-  const dim3 grid(static_cast<unsigned>((a.hidden + 15) / 16), static_cast<unsigned>(shares));
-  note_kernel("dense_moe up to %d rows, %d shares", 8 * XG, shares);
-  const size_t lds = kWaves * (stream_ring<XG, 2>() + a.T * 64) + static_cast<size_t>(a.T) * a.k * (4 + sizeof(MoeSegment));
-  auto* kern = dense_moe_down_kernel<BF, XG>;
-  const hipError_t d = may_use(kern, lds);
-  if (d != hipSuccess) return d;
-  hipLaunchKernelGGL(kern, grid, dim3(kThreads), lds, s, a, layout);
-  return hipGetLastError();
+  auto up = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    return a.experts <= 64    ? launch_up<BF, 2, XG, D>(a, layout, s)
+           : a.experts <= 128 ? launch_up<BF, 4, XG, D>(a, layout, s)
+           : a.experts <= 256 ? launch_up<BF, 8, XG, D>(a, layout, s)
+                              : launch_up<BF, 16, XG, D>(a, layout, s);
+  };
+  hipError_t e = up(std::integral_constant<int, 4>{});
+  if (e == hipErrorNotSupported) e = up(std::integral_constant<int, 2>{});  // (many slots: their tables take the room)
+  // (two workgroups a unit with two blocks ahead: one with four was 1 to 10 % behind, 16 tokens of 128 experts 133 / 137 us in all)
+  return e != hipSuccess ? e : launch_down<BF, XG, 2>(a, layout, s);
 }
 
 hipError_t launch_dense_moe(const DenseMoeArgs& a, hipStream_t s) {

@@ -17,7 +17,7 @@ constexpr uint32_t kNowhere = 0xc0000000u;  // past the end of any buffer here, 
 constexpr int64_t kReach = 0xc0000000ll;    // bytes of a buffer, below
 constexpr int kStreamBlock = 64;            // numbers of K in a block
 constexpr int kStreamWaves = 8;             // of a workgroup
-constexpr int kStreamDepth = 2;             // blocks in flight, D
+constexpr int kStreamUnits = 256;           // workgroups that run at a time, where their rings take most of a unit's LDS
 
 __device__ __forceinline__ rsrc_t dense_buffer(const void* base, int64_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(bytes < kReach ? static_cast<uint32_t>(bytes) : kNowhere), 0x00027000);
@@ -40,8 +40,8 @@ struct StreamPlace {
 
 template <int XG, int PX>
 constexpr int stream_stage() { return 2048 + PX * XG * 1024; }
-template <int XG, int PX>
-constexpr int stream_ring() { return kStreamDepth * stream_stage<XG, PX>(); }
+template <int XG, int PX, int D>
+constexpr int stream_ring() { return D * stream_stage<XG, PX>(); }
 
 // One block from number k of the rows on, into a stage.  Chunk c of 16 bytes of a row lies at place c ^ (row & 7), so that the 16 lanes that LDS
 // serves at a time meet all its banks.
@@ -59,10 +59,11 @@ __device__ __forceinline__ void stream_load(const StreamPlace<XG, PX>& p, int k,
     for (int i = 0; i < PX; ++i) dense_to_lds<false>(p.x[i], at, stage + 2048 + (i * XG + g) * 1024);
   }
 }
-// Waits until all but the newest `newer` blocks have landed.
-template <int XG, int PX>
+// Waits until all but the newest D - 1 blocks have landed.
+template <int XG, int PX, int D>
 __device__ __forceinline__ void stream_wait() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStreamDepth - 1) * (2 + PX * XG)) : "memory");
+  static_assert((D - 1) * (2 + PX * XG) < 64, "the counter of loads");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * (2 + PX * XG)) : "memory");
 }
 // sums += the block in a stage; the lane holds row 16 t + lane % 16 of x and rows 4 (lane / 16) .. + 3 of W.
 template <bool BF, int XG, int PX>
@@ -85,9 +86,9 @@ __device__ __forceinline__ void stream_block(const uint8_t* stage, float4_t (&ac
 
 // `rounds` places one after the other, of each nb blocks (a multiple of D), `step` numbers of K apart; past K they are zeros.  place_of(round)
 // gives a place, done(round, sums) takes its sums.
-template <bool BF, int XG, class PlaceOf, class Done>
+template <bool BF, int XG, int D, class PlaceOf, class Done>
 __device__ __forceinline__ void dense_stream(uint8_t* ring, uint32_t w_pitch, int step, int nb, int rounds, PlaceOf place_of, Done done) {
-  constexpr int D = kStreamDepth, TT = (XG + 1) / 2, kStage = stream_stage<XG, 1>();
+  constexpr int TT = (XG + 1) / 2, kStage = stream_stage<XG, 1>();
   StreamPlace<XG, 1> here = place_of(0);
 #pragma unroll
   for (int s = 0; s < D; ++s) stream_load(here, here.k + s * step, w_pitch, ring + s * kStage);
@@ -98,7 +99,7 @@ __device__ __forceinline__ void dense_stream(uint8_t* ring, uint32_t w_pitch, in
     for (int j = D; j < nb; j += D) {
 #pragma unroll
       for (int s = 0; s < D; ++s) {
-        stream_wait<XG, 1>();
+        stream_wait<XG, 1, D>();
         stream_block<BF, XG, 1>(ring + s * kStage, acc);
         stream_load(here, here.k + (j + s) * step, w_pitch, ring + s * kStage);
       }
@@ -106,7 +107,7 @@ __device__ __forceinline__ void dense_stream(uint8_t* ring, uint32_t w_pitch, in
     here = place_of(round + 1);
 #pragma unroll
     for (int s = 0; s < D; ++s) {
-      stream_wait<XG, 1>();
+      stream_wait<XG, 1, D>();
       stream_block<BF, XG, 1>(ring + s * kStage, acc);
       stream_load(here, here.k + s * step, w_pitch, ring + s * kStage);
     }
@@ -136,16 +137,27 @@ __device__ __forceinline__ float4_t stream_up(float4_t v) {
   return u;
 }
 
-// KW of a workgroup's eight waves share the K of an item, as many as have D blocks each: the rows that a workgroup reads are long then.
+// KW of a workgroup's eight waves share the K of an item.  More of them read longer runs of a row, fewer leave more blocks a wave between two
+// items: the KW of the fewest blocks that a wave takes one after the other, padding and the ends of its rounds (1.6 blocks each; 0.6 of a single one)
+// counted, and a seventh more where rows are not shared.  One row, by KW 8, 4, 2 and 1, us: 28672 x 4096 36.7, 42.9, 40.0, 41.1 (the rule: 8); 28672 x
+// 2048 22.0, 22.4, 20.7, 24.5 (2); 11264 x 2048 11.3, 11.1, 10.4 (2); 5120 x 5120 13.2, 11.6 (4); 6144 x 4096 11.1, 11.9 (4).
 struct StreamPlan {
-  int kw_log2, nb;
+  int kw_log2, nb, rounds;
 };
-inline StreamPlan stream_plan(int64_t K) {
+inline StreamPlan stream_plan(double items, int64_t K, int D) {
   const int64_t blocks = (K + kStreamBlock - 1) / kStreamBlock;
-  int log2 = 0;
-  while (log2 < 3 && (blocks >> (log2 + 1)) >= kStreamDepth) ++log2;
-  const int64_t each = (blocks + (1 << log2) - 1) >> log2;
-  return {log2, static_cast<int>((each + kStreamDepth - 1) / kStreamDepth * kStreamDepth)};
+  StreamPlan best{0, 0, 0};
+  double best_cost = 0;
+  for (int log2 = 3; log2 >= 0; --log2) {
+    const int64_t each = (blocks + (1 << log2) - 1) >> log2, nb = (each + D - 1) / D * D;
+    const double rounds = __builtin_ceil(items / ((kStreamWaves >> log2) * kStreamUnits));
+    const double cost = (rounds * static_cast<double>(nb) + (rounds > 1 ? 1.6 * rounds : 0.6)) * (log2 == 0 ? 1.15 : 1.0);
+    if (best.nb == 0 || cost < best_cost) {
+      best_cost = cost;
+      best = {log2, static_cast<int>(nb), static_cast<int>(rounds)};
+    }
+  }
+  return best;
 }
 
 }  // namespace gq
