@@ -43,18 +43,18 @@ hipError_t launch_dense_join(const DenseArgs& a, int splits, hipStream_t s) {
 namespace {
 
 // A form's tile, the workgroups of it that a unit holds (one or two), and what a block of K of its tiles takes in ns: alone_ns where few run,
-// one_ns where a unit has one each, full_ns where the units are full (L2 and clocks are shared).  Fitted to 10000 timings of 198 shapes, 17 to 4096
-// rows, all forms, 1 to 16 shares: the choice takes 1.0 % longer than the best one on average, 14 % at most.
+// one_ns where a unit has one each, full_ns where the units are full (L2 and clocks are shared).  Fitted to 14000 timings of 242 shapes, 17 to 4096
+// rows, all forms, 1 to 16 shares: the choice takes 0.7 % longer than the best one on average, 13 % at most.
 struct Form {
   int bn, bm, a_unit;
   float alone_ns, one_ns, full_ns;
 };
 constexpr int kForms = 9;
-constexpr Form kForm[kForms] = {{256, 256, 1, 1296.f, 1495.f, 1495.f}, {256, 192, 1, 919.f, 1182.f, 1182.f}, {256, 128, 1, 742.f, 879.f, 879.f},
-                                {128, 192, 1, 545.f, 836.f, 836.f},    {128, 128, 1, 526.f, 597.f, 597.f},   {128, 128, 2, 486.f, 718.f, 881.f},
-                                {64, 128, 1, 276.f, 336.f, 336.f},     {64, 64, 2, 189.f, 220.f, 486.f},     {64, 32, 2, 125.f, 241.f, 666.f}};
-// a round's ends, the launch that joins, a number of a share, a byte of W from memory
-constexpr float kRoundNs = 1306.f, kJoinNs = 1949.f, kShareNs = 1.62e-3f, kByteNs = 1.43e-4f;
+constexpr Form kForm[kForms] = {{256, 256, 1, 989.f, 1470.f, 1470.f}, {256, 192, 1, 869.f, 1209.f, 1209.f}, {256, 128, 1, 741.f, 890.f, 890.f},
+                                {128, 192, 1, 561.f, 852.f, 852.f},   {128, 128, 1, 514.f, 570.f, 570.f},   {128, 128, 2, 477.f, 680.f, 890.f},
+                                {64, 128, 1, 220.f, 378.f, 378.f},    {64, 64, 2, 219.f, 221.f, 564.f},     {64, 32, 2, 172.f, 227.f, 563.f}};
+// a round's ends, the launch that joins, a number of a share, a byte of W from memory, a second launch for the rest of the last round
+constexpr float kRoundNs = 977.f, kJoinNs = 2626.f, kShareNs = 1.67e-3f, kByteNs = 1.27e-4f, kRestNs = 1500.f;
 constexpr int64_t kUnits = 256;
 float ns_of(const Form& f, int64_t tiles, int64_t blocks) {
   const int64_t at_a_time = kUnits * f.a_unit, full = tiles / at_a_time, rest = tiles - full * at_a_time;
@@ -88,7 +88,7 @@ DensePlan plan_of(int64_t rows, int64_t N, int64_t K, bool only_whole = false) {
     const int64_t at_a_time = kUnits * kForm[f].a_unit, whole = tiles / at_a_time * at_a_time / m_tiles;
     if (!only_whole && options().gemm_split_k <= 1 && whole > 0 && whole < n_tiles) {
       const DensePlan rest = plan_of(rows, N - whole * kForm[f].bn, K, true);
-      const float ns = ns_of(kForm[f], whole * m_tiles, blocks) + rest.ns + 2000.f;
+      const float ns = ns_of(kForm[f], whole * m_tiles, blocks) + rest.ns + kRestNs;
       if (ns < best.ns) {
         best = DensePlan{};
         best.form = f;

@@ -45,7 +45,7 @@ __device__ __forceinline__ float16_t tile_mfma(int4_t w, int4_t x, float16_t acc
 // WS stages of W and XS of x in LDS: W is WS - 1 blocks ahead, x XS - 1.
 // ONCE: no other workgroup reads these rows of W.
 template <bool BF, bool GATED, int MI, int WN, int WM, int TN, int TM, int WS, int XS, bool ONCE>
-__global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p, int n_first, int n_tiles, int m_tiles, int per_split) {
+__global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p, int n_first, int n_tiles, int m_tiles, int splits, int per_split) {
   constexpr int kWaves = WN * WM, BN = MI * WN * TN, BM = MI * WM * TM, KS = MI / 8;  // KS: instructions to a block
   constexpr int kWLoads = BN / 8 / kWaves, kXLoads = (BM / 8 + kWaves - 1) / kWaves;  // of 1 KiB, eight rows, a wave and block of K
   constexpr int P = GATED ? 2 : 1, kPart = MI * TN / P;  // parts of a wave's rows of W
@@ -58,15 +58,18 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p
   const int K = static_cast<int>(p.K), N = static_cast<int>(p.N), half = N / P;
   const int blocks = (K + kBlock - 1) / kBlock;
 
-  // Workgroups go to the eight dies in turn; each die takes a run of tiles, x tiles fastest, so that what runs on it at a time
-  // shares rows of W and of x in its L2.
-  const int tiles = n_tiles * m_tiles, per = (tiles + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= per || id >= tiles) return;
-  const int nt = id / m_tiles, mt = id - nt * m_tiles, n0 = n_first + nt * (BN / P);
+  // Workgroups go to the eight dies in turn; each die takes a run of tiles, one share of K after the other and x tiles fastest in groups of kGroup:
+  // what runs on it at a time is about as many rows of W as of x, which its L2 then holds for all of them.
+  const int tiles = n_tiles * m_tiles, per = (tiles * splits + 7) / 8, at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= per || at >= tiles * splits) return;
+  const int part = at / tiles, id = at - part * tiles;  // this workgroup's share
+  constexpr int kGroup = 8;
+  const int group = id / (kGroup * n_tiles), m_first = group * kGroup, m_here = m_tiles - m_first < kGroup ? m_tiles - m_first : kGroup;
+  const int in_group = id - group * kGroup * n_tiles, nt = in_group / m_here, mt = m_first + in_group - nt * m_here, n0 = n_first + nt * (BN / P);
   const int64_t r0 = static_cast<int64_t>(mt) * BM;
   const int rows = p.rows - r0 < BM ? static_cast<int>(p.rows - r0) : BM;  // of x in this tile
   // this workgroup's blocks of K
-  const int first = blockIdx.y * per_split, last = (first + per_split < blocks ? first + per_split : blocks) - 1;
+  const int first = part * per_split, last = (first + per_split < blocks ? first + per_split : blocks) - 1;
 
   // Rows past the end are read from the last one.  A block's loads see the matrix from that block on, and nothing past its end: the last
   // row's bytes past K are zeros, another row's are the next row's, and the last block is masked where it is used.
@@ -233,8 +236,8 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p
   // eight a lane; float32 until the epilogue is through.
   constexpr int kCols = MI * TN, kRow = kCols + 4, kLanes = kPart / 8, kRows = 64 / kLanes < MI ? 64 / kLanes : MI;
   float* const mine = reinterpret_cast<float*>(smem) + wave * MI * kRow;
-  const bool share = gridDim.y > 1;
-  float* const to = static_cast<float*>(p.workspace) + (blockIdx.y * p.rows + r0) * N;
+  const bool share = splits > 1;
+  float* const to = static_cast<float*>(p.workspace) + (part * p.rows + r0) * N;
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
 #pragma unroll
@@ -319,12 +322,12 @@ hipError_t launch_tile(const DenseArgs& a, const DensePlan& plan, int part, hipS
     if (e != hipSuccess) return e;
   }
   note_kernel("dense_tile %dx%d%s, %d shares of K", BN * P, BM, GATED ? " gated" : "", splits);
-  const int64_t most = (0xffffffffll / (64 * kWaves) - 8) / m_tiles;  // columns of tiles a launch, likewise
+  const int64_t most = (0xffffffffll / (64 * kWaves) - 8) / (m_tiles * splits);  // columns of tiles a launch, likewise
   if (most < 1) return hipErrorNotSupported;
   for (int64_t t0 = 0; t0 < n_tiles; t0 += most) {
     const int64_t here = n_tiles - t0 < most ? n_tiles - t0 : most;
-    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((here * m_tiles + 7) / 8 * 8), splits), dim3(64 * kWaves), lds, s, a,
-                       static_cast<int>(n_first + t0 * BN), static_cast<int>(here), static_cast<int>(m_tiles), per_split);
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((here * m_tiles * splits + 7) / 8 * 8)), dim3(64 * kWaves), lds, s, a,
+                       static_cast<int>(n_first + t0 * BN), static_cast<int>(here), static_cast<int>(m_tiles), splits, per_split);
   }
   return splits > 1 ? launch_dense_join(a, splits, s) : hipGetLastError();
 }
