@@ -141,33 +141,33 @@ __device__ __forceinline__ void dense_load_run(const uint16_t* p, float (&f)[CNT
   }
 }
 
-// The epilogue, in float32 with one rounding at its end: CNT (4 or 8) sums o of row r from column n on; gated: u are the up sums of the same columns.
+// CNT numbers from `from` on, `count` of them there
+template <bool BF, int CNT>
+__device__ __forceinline__ void dense_add_run(const DenseArgs& a, const uint16_t* from, int count, float (&to)[CNT]) {
+  if (a.vec) {
+    float f[CNT];
+    dense_load_run<BF, CNT>(from, f);
+#pragma unroll
+    for (int v = 0; v < CNT; ++v) to[v] += f[v];
+  } else {
+#pragma unroll
+    for (int v = 0; v < CNT; ++v)
+      if (v < count) to[v] += dense_widen<BF>(from[v]);
+  }
+}
+
+// The epilogue behind the bias, in float32 with one rounding at its end: CNT (4 or 8) numbers o of row r from column n on; gated: u are the up
+// numbers of the same columns.
 template <bool BF, int CNT, bool GATED>
-__device__ __forceinline__ void dense_store(const DenseArgs& a, int64_t r, int n, float (&o)[CNT], float (&u)[CNT]) {
+__device__ __forceinline__ void dense_finish(const DenseArgs& a, int64_t r, int n, float (&o)[CNT], float (&u)[CNT]) {
   const int cols = static_cast<int>(GATED ? a.N / 2 : a.N), count = cols - n < CNT ? cols - n : CNT;
   const int64_t at = r * cols + n;
-  auto add = [&](const uint16_t* from, float (&to)[CNT]) {
-    if (a.vec) {
-      float f[CNT];
-      dense_load_run<BF, CNT>(from, f);
-#pragma unroll
-      for (int v = 0; v < CNT; ++v) to[v] += f[v];
-    } else {
-#pragma unroll
-      for (int v = 0; v < CNT; ++v)
-        if (v < count) to[v] += dense_widen<BF>(from[v]);
-    }
-  };
-  if (a.bias) {
-    add(a.bias + n, o);
-    if constexpr (GATED) add(a.bias + cols + n, u);
-  }
   dense_act<CNT>(o, a.act);
   if constexpr (GATED) {
 #pragma unroll
     for (int v = 0; v < CNT; ++v) o[v] *= u[v];
   } else if (a.residual) {
-    add(a.residual + at, o);
+    dense_add_run<BF, CNT>(a, a.residual + at, count, o);
   }
   if (a.out_f32) {
     float* y = static_cast<float*>(a.y) + at;
@@ -193,6 +193,17 @@ __device__ __forceinline__ void dense_store(const DenseArgs& a, int64_t r, int n
         if (v < count) y[v] = static_cast<uint16_t>(v % 2 ? q[v / 2] >> 16 : q[v / 2]);
     }
   }
+}
+
+// ... of sums, with the bias
+template <bool BF, int CNT, bool GATED>
+__device__ __forceinline__ void dense_store(const DenseArgs& a, int64_t r, int n, float (&o)[CNT], float (&u)[CNT]) {
+  if (a.bias) {
+    const int cols = static_cast<int>(GATED ? a.N / 2 : a.N), count = cols - n < CNT ? cols - n : CNT;
+    dense_add_run<BF, CNT>(a, a.bias + n, count, o);
+    if constexpr (GATED) dense_add_run<BF, CNT>(a, a.bias + cols + n, count, u);
+  }
+  dense_finish<BF, CNT, GATED>(a, r, n, o, u);
 }
 
 }  // namespace gq

@@ -237,6 +237,13 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p
   constexpr int kCols = MI * TN, kRow = kCols + 4, kLanes = kPart / 8, kRows = 64 / kLanes < MI ? 64 / kLanes : MI;
   float* const mine = reinterpret_cast<float*>(smem) + wave * MI * kRow;
   const bool share = splits > 1;
+  const int n = n0 + (wave % WN) * kPart + (lane % kLanes) * 8;  // this lane's eight columns, in every row that it stores
+  float bias[P][8] = {};
+  const bool biased = !share && p.bias != nullptr;
+  if (biased && n < half) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) dense_add_run<BF, 8>(p, p.bias + i * half + n, half - n < 8 ? half - n : 8, bias[i]);
+  }
   float* const to = static_cast<float*>(p.workspace) + (part * p.rows + r0) * N;
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
@@ -254,7 +261,6 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p
 #pragma unroll
     for (int t = 0; t < (MI + kRows - 1) / kRows; ++t) {
       const int row = t * kRows + lane / kLanes, col = (lane % kLanes) * 8, r = wm + MI * j + row;
-      const int n = n0 + (wave % WN) * kPart + col;
       if (row < MI && lane / kLanes < kRows && r < rows && n < half) {
         float o[2][8];
 #pragma unroll
@@ -266,7 +272,13 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p
             for (int e = 0; e < 4; ++e) o[i][v + e] = a[e];
           }
         if (!share) {
-          dense_store<BF, 8, GATED>(p, r0 + r, n, o[0], o[P - 1]);
+          if (biased) {
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+#pragma unroll
+              for (int v = 0; v < 8; ++v) o[i][v] += bias[i][v];
+          }
+          dense_finish<BF, 8, GATED>(p, r0 + r, n, o[0], o[P - 1]);
         } else {  // a share of K: its sums go to the scratch as they are
           for (int i = 0; i < P; ++i) {
             float* const at = to + static_cast<int64_t>(r) * N + i * half + n;
