@@ -16,6 +16,8 @@ constexpr int64_t kMaxDim = (int64_t(1) << 31) - 256;
 // numbers of a row: 256 rows of a tile are to end below what is left of 2^32 bytes at any block of K
 constexpr int64_t kMaxRow = (int64_t(1) << 23) - 128;
 
+constexpr int64_t kMostRows = int64_t(1) << 20;  // in one launch
+
 bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 bool act_ok(int a) { return a >= MI355GQ_ACT_NONE && a <= MI355GQ_ACT_GELU_TANH; }
 bool dim_ok(int64_t d) { return d >= 0 && d < kMaxDim; }
@@ -62,12 +64,20 @@ int product(const char* what, const void* x, const void* w, const void* bias, co
     a.workspace_bytes = workspace_bytes;
   }
   const hipStream_t s = as_stream(stream);
-  hipError_t e = hipErrorNotSupported;
-  if (gq::dense_aligned(a)) {
-    if (few_rows(M, a.N, K)) e = gq::launch_dense_rows(a, s);
-    if (e == hipErrorNotSupported) e = gq::launch_dense_tile(a, s);
+  const int64_t y_row = cols * (a.out_f32 ? 4 : 2);
+  hipError_t e = hipSuccess;
+  for (int64_t r = 0; r < M && e == hipSuccess; r += kMostRows) {  // (2^32 work items or more in a launch would wrap, without an error)
+    a.rows = M - r < kMostRows ? M - r : kMostRows;
+    e = hipErrorNotSupported;
+    if (gq::dense_aligned(a)) {
+      if (few_rows(a.rows, a.N, K)) e = gq::launch_dense_rows(a, s);
+      if (e == hipErrorNotSupported) e = gq::launch_dense_tile(a, s);
+    }
+    if (e == hipErrorNotSupported) e = gq::launch_dense_simple(a, s);
+    a.x += a.rows * K;
+    if (a.residual != nullptr) a.residual += a.rows * cols;
+    a.y = static_cast<char*>(a.y) + a.rows * y_row;
   }
-  if (e == hipErrorNotSupported) e = gq::launch_dense_simple(a, s);
   return hip_result(e, what);
 }
 
@@ -85,7 +95,7 @@ extern "C" {
 int64_t mi355gq_dense_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated) {
   const int64_t rows_of_w = gated ? 2 * N : N;
   if (!dim_ok(M) || !dim_ok(N) || !dim_ok(rows_of_w) || !dim_ok(K) || M == 0 || N == 0 || K == 0 || few_rows(M, rows_of_w, K) || K % 8 != 0) return 0;
-  return gq::dense_tile_workspace_bytes(M, rows_of_w, K);
+  return gq::dense_tile_workspace_bytes(M < kMostRows ? M : kMostRows, rows_of_w, K);
 }
 
 int mi355gq_dense_linear(const void* x, const void* w, const void* bias, const void* residual, int64_t M, int64_t N, int64_t K, int activation,

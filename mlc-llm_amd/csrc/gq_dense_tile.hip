@@ -102,15 +102,29 @@ DensePlan plan_of(int64_t rows, int64_t N, int64_t K, bool only_whole = false) {
   return best;
 }
 
+// The plan of a call, made for its workspace and needed again for its launch right behind: 2 us of arithmetic.
+DensePlan plan_for(int64_t rows, int64_t N, int64_t K) {
+  struct Last {
+    int64_t rows = 0, N, K;
+    int variant, split;
+    DensePlan plan;
+  };
+  static thread_local Last last;
+  const int variant = options().gemm_variant, split = options().gemm_split_k;
+  if (last.rows != rows || last.N != N || last.K != K || last.variant != variant || last.split != split)
+    last = {rows, N, K, variant, split, plan_of(rows, N, K)};
+  return last.plan;
+}
+
 }  // namespace
 
 int64_t dense_tile_workspace_bytes(int64_t rows, int64_t N, int64_t K) {
-  const DensePlan p = plan_of(rows, N, K);
+  const DensePlan p = plan_for(rows, N, K);
   return p.splits > 1 ? p.splits * rows * N * 4 : 0;
 }
 
 hipError_t launch_dense_tile(const DenseArgs& a, hipStream_t s) {
-  const DensePlan plan = plan_of(a.rows, a.N, a.K);
+  const DensePlan plan = plan_for(a.rows, a.N, a.K);
   auto go = [&](int part) {
     return a.bf16 ? launch_dense_part_bf16(a, plan, part, s) : launch_dense_part_f16(a, plan, part, s);
   };

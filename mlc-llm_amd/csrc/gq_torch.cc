@@ -415,10 +415,15 @@ const Tensor* beside(PyObject* o, const Tensor& x, at::IntArrayRef sizes) {
 
 void* stream_of(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.device().index()).stream(); }
 
-// dense(x, weight, bias | None, activation | None, out_dtype | None, residual | None): GATED without the last
+bool overlap(const Tensor& a, const Tensor& b) {
+  const char *a0 = static_cast<const char*>(a.const_data_ptr()), *b0 = static_cast<const char*>(b.const_data_ptr());
+  return a0 < b0 + b.nbytes() && b0 < a0 + a.nbytes();
+}
+
+// dense(x, weight, bias | None, activation | None, out_dtype | None, residual | None, out | None): GATED without the last two
 template <bool GATED>
 PyObject* dense(PyObject* const* a, Py_ssize_t nargs) {
-  if (nargs != (GATED ? 5 : 6) || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+  if (nargs != (GATED ? 5 : 7) || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
   const Tensor *x = plain(a[0]), *w = plain(a[1]), *bias = nullptr, *residual = nullptr;
   int act = 0, code = 0;
   if (!x || !w || x->dim() < 1 || w->dim() != 2 || !half_code(x->scalar_type(), &code) || w->scalar_type() != x->scalar_type() || w->device() != x->device() ||
@@ -434,13 +439,23 @@ PyObject* dense(PyObject* const* a, Py_ssize_t nargs) {
     if (out_dtype != x->scalar_type() && out_dtype != ScalarType::Float) Py_RETURN_NONE;
   }
   const auto shape = with_last(*x, n);
-  if (!GATED && a[5] != Py_None && !(residual = beside(a[5], *x, shape))) Py_RETURN_NONE;
+  const Tensor* given = nullptr;
+  if constexpr (!GATED) {
+    if (a[5] != Py_None && !(residual = beside(a[5], *x, shape))) Py_RETURN_NONE;
+    if (a[6] != Py_None) {
+      given = plain(a[6]);
+      if (!given || given->scalar_type() != out_dtype || given->device() != x->device() || given->sizes() != at::IntArrayRef(shape) || overlap(*given, *x) ||
+          overlap(*given, *w) || (bias && overlap(*given, *bias)) ||
+          (residual && overlap(*given, *residual) && (given->const_data_ptr() != residual->const_data_ptr() || out_dtype != residual->scalar_type())))
+        Py_RETURN_NONE;
+    }
+  }
   Tensor out;
   int rc;
   {
     pybind11::gil_scoped_release release;
     const c10::DeviceGuard guard(x->device());
-    out = at::empty(shape, x->options().dtype(out_dtype));
+    out = given ? *given : at::empty(shape, x->options().dtype(out_dtype));
     const int64_t bytes = mi355gq_dense_linear_workspace_bytes(m, n, k, GATED);
     Scratch ws(*x, bytes);
     const void *xp = x->const_data_ptr(), *wp = w->const_data_ptr(), *bp = bias ? bias->const_data_ptr() : nullptr;

@@ -990,7 +990,7 @@ def dense_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     activation: None, "relu", "silu", "gelu" (v Phi(v)) or "gelu_tanh".  Sums and epilogue are float32 with one rounding, to out_dtype: x's
     type (the default) or float32.  residual has x's type and y's shape; as `out` too it is updated in place."""
     native = _lib.native()
-    done = native.dense_linear(x, weight, bias, activation, out_dtype, residual) if native is not None and out is None else None
+    done = native.dense_linear(x, weight, bias, activation, out_dtype, residual, out) if native is not None else None
     if isinstance(done, torch.Tensor):
         return done
     if done is not None:

@@ -182,7 +182,7 @@ def test_in_place_residual_and_neighbours(m):
     hidden = wide[1 : m + 1]
     hidden.copy_(_normal(g, torch.float16, m, n))
     want = linear_ref(x, w, None, "gelu_tanh", hidden.clone(), torch.float16)
-    assert ops.dense_linear(x, w, activation="gelu_tanh", residual=hidden, out=hidden) is hidden
+    assert ops.dense_linear(x, w, activation="gelu_tanh", residual=hidden, out=hidden).data_ptr() == hidden.data_ptr()
     close(hidden, want)
     assert (wide[0] == -3).all() and (wide[m + 1] == -3).all()
 
@@ -234,6 +234,31 @@ def test_not_finite():
         x[1, 7] = nan  # one token's trouble is its own
         y = ops.dense_linear(x, w)
         assert y[1].isnan().all() and y[0, 0] == 1
+
+
+@pytest.mark.parametrize("m", [2, 12, 30, 100, 300])
+def test_not_finite_in_the_next_row(m):
+    """Rows that end inside a block of K: what stands behind them, the next row's first numbers, is not theirs."""
+    g = _gen(m)
+    k, n = 200, 81
+    x, w = _normal(g, torch.bfloat16, m, k), _normal(g, torch.bfloat16, n, k, scale=k**-0.5)
+    clean, clean_gated = ops.dense_linear(x, w), ops.dense_linear_gated(x, w[:80])
+    w[1::2], x[1::2] = math.nan, math.inf
+    got = ops.dense_linear(x, w)
+    assert torch.equal(got[::2, ::2], clean[::2, ::2])
+    assert got[:, 1::2].isnan().all()
+    assert torch.equal(ops.dense_linear_gated(x, w[:80])[::2, ::2], clean_gated[::2, ::2])
+
+
+def test_more_rows_than_a_launch_takes():
+    m, n, k = (1 << 20) + 77, 24, 40
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x, w = (torch.randn(r, k, generator=g, device="cuda").to(torch.float16) for r in (m, n))
+    r = torch.randn(m, n, generator=g, device="cuda").to(torch.float16)
+    y = ops.dense_linear(x, w, activation="relu", residual=r, out_dtype=torch.float32)
+    rows = torch.tensor([0, 1, (1 << 20) - 1, 1 << 20, (1 << 20) + 1, m - 1], device="cuda")
+    close(y[rows], linear_ref(x[rows], w, None, "relu", r[rows], torch.float32))
+    close(ops.dense_linear_gated(x, w)[rows], gated_ref(x[rows], w, None, "silu", torch.float16))
 
 
 @pytest.mark.parametrize("m", [3, 40])
@@ -438,7 +463,7 @@ def test_router_layer_and_residual_together():
     shared = ops.dense_linear_gated(x, up, activation="gelu_tanh")
     close(shared, gated_ref(x, up, None, "gelu_tanh", dtype))
     y = ops.dense_linear(shared, down, residual=routed, out=routed)
-    assert y is routed
+    assert y.data_ptr() == routed.data_ptr()
     close(y, linear_ref(shared, down, None, None, ops.dense_moe(x, logits, w13, w2, k), dtype))
 
 
@@ -463,12 +488,13 @@ def test_native_and_python_routes_agree(lead):
         for act in ACTS:
             for out_dtype in (None, torch.float32):
                 for residual in (None, r):
-                    assert isinstance(native.dense_linear(x, w, bias, act, out_dtype, residual), torch.Tensor)
+                    assert isinstance(native.dense_linear(x, w, bias, act, out_dtype, residual, None), torch.Tensor)
                     got = ops.dense_linear(x, w, bias, act, residual, out_dtype)
                     want = ops.dense_linear(x.as_subclass(Plain), w, bias, act, residual, out_dtype)
                     assert got.dtype == want.dtype and got.shape == (*lead, n) and torch.equal(got, want.as_subclass(torch.Tensor))
                     out = torch.empty_like(got)
-                    assert ops.dense_linear(x, w, bias, act, residual, out_dtype, out) is out and torch.equal(out, got)
+                    assert native.dense_linear(x, w, bias, act, out_dtype, residual, out) is not None
+                    assert ops.dense_linear(x, w, bias, act, residual, out_dtype, out).data_ptr() == out.data_ptr() and torch.equal(out, got)
                 assert isinstance(native.dense_linear_gated(x, w, bias, act, out_dtype), torch.Tensor)
                 got, want = ops.dense_linear_gated(x, w, bias, act, out_dtype), ops.dense_linear_gated(x.as_subclass(Plain), w, bias, act, out_dtype)
                 assert got.dtype == want.dtype and got.shape == (*lead, n // 2) and torch.equal(got, want.as_subclass(torch.Tensor))
