@@ -21,17 +21,17 @@ constexpr int kWaves = kStreamWaves, kThreads = 64 * kWaves;
 struct MoeSegment {
   int e, row0, rows;
 };
-// The workspace: what the first kernel leaves for the second.  Offsets; at 0 the number of segments.
+// The workspace: what the first kernel leaves for the second.  Offsets; at 0 the number of segments, at kSegsAt these.
+constexpr int64_t kSegsAt = 256;
 struct MoeLayout {
-  int64_t segs, row_token, tickets, shares, h, bytes;  // h: [2][T k][inter]
+  int64_t row_token, tickets, shares, h, bytes;  // h: [2][T k][inter]
 };
 inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 inline int moe_shares(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k);
 inline MoeLayout moe_layout(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k) {
   const int64_t slots = T * k, tiles = (hidden + 15) / 16;
   MoeLayout l;
-  l.segs = 256;
-  l.row_token = l.segs + up256(slots * static_cast<int64_t>(sizeof(MoeSegment)));
+  l.row_token = kSegsAt + up256(slots * static_cast<int64_t>(sizeof(MoeSegment)));
   l.tickets = l.row_token + up256(slots * 4);
   l.shares = l.tickets + up256(tiles * 4);
   const int shares = moe_shares(T, hidden, inter, experts, k);
@@ -68,18 +68,21 @@ struct MoeTables {  // in LDS, in front of the rest
   float* row_w;        // [T k]
   uint64_t* totals;    // [waves]
 };
-inline size_t moe_tables_bytes(int experts, int slots) { return (64 + static_cast<size_t>(experts) * 12 + static_cast<size_t>(slots) * (16 + sizeof(MoeSegment)) + 15) / 16 * 16; }
+inline size_t moe_tables_bytes(int experts, int slots) {
+  return (64 + static_cast<size_t>(experts) * 12 + static_cast<size_t>(slots) * (16 + sizeof(MoeSegment)) + 15) / 16 * 16;
+}
 
 }  // namespace
 
 // NC: experts a lane in the routing.  XG: eights of rows of a segment.
 template <bool BF, int NC, int XG, int D>
-__global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(DenseMoeArgs a, MoeLayout layout, int group_inv, int logits_vec, int kw_log2, int nb,
-                                                                  int tables_bytes) {
+__global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(
+    const void* __restrict__ logits, int T, int E, int top_k, int logits_dtype, int logits_vec, int tables_bytes, int group_inv, int kw_log2, int nb,
+    DenseMoeArgs a, MoeLayout layout) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   constexpr int TT = (XG + 1) / 2, kSegRows = 8 * XG;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int slots = a.T * a.k, E = a.experts, K = a.hidden, I = a.inter;
+  const int slots = T * top_k, K = a.hidden, I = a.inter;
   MoeTables tab;
   tab.totals = reinterpret_cast<uint64_t*>(smem);
   tab.mask = tab.totals + 8;
@@ -95,19 +98,19 @@ __global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(
   // ---- routing ----
   if (tid < E) tab.mask[tid] = 0;
   __syncthreads();
-  const GateRule rule{a.score_bias, E, a.k, a.sigmoid, a.groups, a.top_groups, group_inv, a.renormalize, a.scale};
-  for (int t0 = 2 * wave; t0 < a.T; t0 += 2 * kWaves) {
+  const GateRule rule{a.score_bias, E, top_k, a.sigmoid, a.groups, a.top_groups, group_inv, a.renormalize, a.scale};
+  for (int t0 = 2 * wave; t0 < T; t0 += 2 * kWaves) {
     const int t = t0 + (lane >> 5), r = lane & 31;
-    const int from = t < a.T ? t : a.T - 1;
+    const int from = t < T ? t : T - 1;
     float score[NC];
-    if (a.logits_dtype == MODEL_F32) gate_load<NC, MODEL_F32>(a.logits, from, E, r, logits_vec, score);
-    else if (a.logits_dtype == MODEL_BF16) gate_load<NC, MODEL_BF16>(a.logits, from, E, r, logits_vec, score);
-    else gate_load<NC, MODEL_F16>(a.logits, from, E, r, logits_vec, score);
+    if (logits_dtype == MODEL_F32) gate_load<NC, MODEL_F32>(logits, from, E, r, logits_vec, score);
+    else if (logits_dtype == MODEL_BF16) gate_load<NC, MODEL_BF16>(logits, from, E, r, logits_vec, score);
+    else gate_load<NC, MODEL_F16>(logits, from, E, r, logits_vec, score);
     int id;
     const float w = gate_pair<NC>(gate, score, rule, &id);
-    if (r < a.k && t < a.T) {
-      tab.slot_id[t * a.k + r] = id;
-      tab.slot_w[t * a.k + r] = w;
+    if (r < top_k && t < T) {
+      tab.slot_id[t * top_k + r] = id;
+      tab.slot_w[t * top_k + r] = w;
       atomicOr(reinterpret_cast<unsigned long long*>(tab.mask) + id, 1ull << t);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -150,7 +153,7 @@ __global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(
   __syncthreads();
   char* const ws = static_cast<char*>(a.workspace);
   if (blockIdx.x == 0) {
-    for (int i = tid; i < segs_all; i += kThreads) reinterpret_cast<MoeSegment*>(ws + layout.segs)[i] = tab.segs[i];
+    for (int i = tid; i < segs_all; i += kThreads) reinterpret_cast<MoeSegment*>(ws + kSegsAt)[i] = tab.segs[i];
     for (int i = tid; i < slots; i += kThreads) reinterpret_cast<int*>(ws + layout.row_token)[i] = tab.row_token[i];
     for (int i = tid; i < (K + 15) / 16; i += kThreads) reinterpret_cast<int*>(ws + layout.tickets)[i] = 0;
     if (tid == 0) *reinterpret_cast<int*>(ws) = segs_all;
@@ -236,24 +239,25 @@ __device__ __forceinline__ void moe_store(uint16_t* to, const float4_t& v) {
 
 // Sixteen columns of the output for all tokens a workgroup; gridDim.y workgroups share the K, which is all segments' inter.
 template <bool BF, int XG, int D>
-__global__ __launch_bounds__(kThreads, XG == 1 && D == 2 ? 4 : 2) void dense_moe_down_kernel(DenseMoeArgs a, MoeLayout layout) {
+__global__ __launch_bounds__(kThreads, XG == 1 && D == 2 ? 4 : 2) void dense_moe_down_kernel(
+    const void* __restrict__ from, const int* __restrict__ tokens, const uint16_t* __restrict__ w2, int T, int slots, int H, int I, DenseMoeArgs a,
+    MoeLayout layout) {
   constexpr int TT = (XG + 1) / 2, kStage = stream_stage<XG, 2>();
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
-  const int slots = a.T * a.k;
   char* const ws = static_cast<char*>(a.workspace);
   uint8_t* const ring = smem + wave * stream_ring<XG, 2, D>();
   float4_t* const sums = reinterpret_cast<float4_t*>(smem + kWaves * stream_ring<XG, 2, D>());  // [waves][T][4]
-  int* const row_token = reinterpret_cast<int*>(sums + kWaves * a.T * 4);                     // [T k]
+  int* const row_token = reinterpret_cast<int*>(sums + kWaves * T * 4);                     // [T k]
   MoeSegment* const segs = reinterpret_cast<MoeSegment*>(row_token + slots);                  // [T k at most]
-  const int n_segs = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(ws));
+  const int n_segs = __builtin_amdgcn_readfirstlane(*static_cast<const int*>(from));
   for (int i = tid; i < slots; i += kThreads) {  // (all that may be there, without a wait for their number)
-    row_token[i] = reinterpret_cast<const int*>(ws + layout.row_token)[i];
-    segs[i] = reinterpret_cast<const MoeSegment*>(ws + layout.segs)[i];
+    row_token[i] = tokens[i];
+    segs[i] = reinterpret_cast<const MoeSegment*>(static_cast<const char*>(from) + kSegsAt)[i];
   }
-  for (int i = tid; i < kWaves * a.T * 4; i += kThreads) sums[i] = float4_t{};
+  for (int i = tid; i < kWaves * T * 4; i += kThreads) sums[i] = float4_t{};
   __syncthreads();
-  const int H = a.hidden, I = a.inter, n0 = blockIdx.x * 16, per = (I + kStreamBlock - 1) / kStreamBlock;  // blocks a segment
+  const int n0 = blockIdx.x * 16, per = (I + kStreamBlock - 1) / kStreamBlock;  // blocks a segment
   const int blocks = n_segs * per;
   const int begin = static_cast<int>(static_cast<int64_t>(blocks) * blockIdx.y / gridDim.y);
   const int end = static_cast<int>(static_cast<int64_t>(blocks) * (blockIdx.y + 1) / gridDim.y);
@@ -282,7 +286,7 @@ __global__ __launch_bounds__(kThreads, XG == 1 && D == 2 ? 4 : 2) void dense_moe
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int64_t left = H - n0 - 8 * i;
-      p.w[i] = dense_buffer(reinterpret_cast<const char*>(a.w2) + (e * H + n0 + 8 * i) * pitch, left > 0 ? 8 * pitch : 0);  // (hidden is a multiple of 8)
+      p.w[i] = dense_buffer(reinterpret_cast<const char*>(w2) + (e * H + n0 + 8 * i) * pitch, left > 0 ? 8 * pitch : 0);  // (hidden is a multiple of 8)
     }
     p.x[0] = h_hi;
     p.x[1] = h_lo;
@@ -302,7 +306,7 @@ __global__ __launch_bounds__(kThreads, XG == 1 && D == 2 ? 4 : 2) void dense_moe
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
       const int c = 16 * t + (lane & 15);
-      if (c < seg.rows) sums[(wave * a.T + row_token[seg.row0 + c]) * 4 + quad] += acc[t];
+      if (c < seg.rows) sums[(wave * T + row_token[seg.row0 + c]) * 4 + quad] += acc[t];
       acc[t] = float4_t{};
     }
   };
@@ -327,10 +331,10 @@ __global__ __launch_bounds__(kThreads, XG == 1 && D == 2 ? 4 : 2) void dense_moe
   __syncthreads();
 
   // The waves' sums in their order: a thread four columns of a token.
-  for (int i = tid; i < a.T * 4; i += kThreads) {
+  for (int i = tid; i < T * 4; i += kThreads) {
     const int n = n0 + 4 * (i & 3);
     float4_t v = sums[i];
-    for (int w = 1; w < kWaves; ++w) v += sums[w * a.T * 4 + i];
+    for (int w = 1; w < kWaves; ++w) v += sums[w * T * 4 + i];
     sums[i] = v;
     if (gridDim.y == 1 && n < H) moe_store<BF>(a.out + static_cast<int64_t>(i >> 2) * H + n, v);
   }
@@ -338,8 +342,8 @@ __global__ __launch_bounds__(kThreads, XG == 1 && D == 2 ? 4 : 2) void dense_moe
   // Shares of several workgroups: the one that comes last adds them all, in their order.  They go past the L2 of a die (agent-scope stores
   // and loads) and are there before the ticket is drawn; a fence would write back the die's whole L2 instead, which took 100 us.
   float* const shares = reinterpret_cast<float*>(ws + layout.shares);  // [shares][tiles][T][16]
-  auto share_of = [&](int s) { return shares + (static_cast<int64_t>(s) * gridDim.x + blockIdx.x) * a.T * 16; };
-  for (int i = tid; i < a.T * 4; i += kThreads)
+  auto share_of = [&](int s) { return shares + (static_cast<int64_t>(s) * gridDim.x + blockIdx.x) * T * 16; };
+  for (int i = tid; i < T * 4; i += kThreads)
 #pragma unroll
     for (int v = 0; v < 4; ++v) __hip_atomic_store(share_of(blockIdx.y) + 4 * i + v, sums[i][v], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -350,7 +354,7 @@ __global__ __launch_bounds__(kThreads, XG == 1 && D == 2 ? 4 : 2) void dense_moe
                static_cast<int>(gridDim.y) - 1;
   __syncthreads();
   if (!*last_one) return;
-  for (int i = tid; i < a.T * 4; i += kThreads) {
+  for (int i = tid; i < T * 4; i += kThreads) {
     float4_t v = {};
     for (int s = 0; s < static_cast<int>(gridDim.y); ++s)
 #pragma unroll
@@ -382,8 +386,8 @@ static hipError_t launch_up(const DenseMoeArgs& a, const MoeLayout& layout, hipS
   if (e != hipSuccess) return e;
   const int vec = a.experts % 8 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0;
   const int64_t at_a_time = kStreamUnits * (lds > 80 * 1024 ? 1 : 2);
-  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(sets < at_a_time ? sets : at_a_time)), dim3(kThreads), lds, s, a, layout, gate_group_inv(a.experts, a.groups),
-                     vec, plan.kw_log2, plan.nb, static_cast<int>(tables));
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(sets < at_a_time ? sets : at_a_time)), dim3(kThreads), lds, s, a.logits, a.T, a.experts,
+                     a.k, a.logits_dtype, vec, static_cast<int>(tables), gate_group_inv(a.experts, a.groups), plan.kw_log2, plan.nb, a, layout);
   return hipGetLastError();
 }
 
@@ -397,7 +401,8 @@ static hipError_t launch_down(const DenseMoeArgs& a, const MoeLayout& layout, hi
   auto* kern = dense_moe_down_kernel<BF, XG, D>;
   const hipError_t e = may_use(kern, lds);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(kern, grid, dim3(kThreads), lds, s, a, layout);
+  hipLaunchKernelGGL(kern, grid, dim3(kThreads), lds, s, a.workspace, reinterpret_cast<const int*>(static_cast<const char*>(a.workspace) + layout.row_token),
+                     a.w2, a.T, a.T * a.k, a.hidden, a.inter, a, layout);
   return hipGetLastError();
 }
 

@@ -7,15 +7,16 @@ namespace {
 constexpr int kDepth = 4;  // blocks in flight a wave
 }
 
+// (The arguments that the loads wait for come first, in scalar registers.)
 // Eight waves: KW of them share the K of an item, 16 rows of W (gated: 8 gate rows and their up rows), and their sums meet in LDS.
 template <bool BF, bool GATED, int XG>
-__global__ __launch_bounds__(64 * kStreamWaves, 2) void dense_rows_kernel(DenseArgs a, int kw_log2, int nb, int rounds) {
+__global__ __launch_bounds__(64 * kStreamWaves, 2) void dense_rows_kernel(
+    const uint16_t* __restrict__ x, const uint16_t* __restrict__ w, int K, int rows, int cols_, int kw_log2, int nb, int rounds, DenseArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   constexpr int TT = (XG + 1) / 2, kCols = GATED ? 8 : 16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int KW = 1 << kw_log2, kw = wave & (KW - 1), nw = wave >> kw_log2;
-  const int K = static_cast<int>(a.K), rows = static_cast<int>(a.rows);
-  const int64_t pitch = a.K * 2, cols = GATED ? a.N / 2 : a.N, stride = static_cast<int64_t>(gridDim.x) * (kStreamWaves >> kw_log2);
+  const int64_t pitch = static_cast<int64_t>(K) * 2, cols = cols_, stride = static_cast<int64_t>(gridDim.x) * (kStreamWaves >> kw_log2);
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (kStreamWaves >> kw_log2) + nw;
   uint8_t* const ring = smem + wave * stream_ring<XG, 1, kDepth>();
   auto place_of = [&](int round) {
@@ -26,9 +27,9 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void dense_rows_kernel(DenseA
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int64_t left = GATED ? cols - n0 : cols - n0 - 8 * i, count = p.end == 0 || left < 0 ? 0 : left < 8 ? left : 8;
-      p.w[i] = dense_buffer(reinterpret_cast<const char*>(a.w) + (n0 + i * (GATED ? cols : 8)) * pitch, count * pitch);
+      p.w[i] = dense_buffer(reinterpret_cast<const char*>(w) + (n0 + i * (GATED ? cols : 8)) * pitch, count * pitch);
     }
-    p.x[0] = dense_buffer(a.x, a.rows * pitch);
+    p.x[0] = dense_buffer(x, rows * pitch);
 #pragma unroll
     for (int g = 0; g < XG; ++g) {
       const int r = 8 * g + (lane >> 3);
@@ -66,8 +67,8 @@ static hipError_t launch(const DenseArgs& a, hipStream_t s) {
   const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kern));
   if (e != hipSuccess) return e;
   note_kernel("dense_rows up to %d rows%s, %d waves share K", 8 * XG, GATED ? " gated" : "", 1 << plan.kw_log2);
-  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((sets + plan.rounds - 1) / plan.rounds)), dim3(64 * kStreamWaves), lds, s, a, plan.kw_log2, plan.nb,
-                     plan.rounds);
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((sets + plan.rounds - 1) / plan.rounds)), dim3(64 * kStreamWaves), lds, s, a.x, a.w,
+                     static_cast<int>(a.K), static_cast<int>(a.rows), static_cast<int>(cols), plan.kw_log2, plan.nb, plan.rounds, a);
   return hipGetLastError();
 }
 

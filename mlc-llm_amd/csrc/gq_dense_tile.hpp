@@ -1,4 +1,4 @@
-// Products with 16-bit weights of more than a few rows: tiles through LDS on v_mfma_f32_16x16x32 or 32x32x16.
+// Products with 16-bit weights of more than a few rows: tiles through LDS on v_mfma_f32_16x16x32.
 #pragma once
 
 #include "gq_dense_common.hpp"
@@ -20,35 +20,23 @@ __device__ __forceinline__ rsrc_t buffer_of(const void* base, uint32_t bytes) {
 // bytes that a tile may reach: rows are below 2^24 bytes, so that a tile's 256 end below what is left of 2^32 at any block of K
 __device__ __forceinline__ uint32_t reach(int64_t bytes) { return bytes > 0xffffffffll ? 0xffffffffu : static_cast<uint32_t>(bytes); }
 
-template <int MI>
-using TileSums = std::conditional_t<MI == 16, float4_t, float16_t>;  // of a lane
 // loads that go out at a time where there are `rows` times to send them
 constexpr int burst_of(int w_loads, int x_loads, int rows) {
   int burst = 2;
   while ((w_loads + burst - 1) / burst + (x_loads + burst - 1) / burst > rows) burst *= 2;
   return burst;
 }
-template <bool BF>
-__device__ __forceinline__ float4_t tile_mfma(int4_t w, int4_t x, float4_t acc) {
-  return dense_mfma<BF>(w, x, acc);
-}
-template <bool BF>
-__device__ __forceinline__ float16_t tile_mfma(int4_t w, int4_t x, float16_t acc) {
-  if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, w), __builtin_bit_cast(bf16x8_t, x), acc, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, w), __builtin_bit_cast(half8_t, x), acc, 0, 0, 0);
-}
-
 }  // namespace
 
-// WN x WM waves, each TN x TM results of MI x MI: a tile of BN = MI WN TN rows of W by BM = MI WM TM rows of x.
+// WN x WM waves, each TN x TM results of 16 x 16: a tile of BN = 16 WN TN rows of W by BM = 16 WM TM rows of x.
 // GATED: half of a wave's rows of W are gate rows and half the up rows that belong to them.
 // WS stages of W and XS of x in LDS: W is WS - 1 blocks ahead, x XS - 1.
 // ONCE: no other workgroup reads these rows of W.
-template <bool BF, bool GATED, int MI, int WN, int WM, int TN, int TM, int WS, int XS, bool ONCE>
+template <bool BF, bool GATED, int WN, int WM, int TN, int TM, int WS, int XS, bool ONCE>
 __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p, int n_first, int n_tiles, int m_tiles, int splits, int per_split) {
-  constexpr int kWaves = WN * WM, BN = MI * WN * TN, BM = MI * WM * TM, KS = MI / 8;  // KS: instructions to a block
+  constexpr int kWaves = WN * WM, BN = 16 * WN * TN, BM = 16 * WM * TM;
   constexpr int kWLoads = BN / 8 / kWaves, kXLoads = (BM / 8 + kWaves - 1) / kWaves;  // of 1 KiB, eight rows, a wave and block of K
-  constexpr int P = GATED ? 2 : 1, kPart = MI * TN / P;  // parts of a wave's rows of W
+  constexpr int P = GATED ? 2 : 1, kPart = 16 * TN / P;  // parts of a wave's rows of W
   constexpr int kWStage = BN * 128, kXStage = kXLoads * kWaves * 1024;  // of a block
   static_assert(XS == WS || XS == WS - 1, "hand_over's count");
   static_assert(BN / 8 % kWaves == 0 && kPart % 8 == 0, "whole loads");
@@ -78,9 +66,9 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p
   const char* const x0 = reinterpret_cast<const char*>(p.x) + r0 * pitch;
   const uint32_t w_bytes = reach(static_cast<int64_t>(half - n0) * pitch), x_bytes = reach((p.rows - r0) * pitch);
   // row of the tile -> (gate or up, row of W from n0 on)
-  auto w_part = [&](int row) { return row % (MI * TN) / kPart; };
+  auto w_part = [&](int row) { return row % (16 * TN) / kPart; };
   auto w_row = [&](int row) {
-    const int n = row / (MI * TN) * kPart + row % kPart;
+    const int n = row / (16 * TN) * kPart + row % kPart;
     return n0 + n < half ? n : half - 1 - n0;
   };
 
@@ -116,23 +104,22 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p
     for (int i = from; i < to; ++i) load_to_lds<false>(rsrc, x_off[i], smem + WS * kWStage + slot + (i * kWaves + wave) * 1024);
   };
 
-  const int wn = (wave % WN) * MI * TN, wm = (wave / WN) * MI * TM, frow = lane & (MI - 1), fpart = lane / MI;
-  typedef TileSums<MI> Acc;
-  Acc acc[TN][TM];
+  const int wn = (wave % WN) * 16 * TN, wm = (wave / WN) * 16 * TM, frow = lane & 15, fpart = lane >> 4;
+  float4_t acc[TN][TM];
 #pragma unroll
   for (int i = 0; i < TN; ++i)
 #pragma unroll
-    for (int j = 0; j < TM; ++j) acc[i][j] = Acc{};
+    for (int j = 0; j < TM; ++j) acc[i][j] = float4_t{};
 
   struct Operand {
-    int4_t v[KS];  // chunks fpart, fpart + 64 / MI, ... of a row
+    int4_t v[2];  // chunks fpart and fpart + 4 of a row
   };
   auto frag = [&](const uint8_t* stage, int g, int row, auto tail) {
     const uint8_t* base = stage + row * 128;
     Operand o;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int c = fpart + s * (64 / MI);
+    for (int s = 0; s < 2; ++s) {
+      const int c = fpart + 4 * s;
       o.v[s] = *reinterpret_cast<const int4_t*>(base + ((c ^ (row & 7)) << 4));
       if constexpr (decltype(tail)::value) {  // (K is a multiple of 8)
         if (g * kBlock + 8 * c >= K) o.v[s] = int4_t{};
@@ -145,8 +132,8 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p
   int w_now = 0, x_now = 0;
   auto after = [](int slot, int stage, int count) { return slot + stage == count * stage ? 0 : slot + stage; };
   auto before = [](int slot, int stage, int count) { return (slot == 0 ? count * stage : slot) - stage; };
-  auto frag_w = [&](int g, int slot, int i, auto tail) { return frag(smem + slot, g, wn + MI * i + frow, tail); };
-  auto frag_x = [&](int g, int slot, int j, auto tail) { return frag(smem + WS * kWStage + slot, g, wm + MI * j + frow, tail); };
+  auto frag_w = [&](int g, int slot, int i, auto tail) { return frag(smem + slot, g, wn + 16 * i + frow, tail); };
+  auto frag_x = [&](int g, int slot, int j, auto tail) { return frag(smem + WS * kWStage + slot, g, wm + 16 * j + frow, tail); };
   // Waits for the next block's stages and hands them over.  Loads come back in order; those of the blocks behind it may still be on
   // their way.  Every wave has read the block before by then, whose stages take the next loads.
   auto hand_over = [&] {
@@ -185,7 +172,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) acc[i][j] = tile_mfma<BF>(fw[i & 1].v[s], fx[j].v[s], acc[i][j]);
+        for (int s = 0; s < 2; ++s) acc[i][j] = dense_mfma<BF>(fw[i & 1].v[s], fx[j].v[s], acc[i][j]);
         if (i + 1 == TN && decltype(has_next)::value) {
           fx[j] = frag_x(g + 1, after(x_now, kXStage, XS), j, next_tail);
           __builtin_amdgcn_sched_barrier(0);  // (at once, not behind the row's other instructions)
@@ -232,10 +219,10 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads that nobody reads may still land in the stages
   __syncthreads();  // (and the last stage has been read)
 
-  // The results change hands through LDS, MI rows of x at a time and each wave in a part of its own, so that a row's columns go out as runs of
+  // The results change hands through LDS, 16 rows of x at a time and each wave in a part of its own, so that a row's columns go out as runs of
   // eight a lane; float32 until the epilogue is through.
-  constexpr int kCols = MI * TN, kRow = kCols + 4, kLanes = kPart / 8, kRows = 64 / kLanes < MI ? 64 / kLanes : MI;
-  float* const mine = reinterpret_cast<float*>(smem) + wave * MI * kRow;
+  constexpr int kRow = 16 * TN + 4, kLanes = kPart / 8, kRows = 64 / kLanes < 16 ? 64 / kLanes : 16;
+  float* const mine = reinterpret_cast<float*>(smem) + wave * 16 * kRow;
   const bool share = splits > 1;
   const int n = n0 + (wave % WN) * kPart + (lane % kLanes) * 8;  // this lane's eight columns, in every row that it stores
   float bias[P][8] = {};
@@ -248,20 +235,13 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
 #pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-      for (int q = 0; q < MI * MI / 256; ++q) {
-        float4_t v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
-        *reinterpret_cast<float4_t*>(mine + frow * kRow + MI * i + (MI == 16 ? 4 * fpart : 8 * q + 4 * fpart)) = v;
-      }
+    for (int i = 0; i < TN; ++i) *reinterpret_cast<float4_t*>(mine + frow * kRow + 16 * i + 4 * fpart) = acc[i][j];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int t = 0; t < (MI + kRows - 1) / kRows; ++t) {
-      const int row = t * kRows + lane / kLanes, col = (lane % kLanes) * 8, r = wm + MI * j + row;
-      if (row < MI && lane / kLanes < kRows && r < rows && n < half) {
+    for (int t = 0; t < (16 + kRows - 1) / kRows; ++t) {
+      const int row = t * kRows + lane / kLanes, col = (lane % kLanes) * 8, r = wm + 16 * j + row;
+      if (row < 16 && lane / kLanes < kRows && r < rows && n < half) {
         float o[2][8];
 #pragma unroll
         for (int i = 0; i < P; ++i)
@@ -314,10 +294,10 @@ hipError_t launch_dense_join(const DenseArgs& a, int splits, hipStream_t s);
 
 namespace {
 
-template <bool BF, bool GATED, int MI, int WN, int WM, int TN, int TM, int WS, int XS, bool ONCE>
+template <bool BF, bool GATED, int WN, int WM, int TN, int TM, int WS, int XS, bool ONCE>
 hipError_t launch_tile(const DenseArgs& a, const DensePlan& plan, int part, hipStream_t s) {
-  constexpr int P = GATED ? 2 : 1, BN = MI * WN * TN / P, BM = MI * WM * TM, kWaves = WN * WM;  // (BN: columns of y)
-  constexpr size_t stages = size_t(WS * BN * P) * 128 + XS * ((BM / 8 + kWaves - 1) / kWaves * kWaves * 1024), results = size_t(kWaves) * MI * (MI * TN + 4) * 4;
+  constexpr int P = GATED ? 2 : 1, BN = 16 * WN * TN / P, BM = 16 * WM * TM, kWaves = WN * WM;  // (BN: columns of y)
+  constexpr size_t stages = size_t(WS * BN * P) * 128 + XS * ((BM / 8 + kWaves - 1) / kWaves * kWaves * 1024), results = size_t(kWaves) * 16 * (16 * TN + 4) * 4;
   constexpr size_t lds = stages > results ? stages : results;
   static_assert(lds <= 160 * 1024, "LDS of a unit");
   const int64_t blocks = (a.K + kBlock - 1) / kBlock, cols = a.N / P, m_tiles = (a.rows + BM - 1) / BM;
@@ -328,7 +308,7 @@ hipError_t launch_tile(const DenseArgs& a, const DensePlan& plan, int part, hipS
     splits = plan.splits;
     per_split = plan.per_split;
   }
-  auto* kern = dense_tile_kernel<BF, GATED, MI, WN, WM, TN, TM, WS, XS, ONCE>;
+  auto* kern = dense_tile_kernel<BF, GATED, WN, WM, TN, TM, WS, XS, ONCE>;
   if (lds > 65536) {
     const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kern));
     if (e != hipSuccess) return e;
@@ -347,15 +327,21 @@ hipError_t launch_tile(const DenseArgs& a, const DensePlan& plan, int part, hipS
 template <bool BF, bool GATED>
 hipError_t launch_form(const DenseArgs& a, const DensePlan& plan, int part, hipStream_t s) {
   switch (part == 0 ? plan.form : plan.form_rest) {  // rows of W x rows of x
-    case 0: return launch_tile<BF, GATED, 16, 2, 4, 8, 4, 3, 2, false>(a, plan, part, s);  // 256 x 256
-    case 1: return launch_tile<BF, GATED, 16, 4, 2, 4, 6, 3, 2, false>(a, plan, part, s);  // 256 x 192
-    case 2: return launch_tile<BF, GATED, 16, 4, 2, 4, 4, 3, 2, false>(a, plan, part, s);  // 256 x 128
-    case 3: return launch_tile<BF, GATED, 16, 2, 4, 4, 3, 3, 2, false>(a, plan, part, s);  // 128 x 192
-    case 4: return a.rows <= 128 ? launch_tile<BF, GATED, 16, 4, 2, 2, 4, 4, 4, true>(a, plan, part, s) : launch_tile<BF, GATED, 16, 4, 2, 2, 4, 4, 4, false>(a, plan, part, s);  // 128 x 128
-    case 5: return launch_tile<BF, GATED, 16, 2, 2, 4, 4, 3, 2, false>(a, plan, part, s);  // 128 x 128, two a unit
-    case 6: return a.rows <= 128 ? launch_tile<BF, GATED, 16, 2, 4, 2, 2, 4, 4, true>(a, plan, part, s) : launch_tile<BF, GATED, 16, 2, 4, 2, 2, 4, 4, false>(a, plan, part, s);  // 64 x 128
-    case 7: return a.rows <= 64 ? launch_tile<BF, GATED, 16, 2, 2, 2, 2, 5, 5, true>(a, plan, part, s) : launch_tile<BF, GATED, 16, 2, 2, 2, 2, 5, 5, false>(a, plan, part, s);  // 64 x 64, two a unit
-    default: return launch_tile<BF, GATED, 16, 2, 2, 2, 1, 6, 6, true>(a, plan, part, s);  // 64 x 32, two a unit
+    case 0: return launch_tile<BF, GATED, 2, 4, 8, 4, 3, 2, false>(a, plan, part, s);  // 256 x 256
+    case 1: return launch_tile<BF, GATED, 4, 2, 4, 6, 3, 2, false>(a, plan, part, s);  // 256 x 192
+    case 2: return launch_tile<BF, GATED, 4, 2, 4, 4, 3, 2, false>(a, plan, part, s);  // 256 x 128
+    case 3: return launch_tile<BF, GATED, 2, 4, 4, 3, 3, 2, false>(a, plan, part, s);  // 128 x 192
+    case 4:  // 128 x 128
+      return a.rows <= 128 ? launch_tile<BF, GATED, 4, 2, 2, 4, 4, 4, true>(a, plan, part, s)
+                           : launch_tile<BF, GATED, 4, 2, 2, 4, 4, 4, false>(a, plan, part, s);
+    case 5: return launch_tile<BF, GATED, 2, 2, 4, 4, 3, 2, false>(a, plan, part, s);  // 128 x 128, two a unit
+    case 6:  // 64 x 128
+      return a.rows <= 128 ? launch_tile<BF, GATED, 2, 4, 2, 2, 4, 4, true>(a, plan, part, s)
+                           : launch_tile<BF, GATED, 2, 4, 2, 2, 4, 4, false>(a, plan, part, s);
+    case 7:  // 64 x 64, two a unit
+      return a.rows <= 64 ? launch_tile<BF, GATED, 2, 2, 2, 2, 5, 5, true>(a, plan, part, s)
+                          : launch_tile<BF, GATED, 2, 2, 2, 2, 5, 5, false>(a, plan, part, s);
+    default: return launch_tile<BF, GATED, 2, 2, 2, 1, 6, 6, true>(a, plan, part, s);  // 64 x 32, two a unit
   }
 }
 
