@@ -122,7 +122,10 @@ __device__ __forceinline__ void stream_join(float4_t* buf, int wave, int KW, flo
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int t = 0; t < TT; ++t) buf[(wave * TT + t) * 64 + lane] = acc[t];
-  __syncthreads();
+  // (no __syncthreads, which waits for the loads ahead as well)
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
   if ((wave & (KW - 1)) != 0) return;
   for (int w = 1; w < KW; ++w)
 #pragma unroll
