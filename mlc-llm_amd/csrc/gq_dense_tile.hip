@@ -42,26 +42,34 @@ hipError_t launch_dense_join(const DenseArgs& a, int splits, hipStream_t s) {
 
 namespace {
 
-// A form's tile, the workgroups of it that a unit holds (one or two), and what a block of K of its tiles takes in ns: alone_ns where few run,
-// one_ns where a unit has one each, full_ns where the units are full (L2 and clocks are shared).  Fitted to 14000 timings of 242 shapes, 17 to 4096
-// rows, all forms, 1 to 16 shares: the choice takes 0.7 % longer than the best one on average, 13 % at most.
+// A form's tile, the workgroups of it that a unit holds (one or two), what a block of K of its tiles takes in ns: alone_ns where few run, one_ns where
+// a unit has one each, full_ns where the units are full (L2 and clocks are shared), and what a byte of W takes from memory, with loads of lines that
+// are read once for up to once_rows rows of x (6.8 TB/s where all the others get 4.8).  Fitted to 21000 timings of 376 shapes, 9 to 4096 rows, all
+// forms, 1 to 16 shares: the choice takes 1.5 % longer than the best one on average, 20 % at most.
 struct Form {
   int bn, bm, a_unit;
   float alone_ns, one_ns, full_ns;
+  int once_rows;
+  float once_ns;
 };
 constexpr int kForms = 9;
-constexpr Form kForm[kForms] = {{256, 256, 1, 989.f, 1470.f, 1470.f}, {256, 192, 1, 869.f, 1209.f, 1209.f}, {256, 128, 1, 741.f, 890.f, 890.f},
-                                {128, 192, 1, 561.f, 852.f, 852.f},   {128, 128, 1, 514.f, 570.f, 570.f},   {128, 128, 2, 477.f, 680.f, 890.f},
-                                {64, 128, 1, 220.f, 378.f, 378.f},    {64, 64, 2, 219.f, 221.f, 564.f},     {64, 32, 2, 172.f, 227.f, 563.f}};
-// a round's ends, the launch that joins, a number of a share, a byte of W from memory, a second launch for the rest of the last round
-constexpr float kRoundNs = 977.f, kJoinNs = 2626.f, kShareNs = 1.67e-3f, kByteNs = 1.27e-4f, kRestNs = 1500.f;
+constexpr Form kForm[kForms] = {{256, 256, 1, 933.f, 1493.f, 1493.f, 0, 0.f},         {256, 192, 1, 1015.f, 1299.f, 1299.f, 0, 0.f},
+                                {256, 128, 1, 857.f, 884.f, 884.f, 0, 0.f},           {128, 192, 1, 674.f, 859.f, 859.f, 0, 0.f},
+                                {128, 128, 1, 664.f, 561.f, 561.f, 128, 1.56e-4f},    {128, 128, 2, 498.f, 909.f, 915.f, 0, 0.f},
+                                {64, 128, 1, 249.f, 368.f, 368.f, 128, 1.75e-4f},     {64, 64, 2, 217.f, 218.f, 658.f, 64, 1.48e-4f},
+                                {64, 32, 2, 158.f, 217.f, 561.f, 32, 1.48e-4f}};
+// a round's ends, the launch that joins, a number of a share, a byte of W from memory and how much more it takes with no unit busy, a second launch
+// for the rest of the last round
+constexpr float kRoundNs = 3382.f, kJoinNs = 2530.f, kShareNs = 1.66e-3f, kByteNs = 2.1e-4f, kIdle = 0.17f, kRestNs = 1500.f;
 constexpr int64_t kUnits = 256;
-float ns_of(const Form& f, int64_t tiles, int64_t blocks) {
+// tiles, of `blocks` blocks each, that read w_bytes of W
+float ns_of(const Form& f, int64_t rows, int64_t tiles, int64_t blocks, int64_t w_bytes) {
   const int64_t at_a_time = kUnits * f.a_unit, full = tiles / at_a_time, rest = tiles - full * at_a_time;
   float ns = full * (blocks * f.full_ns + kRoundNs);
   if (rest > kUnits) ns += blocks * f.full_ns + kRoundNs;
   else if (rest > 0) ns += blocks * (f.alone_ns + (f.one_ns - f.alone_ns) * rest / kUnits) + kRoundNs;
-  return ns;
+  const float from_memory = w_bytes * (rows <= f.once_rows ? f.once_ns : kByteNs) * (full > 0 ? 1.f : 1.f + kIdle * (at_a_time - tiles) / at_a_time);
+  return ns > from_memory ? ns : from_memory;
 }
 bool may_take(int form) { return options().gemm_variant < 0 || options().gemm_variant >= kForms || options().gemm_variant == form; }
 // N: rows of W
@@ -74,8 +82,7 @@ DensePlan plan_of(int64_t rows, int64_t N, int64_t K, bool only_whole = false) {
     for (int64_t want = 1; want <= 16 && want <= (only_whole || blocks < 4 ? 1 : blocks / 4); ++want) {
       if (options().gemm_split_k > 0 && options().gemm_split_k != want) continue;
       const int64_t per = (blocks + want - 1) / want, splits = (blocks + per - 1) / per;
-      const float whole_ns = ns_of(kForm[f], tiles * splits, per), from_memory = N * K * 2 * kByteNs;
-      const float ns = (whole_ns > from_memory ? whole_ns : from_memory) + (splits > 1 ? kJoinNs + splits * rows * N * kShareNs : 0.f);
+      const float ns = ns_of(kForm[f], rows, tiles * splits, per, N * K * 2) + (splits > 1 ? kJoinNs + splits * rows * N * kShareNs : 0.f);
       if (best.per_split == 0 || ns < best.ns) {
         best = DensePlan{};
         best.form = f;
@@ -88,7 +95,7 @@ DensePlan plan_of(int64_t rows, int64_t N, int64_t K, bool only_whole = false) {
     const int64_t at_a_time = kUnits * kForm[f].a_unit, whole = tiles / at_a_time * at_a_time / m_tiles;
     if (!only_whole && options().gemm_split_k <= 1 && whole > 0 && whole < n_tiles) {
       const DensePlan rest = plan_of(rows, N - whole * kForm[f].bn, K, true);
-      const float ns = ns_of(kForm[f], whole * m_tiles, blocks) + rest.ns + kRestNs;
+      const float ns = ns_of(kForm[f], rows, whole * m_tiles, blocks, whole * kForm[f].bn * K * 2) + rest.ns + kRestNs;
       if (ns < best.ns) {
         best = DensePlan{};
         best.form = f;
