@@ -61,6 +61,17 @@ inline int moe_shares(int64_t T, int64_t hidden, int64_t inter, int64_t experts,
   return s;
 }
 
+// blocks of K of the first product a wave where all waves of a workgroup share them
+inline int moe_blocks(int64_t hidden) { return static_cast<int>((hidden + kWaves * kStreamBlock - 1) / (kWaves * kStreamBlock)); }
+// Whether the first kernel keeps x in registers, in segments of 32 rows, rather than load it beside W, in segments of 8 or 16.  It does where that
+// fits (4 blocks a wave, or 7 and 8) and a segment is long enough for the wait that each change of x is.  The first kernel's us, with W / kept:
+// 8 experts of 4096 x 14336, 2 a token, 4 tokens 204 / 204, 8 tokens 298 / 284, 32 348 / 328, 48 373 / 327, 64 553 / 323; 64 of 64 experts of 2048 x
+// 1408, 6 a token, 156 / 150; 128 experts of 2048 x 768, 8 a token, 16 tokens 99 / 108, 64 tokens 141 / 147.
+inline bool moe_keeps(const DenseMoeArgs& a) {
+  const int blocks = moe_blocks(a.hidden);
+  return (blocks == 4 || blocks == 7 || blocks == 8) && a.T * a.k >= 2 * a.experts && a.inter >= 1024;
+}
+
 struct MoeTables {  // in LDS, in front of the rest
   uint64_t* mask;      // [experts] tokens of each
   MoeSegment* segs;    // [T k at most]
@@ -77,11 +88,12 @@ inline size_t moe_tables_bytes(int experts, int slots) {
 
 }  // namespace
 
-// NC: experts a lane in the routing.  XG: eights of rows of a segment.
-template <bool BF, int NC, int XG, int D>
+// NC: experts a lane in the routing.  XG: eights of rows of a segment.  NB: blocks of K a wave whose x it keeps in registers; 0: x comes with every
+// item.  down_rows: rows of a segment of the second kernel, 8 XG where NB is 0.
+template <bool BF, int NC, int XG, int D, int NB>
 __global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(
     const void* __restrict__ logits, int T, int E, int top_k, int logits_dtype, int logits_vec, int tables_bytes, int group_inv, int kw_log2, int nb,
-    DenseMoeArgs a, MoeLayout layout) {
+    int down_rows, DenseMoeArgs a, MoeLayout layout) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   constexpr int TT = (XG + 1) / 2, kSegRows = 8 * XG;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -120,29 +132,31 @@ __global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(
     __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
-  // Rows and segments in front of each expert: two sums in one number.
+  // Rows and segments in front of each expert: the sums in one number.
   const uint64_t mine = tid < E ? tab.mask[tid] : 0;
   const int n_rows = __popcll(mine), n_segs = (n_rows + kSegRows - 1) / kSegRows;
-  const uint32_t own = static_cast<uint32_t>(n_rows) | static_cast<uint32_t>(n_segs) << 16;
-  uint32_t upto = own;
+  typedef std::conditional_t<(NB > 0), uint64_t, uint32_t> Sums;  // the second kernel's segments are others where x is kept: a third sum
+  const Sums own = static_cast<Sums>(n_rows) | static_cast<Sums>(n_segs) << 16 |
+                   (NB > 0 ? static_cast<uint64_t>((n_rows + down_rows - 1) / down_rows) << 32 : 0);
+  Sums upto = own;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const uint32_t other = __shfl_up(upto, d);
+    const Sums other = __shfl_up(upto, d);
     if (lane >= d) upto += other;
   }
   if (lane == 63) tab.totals[wave] = upto;
   __syncthreads();
-  uint32_t before = upto - own, all = 0;
+  Sums before = upto - own, all = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    const uint32_t v = static_cast<uint32_t>(tab.totals[w]);
+    const Sums v = static_cast<Sums>(tab.totals[w]);
     if (w < wave) before += v;
     all += v;
   }
-  const int row0 = before & 0xffff, segs_all = __builtin_amdgcn_readfirstlane(all >> 16);
+  const int row0 = before & 0xffff, segs_all = __builtin_amdgcn_readfirstlane(static_cast<int>(all >> 16 & 0xffff));
   for (int s = 0; s < n_segs; ++s) {
     const int left = n_rows - kSegRows * s;
-    tab.segs[(before >> 16) + s] = MoeSegment{tid, row0 + kSegRows * s, left < kSegRows ? left : kSegRows};
+    tab.segs[(before >> 16 & 0xffff) + s] = MoeSegment{tid, row0 + kSegRows * s, left < kSegRows ? left : kSegRows};
   }
   if (tid < E) tab.expert_row[tid] = row0;
   __syncthreads();
@@ -156,16 +170,27 @@ __global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(
   __syncthreads();
   char* const ws = static_cast<char*>(a.workspace);
   if (blockIdx.x == 0) {
-    for (int i = tid; i < segs_all; i += kThreads) reinterpret_cast<MoeSegment*>(ws + kSegsAt)[i] = tab.segs[i];
+    MoeSegment* const segs = reinterpret_cast<MoeSegment*>(ws + kSegsAt);
+    if constexpr (NB > 0) {
+      for (int s = 0; s * down_rows < n_rows; ++s) {
+        const int left = n_rows - s * down_rows;
+        segs[(before >> 32) + s] = MoeSegment{tid, row0 + s * down_rows, left < down_rows ? left : down_rows};
+      }
+    } else {
+      for (int i = tid; i < segs_all; i += kThreads) segs[i] = tab.segs[i];
+    }
     for (int i = tid; i < slots; i += kThreads) reinterpret_cast<int*>(ws + layout.row_token)[i] = tab.row_token[i];
     for (int i = tid; i < (K + 15) / 16; i += kThreads) reinterpret_cast<int*>(ws + layout.tickets)[i] = 0;
-    if (tid == 0) *reinterpret_cast<int*>(ws) = segs_all;
+    if (tid == 0) *reinterpret_cast<int*>(ws) = NB > 0 ? static_cast<int>(static_cast<uint64_t>(all) >> 32) : segs_all;
   }
 
   // ---- the product: items of 8 gate rows and their up rows of one segment ----
-  const int KW = 1 << kw_log2, kw = wave & (KW - 1), nw = wave >> kw_log2, stride = gridDim.x * (kWaves >> kw_log2);
-  const int n_tiles = (I + 7) / 8, items = segs_all * n_tiles, first = blockIdx.x * (kWaves >> kw_log2) + nw;
-  const int rounds = (items + stride - 1) / stride;
+  const int n_tiles = (I + 7) / 8, items = segs_all * n_tiles;
+  // all waves share an item and a workgroup has a run of items, or KW share one and they go around
+  const int KW = NB > 0 ? kWaves : 1 << kw_log2, kw = wave & (KW - 1), nw = NB > 0 ? 0 : wave >> kw_log2;
+  const int stride = NB > 0 ? 1 : gridDim.x * (kWaves >> kw_log2);
+  const int first = NB > 0 ? static_cast<int>(static_cast<int64_t>(items) * blockIdx.x / gridDim.x) : blockIdx.x * (kWaves >> kw_log2) + nw;
+  const int rounds = NB > 0 ? static_cast<int>(static_cast<int64_t>(items) * (blockIdx.x + 1) / gridDim.x) - first : (items + stride - 1) / stride;
   const int64_t pitch = static_cast<int64_t>(K) * 2;
   struct Item {
     int e, n0, row0, rows;
@@ -202,7 +227,7 @@ __global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(
   };
   auto done = [&](int round, float4_t (&acc)[TT]) {
     if (KW > 1) {  // (two buffers in turn: one barrier a round)
-      stream_join(reinterpret_cast<float4_t*>(rest + kWaves * stream_ring<XG, 1, D>()) + (round & 1) * kWaves * TT * 64, wave, KW, acc);
+      stream_join(reinterpret_cast<float4_t*>(rest + kWaves * (NB > 0 ? D * kKeptStage : stream_ring<XG, 1, D>())) + (round & 1) * kWaves * TT * 64, wave, KW, acc);
       if (kw != 0) return;
     }
     const Item it = item_of(round);
@@ -232,7 +257,33 @@ __global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(
     }
   };
   __syncthreads();  // (the routing's part of LDS is the rings' now)
-  dense_stream<BF, XG, D>(rest + wave * stream_ring<XG, 1, D>(), static_cast<uint32_t>(pitch), KW * kStreamBlock, nb, rounds, place_of, done);
+  if constexpr (NB == 0) {
+    dense_stream<BF, XG, D>(rest + wave * stream_ring<XG, 1, D>(), static_cast<uint32_t>(pitch), KW * kStreamBlock, nb, rounds, place_of, done);
+  } else {
+    auto rows_of = [&](int round) {
+      const Item it = item_of(round);
+      StreamRows p;
+      p.end = it.there ? K : 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        p.w[i] = dense_buffer(reinterpret_cast<const char*>(a.w13) + ((static_cast<int64_t>(it.e) * 2 + i) * I + it.n0) * pitch, 8 * pitch);
+      return p;
+    };
+    int kept = -1;  // first row of the segment
+    auto keep = [&](int round, StreamKept<NB, TT>& of) {
+      const Item it = item_of(round);
+      if (it.row0 == kept) return;
+      kept = it.row0;
+      uint32_t at[TT];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const int c = 16 * t + (lane & 15);
+        at[t] = c < it.rows ? static_cast<uint32_t>(tab.row_token[it.row0 + c]) * static_cast<uint32_t>(pitch) : kNowhere;
+      }
+      kept_x(of, x, at, wave * kStreamBlock, kWaves * kStreamBlock, K);
+    };
+    dense_stream_kept<BF, TT, NB, D>(rest + wave * D * kKeptStage, static_cast<uint32_t>(pitch), wave * kStreamBlock, kWaves * kStreamBlock, rounds, rows_of, keep, done);
+  }
 }
 
 template <bool BF>
@@ -374,23 +425,23 @@ static hipError_t may_use(Kernel* kern, size_t lds) {
   return lds > 65536 ? allow_large_lds(reinterpret_cast<const void*>(kern)) : hipSuccess;
 }
 
-template <bool BF, int NC, int XG, int D>
-static hipError_t launch_up(const DenseMoeArgs& a, const MoeLayout& layout, hipStream_t s) {
+template <bool BF, int NC, int XG, int D, int NB>
+static hipError_t launch_up(const DenseMoeArgs& a, const MoeLayout& layout, int down_rows, hipStream_t s) {
   const int slots = a.T * a.k, n_tiles = a.inter / 8;
   const StreamPlan plan = stream_plan(experts_chosen(a.T, a.experts, a.k) * n_tiles, a.hidden, D);
   const int64_t most = static_cast<int64_t>(slots < a.experts ? slots : a.experts + slots / (8 * XG)) * n_tiles;  // items
   const int nw = kWaves >> plan.kw_log2;
   const int64_t sets = (most + nw - 1) / nw;
   const size_t tables = moe_tables_bytes(a.experts, slots), gate = kWaves * sizeof(GateScratch<NC>);
-  const size_t rings = kWaves * (stream_ring<XG, 1, D>() + 2 * ((XG + 1) / 2) * 1024), lds = tables + (rings > gate ? rings : gate);
+  const size_t rings = kWaves * ((NB > 0 ? D * kKeptStage : stream_ring<XG, 1, D>()) + 2 * ((XG + 1) / 2) * 1024), lds = tables + (rings > gate ? rings : gate);
   if (lds > 160 * 1024) return hipErrorNotSupported;
-  auto* kern = dense_moe_up_kernel<BF, NC, XG, D>;
+  auto* kern = dense_moe_up_kernel<BF, NC, XG, D, NB>;
   const hipError_t e = may_use(kern, lds);
   if (e != hipSuccess) return e;
   const int vec = a.experts % 8 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0;
-  const int64_t at_a_time = kStreamUnits * (lds > 80 * 1024 ? 1 : 2);
+  const int64_t at_a_time = kStreamUnits * (lds > 80 * 1024 || NB > 0 ? 1 : 2);
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(sets < at_a_time ? sets : at_a_time)), dim3(kThreads), lds, s, a.logits, a.T, a.experts,
-                     a.k, a.logits_dtype, vec, static_cast<int>(tables), gate_group_inv(a.experts, a.groups), plan.kw_log2, plan.nb, a, layout);
+                     a.k, a.logits_dtype, vec, static_cast<int>(tables), gate_group_inv(a.experts, a.groups), plan.kw_log2, plan.nb, down_rows, a, layout);
   return hipGetLastError();
 }
 
@@ -398,7 +449,7 @@ template <bool BF, int XG, int D>
 static hipError_t launch_down(const DenseMoeArgs& a, const MoeLayout& layout, hipStream_t s) {
   const int shares = moe_shares(a.T, a.hidden, a.inter, a.experts, a.k);
   const dim3 grid(static_cast<unsigned>((a.hidden + 15) / 16), static_cast<unsigned>(shares));
-  note_kernel("dense_moe up to %d rows, %d shares", 8 * XG, shares);
+  note_kernel("dense_moe up to %d rows, %d shares%s", 8 * XG, shares, moe_keeps(a) ? ", x kept" : "");
   const size_t lds = kWaves * (stream_ring<XG, 2, D>() + a.T * 64) + static_cast<size_t>(a.T) * a.k * (4 + sizeof(MoeSegment));
   if (lds > 160 * 1024) return hipErrorNotSupported;
   auto* kern = dense_moe_down_kernel<BF, XG, D>;
@@ -412,15 +463,22 @@ static hipError_t launch_down(const DenseMoeArgs& a, const MoeLayout& layout, hi
 template <bool BF, int XG>
 static hipError_t launch(const DenseMoeArgs& a, hipStream_t s) {
   const MoeLayout layout = moe_layout(a.T, a.hidden, a.inter, a.experts, a.k);
-  auto up = [&](auto d) {
-    constexpr int D = decltype(d)::value;
-    return a.experts <= 64    ? launch_up<BF, 2, XG, D>(a, layout, s)
-           : a.experts <= 128 ? launch_up<BF, 4, XG, D>(a, layout, s)
-           : a.experts <= 256 ? launch_up<BF, 8, XG, D>(a, layout, s)
-                              : launch_up<BF, 16, XG, D>(a, layout, s);
+  auto up = [&](auto xg, auto d, auto nb) {
+    constexpr int U = decltype(xg)::value, D = decltype(d)::value, NB = decltype(nb)::value;
+    return a.experts <= 64    ? launch_up<BF, 2, U, D, NB>(a, layout, 8 * XG, s)
+           : a.experts <= 128 ? launch_up<BF, 4, U, D, NB>(a, layout, 8 * XG, s)
+           : a.experts <= 256 ? launch_up<BF, 8, U, D, NB>(a, layout, 8 * XG, s)
+                              : launch_up<BF, 16, U, D, NB>(a, layout, 8 * XG, s);
   };
-  hipError_t e = up(std::integral_constant<int, 4>{});
-  if (e == hipErrorNotSupported) e = up(std::integral_constant<int, 2>{});  // (many slots: their tables take the room)
+  const std::integral_constant<int, 0> none{};
+  const std::integral_constant<int, 2> two{};
+  const std::integral_constant<int, 4> four{};
+  const std::integral_constant<int, 8> eight{};
+  const std::integral_constant<int, XG> rows{};
+  hipError_t e = hipErrorNotSupported;
+  if (moe_keeps(a)) e = moe_blocks(a.hidden) == 4 ? up(four, four, four) : up(four, four, eight);
+  if (e == hipErrorNotSupported) e = up(rows, four, none);
+  if (e == hipErrorNotSupported) e = up(rows, two, none);  // (many slots: their tables take the room)
   // (two workgroups a unit with two blocks ahead: one with four was 1 to 10 % behind, 16 tokens of 128 experts 133 / 137 us in all)
   return e != hipSuccess ? e : launch_down<BF, XG, 2>(a, layout, s);
 }

@@ -116,6 +116,83 @@ __device__ __forceinline__ void dense_stream(uint8_t* ring, uint32_t w_pitch, in
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (loads of nothing may still land in the ring)
 }
 
+// The same with this wave's part of x in registers, loaded where the item's rows of x change: NB blocks of an item, those of K that the wave takes.
+// x of a segment comes once a workgroup and not with every item, and the ring holds weights alone.
+template <int NB, int TT>
+struct StreamKept {
+  int4_t v[NB][2][TT];
+};
+struct StreamRows {
+  rsrc_t w[2];
+  int end;  // K, or 0: nothing to do
+};
+constexpr int kKeptStage = 2048;
+// at[t]: byte offset of row 16 t + lane % 16 of x; k: this wave's first number of K, its blocks `step` apart.
+template <int NB, int TT>
+__device__ __forceinline__ void kept_x(StreamKept<NB, TT>& to, rsrc_t x, const uint32_t (&at)[TT], int k, int step, int K) {
+  const int kc = k + 8 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const int at_k = kc + j * step + 32 * i;
+        to.v[j][i][t] = __builtin_bit_cast(int4_t, __builtin_amdgcn_raw_buffer_load_b128(x, at_k < K ? at[t] + 2u * at_k : kNowhere, 0, 0));
+      }
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) asm volatile("" : "+v"(to.v[j][i][t]));  // (waited for here, not behind the loads of weights that follow)
+}
+__device__ __forceinline__ void kept_load(const StreamRows& p, int k, uint32_t w_pitch, uint8_t* stage) {
+  const int lane = threadIdx.x & 63, kc = k + 8 * ((lane & 7) ^ (lane >> 3));
+  const uint32_t at = kc < p.end ? static_cast<uint32_t>(lane >> 3) * w_pitch + 2u * kc : kNowhere;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) dense_to_lds<true>(p.w[i], at, stage + 1024 * i);
+}
+// keep(round, kept) brings x where it changes, rows_of(round) gives the rows of W.  k: this wave's first number of K.
+template <bool BF, int TT, int NB, int D, class RowsOf, class Keep, class Done>
+__device__ __forceinline__ void dense_stream_kept(uint8_t* ring, uint32_t w_pitch, int k, int step, int rounds, RowsOf rows_of, Keep keep, Done done) {
+  static_assert(D % NB == 0 || NB % D == 0, "whole items or whole parts of one");
+  constexpr int kAhead = D >= NB ? D / NB : 1;
+  const int lane = threadIdx.x & 63, quad = lane >> 4, row = lane & 15;
+  const int c0 = (quad ^ (row & 7)) << 4, c1 = ((quad + 4) ^ (row & 7)) << 4;
+  StreamRows here = rows_of(0), next = here;
+#pragma unroll
+  for (int s = 0; s < D; ++s) {
+    if (s > 0 && s % NB == 0) next = rows_of(s / NB);
+    kept_load(s < NB ? here : next, k + s % NB * step, w_pitch, ring + s * kKeptStage);
+  }
+  StreamKept<NB, TT> x;
+  for (int round = 0; round < rounds; ++round) {
+    keep(round, x);
+    float4_t acc[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[t] = float4_t{};
+    next = rows_of(round + kAhead);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      uint8_t* const stage = ring + (D > NB ? (round % kAhead) * NB + j : j % D) * kKeptStage;
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (D - 1)) : "memory");
+      const int4_t w0 = *reinterpret_cast<const int4_t*>(stage + row * 128 + c0), w1 = *reinterpret_cast<const int4_t*>(stage + row * 128 + c1);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        acc[t] = dense_mfma<BF>(w0, x.v[j][0][t], acc[t]);
+        acc[t] = dense_mfma<BF>(w1, x.v[j][1][t], acc[t]);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read, before the stage is loaded again)
+      const bool same = j + D < NB;
+      kept_load(same ? here : next, k + (j + D) % NB * step, w_pitch, stage);
+    }
+    here = next;
+    done(round, acc);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
 // The sums of the KW waves that share an item, in the first one's acc; buf: kStreamWaves TT KiB, no use of it may be left.
 template <int TT>
 __device__ __forceinline__ void stream_join(float4_t* buf, int wave, int KW, float4_t (&acc)[TT]) {

@@ -391,6 +391,32 @@ def test_moe_skewed_routing(t):
     close(ops.dense_moe(x, logits, w13, w2, 4), moe_ref(x, weights, ids, w13, w2, "silu", torch.bfloat16))
 
 
+# x in registers: four, seven and eight blocks of K a wave, K that ends inside a block; segments of 32 rows in the first kernel, of 8 or 16 in the second
+KEPT = [(64, 2048, 1024, 4, 2), (33, 1544, 1032, 3, 1), (40, 4096, 1024, 2, 2), (8, 3592, 1024, 4, 2), (64, 2000, 1096, 8, 8), (7, 3584, 1032, 1, 1), (64, 1600, 1024, 60, 3)]
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t,hidden,inter,experts,k", KEPT)
+def test_moe_x_in_registers(t, hidden, inter, experts, k, dtype):
+    g = _gen(t + hidden + inter)
+    x, logits, w13, w2 = _layer(g, dtype, t, hidden, inter, experts)
+    for skewed in (False, True):
+        if skewed:  # all tokens to the same experts, the last among them
+            logits[:, -k:] += 20.0
+        weights, ids = ops.moe_gating(logits, k)
+        got = ops.dense_moe(x, logits, w13, w2, k)
+        assert gq._lib.last_kernel().endswith("x kept")
+        close(got, moe_ref(x, weights, ids, w13, w2, "silu", dtype))
+        assert torch.equal(got, ops.dense_moe(x, logits, w13, w2, k))
+    if experts > k:  # what others chose, or nobody, stays away from a token
+        logits[:, 0], logits[0, 0] = -50.0, 60.0
+        weights, ids = ops.moe_gating(logits, k)
+        want = ops.dense_moe(x, logits, w13, w2, k)
+        w13[0, 0] = math.inf
+        got = ops.dense_moe(x, logits, w13, w2, k)
+        assert not got[0].isfinite().all() and torch.equal(got[1:], want[1:])
+
+
 @pytest.mark.parametrize("t", [2, 40])
 def test_moe_troubles_stay_where_they_are(t):
     """Experts that nobody chose, and those that others chose, may hold anything; a token's NaN is its own."""
