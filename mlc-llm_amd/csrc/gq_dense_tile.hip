@@ -44,23 +44,25 @@ namespace {
 
 // A form's tile, the workgroups of it that a unit holds (one or two), what a block of K of its tiles takes in ns: alone_ns where few run, one_ns where
 // a unit has one each, full_ns where the units are full (L2 and clocks are shared), and what a byte of W takes from memory, with loads of lines that
-// are read once for up to once_rows rows of x (6.8 TB/s where all the others get 4.8).  Fitted to 21000 timings of 376 shapes, 9 to 4096 rows, all
-// forms, 1 to 16 shares: the choice takes 1.5 % longer than the best one on average, 20 % at most.
+// are read once for up to once_rows rows of x (6.8 TB/s where all the others get 4.8).  Fitted to 20000 timings of 420 shapes, 9 to 4096 rows, all
+// forms, 1 to 16 shares: the choice takes 1.4 % longer than the best one on average, 21 % at most.  (160 rows of x: 1.5 % on average over 130 to 2048
+// rows, 10 % at 160, 320 and 800 of them.)
 struct Form {
   int bn, bm, a_unit;
   float alone_ns, one_ns, full_ns;
   int once_rows;
   float once_ns;
 };
-constexpr int kForms = 9;
-constexpr Form kForm[kForms] = {{256, 256, 1, 933.f, 1493.f, 1493.f, 0, 0.f},         {256, 192, 1, 1015.f, 1299.f, 1299.f, 0, 0.f},
-                                {256, 128, 1, 857.f, 884.f, 884.f, 0, 0.f},           {128, 192, 1, 674.f, 859.f, 859.f, 0, 0.f},
-                                {128, 128, 1, 664.f, 561.f, 561.f, 128, 1.56e-4f},    {128, 128, 2, 498.f, 909.f, 915.f, 0, 0.f},
-                                {64, 128, 1, 249.f, 368.f, 368.f, 128, 1.75e-4f},     {64, 64, 2, 217.f, 218.f, 658.f, 64, 1.48e-4f},
-                                {64, 32, 2, 158.f, 217.f, 561.f, 32, 1.48e-4f}};
+constexpr int kForms = 11;
+constexpr Form kForm[kForms] = {{256, 256, 1, 813.f, 1479.f, 1479.f, 0, 0.f},      {256, 192, 1, 794.f, 1298.f, 1298.f, 0, 0.f},
+                                {256, 128, 1, 645.f, 920.f, 920.f, 0, 0.f},        {128, 192, 1, 642.f, 753.f, 753.f, 0, 0.f},
+                                {128, 128, 1, 453.f, 561.f, 561.f, 128, 1.56e-4f}, {128, 128, 2, 530.f, 601.f, 925.f, 0, 0.f},
+                                {64, 128, 1, 275.f, 326.f, 326.f, 128, 1.75e-4f},  {64, 64, 2, 205.f, 218.f, 654.f, 64, 1.48e-4f},
+                                {64, 32, 2, 142.f, 216.f, 546.f, 32, 1.48e-4f},    {128, 160, 1, 569.f, 643.f, 643.f, 0, 0.f},
+                                {256, 160, 1, 784.f, 1079.f, 1079.f, 0, 0.f}};
 // a round's ends, the launch that joins, a number of a share, a byte of W from memory and how much more it takes with no unit busy, a second launch
 // for the rest of the last round
-constexpr float kRoundNs = 3382.f, kJoinNs = 2530.f, kShareNs = 1.66e-3f, kByteNs = 2.1e-4f, kIdle = 0.17f, kRestNs = 1500.f;
+constexpr float kRoundNs = 3325.f, kJoinNs = 2216.f, kShareNs = 1.94e-3f, kByteNs = 2.1e-4f, kIdle = 0.17f, kRestNs = 1500.f;
 constexpr int64_t kUnits = 256;
 // tiles, of `blocks` blocks each, that read w_bytes of W
 float ns_of(const Form& f, int64_t rows, int64_t tiles, int64_t blocks, int64_t w_bytes) {
@@ -77,7 +79,7 @@ DensePlan plan_of(int64_t rows, int64_t N, int64_t K, bool only_whole = false) {
   const int64_t blocks = (K + kBlock - 1) / kBlock;
   DensePlan best;
   for (int f = 0; f < kForms; ++f) {
-    if (!may_take(f) || (f == kForms - 1 && rows > 32 && options().gemm_variant != f)) continue;
+    if (!may_take(f) || (kForm[f].bm == 32 && rows > 32 && options().gemm_variant != f)) continue;
     const int64_t m_tiles = (rows + kForm[f].bm - 1) / kForm[f].bm, n_tiles = (N + kForm[f].bn - 1) / kForm[f].bn, tiles = m_tiles * n_tiles;
     for (int64_t want = 1; want <= 16 && want <= (only_whole || blocks < 4 ? 1 : blocks / 4); ++want) {
       if (options().gemm_split_k > 0 && options().gemm_split_k != want) continue;

@@ -12,7 +12,8 @@ namespace gq {
 namespace {
 
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
-constexpr int kBlock = 64;  // numbers of K, 128 bytes of a row
+constexpr int kBlock = 64;                  // numbers of K, 128 bytes of a row
+constexpr uint32_t kNowhere = 0xfffffff0u;  // past the end of any buffer here, or inside of it
 
 template <bool ONCE>
 __device__ __forceinline__ void load_to_lds(rsrc_t rsrc, uint32_t off, uint8_t* lds) {
@@ -89,6 +90,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void dense_tile_kernel(DenseArgs p
   for (int i = 0; i < kXLoads; ++i) {
     const int r = (i * kWaves + wave) * 8 + (lane >> 3);
     x_off[i] = static_cast<uint32_t>(r < rows ? r : rows - 1) * pitch + my_chunk;
+    if (BM % (8 * kWaves) != 0 && r >= BM) x_off[i] = kNowhere;  // (a load for the count of loads alone)
     asm volatile("" : "+v"(x_off[i]));
   }
   // Loads [from, to) of block g; past the last block, that one's again (nobody reads them).  No branches and no vector instructions
@@ -345,7 +347,9 @@ hipError_t launch_form(const DenseArgs& a, const DensePlan& plan, int part, hipS
     case 7:  // 64 x 64, two a unit
       return a.rows <= 64 ? launch_tile<BF, GATED, 2, 2, 2, 2, 5, 5, true>(a, plan, part, s)
                           : launch_tile<BF, GATED, 2, 2, 2, 2, 5, 5, false>(a, plan, part, s);
-    default: return launch_tile<BF, GATED, 2, 2, 2, 1, 6, 6, true>(a, plan, part, s);  // 64 x 32, two a unit
+    case 8: return launch_tile<BF, GATED, 2, 2, 2, 1, 6, 6, true>(a, plan, part, s);    // 64 x 32, two a unit
+    case 9: return launch_tile<BF, GATED, 4, 2, 2, 5, 4, 3, false>(a, plan, part, s);   // 128 x 160
+    default: return launch_tile<BF, GATED, 4, 2, 4, 5, 3, 2, false>(a, plan, part, s);  // 256 x 160
   }
 }
 

@@ -15,7 +15,7 @@
  *   "quad_pairs"          1, 2           weight quads per item of the quad-row kernel
  *   "gemm_variant"        0..15          GEMM tile (1: GEMM only, 2: GEMV up to 8 rows, others pick a tile)
  *   "gemm_split_k"        1..4096        split of K in the few-row GEMM
- *                                        (16-bit weights: gemm_variant 0..8 a tile form, above any of them, both without the kernel of few
+ *                                        (16-bit weights: gemm_variant 0..10 a tile form, above any of them, both without the kernel of few
  *                                        rows; gemm_split_k the shares of K, of an expert layer's second kernel up to 8)
  *   "gemm_fast_loop"      0              0 forces the GEMM's general K loop (zero-selects kept)
  * Returns 0, or MI355GQ_ERR_ARG for an unknown name or a value out of range.

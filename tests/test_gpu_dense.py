@@ -115,14 +115,14 @@ def test_gated(m, n, k, dtype):
 
 
 @pytest.mark.parametrize("shares", [1, 3])
-@pytest.mark.parametrize("form", range(9))
+@pytest.mark.parametrize("form", range(11))
 def test_tile_forms(form, shares):
     """Every tile form, whole and in shares of K, on tiles that end inside in all directions."""
     g = _gen(form * 10 + shares)
     gq._lib.set_option("gemm_variant", form)
     gq._lib.set_option("gemm_split_k", shares)
     try:
-        for i, (m, n, k) in enumerate([(17, 40, 776), (33, 257, 1032), (200, 520, 776), (300, 129, 968), (521, 392, 1288)]):
+        for i, (m, n, k) in enumerate([(17, 40, 776), (33, 257, 1032), (160, 130, 776), (200, 520, 776), (300, 129, 968), (521, 392, 1288)]):
             dtype = HALVES[i % 2]
             x, w, bias = _normal(g, dtype, m, k), _normal(g, dtype, n, k, scale=k**-0.5), _normal(g, dtype, n)
             r = _normal(g, dtype, m, n)
