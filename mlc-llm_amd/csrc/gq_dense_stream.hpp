@@ -218,9 +218,10 @@ __device__ __forceinline__ float4_t stream_up(float4_t v) {
 }
 
 // KW of a workgroup's eight waves share the K of an item.  More of them read longer runs of a row, fewer leave more blocks a wave between two
-// items: the KW of the fewest blocks that a wave takes one after the other, padding and the ends of up to six rounds (2.2 blocks each; 0.6 of a
-// single one) counted, a tenth more for a KW of four or two and three for one.  One row, by KW 8, 4, 2 and 1, us: 28672 x 4096 36.7, 42.9, 40.0, 41.1
-// (the rule: 8); 28672 x 2048 22.0, 22.4, 20.7, 24.5 (2); 11264 x 2048 11.3, 11.1, 10.4 (2); 5120 x 5120 13.2, 11.6 (4); 6144 x 4096 11.1, 11.9 (4).
+// items: the KW of the fewest blocks that a wave takes one after the other, padding and the ends of up to six rounds (0.65 of a block each) counted,
+// a twelfth more for a KW of four or two and a third for one.  One row, by KW 8, 4, 2 and 1, us: 28672 x 4096 38.4, 36.2, 45.4, 40.4 (the rule: 8);
+// 8192 x 8192 27.0, 29.7, 28.0, 52.2 (8); 6144 x 4096 11.1, 12.3, 15.3, 24.2 (8); 5120 x 5120, of whose 10 blocks a wave of eight has two empty
+// ones, 13.4, 12.1, 18.1, 30.7 (4); 152064 x 3584 162.6, 151.8, 153.4, 155.2 (2).
 struct StreamPlan {
   int kw_log2, nb, rounds;
 };
@@ -231,8 +232,8 @@ inline StreamPlan stream_plan(double items, int64_t K, int D) {
   for (int log2 = 3; log2 >= 0; --log2) {
     const int64_t each = (blocks + (1 << log2) - 1) >> log2, nb = (each + D - 1) / D * D;
     const double rounds = __builtin_ceil(items / ((kStreamWaves >> log2) * kStreamUnits));
-    const double ends = rounds > 6 ? 13.2 : rounds > 1 ? 2.2 * rounds : 0.6;
-    const double cost = (rounds * static_cast<double>(nb) + ends) * (log2 == 0 ? 1.3 : log2 < 3 ? 1.1 : 1.0);
+    const double ends = 0.65 * (rounds < 6 ? rounds : 6);
+    const double cost = (rounds * static_cast<double>(nb) + ends) * (log2 == 0 ? 1.3 : log2 < 3 ? 1.08 : 1.0);
     if (best.nb == 0 || cost < best_cost) {
       best_cost = cost;
       best = {log2, static_cast<int>(nb), static_cast<int>(rounds)};
