@@ -32,7 +32,7 @@ struct MoeLayout {
 inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 inline int moe_shares(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k);
 inline MoeLayout moe_layout(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k) {
-  const int64_t slots = T * k, tiles = (hidden + 15) / 16;
+  const int64_t slots = T * k, tiles = (hidden + 31) / 32 * 2;
   MoeLayout l;
   l.row_token = kSegsAt + up256(slots * static_cast<int64_t>(sizeof(MoeSegment)));
   l.tickets = l.row_token + up256(slots * 4);
@@ -48,13 +48,15 @@ inline double experts_chosen(int64_t T, int64_t experts, int64_t k) {
   for (int64_t t = 0; t < T; ++t) none *= 1 - static_cast<double>(k) / static_cast<double>(experts);
   return static_cast<double>(experts) * (1 - none);
 }
-// eights of rows of a segment: sixteen rows where experts have more than four on average
+// Eights of rows of a segment: sixteen rows where experts have more than four on average.  The second kernel then takes 32 columns a workgroup and not
+// 16, and x, which comes half as often, goes straight into registers: 8 experts of 4096 x 14336, 2 a token, 32 tokens 213 -> 200 us, 48 226 -> 213; 16
+// experts of 7168 x 2048, 4 a token, 32 tokens 110 -> 95; (16 tokens of 128 experts of 2048 x 768, 8 a token, would take 48 and take 46).
 inline int moe_eights(int64_t T, int64_t experts, int64_t k) { return T > 8 && T * k > 4 * experts ? 2 : 1; }
 // Workgroups that share the K (all chosen experts' inter) of sixteen columns in the second kernel: about one a unit (sixteen tokens
 // of 128 experts, 128 tiles: 131 us with two shares, 159 with one and 136 with four; 224 tiles: 212 with one, 219 with two).
 inline int moe_shares(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k) {
   if (options().gemm_split_k > 0) return options().gemm_split_k < 8 ? options().gemm_split_k : 8;
-  const int64_t tiles = (hidden + 15) / 16;
+  const int64_t tiles = moe_eights(T, experts, k) == 2 ? (hidden + 31) / 32 : (hidden + 15) / 16;
   const double blocks = experts_chosen(T, experts, k) * static_cast<double>((inter + kStreamBlock - 1) / kStreamBlock);
   int s = 1;
   while (s < 8 && tiles * s < 200 && blocks / (2 * s) >= 4 * kWaves) s *= 2;
@@ -70,6 +72,12 @@ inline int moe_blocks(int64_t hidden) { return static_cast<int>((hidden + kWaves
 inline bool moe_keeps(const DenseMoeArgs& a) {
   const int blocks = moe_blocks(a.hidden);
   return (blocks == 4 || blocks == 7 || blocks == 8) && a.T * a.k >= 2 * a.experts && a.inter >= 1024;
+}
+
+// Rows of a segment of the second kernel: 32 where the first one keeps x and experts have more than twelve on average (64 tokens, 2 of 8 experts of 4096
+// x 14336, 302 -> 232 us; 48 tokens would take 221 and take 213).
+inline int moe_down_rows(const DenseMoeArgs& a) {
+  return moe_keeps(a) && a.T * a.k > 12 * a.experts ? 32 : 8 * moe_eights(a.T, a.experts, a.k);
 }
 
 struct MoeTables {  // in LDS, in front of the rest
@@ -282,7 +290,8 @@ __global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(
       }
       kept_x(of, x, at, wave * kStreamBlock, kWaves * kStreamBlock, K);
     };
-    dense_stream_kept<BF, TT, NB, D>(rest + wave * D * kKeptStage, static_cast<uint32_t>(pitch), wave * kStreamBlock, kWaves * kStreamBlock, rounds, rows_of, keep, done);
+    dense_stream_kept<BF, TT, NB, D>(rest + wave * D * kKeptStage, static_cast<uint32_t>(pitch), wave * kStreamBlock, kWaves * kStreamBlock, rounds,
+                                     rows_of, keep, done);
   }
 }
 
@@ -291,27 +300,31 @@ __device__ __forceinline__ void moe_store(uint16_t* to, const float4_t& v) {
   *reinterpret_cast<uint2*>(to) = uint2{dense_pair<BF>(v[0], v[1]), dense_pair<BF>(v[2], v[3])};
 }
 
-// Sixteen columns of the output for all tokens a workgroup; gridDim.y workgroups share the K, which is all segments' inter.
-template <bool BF, int XG, int D>
-__global__ __launch_bounds__(kThreads, XG == 1 && D == 2 ? 4 : 2) void dense_moe_down_kernel(
+template <int XG, int C>
+constexpr int down_stage() { return C == 1 ? stream_stage<XG, 2>() : 2048 * C; }
+
+// 16 C columns of the output for all tokens a workgroup; gridDim.y workgroups share the K, which is all segments' inter.  x comes through LDS beside W,
+// or, with C 2, straight into registers.
+template <bool BF, int XG, int D, int C>
+__global__ __launch_bounds__(kThreads, XG == 1 && C == 1 && D == 2 ? 4 : 2) void dense_moe_down_kernel(
     const void* __restrict__ from, const int* __restrict__ tokens, const uint16_t* __restrict__ w2, int T, int slots, int H, int I, DenseMoeArgs a,
     MoeLayout layout) {
-  constexpr int TT = (XG + 1) / 2, kStage = stream_stage<XG, 2>();
+  constexpr int TT = (XG + 1) / 2, kStage = down_stage<XG, C>();
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
   char* const ws = static_cast<char*>(a.workspace);
-  uint8_t* const ring = smem + wave * stream_ring<XG, 2, D>();
-  float4_t* const sums = reinterpret_cast<float4_t*>(smem + kWaves * stream_ring<XG, 2, D>());  // [waves][T][4]
-  int* const row_token = reinterpret_cast<int*>(sums + kWaves * T * 4);                     // [T k]
-  MoeSegment* const segs = reinterpret_cast<MoeSegment*>(row_token + slots);                  // [T k at most]
+  uint8_t* const ring = smem + wave * D * kStage;
+  float4_t* const sums = reinterpret_cast<float4_t*>(smem + kWaves * D * kStage);  // [waves][T][4 C]
+  int* const row_token = reinterpret_cast<int*>(sums + kWaves * T * 4 * C);      // [T k]
+  MoeSegment* const segs = reinterpret_cast<MoeSegment*>(row_token + slots);     // [T k at most]
   const int n_segs = __builtin_amdgcn_readfirstlane(*static_cast<const int*>(from));
   for (int i = tid; i < slots; i += kThreads) {  // (all that may be there, without a wait for their number)
     row_token[i] = tokens[i];
     segs[i] = reinterpret_cast<const MoeSegment*>(static_cast<const char*>(from) + kSegsAt)[i];
   }
-  for (int i = tid; i < kWaves * T * 4; i += kThreads) sums[i] = float4_t{};
+  for (int i = tid; i < kWaves * T * 4 * C; i += kThreads) sums[i] = float4_t{};
   __syncthreads();
-  const int n0 = blockIdx.x * 16, per = (I + kStreamBlock - 1) / kStreamBlock;  // blocks a segment
+  const int n0 = blockIdx.x * 16 * C, per = (I + kStreamBlock - 1) / kStreamBlock;  // blocks a segment
   const int blocks = n_segs * per;
   const int begin = static_cast<int>(static_cast<int64_t>(blocks) * blockIdx.y / gridDim.y);
   const int end = static_cast<int>(static_cast<int64_t>(blocks) * (blockIdx.y + 1) / gridDim.y);
@@ -331,38 +344,66 @@ __global__ __launch_bounds__(kThreads, XG == 1 && D == 2 ? 4 : 2) void dense_moe
     }
   };
   At ahead{begin + wave, (begin + wave) / per, (begin + wave) % per}, now = ahead;
+  int4_t x_of[C == 2 ? D : 1][2][2][TT];  // [stage][plane][half of a block][16 rows]
   auto load = [&](int s) {
     const bool there = ahead.b < end;
     const MoeSegment seg = segs[there ? ahead.i : 0];
     const int64_t e = __builtin_amdgcn_readfirstlane(seg.e);
-    StreamPlace<XG, 2> p;
-    p.end = there ? I : 0;
+    rsrc_t w[2 * C];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 2 * C; ++i) {
       const int64_t left = H - n0 - 8 * i;
-      p.w[i] = dense_buffer(reinterpret_cast<const char*>(w2) + (e * H + n0 + 8 * i) * pitch, left > 0 ? 8 * pitch : 0);  // (hidden is a multiple of 8)
+      w[i] = dense_buffer(reinterpret_cast<const char*>(w2) + (e * H + n0 + 8 * i) * pitch, left > 0 ? 8 * pitch : 0);  // (hidden is a multiple of 8)
     }
-    p.x[0] = h_hi;
-    p.x[1] = h_lo;
+    const int k = ahead.kb * kStreamBlock, last = there ? I : 0;
+    if constexpr (C == 1) {
+      StreamPlace<XG, 2> p;
+      p.end = last;
+      p.w[0] = w[0];
+      p.w[1] = w[1];
+      p.x[0] = h_hi;
+      p.x[1] = h_lo;
 #pragma unroll
-    for (int g = 0; g < XG; ++g) {
-      const int c = 8 * g + (lane >> 3);
-      p.x_at[g] = c < seg.rows ? static_cast<uint32_t>(seg.row0 + c) * static_cast<uint32_t>(pitch) : kNowhere;
+      for (int g = 0; g < XG; ++g) {
+        const int c = 8 * g + (lane >> 3);
+        p.x_at[g] = c < seg.rows ? static_cast<uint32_t>(seg.row0 + c) * static_cast<uint32_t>(pitch) : kNowhere;
+      }
+      stream_load(p, k, static_cast<uint32_t>(pitch), ring + s * kStage);
+    } else {
+      const int kc = k + 8 * ((lane & 7) ^ (lane >> 3));
+      const uint32_t w_at = kc < last ? static_cast<uint32_t>(lane >> 3) * static_cast<uint32_t>(pitch) + 2u * kc : kNowhere;
+#pragma unroll
+      for (int i = 0; i < 2 * C; ++i) dense_to_lds<true>(w[i], w_at, ring + s * kStage + 1024 * i);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const int c = 16 * t + (lane & 15);
+        const uint32_t row = static_cast<uint32_t>(seg.row0 + c) * static_cast<uint32_t>(pitch);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int at_k = k + 32 * i + 8 * quad;
+          const uint32_t at = c < seg.rows && at_k < last ? row + 2u * at_k : kNowhere;
+          x_of[s][0][i][t] = __builtin_bit_cast(int4_t, __builtin_amdgcn_raw_buffer_load_b128(h_hi, at, 0, 0));
+          x_of[s][1][i][t] = __builtin_bit_cast(int4_t, __builtin_amdgcn_raw_buffer_load_b128(h_lo, at, 0, 0));
+        }
+      }
     }
-    stream_load(p, ahead.kb * kStreamBlock, static_cast<uint32_t>(pitch), ring + s * kStage);
     next(ahead);
   };
-  float4_t acc[TT];
+  float4_t acc[C][TT];
 #pragma unroll
-  for (int t = 0; t < TT; ++t) acc[t] = float4_t{};
+  for (int u = 0; u < C; ++u)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[u][t] = float4_t{};
   auto join = [&](int i) {  // a segment's sums go to its tokens'
     const MoeSegment seg = segs[i];
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      const int c = 16 * t + (lane & 15);
-      if (c < seg.rows) sums[(wave * T + row_token[seg.row0 + c]) * 4 + quad] += acc[t];
-      acc[t] = float4_t{};
-    }
+    for (int u = 0; u < C; ++u)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const int c = 16 * t + (lane & 15);
+        if (c < seg.rows) sums[(wave * T + row_token[seg.row0 + c]) * 4 * C + 4 * u + quad] += acc[u][t];
+        acc[u][t] = float4_t{};
+      }
   };
 #pragma unroll
   for (int s = 0; s < D; ++s) load(s);
@@ -374,8 +415,29 @@ __global__ __launch_bounds__(kThreads, XG == 1 && D == 2 ? 4 : 2) void dense_moe
         join(current);
         current = now.i;
       }
-      stream_wait<XG, 2, D>();
-      stream_block<BF, XG, 2>(ring + s * kStage, acc);  // (past the end: zeros)
+      // (past the end: zeros)
+      if constexpr (C == 1) {
+        stream_wait<XG, 2, D>();
+        stream_block<BF, XG, 2>(ring + s * kStage, acc[0]);
+      } else {
+        constexpr int kLoads = 2 * C + 4 * TT;
+        static_assert((D - 1) * kLoads < 64, "the counter of loads");
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * kLoads) : "memory");
+        const int row = lane & 15;
+#pragma unroll
+        for (int u = 0; u < C; ++u) {
+          int4_t w[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) w[i] = *reinterpret_cast<const int4_t*>(ring + s * kStage + 2048 * u + row * 128 + (((quad + 4 * i) ^ (row & 7)) << 4));
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int t = 0; t < TT; ++t) acc[u][t] = dense_mfma<BF>(w[i], x_of[s][p][i][t], acc[u][t]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read, before the stage is loaded again)
+      }
       next(now);
       load(s);
     }
@@ -385,19 +447,19 @@ __global__ __launch_bounds__(kThreads, XG == 1 && D == 2 ? 4 : 2) void dense_moe
   __syncthreads();
 
   // The waves' sums in their order: a thread four columns of a token.
-  for (int i = tid; i < T * 4; i += kThreads) {
-    const int n = n0 + 4 * (i & 3);
+  for (int i = tid; i < T * 4 * C; i += kThreads) {
+    const int n = n0 + 4 * (i % (4 * C));
     float4_t v = sums[i];
-    for (int w = 1; w < kWaves; ++w) v += sums[w * T * 4 + i];
+    for (int w = 1; w < kWaves; ++w) v += sums[w * T * 4 * C + i];
     sums[i] = v;
-    if (gridDim.y == 1 && n < H) moe_store<BF>(a.out + static_cast<int64_t>(i >> 2) * H + n, v);
+    if (gridDim.y == 1 && n < H) moe_store<BF>(a.out + static_cast<int64_t>(i / (4 * C)) * H + n, v);
   }
   if (gridDim.y == 1) return;
   // Shares of several workgroups: the one that comes last adds them all, in their order.  They go past the L2 of a die (agent-scope stores
   // and loads) and are there before the ticket is drawn; a fence would write back the die's whole L2 instead, which took 100 us.
-  float* const shares = reinterpret_cast<float*>(ws + layout.shares);  // [shares][tiles][T][16]
-  auto share_of = [&](int s) { return shares + (static_cast<int64_t>(s) * gridDim.x + blockIdx.x) * T * 16; };
-  for (int i = tid; i < T * 4; i += kThreads)
+  float* const shares = reinterpret_cast<float*>(ws + layout.shares);  // [shares][tiles][T][16 C]
+  auto share_of = [&](int s) { return shares + (static_cast<int64_t>(s) * gridDim.x + blockIdx.x) * T * 16 * C; };
+  for (int i = tid; i < T * 4 * C; i += kThreads)
 #pragma unroll
     for (int v = 0; v < 4; ++v) __hip_atomic_store(share_of(blockIdx.y) + 4 * i + v, sums[i][v], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -408,13 +470,13 @@ __global__ __launch_bounds__(kThreads, XG == 1 && D == 2 ? 4 : 2) void dense_moe
                static_cast<int>(gridDim.y) - 1;
   __syncthreads();
   if (!*last_one) return;
-  for (int i = tid; i < T * 4; i += kThreads) {
+  for (int i = tid; i < T * 4 * C; i += kThreads) {
     float4_t v = {};
     for (int s = 0; s < static_cast<int>(gridDim.y); ++s)
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] += __hip_atomic_load(share_of(s) + 4 * i + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const int n = n0 + 4 * (i & 3);
-    if (n < H) moe_store<BF>(a.out + static_cast<int64_t>(i >> 2) * H + n, v);
+    const int n = n0 + 4 * (i % (4 * C));
+    if (n < H) moe_store<BF>(a.out + static_cast<int64_t>(i / (4 * C)) * H + n, v);
   }
 }
 
@@ -445,30 +507,33 @@ static hipError_t launch_up(const DenseMoeArgs& a, const MoeLayout& layout, int 
   return hipGetLastError();
 }
 
-template <bool BF, int XG, int D>
+template <bool BF, int XG, int C>
 static hipError_t launch_down(const DenseMoeArgs& a, const MoeLayout& layout, hipStream_t s) {
+  constexpr int D = 2;  // (two workgroups a unit with two blocks ahead, C 1: one with four was 1 to 10 % behind)
   const int shares = moe_shares(a.T, a.hidden, a.inter, a.experts, a.k);
-  const dim3 grid(static_cast<unsigned>((a.hidden + 15) / 16), static_cast<unsigned>(shares));
+  const dim3 grid(static_cast<unsigned>((a.hidden + 16 * C - 1) / (16 * C)), static_cast<unsigned>(shares));
   note_kernel("dense_moe up to %d rows, %d shares%s", 8 * XG, shares, moe_keeps(a) ? ", x kept" : "");
-  const size_t lds = kWaves * (stream_ring<XG, 2, D>() + a.T * 64) + static_cast<size_t>(a.T) * a.k * (4 + sizeof(MoeSegment));
-  if (lds > 160 * 1024) return hipErrorNotSupported;
-  auto* kern = dense_moe_down_kernel<BF, XG, D>;
+  const size_t lds = kWaves * (D * down_stage<XG, C>() + static_cast<size_t>(a.T) * 64 * C) + static_cast<size_t>(a.T) * a.k * (4 + sizeof(MoeSegment));
+  static_assert(kWaves * (D * down_stage<XG, C>() + kMoeTokens * 64 * C) + kMoeTokens * 32 * (4 + sizeof(MoeSegment)) <= 160 * 1024, "LDS of a unit");
+  auto* kern = dense_moe_down_kernel<BF, XG, D, C>;
   const hipError_t e = may_use(kern, lds);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(kern, grid, dim3(kThreads), lds, s, a.workspace, reinterpret_cast<const int*>(static_cast<const char*>(a.workspace) + layout.row_token),
-                     a.w2, a.T, a.T * a.k, a.hidden, a.inter, a, layout);
+  hipLaunchKernelGGL(kern, grid, dim3(kThreads), lds, s, a.workspace,
+                     reinterpret_cast<const int*>(static_cast<const char*>(a.workspace) + layout.row_token), a.w2, a.T, a.T * a.k, a.hidden, a.inter, a,
+                     layout);
   return hipGetLastError();
 }
 
 template <bool BF, int XG>
 static hipError_t launch(const DenseMoeArgs& a, hipStream_t s) {
   const MoeLayout layout = moe_layout(a.T, a.hidden, a.inter, a.experts, a.k);
+  const int down_rows = moe_down_rows(a);
   auto up = [&](auto xg, auto d, auto nb) {
     constexpr int U = decltype(xg)::value, D = decltype(d)::value, NB = decltype(nb)::value;
-    return a.experts <= 64    ? launch_up<BF, 2, U, D, NB>(a, layout, 8 * XG, s)
-           : a.experts <= 128 ? launch_up<BF, 4, U, D, NB>(a, layout, 8 * XG, s)
-           : a.experts <= 256 ? launch_up<BF, 8, U, D, NB>(a, layout, 8 * XG, s)
-                              : launch_up<BF, 16, U, D, NB>(a, layout, 8 * XG, s);
+    return a.experts <= 64    ? launch_up<BF, 2, U, D, NB>(a, layout, down_rows, s)
+           : a.experts <= 128 ? launch_up<BF, 4, U, D, NB>(a, layout, down_rows, s)
+           : a.experts <= 256 ? launch_up<BF, 8, U, D, NB>(a, layout, down_rows, s)
+                              : launch_up<BF, 16, U, D, NB>(a, layout, down_rows, s);
   };
   const std::integral_constant<int, 0> none{};
   const std::integral_constant<int, 2> two{};
@@ -479,8 +544,9 @@ static hipError_t launch(const DenseMoeArgs& a, hipStream_t s) {
   if (moe_keeps(a)) e = moe_blocks(a.hidden) == 4 ? up(four, four, four) : up(four, four, eight);
   if (e == hipErrorNotSupported) e = up(rows, four, none);
   if (e == hipErrorNotSupported) e = up(rows, two, none);  // (many slots: their tables take the room)
-  // (two workgroups a unit with two blocks ahead: one with four was 1 to 10 % behind, 16 tokens of 128 experts 133 / 137 us in all)
-  return e != hipSuccess ? e : launch_down<BF, XG, 2>(a, layout, s);
+  if (e != hipSuccess) return e;
+  if constexpr (XG == 1) return launch_down<BF, 1, 1>(a, layout, s);  // (8 tokens, or few an expert)
+  else return down_rows == 32 ? launch_down<BF, 4, 2>(a, layout, s) : launch_down<BF, 2, 2>(a, layout, s);
 }
 
 hipError_t launch_dense_moe(const DenseMoeArgs& a, hipStream_t s) {
