@@ -8,9 +8,9 @@
 // left, so that the second product loses nothing to it.
 // The second streams the down rows past the same rows of w h; what comes out of an expert joins the sums of its tokens, which lie in LDS.  An
 // expert meets the tokens that chose it alone, whatever W or the other tokens hold.
-// Bound by HBM.  Both kernels, us (of their bytes at 6.85 TB/s): one token, 6 of 64 experts of 2048 x 1408, 29.7 (15.2); 4 tokens, 2 of 8 experts of 4096
-// x 14336, 294 (283), 16 tokens 577 (407), 32 tokens 574 (411): with more rows an expert the way of x from the L2 counts beside W's; 16 tokens, 8 of
-// 128 experts of 2048 x 768, 134 (114).
+// Bound by HBM.  Both kernels, us (of their bytes at 6.85 TB/s): one token, 6 of 64 experts of 2048 x 1408, 27.5 (15.2); 2 of 8 experts of 4096 x 14336,
+// 4 tokens 298 (283), 16 tokens 522 (411), 64 tokens 567 (411): the way of x from the L2 counts beside W's; 16 tokens, 8 of 128 experts of 2048 x 768,
+// 126 (114).
 #include "gq_dense_stream.hpp"
 #include "gq_gating.hpp"
 
@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kWaves = kStreamWaves, kThreads = 64 * kWaves;
 
-// Up to 8 XG rows of one expert, the columns of x of both products.
+// Up to 8 XG rows of one expert, a matrix instruction's columns in both products.
 struct MoeSegment {
   int e, row0, rows;
 };
@@ -374,6 +374,7 @@ __global__ __launch_bounds__(kThreads, XG == 1 && C == 1 && D == 2 ? 4 : 2) void
       const uint32_t w_at = kc < last ? static_cast<uint32_t>(lane >> 3) * static_cast<uint32_t>(pitch) + 2u * kc : kNowhere;
 #pragma unroll
       for (int i = 0; i < 2 * C; ++i) dense_to_lds<true>(w[i], w_at, ring + s * kStage + 1024 * i);
+      asm volatile("" ::: "memory");  // (in this order)
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
         const int c = 16 * t + (lane & 15);
@@ -386,6 +387,7 @@ __global__ __launch_bounds__(kThreads, XG == 1 && C == 1 && D == 2 ? 4 : 2) void
           x_of[s][1][i][t] = __builtin_bit_cast(int4_t, __builtin_amdgcn_raw_buffer_load_b128(h_lo, at, 0, 0));
         }
       }
+      asm volatile("" ::: "memory");
     }
     next(ahead);
   };
@@ -492,7 +494,7 @@ static hipError_t launch_up(const DenseMoeArgs& a, const MoeLayout& layout, int 
   const int slots = a.T * a.k, n_tiles = a.inter / 8;
   const StreamPlan plan = stream_plan(experts_chosen(a.T, a.experts, a.k) * n_tiles, a.hidden, D);
   const int64_t most = static_cast<int64_t>(slots < a.experts ? slots : a.experts + slots / (8 * XG)) * n_tiles;  // items
-  const int nw = kWaves >> plan.kw_log2;
+  const int nw = NB > 0 ? 1 : kWaves >> plan.kw_log2;
   const int64_t sets = (most + nw - 1) / nw;
   const size_t tables = moe_tables_bytes(a.experts, slots), gate = kWaves * sizeof(GateScratch<NC>);
   const size_t rings = kWaves * ((NB > 0 ? D * kKeptStage : stream_ring<XG, 1, D>()) + 2 * ((XG + 1) / 2) * 1024), lds = tables + (rings > gate ? rings : gate);

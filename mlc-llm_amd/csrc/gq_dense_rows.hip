@@ -1,8 +1,8 @@
 // Products of up to 16 rows with 16-bit weights: the weights stream through once, bound by HBM.
 //
 // 256 workgroups of eight waves, one a unit: together 64 KiB of weights a unit are on their way, which keeps the memory busy over a load's 1 to 2 us, and
-// a launch has no second round of workgroups to ramp up.  Measured, us (TB/s of weights): 128256 x 4096 of 5 rows 156 (6.7); 28672 x 4096, gated, of one
-// row 37.3 (6.3); 4096 x 4096 of one row 7.2 (4.7, of which 2.3 us are the launch); 128 x 2048 of 16 rows 5.4 with its call.
+// a launch has no second round of workgroups to ramp up.  Measured, us (TB/s of weights): 128256 x 4096 of 5 rows 152 (6.9); 28672 x 4096, gated, of one
+// row 37.0 (6.3); 4096 x 4096 of one row 7.2 (4.7, of which 2.3 us are the launch); 128 x 2048 of 16 rows 5.4 with its call.
 #include "gq_dense_stream.hpp"
 
 namespace gq {

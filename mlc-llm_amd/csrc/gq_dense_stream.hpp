@@ -58,6 +58,7 @@ __device__ __forceinline__ void stream_load(const StreamPlace<XG, PX>& p, int k,
 #pragma unroll
     for (int i = 0; i < PX; ++i) dense_to_lds<false>(p.x[i], at, stage + 2048 + (i * XG + g) * 1024);
   }
+  asm volatile("" ::: "memory");  // (before the next block's, by which the wait counts)
 }
 // Waits until all but the newest D - 1 blocks have landed.
 template <int XG, int PX, int D>
@@ -152,30 +153,27 @@ __device__ __forceinline__ void kept_load(const StreamRows& p, int k, uint32_t w
   const uint32_t at = kc < p.end ? static_cast<uint32_t>(lane >> 3) * w_pitch + 2u * kc : kNowhere;
 #pragma unroll
   for (int i = 0; i < 2; ++i) dense_to_lds<true>(p.w[i], at, stage + 1024 * i);
+  asm volatile("" ::: "memory");  // (before the next block's, by which the wait counts)
 }
 // keep(round, kept) brings x where it changes, rows_of(round) gives the rows of W.  k: this wave's first number of K.
 template <bool BF, int TT, int NB, int D, class RowsOf, class Keep, class Done>
 __device__ __forceinline__ void dense_stream_kept(uint8_t* ring, uint32_t w_pitch, int k, int step, int rounds, RowsOf rows_of, Keep keep, Done done) {
-  static_assert(D % NB == 0 || NB % D == 0, "whole items or whole parts of one");
-  constexpr int kAhead = D >= NB ? D / NB : 1;
+  static_assert(NB % D == 0, "the stages of a block in every item");
   const int lane = threadIdx.x & 63, quad = lane >> 4, row = lane & 15;
   const int c0 = (quad ^ (row & 7)) << 4, c1 = ((quad + 4) ^ (row & 7)) << 4;
-  StreamRows here = rows_of(0), next = here;
+  StreamRows here = rows_of(0);
 #pragma unroll
-  for (int s = 0; s < D; ++s) {
-    if (s > 0 && s % NB == 0) next = rows_of(s / NB);
-    kept_load(s < NB ? here : next, k + s % NB * step, w_pitch, ring + s * kKeptStage);
-  }
+  for (int s = 0; s < D; ++s) kept_load(here, k + s * step, w_pitch, ring + s * kKeptStage);
   StreamKept<NB, TT> x;
   for (int round = 0; round < rounds; ++round) {
     keep(round, x);
     float4_t acc[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) acc[t] = float4_t{};
-    next = rows_of(round + kAhead);
+    const StreamRows next = rows_of(round + 1);
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      uint8_t* const stage = ring + (D > NB ? (round % kAhead) * NB + j : j % D) * kKeptStage;
+      uint8_t* const stage = ring + j % D * kKeptStage;
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (D - 1)) : "memory");
       const int4_t w0 = *reinterpret_cast<const int4_t*>(stage + row * 128 + c0), w1 = *reinterpret_cast<const int4_t*>(stage + row * 128 + c1);
 #pragma unroll
@@ -184,8 +182,7 @@ __device__ __forceinline__ void dense_stream_kept(uint8_t* ring, uint32_t w_pitc
         acc[t] = dense_mfma<BF>(w1, x.v[j][1][t], acc[t]);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read, before the stage is loaded again)
-      const bool same = j + D < NB;
-      kept_load(same ? here : next, k + (j + D) % NB * step, w_pitch, stage);
+      kept_load(j + D < NB ? here : next, k + (j + D) % NB * step, w_pitch, stage);
     }
     here = next;
     done(round, acc);
