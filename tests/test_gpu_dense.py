@@ -474,6 +474,47 @@ def test_moe_graph_replays(t):
             assert torch.equal(out, ops.dense_moe(x, logits, w13, w2, k))
 
 
+def test_moe_graph_replays_with_x_in_registers():
+    g = _gen(77)
+    x, logits, w13, w2 = _layer(g, torch.float16, 64, 2048, 1024, 4)
+    ops.dense_moe(x, logits, w13, w2, 2)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.dense_moe(x, logits, w13, w2, 2)
+    for i in range(4):
+        x.copy_(_normal(g, torch.float16, *x.shape))
+        logits.copy_(_normal(g, torch.float32, *logits.shape, scale=0.1 + 3 * i))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.dense_moe(x, logits, w13, w2, 2))
+
+
+# (tokens, hidden, inter, experts, top_k): one token, shares of the second product, 32 columns a workgroup, x in registers with segments of 16 and 32 rows
+@pytest.mark.parametrize("t,hidden,inter,experts,k", [(1, 2048, 1408, 64, 6), (16, 2048, 768, 128, 8), (33, 104, 64, 300, 32), (40, 264, 136, 8, 3),
+                                                      (40, 2048, 1024, 8, 2), (64, 2048, 1032, 4, 2)])
+def test_moe_whatever_its_workspace_holds(t, hidden, inter, experts, k):
+    """Scratch full of ones or of an earlier call's, guards behind it and the output, NaN and infinite logits."""
+    g = _gen(t + inter)
+    x, logits, w13, w2 = _layer(g, torch.bfloat16, t, hidden, inter, experts)
+    logits[0] = math.nan
+    logits[t // 2, : experts // 2] = math.inf
+    logits[t - 1] = -math.inf
+    want = ops.dense_moe(x, logits, w13, w2, k)
+    weights, ids = ops.moe_gating(logits, k)
+    assert ((ids >= 0) & (ids < experts)).all() and all(len(set(row)) == k for row in ids.tolist())
+    close(want, moe_ref(x, weights, ids, w13, w2, "silu", torch.bfloat16))
+    size = gq._lib.lib().mi355gq_dense_moe_workspace_bytes(t, hidden, inter, experts, k)
+    ws = torch.full((size + 256,), 255, dtype=torch.uint8, device="cuda")
+    out = torch.full((t * hidden + 64,), 7.0, dtype=torch.bfloat16, device="cuda")
+    for _ in range(3):
+        gq._lib.call("mi355gq_dense_moe", x.data_ptr(), logits.data_ptr(), None, t, hidden, inter, experts, k, 0, 1, 1, 1, 1.0, ops._MODEL_DTYPES[logits.dtype],
+                     w13.data_ptr(), w2.data_ptr(), ops._activation("silu"), ops._MODEL_DTYPES[x.dtype], out.data_ptr(), ws.data_ptr(), size, ops._stream())
+        assert torch.equal(out[: t * hidden].view(t, hidden), want)
+        assert (ws[size:] == 255).all() and (out[t * hidden :] == 7).all()
+        out[: t * hidden] = math.nan
+
+
 def test_router_layer_and_residual_together():
     """As a decoder layer runs them: router logits in float32, experts, a shared gated MLP whose down projection adds the rest up."""
     g = _gen(9)
