@@ -266,7 +266,7 @@ __global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(
   };
   __syncthreads();  // (the routing's part of LDS is the rings' now)
   if constexpr (NB == 0) {
-    dense_stream<BF, XG, D>(rest + wave * stream_ring<XG, 1, D>(), static_cast<uint32_t>(pitch), KW * kStreamBlock, nb, rounds, place_of, done);
+    dense_stream<BF, XG, D, false>(rest + wave * stream_ring<XG, 1, D>(), static_cast<uint32_t>(pitch), KW * kStreamBlock, nb, rounds, place_of, done);
   } else {
     auto rows_of = [&](int round) {
       const Item it = item_of(round);
@@ -492,7 +492,7 @@ static hipError_t may_use(Kernel* kern, size_t lds) {
 template <bool BF, int NC, int XG, int D, int NB>
 static hipError_t launch_up(const DenseMoeArgs& a, const MoeLayout& layout, int down_rows, hipStream_t s) {
   const int slots = a.T * a.k, n_tiles = a.inter / 8;
-  const StreamPlan plan = stream_plan(experts_chosen(a.T, a.experts, a.k) * n_tiles, a.hidden, D);
+  const StreamPlan plan = stream_plan(experts_chosen(a.T, a.experts, a.k) * n_tiles, a.hidden, D, false);
   const int64_t most = static_cast<int64_t>(slots < a.experts ? slots : a.experts + slots / (8 * XG)) * n_tiles;  // items
   const int nw = NB > 0 ? 1 : kWaves >> plan.kw_log2;
   const int64_t sets = (most + nw - 1) / nw;

@@ -13,7 +13,7 @@ constexpr int kDepth = 4;  // blocks in flight a wave
 
 // Eight waves: KW of them share the K of an item, 16 rows of W (gated: 8 gate rows and their up rows), and their sums meet in LDS.  The arguments
 // that the first loads wait for come first: a launch brings them in scalar registers (4096 x 4096 of one row 7.5 -> 7.2 us).
-template <bool BF, bool GATED, int XG>
+template <bool BF, bool GATED, int XG, bool ANY>
 __global__ __launch_bounds__(64 * kStreamWaves, 2) void dense_rows_kernel(
     const uint16_t* __restrict__ x, const uint16_t* __restrict__ w, int K, int rows, int cols_, int kw_log2, int nb, int rounds, DenseArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -56,18 +56,18 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void dense_rows_kernel(
       if (r < rows && n < cols && (!GATED || lane < 32)) dense_store<BF, 4, GATED>(a, r, static_cast<int>(n), o, u);
     }
   };
-  dense_stream<BF, XG, kDepth>(ring, static_cast<uint32_t>(pitch), KW * kStreamBlock, nb, rounds, place_of, done);
+  dense_stream<BF, XG, kDepth, ANY>(ring, static_cast<uint32_t>(pitch), KW * kStreamBlock, nb, rounds, place_of, done);
 }
 
 template <bool BF, bool GATED, int XG>
 static hipError_t launch(const DenseArgs& a, hipStream_t s) {
   const int64_t cols = GATED ? a.N / 2 : a.N, items = (cols + (GATED ? 7 : 15)) / (GATED ? 8 : 16);
-  const StreamPlan plan = stream_plan(static_cast<double>(items), a.K, kDepth);
+  const StreamPlan plan = stream_plan(static_cast<double>(items), a.K, kDepth, true);
   const int nw = kStreamWaves >> plan.kw_log2;
   const int64_t sets = (items + nw - 1) / nw;
   constexpr size_t lds = kStreamWaves * (stream_ring<XG, 1, kDepth>() + 2 * ((XG + 1) / 2) * 1024);
   static_assert(lds <= 160 * 1024, "LDS of a unit");
-  auto* kern = dense_rows_kernel<BF, GATED, XG>;
+  auto* kern = plan.nb % kDepth == 0 ? dense_rows_kernel<BF, GATED, XG, false> : dense_rows_kernel<BF, GATED, XG, true>;
   const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kern));
   if (e != hipSuccess) return e;
   note_kernel("dense_rows up to %d rows%s, %d waves share K", 8 * XG, GATED ? " gated" : "", 1 << plan.kw_log2);

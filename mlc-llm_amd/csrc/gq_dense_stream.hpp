@@ -85,34 +85,64 @@ __device__ __forceinline__ void stream_block(const uint8_t* stage, float4_t (&ac
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read, before the stage is loaded again)
 }
 
-// `rounds` places one after the other, of each nb blocks (a multiple of D), `step` numbers of K apart; past K they are zeros.  place_of(round)
-// gives a place, done(round, sums) takes its sums.
-template <bool BF, int XG, int D, class PlaceOf, class Done>
+// `rounds` places one after the other, of each nb blocks, `step` numbers of K apart; past K they are zeros.  place_of(round) gives a place,
+// done(round, sums) takes its sums.  nb a multiple of D goes around the ring without a branch (128 x 2048 of one row 3.7 us, and 4.2 the other way);
+// with ANY it may be anything, and a place's last stage is followed by the next one's first (2 x 9728 x 2560, five blocks a wave, 12.1 us, and 13.8
+// padded to eight).
+template <bool BF, int XG, int D, bool ANY, class PlaceOf, class Done>
 __device__ __forceinline__ void dense_stream(uint8_t* ring, uint32_t w_pitch, int step, int nb, int rounds, PlaceOf place_of, Done done) {
   constexpr int TT = (XG + 1) / 2, kStage = stream_stage<XG, 1>();
   StreamPlace<XG, 1> here = place_of(0);
-#pragma unroll
-  for (int s = 0; s < D; ++s) stream_load(here, here.k + s * step, w_pitch, ring + s * kStage);
-  for (int round = 0; round < rounds; ++round) {
-    float4_t acc[TT];
+  float4_t acc[TT];
+  auto clear = [&] {
 #pragma unroll
     for (int t = 0; t < TT; ++t) acc[t] = float4_t{};
-    for (int j = D; j < nb; j += D) {
+  };
+  if constexpr (!ANY) {
+#pragma unroll
+    for (int s = 0; s < D; ++s) stream_load(here, here.k + s * step, w_pitch, ring + s * kStage);
+    for (int round = 0; round < rounds; ++round) {
+      clear();
+      for (int j = D; j < nb; j += D) {
+#pragma unroll
+        for (int s = 0; s < D; ++s) {
+          stream_wait<XG, 1, D>();
+          stream_block<BF, XG, 1>(ring + s * kStage, acc);
+          stream_load(here, here.k + (j + s) * step, w_pitch, ring + s * kStage);
+        }
+      }
+      here = place_of(round + 1);
 #pragma unroll
       for (int s = 0; s < D; ++s) {
         stream_wait<XG, 1, D>();
         stream_block<BF, XG, 1>(ring + s * kStage, acc);
-        stream_load(here, here.k + (j + s) * step, w_pitch, ring + s * kStage);
+        stream_load(here, here.k + s * step, w_pitch, ring + s * kStage);
       }
+      done(round, acc);
     }
-    here = place_of(round + 1);
-#pragma unroll
-    for (int s = 0; s < D; ++s) {
-      stream_wait<XG, 1, D>();
-      stream_block<BF, XG, 1>(ring + s * kStage, acc);
-      stream_load(here, here.k + s * step, w_pitch, ring + s * kStage);
+  } else {
+    int at = 0, block = 0;  // place and number there of the next block to load
+    auto load = [&](uint8_t* stage) {
+      stream_load(here, here.k + block * step, w_pitch, stage);
+      if (++block == nb) {
+        block = 0;
+        here = place_of(++at);
+      }
+    };
+#pragma unroll 1
+    for (int s = 0; s < D; ++s) load(ring + s * kStage);
+    uint8_t* stage = ring;
+    for (int round = 0; round < rounds; ++round) {
+      clear();
+#pragma unroll 1
+      for (int j = 0; j < nb; ++j) {
+        stream_wait<XG, 1, D>();
+        stream_block<BF, XG, 1>(stage, acc);
+        load(stage);
+        stage = stage == ring + (D - 1) * kStage ? ring : stage + kStage;
+      }
+      done(round, acc);
     }
-    done(round, acc);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (loads of nothing may still land in the ring)
 }
@@ -219,18 +249,19 @@ __device__ __forceinline__ float4_t stream_up(float4_t v) {
 // a twelfth more for a KW of four or two and a third for one.  One row, by KW 8, 4, 2 and 1, us: 28672 x 4096 38.4, 36.2, 45.4, 40.4 (the rule: 8);
 // 8192 x 8192 27.0, 29.7, 28.0, 52.2 (8); 6144 x 4096 11.1, 12.3, 15.3, 24.2 (8); 5120 x 5120, of whose 10 blocks a wave of eight has two empty
 // ones, 13.4, 12.1, 18.1, 30.7 (4); 152064 x 3584 162.6, 151.8, 153.4, 155.2 (2).
+// any: nb may be no multiple of D where it is more, at a seventh more for a block.
 struct StreamPlan {
   int kw_log2, nb, rounds;
 };
-inline StreamPlan stream_plan(double items, int64_t K, int D) {
+inline StreamPlan stream_plan(double items, int64_t K, int D, bool any) {
   const int64_t blocks = (K + kStreamBlock - 1) / kStreamBlock;
   StreamPlan best{0, 0, 0};
   double best_cost = 0;
   for (int log2 = 3; log2 >= 0; --log2) {
-    const int64_t each = (blocks + (1 << log2) - 1) >> log2, nb = (each + D - 1) / D * D;
+    const int64_t each = (blocks + (1 << log2) - 1) >> log2, whole = (each + D - 1) / D * D, nb = any && each > D ? each : whole;
     const double rounds = __builtin_ceil(items / ((kStreamWaves >> log2) * kStreamUnits));
     const double ends = 0.65 * (rounds < 6 ? rounds : 6);
-    const double cost = (rounds * static_cast<double>(nb) + ends) * (log2 == 0 ? 1.3 : log2 < 3 ? 1.08 : 1.0);
+    const double cost = (rounds * static_cast<double>(nb) + ends) * (log2 == 0 ? 1.3 : log2 < 3 ? 1.08 : 1.0) * (nb < whole ? 1.15 : 1.0);
     if (best.nb == 0 || cost < best_cost) {
       best_cost = cost;
       best = {log2, static_cast<int>(nb), static_cast<int>(rounds)};

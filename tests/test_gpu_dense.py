@@ -114,6 +114,17 @@ def test_gated(m, n, k, dtype):
         close(ops.dense_linear_gated(x, w, bias=b, activation=act, out_dtype=out_dtype), gated_ref(x, w, b, act, out_dtype))
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 9728, 2560), (8, 4872, 2600), (3, 8200, 2888), (16, 4868, 2600), (2, 100, 5000)])
+def test_blocks_of_a_wave_past_its_ring(m, n, k):
+    """K of five to eleven blocks a wave, over several items each."""
+    g = _gen(n + k)
+    for dtype in HALVES:
+        x, w, bias = _normal(g, dtype, m, k), _normal(g, dtype, n, k, scale=k**-0.5), _normal(g, dtype, n)
+        close(ops.dense_linear(x, w, bias=bias, activation="silu"), linear_ref(x, w, bias, "silu", None, dtype))
+        assert "dense_rows" in gq._lib.last_kernel()
+        close(ops.dense_linear_gated(x, w), gated_ref(x, w, None, "silu", dtype))
+
+
 @pytest.mark.parametrize("shares", [1, 3])
 @pytest.mark.parametrize("form", range(11))
 def test_tile_forms(form, shares):
