@@ -27,9 +27,9 @@ int hip_result(hipError_t e, const char* what) {
 }
 hipStream_t as_stream(mi355gq_stream_t s) { return static_cast<hipStream_t>(s); }
 
-// Where the kernel that streams the weights past up to sixteen rows of x is faster than the tiles; N rows of W.  us, it / the best tiles:
-// 4096 x 4096 of 2 rows 8.5 / 10.6, of 16 9.8 / 11.3; 28672 x 4096 of 2 rows 38.5 / 37.6, of 8 39.9 / 39.0, of 12 42.7 / 39.0; 5120 x 5120 of 2
-// rows 12.7 / 13.2, of 8 14.3 / 13.7, of 12 16.2 / 14.1; 11264 x 2048 of 8 rows 11.7 / 11.0, of 12 12.6 / 11.2; 8192 x 2048 of 12 9.9 / 9.9.
+// Where the kernel that streams the weights past up to sixteen rows of x is faster than the tiles; N rows of W.  us, it / the tiles: 4096 x 4096 of 4
+// rows 8.3 / 10.7, of 16 9.3 / 11.2; 6144 x 4096 of 8 rows 11.9 / 13.9, of 16 13.9 / 14.4; 11264 x 2048 of 8 rows 10.6 / 11.0, of 12 11.7 / 11.1; 5120 x 5120
+// of 8 rows 14.3 / 13.6, of 12 16.0 / 13.9; 28672 x 4096 of 8 rows 37.5 / 37.9, of 12 39.4 / 38.2; 128256 x 4096 of 8 rows 157 / 154, of 16 186 / 160.
 bool few_rows(int64_t M, int64_t N, int64_t K) { return gq::options().gemm_variant < 0 && (M <= 8 || (M <= 16 && N * K < 20000000)); }
 
 // cols: of y
