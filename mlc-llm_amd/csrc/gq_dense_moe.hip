@@ -9,8 +9,8 @@
 // The second streams the down rows past the same rows of w h; what comes out of an expert joins the sums of its tokens, which lie in LDS.  An
 // expert meets the tokens that chose it alone, whatever W or the other tokens hold.
 // Bound by HBM.  Both kernels, us (of their bytes at 6.85 TB/s): one token, 6 of 64 experts of 2048 x 1408, 27.5 (15.2); 2 of 8 experts of 4096 x 14336,
-// 4 tokens 298 (283), 16 tokens 522 (411), 64 tokens 567 (411): the way of x from the L2 counts beside W's; 16 tokens, 8 of 128 experts of 2048 x 768,
-// 126 (114).
+// 4 tokens 290 (283), 16 tokens 440 (411), 32 tokens 447 (411), 64 tokens 527 (411), where the way of x from the L2 counts beside W's; 16 tokens, 8
+// of 128 experts of 2048 x 768, 126 (119).  In memory that a process has given back and taken again all of these take 10 to 20 % more.
 #include "gq_dense_stream.hpp"
 #include "gq_gating.hpp"
 
@@ -49,7 +49,7 @@ inline double experts_chosen(int64_t T, int64_t experts, int64_t k) {
   return static_cast<double>(experts) * (1 - none);
 }
 // Eights of rows of a segment: sixteen rows where experts have more than four on average.  The second kernel then takes 32 columns a workgroup and not
-// 16, and x, which comes half as often, goes straight into registers: 8 experts of 4096 x 14336, 2 a token, 32 tokens 213 -> 200 us, 48 226 -> 213; 16
+// 16, and x, which comes half as often, goes straight into registers (each pair in the same memory): 8 experts of 4096 x 14336, 2 a token, 32 tokens 213 -> 200 us, 48 226 -> 213; 16
 // experts of 7168 x 2048, 4 a token, 32 tokens 110 -> 95; (16 tokens of 128 experts of 2048 x 768, 8 a token, would take 48 and take 46).
 inline int moe_eights(int64_t T, int64_t experts, int64_t k) { return T > 8 && T * k > 4 * experts ? 2 : 1; }
 // Workgroups that share the K (all chosen experts' inter) of sixteen columns in the second kernel: about one a unit (sixteen tokens
@@ -66,7 +66,8 @@ inline int moe_shares(int64_t T, int64_t hidden, int64_t inter, int64_t experts,
 // blocks of K of the first product a wave where all waves of a workgroup share them
 inline int moe_blocks(int64_t hidden) { return static_cast<int>((hidden + kWaves * kStreamBlock - 1) / (kWaves * kStreamBlock)); }
 // Whether the first kernel keeps x in registers, in segments of 32 rows, rather than load it beside W, in segments of 8 or 16.  It does where that
-// fits (4 blocks a wave, or 7 and 8) and a segment is long enough for the wait that each change of x is.  The first kernel's us, with W / kept:
+// fits (4 blocks a wave, or 7 and 8) and a segment is long enough for the wait that each change of x is.  The first kernel's us, with W / kept
+// in the same memory:
 // 8 experts of 4096 x 14336, 2 a token, 4 tokens 204 / 204, 8 tokens 298 / 284, 32 348 / 328, 48 373 / 327, 64 553 / 323; 64 of 64 experts of 2048 x
 // 1408, 6 a token, 156 / 150; 128 experts of 2048 x 768, 8 a token, 16 tokens 99 / 108, 64 tokens 141 / 147.
 inline bool moe_keeps(const DenseMoeArgs& a) {
