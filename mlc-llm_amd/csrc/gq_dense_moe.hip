@@ -10,7 +10,7 @@
 // expert meets the tokens that chose it alone, whatever W or the other tokens hold.
 // Bound by HBM.  Both kernels, us (of their bytes at 6.85 TB/s): one token, 6 of 64 experts of 2048 x 1408, 27.5 (15.2); 2 of 8 experts of 4096 x 14336,
 // 4 tokens 290 (283), 16 tokens 440 (411), 32 tokens 447 (411), 64 tokens 527 (411), where the way of x from the L2 counts beside W's; 16 tokens, 8
-// of 128 experts of 2048 x 768, 126 (119).  In memory that a process has given back and taken again all of these take 10 to 20 % more.
+// of 128 experts of 2048 x 768, 126 (114).  In memory that a process has given back and taken again all of these take 10 to 20 % more.
 #include "gq_dense_stream.hpp"
 #include "gq_gating.hpp"
 
