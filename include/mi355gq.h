@@ -574,8 +574,8 @@ MI355GQ_API int mi355gq_dense_linear_gated(const void* x, const void* w, const v
  *   out[t] = sum over j of weights[t, j] * w2[e] . (act(g) * u),  [g, u] = w13[e] . x[t],  e = ids[t, j]
  * weights and ids are mi355gq_moe_gating's of logits [T, num_experts] in logits_dtype (score_bias is its bias); w13 [num_experts,
  * 2 inter, hidden] (gate rows, then up rows) and w2 [num_experts, hidden, inter] in model_dtype, dense.  All sums are in float32;
- * weights * act(g) * u is held as the sum of two numbers of model_dtype (an infinity beyond its range), the output rounded once.  An expert touches no token
- * that did not choose it, whatever its weights hold.  hidden and inter: multiples of 8.  x, w13, w2 and out start at 16 bytes; out may be x.
+ * weights * act(g) * u is held in float32, of which the second product takes all 24 bits (bfloat16), or what is above 2^-23 of the number or 2^-27 of the
+ * largest one of its token and expert (float16); the output is rounded once.  An expert touches no token that did not choose it, whatever its weights hold.  hidden and inter: multiples of 8.  x, w13, w2 and out start at 16 bytes; out may be x.
  * workspace: mi355gq_dense_moe_workspace_bytes() bytes, 16-byte aligned; MI355GQ_ERR_WORKSPACE where it is smaller.  Undefined afterwards; calls
  * that share one must be stream-ordered.  More than 64 tokens, or 2 T top_k inter of 3 * 2^30 and more: MI355GQ_ERR_UNSUPPORTED.
  */

@@ -85,7 +85,7 @@ bool moe_sizes_ok(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int
   return T >= 0 && T < kMaxDim && hidden > 0 && hidden % 8 == 0 && hidden < kMaxRow && inter > 0 && inter % 8 == 0 && inter < kMaxRow && experts > 0 &&
          experts <= 512 && top_k > 0 && top_k <= 32 && top_k <= experts;
 }
-// the rows of the workspace are reached by 32-bit offsets
+// (work items are counted in 32 bits)
 bool moe_takes(int64_t T, int64_t inter, int64_t top_k) { return T <= gq::kMoeTokens && T * top_k * inter * 2 < 0xc0000000ll; }
 
 }  // namespace
@@ -131,7 +131,7 @@ int mi355gq_dense_moe(const void* x, const void* logits, const void* score_bias,
                 (long long)num_experts, (long long)top_k);
   if (T == 0) return MI355GQ_OK;
   if (!moe_takes(T, inter, top_k))
-    return set_error(MI355GQ_ERR_UNSUPPORTED, "dense_moe: %lld tokens of %lld experts of %lld (%d tokens at most, and 3 GiB of activations)", (long long)T,
+    return set_error(MI355GQ_ERR_UNSUPPORTED, "dense_moe: %lld tokens of %lld experts of %lld (%d tokens at most, and 3 GiB of activations in 16 bits)", (long long)T,
                      (long long)top_k, (long long)inter, gq::kMoeTokens);
   DENSE_REQUIRE(x && logits && w13 && w2 && out, "dense_moe: null pointer");
   DENSE_REQUIRE(aligned(x, 16) && aligned(w13, 16) && aligned(w2, 16) && aligned(out, 16) && aligned(score_bias, 4) &&

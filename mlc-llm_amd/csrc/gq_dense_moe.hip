@@ -4,10 +4,9 @@
 //
 // The first routes (every workgroup all tokens for itself: a microsecond, where a launch of its own and its results' way through memory
 // are three) and streams the gate and up rows of the experts that some token chose past these experts' tokens.  A row of w h, the
-// weighted activation of one token and expert, goes to the workspace as two 16-bit numbers, the rounded value and what the rounding
-// left, so that the second product loses nothing to it.
-// The second streams the down rows past the same rows of w h; what comes out of an expert joins the sums of its tokens, which lie in LDS.  An
-// expert meets the tokens that chose it alone, whatever W or the other tokens hold.
+// weighted activation of one token and expert, goes to the workspace in float32.
+// The second streams the down rows past the same rows of w h, which go through the matrix instruction as two or three 16-bit planes (down_planes); what
+// comes out of an expert joins the sums of its tokens, which lie in LDS.  An expert meets the tokens that chose it alone, whatever W or the other tokens hold.
 // Bound by HBM.  Both kernels, us (of their bytes at 6.85 TB/s): one token, 6 of 64 experts of 2048 x 1408, 27.5 (15.2); 2 of 8 experts of 4096 x 14336,
 // 4 tokens 290 (283), 16 tokens 440 (411), 32 tokens 447 (411), 64 tokens 527 (411), where the way of x from the L2 counts beside W's; 16 tokens, 8
 // of 128 experts of 2048 x 768, 126 (114).  In memory that a process has given back and taken again all of these take 10 to 20 % more.
@@ -27,7 +26,7 @@ struct MoeSegment {
 // The workspace: what the first kernel leaves for the second.  Offsets; at 0 the number of segments, at kSegsAt these.
 constexpr int64_t kSegsAt = 256;
 struct MoeLayout {
-  int64_t row_token, tickets, shares, h, bytes;  // h: [2][T k][inter]
+  int64_t row_token, tickets, shares, h, bytes;  // h: float32 [T k][inter]
 };
 inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 inline int moe_shares(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k);
@@ -39,7 +38,7 @@ inline MoeLayout moe_layout(int64_t T, int64_t hidden, int64_t inter, int64_t ex
   l.shares = l.tickets + up256(tiles * 4);
   const int shares = moe_shares(T, hidden, inter, experts, k);
   l.h = l.shares + (shares > 1 ? up256(static_cast<int64_t>(shares) * tiles * T * 64) : 0);
-  l.bytes = l.h + up256(2 * slots * inter * 2);
+  l.bytes = l.h + up256(slots * inter * 4);
   return l;
 }
 // experts that some token chooses, where all are alike
@@ -220,13 +219,13 @@ __global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(
   const rsrc_t x = dense_buffer(a.x, a.T * pitch);
   auto place_of = [&](int round) {
     const Item it = item_of(round);
-    StreamPlace<XG, 1> p;
+    StreamPlace<XG> p;
     p.k = kw * kStreamBlock;
     p.end = it.there ? K : 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i)  // (inter is a multiple of 8)
       p.w[i] = dense_buffer(reinterpret_cast<const char*>(a.w13) + ((static_cast<int64_t>(it.e) * 2 + i) * I + it.n0) * pitch, 8 * pitch);
-    p.x[0] = x;
+    p.x = x;
 #pragma unroll
     for (int g = 0; g < XG; ++g) {
       const int c = 8 * g + (lane >> 3);
@@ -236,38 +235,28 @@ __global__ __launch_bounds__(kThreads, D == 2 ? 4 : 2) void dense_moe_up_kernel(
   };
   auto done = [&](int round, float4_t (&acc)[TT]) {
     if (KW > 1) {  // (two buffers in turn: one barrier a round)
-      stream_join(reinterpret_cast<float4_t*>(rest + kWaves * (NB > 0 ? D * kKeptStage : stream_ring<XG, 1, D>())) + (round & 1) * kWaves * TT * 64, wave, KW, acc);
+      stream_join(reinterpret_cast<float4_t*>(rest + kWaves * (NB > 0 ? D * kKeptStage : stream_ring<XG, D>())) + (round & 1) * kWaves * TT * 64, wave, KW, acc);
       if (kw != 0) return;
     }
     const Item it = item_of(round);
     const int n = it.n0 + 4 * (lane >> 4);
-    uint16_t* const h = reinterpret_cast<uint16_t*>(ws + layout.h);
+    float* const h = reinterpret_cast<float*>(ws + layout.h);
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
       const int c = 16 * t + (lane & 15);
       const float4_t g = acc[t], up = stream_up(g);
       if (!it.there || c >= it.rows || lane >= 32) continue;
       const int row = it.row0 + c;
-      const int64_t at = static_cast<int64_t>(row) * I + n;
       const float w = tab.row_w[row];
       float f[4] = {g[0], g[1], g[2], g[3]};
       dense_act<4>(f, a.act);
-      uint32_t hi[2], lo[2];
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const float f0 = w * (f[2 * v] * up[2 * v]), f1 = w * (f[2 * v + 1] * up[2 * v + 1]);
-        hi[v] = dense_pair<BF>(f0, f1);
-        const float r0 = dense_widen<BF>(hi[v] & 0xffffu), r1 = dense_widen<BF>(hi[v] >> 16);
-        auto left = [](float of, float rounded) { return __builtin_fabsf(rounded) <= 3.402823466e38f ? of - rounded : 0.f; };  // (nothing is left of an infinity)
-        lo[v] = dense_pair<BF>(left(f0, r0), left(f1, r1));
-      }
-      *reinterpret_cast<uint2*>(h + at) = uint2{hi[0], hi[1]};
-      *reinterpret_cast<uint2*>(h + static_cast<int64_t>(slots) * I + at) = uint2{lo[0], lo[1]};
+      *reinterpret_cast<float4_t*>(h + static_cast<int64_t>(row) * I + n) =
+          float4_t{w * (f[0] * up[0]), w * (f[1] * up[1]), w * (f[2] * up[2]), w * (f[3] * up[3])};
     }
   };
   __syncthreads();  // (the routing's part of LDS is the rings' now)
   if constexpr (NB == 0) {
-    dense_stream<BF, XG, D, false>(rest + wave * stream_ring<XG, 1, D>(), static_cast<uint32_t>(pitch), KW * kStreamBlock, nb, rounds, place_of, done);
+    dense_stream<BF, XG, D, false>(rest + wave * stream_ring<XG, D>(), static_cast<uint32_t>(pitch), KW * kStreamBlock, nb, rounds, place_of, done);
   } else {
     auto rows_of = [&](int round) {
       const Item it = item_of(round);
@@ -301,15 +290,62 @@ __device__ __forceinline__ void moe_store(uint16_t* to, const float4_t& v) {
   *reinterpret_cast<uint2*>(to) = uint2{dense_pair<BF>(v[0], v[1]), dense_pair<BF>(v[2], v[3])};
 }
 
-template <int XG, int C>
-constexpr int down_stage() { return C == 1 ? stream_stage<XG, 2>() : 2048 * C; }
+// Eight float32 numbers as 16-bit planes for the matrix instruction.
+// bfloat16: three planes, the upper 16 bits of what is left each time, which is all 24 bits of the number.
+// float16: two planes of v = scale f, a power of two times the number: v rounded, and what that left rounded.  Together they are off by at most 2^-23 of v, or
+// 2^-25 where that is more; a row's largest v is between 4 and 2^15, so that this is 2^-27 of it.  (float32, of which they take the place, has 2^-24 of v.)
+template <bool BF>
+struct DownPlanes {
+  int4_t v[BF ? 3 : 2];
+};
+template <bool BF>
+__device__ __forceinline__ DownPlanes<BF> down_planes(const float* f, float scale) {
+  DownPlanes<BF> p;
+  float minus = -1.f;
+  asm("" : "+s"(minus));  // (not folded into a subtraction, which would widen its float16 operand first)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a = f[2 * i], b = f[2 * i + 1];
+    if constexpr (BF) {
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        const uint32_t ua = __builtin_bit_cast(uint32_t, a), ub = __builtin_bit_cast(uint32_t, b);
+        p.v[j][i] = static_cast<int>(__builtin_amdgcn_perm(ub, ua, 0x07060302u));
+        if (j < 2) {
+          a -= __builtin_bit_cast(float, ua & 0xffff0000u);
+          b -= __builtin_bit_cast(float, ub & 0xffff0000u);
+        }
+      }
+    } else {
+      a *= scale;
+      b *= scale;
+      const uint32_t h = dense_pair<false>(a, b);
+      p.v[0][i] = static_cast<int>(h);
+      p.v[1][i] = static_cast<int>(dense_pair<false>(__builtin_fmaf(dense_widen<false>(h & 0xffffu), minus, a), __builtin_fmaf(dense_widen<false>(h >> 16), minus, b)));
+    }
+  }
+  return p;
+}
+// the largest over the four lanes of a row
+__device__ __forceinline__ float down_row_max(float v) {
+  auto larger = [](uint32_t x, uint32_t y) { return __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y))); };
+  uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto sixteens = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  u = larger(sixteens[0], sixteens[1]);
+  const auto halves = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, larger(halves[0], halves[1]));
+}
 
-// 16 C columns of the output for all tokens a workgroup; gridDim.y workgroups share the K, which is all segments' inter.  x comes through LDS beside W,
-// or, with C 2, straight into registers.
+template <int XG, int C>
+constexpr int down_stage() { return C == 1 ? 2048 + 2048 * XG : 2048 * C; }
+
+// 16 C columns of the output for all tokens a workgroup; gridDim.y workgroups share the K, which is all segments' inter.  The activations come through
+// LDS beside W, or, with C 2, straight into registers; as float32, of which the wave that multiplies makes 16-bit planes.
 template <bool BF, int XG, int D, int C>
 __global__ __launch_bounds__(kThreads, XG == 1 && C == 1 && D == 2 ? 4 : 2) void dense_moe_down_kernel(
     const void* __restrict__ from, const int* __restrict__ tokens, const uint16_t* __restrict__ w2, int T, int slots, int H, int I, DenseMoeArgs a,
     MoeLayout layout) {
+  static_assert(C == 2 || XG == 1, "eight rows a stage");
   constexpr int TT = (XG + 1) / 2, kStage = down_stage<XG, C>();
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
@@ -329,8 +365,9 @@ __global__ __launch_bounds__(kThreads, XG == 1 && C == 1 && D == 2 ? 4 : 2) void
   const int blocks = n_segs * per;
   const int begin = static_cast<int>(static_cast<int64_t>(blocks) * blockIdx.y / gridDim.y);
   const int end = static_cast<int>(static_cast<int64_t>(blocks) * (blockIdx.y + 1) / gridDim.y);
-  const int64_t pitch = static_cast<int64_t>(I) * 2, plane = slots * pitch;
-  const rsrc_t h_hi = dense_buffer(ws + layout.h, plane), h_lo = dense_buffer(ws + layout.h + plane, plane);
+  const uint32_t pitch = static_cast<uint32_t>(I) * 2u, h_pitch = 2u * pitch;  // (below 2^25)
+  const uint64_t expert = static_cast<uint64_t>(static_cast<uint32_t>(H)) * pitch;
+  const char* const w_first = reinterpret_cast<const char*>(w2) + static_cast<uint64_t>(static_cast<uint32_t>(n0)) * pitch;
 
   // this wave's blocks: every kWaves-th; (segment, block of it) of the next one to load, and of the one to compute
   struct At {
@@ -345,107 +382,192 @@ __global__ __launch_bounds__(kThreads, XG == 1 && C == 1 && D == 2 ? 4 : 2) void
     }
   };
   At ahead{begin + wave, (begin + wave) / per, (begin + wave) % per}, now = ahead;
-  int4_t x_of[C == 2 ? D : 1][2][2][TT];  // [stage][plane][half of a block][16 rows]
+  int4_t x_of[C == 2 ? D : 1][TT][2][2];  // [stage][16 rows][half of a block][four numbers]
+  MoeSegment coming = segs[ahead.b < end ? ahead.i : 0];  // of the next block to load, read ahead
   auto load = [&](int s) {
     const bool there = ahead.b < end;
-    const MoeSegment seg = segs[there ? ahead.i : 0];
-    const int64_t e = __builtin_amdgcn_readfirstlane(seg.e);
+    const uint32_t e = __builtin_amdgcn_readfirstlane(coming.e), row0 = __builtin_amdgcn_readfirstlane(coming.row0);
+    const int rows = __builtin_amdgcn_readfirstlane(coming.rows);
     rsrc_t w[2 * C];
 #pragma unroll
-    for (int i = 0; i < 2 * C; ++i) {
-      const int64_t left = H - n0 - 8 * i;
-      w[i] = dense_buffer(reinterpret_cast<const char*>(w2) + (e * H + n0 + 8 * i) * pitch, left > 0 ? 8 * pitch : 0);  // (hidden is a multiple of 8)
-    }
+    for (int i = 0; i < 2 * C; ++i)  // (hidden is a multiple of 8)
+      w[i] = dense_buffer(w_first + e * expert + static_cast<uint64_t>(8 * i) * pitch, H - n0 > 8 * i ? static_cast<int64_t>(8 * pitch) : 0);
+    const rsrc_t h = dense_buffer(ws + layout.h + static_cast<uint64_t>(row0) * h_pitch, static_cast<int64_t>(static_cast<uint32_t>(rows) * h_pitch));
     const int k = ahead.kb * kStreamBlock, last = there ? I : 0;
+    const int kc = k + 8 * ((lane & 7) ^ (lane >> 3));
+    const uint32_t w_at = kc < last ? static_cast<uint32_t>(lane >> 3) * pitch + 2u * kc : kNowhere;
+#pragma unroll
+    for (int i = 0; i < 2 * C; ++i) dense_to_lds<true>(w[i], w_at, ring + s * kStage + 1024 * i);
+    asm volatile("" ::: "memory");  // (in this order)
     if constexpr (C == 1) {
-      StreamPlace<XG, 2> p;
-      p.end = last;
-      p.w[0] = w[0];
-      p.w[1] = w[1];
-      p.x[0] = h_hi;
-      p.x[1] = h_lo;
+      // four rows of 256 bytes an instruction, chunk c of four numbers of a row at place c ^ (row & 7)
 #pragma unroll
-      for (int g = 0; g < XG; ++g) {
-        const int c = 8 * g + (lane >> 3);
-        p.x_at[g] = c < seg.rows ? static_cast<uint32_t>(seg.row0 + c) * static_cast<uint32_t>(pitch) : kNowhere;
+      for (int i = 0; i < 2; ++i) {
+        const int row = 4 * i + quad, at_k = k + 4 * ((lane & 15) ^ row);
+        const uint32_t at = row < rows && at_k < last ? static_cast<uint32_t>(row) * h_pitch + 4u * at_k : kNowhere;
+        dense_to_lds<false>(h, at, ring + s * kStage + 2048 + 1024 * i);
       }
-      stream_load(p, k, static_cast<uint32_t>(pitch), ring + s * kStage);
     } else {
-      const int kc = k + 8 * ((lane & 7) ^ (lane >> 3));
-      const uint32_t w_at = kc < last ? static_cast<uint32_t>(lane >> 3) * static_cast<uint32_t>(pitch) + 2u * kc : kNowhere;
-#pragma unroll
-      for (int i = 0; i < 2 * C; ++i) dense_to_lds<true>(w[i], w_at, ring + s * kStage + 1024 * i);
-      asm volatile("" ::: "memory");  // (in this order)
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
         const int c = 16 * t + (lane & 15);
-        const uint32_t row = static_cast<uint32_t>(seg.row0 + c) * static_cast<uint32_t>(pitch);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int at_k = k + 32 * i + 8 * quad;
-          const uint32_t at = c < seg.rows && at_k < last ? row + 2u * at_k : kNowhere;
-          x_of[s][0][i][t] = __builtin_bit_cast(int4_t, __builtin_amdgcn_raw_buffer_load_b128(h_hi, at, 0, 0));
-          x_of[s][1][i][t] = __builtin_bit_cast(int4_t, __builtin_amdgcn_raw_buffer_load_b128(h_lo, at, 0, 0));
+          const uint32_t at = c < rows && at_k < last ? static_cast<uint32_t>(c) * h_pitch + 4u * at_k : kNowhere;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) x_of[s][t][i][j] = __builtin_bit_cast(int4_t, __builtin_amdgcn_raw_buffer_load_b128(h, at + 16u * j, 0, 0));
         }
       }
-      asm volatile("" ::: "memory");
     }
+    asm volatile("" ::: "memory");
     next(ahead);
+    coming = segs[ahead.b < end ? ahead.i : 0];
   };
-  float4_t acc[C][TT];
+  // Sums of the first planes, and of the others: where the first ones' are infinite or NaN, they are the result, and the others', in which an infinity meets
+  // zeros and numbers of the other sign, are nothing.
+  // C 1: eight rows of x are columns 0 to 7 of the operand with the first half of a block's K and columns 8 to 15 with the second.  The sums of W's first
+  // half have the results in columns 0 to 7, those of W's second half in columns 8 to 15, and half the numbers go through down_planes.
+  constexpr int NF = C == 1 ? 8 : 16;  // numbers of a lane in a block
+  float4_t acc[2][TT], left[2][TT];    // C 1: halves of K, C 2: of the columns
+  // float16: the scale of this lane's row of each 16, 2^scale_log2; it starts where it may well stay
+  constexpr int kScaleStart = 12, kScaleMost = 126;
+  constexpr float kSmallest = 4.f, kLargest = 0x1p15f;
+  int scale_log2[TT];
+  float scale[TT], small[TT];  // small: kSmallest, or 0 once the lane has met a number other than 0
+  auto clear = [&] {
 #pragma unroll
-  for (int u = 0; u < C; ++u)
+    for (int t = 0; t < TT; ++t) {
+      scale_log2[t] = kScaleStart;
+      scale[t] = static_cast<float>(1 << kScaleStart);
+      small[t] = kSmallest;
 #pragma unroll
-    for (int t = 0; t < TT; ++t) acc[u][t] = float4_t{};
-  auto join = [&](int i) {  // a segment's sums go to its tokens'
+      for (int u = 0; u < 2; ++u) acc[u][t] = left[u][t] = float4_t{};
+    }
+  };
+  clear();
+  // Moves the scale of the rows, and their sums with it, where a block has numbers that it would bring past kLargest, or none above kSmallest in the first block
+  // that is not all zeros.
+  auto fit = [&](int t, const float (&f)[NF]) {
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < NF; ++i) most = fmaxf(most, __builtin_fabsf(f[i]));
+    const float v = most * scale[t], was = small[t];
+    small[t] = most > 0.f ? 0.f : was;
+    if (__any(v >= kLargest || (v < was && most > 0.f)) == 0) return;
+    asm volatile("");  // (a branch: few blocks come here)
+    if (__any(most == __builtin_inff())) {  // the largest finite one
+      most = 0.f;
+#pragma unroll
+      for (int i = 0; i < NF; ++i) {
+        const float v = __builtin_fabsf(f[i]);
+        most = v < __builtin_inff() ? fmaxf(most, v) : most;
+      }
+    }
+    most = down_row_max(most);
+    const bool first = down_row_max(was == 0.f ? 1.f : 0.f) == 0.f;
+    const bool move = most * scale[t] >= kLargest || (first && most > 0.f && most * scale[t] < kSmallest);
+    const int fitting = 13 - __builtin_amdgcn_frexp_expf(most);  // to 2^12 to 2^13: there is room above
+    const int to = !move ? scale_log2[t] : fitting < kScaleMost ? fitting : kScaleMost, by = to - scale_log2[t];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        acc[u][t][v] = __builtin_amdgcn_ldexpf(acc[u][t][v], by);
+        left[u][t][v] = __builtin_amdgcn_ldexpf(left[u][t][v], by);
+      }
+    scale_log2[t] = to;
+    scale[t] = __builtin_amdgcn_ldexpf(1.f, to);
+  };
+  int token[TT];  // of this lane's row of the segment in hand, -1: none
+  auto take = [&](int i) {
     const MoeSegment seg = segs[i];
 #pragma unroll
-    for (int u = 0; u < C; ++u)
+    for (int t = 0; t < TT; ++t) {
+      const int c = 16 * t + (lane & 15);
+      token[t] = c < seg.rows ? row_token[seg.row0 + c] : -1;
+    }
+  };
+  auto join = [&] {  // the segment's sums go to its tokens'
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        const int c = 16 * t + (lane & 15);
-        if (c < seg.rows) sums[(wave * T + row_token[seg.row0 + c]) * 4 * C + 4 * u + quad] += acc[u][t];
-        acc[u][t] = float4_t{};
-      }
+    for (int t = 0; t < TT; ++t) {
+      float4_t v[C];
+#pragma unroll
+      for (int u = 0; u < C; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool second = C == 1 && (lane & 8) != 0;  // this lane's half of K
+          const float first = second ? acc[1][t][j] : acc[u][t][j], others = second ? left[1][t][j] : left[u][t][j];
+          float sum = __builtin_fabsf(first) < __builtin_inff() ? first + others : first;
+          if constexpr (!BF) sum = __builtin_amdgcn_ldexpf(sum, -scale_log2[t]);
+          if constexpr (C == 1) {
+            const int bits = __builtin_bit_cast(int, sum);
+            sum += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, bits, 0x128, 0xf, 0xf, false));  // row_ror:8
+          }
+          v[u][j] = sum;
+        }
+      if (token[t] >= 0)
+#pragma unroll
+        for (int u = 0; u < C; ++u) sums[(wave * T + token[t]) * 4 * C + 4 * u + quad] += v[u];
+    }
+    clear();
   };
 #pragma unroll
   for (int s = 0; s < D; ++s) load(s);
   int current = now.i;
+  if (now.b < end) take(current);
   while (now.b < end) {
 #pragma unroll
     for (int s = 0; s < D; ++s) {
-      if (now.b < end && now.i != current) {
-        join(current);
-        current = now.i;
-      }
-      // (past the end: zeros)
-      if constexpr (C == 1) {
-        stream_wait<XG, 2, D>();
-        stream_block<BF, XG, 2>(ring + s * kStage, acc[0]);
-      } else {
-        constexpr int kLoads = 2 * C + 4 * TT;
-        static_assert((D - 1) * kLoads < 64, "the counter of loads");
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * kLoads) : "memory");
-        const int row = lane & 15;
+      const int segment = now.b < end ? now.i : current;  // (past the end: zeros)
+      constexpr int kLoads = C == 1 ? 4 : 2 * C + 4 * TT;
+      static_assert((D - 1) * kLoads < 64, "the counter of loads");
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * kLoads) : "memory");
+      const uint8_t* const stage = ring + s * kStage;
+      const int row = lane & 15;
+      int4_t w[C][2];
 #pragma unroll
-        for (int u = 0; u < C; ++u) {
-          int4_t w[2];
+      for (int u = 0; u < C; ++u)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) w[i] = *reinterpret_cast<const int4_t*>(ring + s * kStage + 2048 * u + row * 128 + (((quad + 4 * i) ^ (row & 7)) << 4));
+        for (int i = 0; i < 2; ++i) w[u][i] = *reinterpret_cast<const int4_t*>(stage + 2048 * u + row * 128 + (((quad + 4 * i) ^ (row & 7)) << 4));
+      float f[TT][NF];
 #pragma unroll
-          for (int p = 0; p < 2; ++p)
+      for (int t = 0; t < TT; ++t)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < NF / 4; ++j) {
+          float4_t v;
+          if constexpr (C == 1) v = *reinterpret_cast<const float4_t*>(stage + 2048 + (row & 7) * 256 + (((row & 8) + ((2 * quad + j) ^ (row & 7))) << 4));
+          else v = __builtin_bit_cast(float4_t, x_of[s][t][j / 2][j % 2]);
 #pragma unroll
-              for (int t = 0; t < TT; ++t) acc[u][t] = dense_mfma<BF>(w[i], x_of[s][p][i][t], acc[u][t]);
+          for (int n = 0; n < 4; ++n) f[t][4 * j + n] = v[n];
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read, before the stage is loaded again)
-      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read, before the stage is loaded again)
       next(now);
-      load(s);
+      load(s);  // (in front of the arithmetic, so that it has this time as well)
+      if (segment != current) {
+        join();
+        take(segment);
+        current = segment;
+      }
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        if constexpr (!BF) fit(t, f[t]);
+#pragma unroll
+        for (int i = 0; i < NF / 8; ++i) {
+          const DownPlanes<BF> p = down_planes<BF>(f[t] + 8 * i, scale[t]);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int4_t& m = C == 1 ? w[0][u] : w[C - 1 < u ? 0 : u][i];
+            acc[u][t] = dense_mfma<BF>(m, p.v[0], acc[u][t]);
+            left[u][t] = dense_mfma<BF>(m, p.v[1], left[u][t]);
+            if constexpr (BF) left[u][t] = dense_mfma<BF>(m, p.v[2], left[u][t]);
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);  // (and none of it behind the next wait)
     }
   }
-  if (begin + wave < end) join(current);
+  if (begin + wave < end) join();
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 
@@ -498,7 +620,7 @@ static hipError_t launch_up(const DenseMoeArgs& a, const MoeLayout& layout, int 
   const int nw = NB > 0 ? 1 : kWaves >> plan.kw_log2;
   const int64_t sets = (most + nw - 1) / nw;
   const size_t tables = moe_tables_bytes(a.experts, slots), gate = kWaves * sizeof(GateScratch<NC>);
-  const size_t rings = kWaves * ((NB > 0 ? D * kKeptStage : stream_ring<XG, 1, D>()) + 2 * ((XG + 1) / 2) * 1024), lds = tables + (rings > gate ? rings : gate);
+  const size_t rings = kWaves * ((NB > 0 ? D * kKeptStage : stream_ring<XG, D>()) + 2 * ((XG + 1) / 2) * 1024), lds = tables + (rings > gate ? rings : gate);
   if (lds > 160 * 1024) return hipErrorNotSupported;
   auto* kern = dense_moe_up_kernel<BF, NC, XG, D, NB>;
   const hipError_t e = may_use(kern, lds);

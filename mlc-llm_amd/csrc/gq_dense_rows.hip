@@ -22,9 +22,9 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void dense_rows_kernel(
   const int KW = 1 << kw_log2, kw = wave & (KW - 1), nw = wave >> kw_log2;
   const int64_t pitch = static_cast<int64_t>(K) * 2, cols = cols_, stride = static_cast<int64_t>(gridDim.x) * (kStreamWaves >> kw_log2);
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (kStreamWaves >> kw_log2) + nw;
-  uint8_t* const ring = smem + wave * stream_ring<XG, 1, kDepth>();
+  uint8_t* const ring = smem + wave * stream_ring<XG, kDepth>();
   auto place_of = [&](int round) {
-    StreamPlace<XG, 1> p;
+    StreamPlace<XG> p;
     p.k = kw * kStreamBlock;
     const int64_t n0 = (round * stride + first) * kCols;
     p.end = round < rounds && n0 < cols ? K : 0;
@@ -33,7 +33,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void dense_rows_kernel(
       const int64_t left = GATED ? cols - n0 : cols - n0 - 8 * i, count = p.end == 0 || left < 0 ? 0 : left < 8 ? left : 8;
       p.w[i] = dense_buffer(reinterpret_cast<const char*>(w) + (n0 + i * (GATED ? cols : 8)) * pitch, count * pitch);
     }
-    p.x[0] = dense_buffer(x, rows * pitch);
+    p.x = dense_buffer(x, rows * pitch);
 #pragma unroll
     for (int g = 0; g < XG; ++g) {
       const int r = 8 * g + (lane >> 3);
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void dense_rows_kernel(
   auto done = [&](int round, float4_t (&acc)[TT]) {
     if (KW > 1) {
       // (two buffers in turn: one barrier a round)
-      stream_join(reinterpret_cast<float4_t*>(smem + kStreamWaves * stream_ring<XG, 1, kDepth>()) + (round & 1) * kStreamWaves * TT * 64, wave, KW, acc);
+      stream_join(reinterpret_cast<float4_t*>(smem + kStreamWaves * stream_ring<XG, kDepth>()) + (round & 1) * kStreamWaves * TT * 64, wave, KW, acc);
       if (kw != 0) return;
     }
     const int64_t n = (round * stride + first) * kCols + 4 * (lane >> 4);
@@ -65,7 +65,7 @@ static hipError_t launch(const DenseArgs& a, hipStream_t s) {
   const StreamPlan plan = stream_plan(static_cast<double>(items), a.K, kDepth, true);
   const int nw = kStreamWaves >> plan.kw_log2;
   const int64_t sets = (items + nw - 1) / nw;
-  constexpr size_t lds = kStreamWaves * (stream_ring<XG, 1, kDepth>() + 2 * ((XG + 1) / 2) * 1024);
+  constexpr size_t lds = kStreamWaves * (stream_ring<XG, kDepth>() + 2 * ((XG + 1) / 2) * 1024);
   static_assert(lds <= 160 * 1024, "LDS of a unit");
   auto* kern = plan.nb % kDepth == 0 ? dense_rows_kernel<BF, GATED, XG, false> : dense_rows_kernel<BF, GATED, XG, true>;
   const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kern));

@@ -29,59 +29,53 @@ __device__ __forceinline__ void dense_to_lds(rsrc_t r, uint32_t at, uint8_t* lds
 }
 
 // What a wave works on: twice eight rows of W, each from the start of its buffer (which ends behind the last row that is there: the
-// others read as zeros), and XG times eight rows of x, in PX planes whose products add up.
-template <int XG, int PX>
+// others read as zeros), and XG times eight rows of x.
+template <int XG>
 struct StreamPlace {
   rsrc_t w[2];
-  rsrc_t x[PX];
+  rsrc_t x;
   uint32_t x_at[XG];  // byte offset of this lane's row of x, row lane / 8 of eight
   int k, end;         // this wave's first number of K and the end of K in a row (0: nothing to do)
 };
 
-template <int XG, int PX>
-constexpr int stream_stage() { return 2048 + PX * XG * 1024; }
-template <int XG, int PX, int D>
-constexpr int stream_ring() { return D * stream_stage<XG, PX>(); }
+template <int XG>
+constexpr int stream_stage() { return 2048 + XG * 1024; }
+template <int XG, int D>
+constexpr int stream_ring() { return D * stream_stage<XG>(); }
 
 // One block from number k of the rows on, into a stage.  Chunk c of 16 bytes of a row lies at place c ^ (row & 7), so that the 16 lanes that LDS
 // serves at a time meet all its banks.
-template <int XG, int PX>
-__device__ __forceinline__ void stream_load(const StreamPlace<XG, PX>& p, int k, uint32_t w_pitch, uint8_t* stage) {
+template <int XG>
+__device__ __forceinline__ void stream_load(const StreamPlace<XG>& p, int k, uint32_t w_pitch, uint8_t* stage) {
   const int lane = threadIdx.x & 63, kc = k + 8 * ((lane & 7) ^ (lane >> 3));  // a chunk of 8; K is a multiple of 8
   const bool in = kc < p.end;
   const uint32_t w_at = in ? static_cast<uint32_t>(lane >> 3) * w_pitch + 2u * kc : kNowhere;
 #pragma unroll
   for (int i = 0; i < 2; ++i) dense_to_lds<true>(p.w[i], w_at, stage + 1024 * i);
 #pragma unroll
-  for (int g = 0; g < XG; ++g) {
-    const uint32_t at = in ? p.x_at[g] + 2u * kc : kNowhere;
-#pragma unroll
-    for (int i = 0; i < PX; ++i) dense_to_lds<false>(p.x[i], at, stage + 2048 + (i * XG + g) * 1024);
-  }
+  for (int g = 0; g < XG; ++g) dense_to_lds<false>(p.x, in ? p.x_at[g] + 2u * kc : kNowhere, stage + 2048 + g * 1024);
   asm volatile("" ::: "memory");  // (before the next block's, by which the wait counts)
 }
 // Waits until all but the newest D - 1 blocks have landed.
-template <int XG, int PX, int D>
+template <int XG, int D>
 __device__ __forceinline__ void stream_wait() {
-  static_assert((D - 1) * (2 + PX * XG) < 64, "the counter of loads");
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * (2 + PX * XG)) : "memory");
+  static_assert((D - 1) * (2 + XG) < 64, "the counter of loads");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * (2 + XG)) : "memory");
 }
 // sums += the block in a stage; the lane holds row 16 t + lane % 16 of x and rows 4 (lane / 16) .. + 3 of W.
-template <bool BF, int XG, int PX>
+template <bool BF, int XG>
 __device__ __forceinline__ void stream_block(const uint8_t* stage, float4_t (&acc)[(XG + 1) / 2]) {
   constexpr int TT = (XG + 1) / 2;
   const int lane = threadIdx.x & 63, quad = lane >> 4, row = lane & 15;
   const int c0 = (quad ^ (row & 7)) << 4, c1 = ((quad + 4) ^ (row & 7)) << 4;
   const int4_t w0 = *reinterpret_cast<const int4_t*>(stage + row * 128 + c0), w1 = *reinterpret_cast<const int4_t*>(stage + row * 128 + c1);
 #pragma unroll
-  for (int i = 0; i < PX; ++i)
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      // (eight rows of x: rows 8 to 15 of the operand are those again, and their sums nobody's)
-      const uint8_t* const x = stage + 2048 + i * XG * 1024 + (XG == 1 ? row & 7 : 16 * t + row) * 128;
-      acc[t] = dense_mfma<BF>(w0, *reinterpret_cast<const int4_t*>(x + c0), acc[t]);
-      acc[t] = dense_mfma<BF>(w1, *reinterpret_cast<const int4_t*>(x + c1), acc[t]);
-    }
+  for (int t = 0; t < TT; ++t) {
+    // (eight rows of x: rows 8 to 15 of the operand are those again, and their sums nobody's)
+    const uint8_t* const x = stage + 2048 + (XG == 1 ? row & 7 : 16 * t + row) * 128;
+    acc[t] = dense_mfma<BF>(w0, *reinterpret_cast<const int4_t*>(x + c0), acc[t]);
+    acc[t] = dense_mfma<BF>(w1, *reinterpret_cast<const int4_t*>(x + c1), acc[t]);
+  }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read, before the stage is loaded again)
 }
 
@@ -91,8 +85,8 @@ __device__ __forceinline__ void stream_block(const uint8_t* stage, float4_t (&ac
 // padded to eight).
 template <bool BF, int XG, int D, bool ANY, class PlaceOf, class Done>
 __device__ __forceinline__ void dense_stream(uint8_t* ring, uint32_t w_pitch, int step, int nb, int rounds, PlaceOf place_of, Done done) {
-  constexpr int TT = (XG + 1) / 2, kStage = stream_stage<XG, 1>();
-  StreamPlace<XG, 1> here = place_of(0);
+  constexpr int TT = (XG + 1) / 2, kStage = stream_stage<XG>();
+  StreamPlace<XG> here = place_of(0);
   float4_t acc[TT];
   auto clear = [&] {
 #pragma unroll
@@ -106,16 +100,16 @@ __device__ __forceinline__ void dense_stream(uint8_t* ring, uint32_t w_pitch, in
       for (int j = D; j < nb; j += D) {
 #pragma unroll
         for (int s = 0; s < D; ++s) {
-          stream_wait<XG, 1, D>();
-          stream_block<BF, XG, 1>(ring + s * kStage, acc);
+          stream_wait<XG, D>();
+          stream_block<BF, XG>(ring + s * kStage, acc);
           stream_load(here, here.k + (j + s) * step, w_pitch, ring + s * kStage);
         }
       }
       here = place_of(round + 1);
 #pragma unroll
       for (int s = 0; s < D; ++s) {
-        stream_wait<XG, 1, D>();
-        stream_block<BF, XG, 1>(ring + s * kStage, acc);
+        stream_wait<XG, D>();
+        stream_block<BF, XG>(ring + s * kStage, acc);
         stream_load(here, here.k + s * step, w_pitch, ring + s * kStage);
       }
       done(round, acc);
@@ -136,8 +130,8 @@ __device__ __forceinline__ void dense_stream(uint8_t* ring, uint32_t w_pitch, in
       clear();
 #pragma unroll 1
       for (int j = 0; j < nb; ++j) {
-        stream_wait<XG, 1, D>();
-        stream_block<BF, XG, 1>(stage, acc);
+        stream_wait<XG, D>();
+        stream_block<BF, XG>(stage, acc);
         load(stage);
         stage = stage == ring + (D - 1) * kStage ? ring : stage + kStage;
       }

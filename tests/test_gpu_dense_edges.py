@@ -1,0 +1,123 @@
+"""The expert layer on 16-bit weights where its activation needs all of float32: sums that are known exactly, in float32 too."""
+
+import math
+
+import pytest
+import torch
+
+import mlc_llm_amd as gq
+from mlc_llm_amd import ops
+
+HALVES = [torch.float16, torch.bfloat16]
+pytestmark = pytest.mark.gpu
+
+
+def _ints(g, most, *shape):
+    return torch.randint(-most, most + 1, shape, generator=g).double()
+
+
+def _pow2(exponents):
+    return 2.0 ** torch.as_tensor(exponents, dtype=torch.float64)
+
+
+# Whole numbers times powers of two.  x has 48 numbers other than 0 in a row, of at most 8, as W13's: a gate or an up value is at most 48 * 64 = 3072 units, most
+# are below 1000, and their product takes up to 23 bits.  Experts of equal logits weigh 1, 1/2 or 1/4.  A row of W2 has four numbers other than 0, so that all sums of
+# products stay below 2^24 units (asserted below) and are exact in float32, in any order.  The one rounding is the output's.
+def _layer(g, dtype, t, hidden, inter, experts, k, x_exp, gate_exp, up_exp, w2_exp, without=()):
+    """x_exp: [t] exponents; gate_exp, up_exp: [inter]; w2_exp: [inter], of the numbers that the columns of W2 hold; without: activations that are 0."""
+    x = torch.zeros(t, hidden, dtype=torch.float64)
+    count = min(48, hidden)
+    at = torch.stack([torch.randperm(hidden, generator=g)[:count] for _ in range(t)])
+    x.scatter_(1, at, _ints(g, 8, t, count))
+    unit = _pow2(x_exp)[:, None]
+    w13 = _ints(g, 8, experts, 2 * inter, hidden)
+    w13[:, list(without)] = 0
+    w2 = torch.zeros(experts, hidden, inter, dtype=torch.float64)
+    # the four columns of a row are of one block of 64, in all experts the same block
+    blocks = (inter + 63) // 64
+    first = 64 * torch.randint(0, blocks, (1, hidden, 1), generator=g)
+    column = (first + torch.randint(0, 64, (experts, hidden, 4), generator=g)).clamp(max=inter - 1)
+    sign = 2.0 * torch.randint(0, 2, (experts, hidden, 4), generator=g).double() - 1
+    w2.scatter_(2, column, sign)
+    logits = torch.full((t, experts), -60.0)
+    ids = torch.stack([torch.randperm(experts, generator=g)[:k] for _ in range(t)])
+    logits.scatter_(1, ids, 30.0)
+    y, size = torch.zeros(t, hidden, dtype=torch.float64), torch.zeros(t, hidden, dtype=torch.float64)
+    scale = _pow2(gate_exp) + 0 * _pow2(up_exp)
+    for e in range(experts):
+        rows = (ids == e).any(1)
+        gate, up = (x[rows] @ w13[e].t()).chunk(2, 1)
+        h = gate * up
+        w = w2[e] * (scale * _pow2(up_exp) * _pow2(w2_exp))
+        y[rows] += h @ w.t() / k
+        size[rows] += h.abs() @ w2[e].abs().t() / k
+    assert size.max() * k < 2**24
+    y = y * unit * unit
+    w13 = w13 * torch.cat([_pow2(gate_exp), _pow2(up_exp)])[:, None]
+    w2 = w2 * _pow2(w2_exp)
+    assert y.abs().max() < torch.finfo(dtype).max
+    for of in (x * unit, w13, w2):
+        assert torch.equal(of.to(dtype).double(), of)
+    return ((x * unit).to(dtype).cuda(), logits.cuda(), w13.to(dtype).cuda(), w2.to(dtype).cuda()), y.float().to(dtype).cuda()
+
+
+# (tokens, hidden, inter, experts, top_k, end of the kernel's note): eight rows a segment through LDS, sixteen and 32 in registers, x kept in the first
+# kernel and not, one and several shares
+LAYERS = [(1, 2048, 1408, 16, 4, "up to 8 rows"), (3, 64, 72, 4, 1, "up to 8 rows"), (8, 520, 200, 9, 2, "up to 8 rows"), (16, 1032, 264, 20, 4, "up to 8 rows"),
+          (12, 264, 328, 2, 2, "up to 16 rows"), (40, 136, 1032, 6, 2, "up to 16 rows"), (40, 2048, 1024, 8, 2, "up to 16 rows"),
+          (64, 2048, 1032, 4, 2, "up to 32 rows")]
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t,hidden,inter,experts,k,note", LAYERS)
+def test_activation_is_held_in_float32(t, hidden, inter, experts, k, note, dtype):
+    """Products of 23 bits that cancel, of sizes that a 16-bit type does not hold or hardly: large and small tokens, magnitudes that rise and fall along K."""
+    g = torch.Generator().manual_seed(t + hidden + inter)
+    flat, steps = torch.zeros(inter), (torch.arange(inter) // 64).double()
+    rise = torch.floor(steps * (12 / max(1.0, steps.max().item())))
+    tokens = torch.arange(t) % 5
+    if dtype == torch.float16:
+        # activations beyond float16's largest number, by 2^2 and 2^8; in units of 2^-40, below its smallest; of many sizes
+        scales = [(torch.zeros(t), flat, flat, flat - 12), (torch.zeros(t), flat + 3, flat + 3, flat - 14), (tokens - 10, flat - 10, flat - 10, flat + 12),
+                  (torch.zeros(t), rise - 10, flat, -rise + 2), (torch.zeros(t), -rise + 2, flat, rise - 14)]
+    else:
+        scales = [(torch.zeros(t), flat, flat, flat), (tokens + 40, flat, flat + 10, flat - 60), (tokens - 30, flat - 20, flat - 20, flat + 60),
+                  (tokens, rise - 10, flat, -rise + 2), (tokens, -rise + 2, flat, rise - 14)]
+    scales.append((*scales[2], [n for n in range(inter) if n // 64 < 9 or n % 64 < 16]))  # small ones behind zeros
+    for i, exps in enumerate(scales):
+        args, want = _layer(g, dtype, t, hidden, inter, experts, k, *exps)
+        got = ops.dense_moe(*args, k, activation=None)
+        assert note in gq._lib.last_kernel()
+        assert torch.equal(got, want), (i, (got != want).sum().item(), got.numel())
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t,experts", [(2, 4), (24, 3), (60, 2)])
+def test_infinities_of_the_second_product(t, experts, dtype):
+    """An infinity among w2's numbers, or an activation beyond float32, gives what the formula gives: an infinity of its sign, and NaN where infinities of
+    both signs or an infinity and a zero meet."""
+    hidden, inter = 64, 1032
+    x = torch.zeros(t, hidden, dtype=dtype, device="cuda")
+    x[:, 0], x[:, 1] = 3.0, 1.0
+    w13 = torch.zeros(experts, 2 * inter, hidden, dtype=dtype, device="cuda")
+    w13[:, :, 0], w13[:, :, 1] = 1 / 3, 2.0**-10  # activations near 1 with many bits
+    w2 = torch.ones(experts, hidden, inter, dtype=dtype, device="cuda")
+    logits = torch.full((t, experts), -50.0, device="cuda")
+    logits[:, 1] = 50.0
+    plain = ops.dense_moe(x, logits, w13, w2, 1, activation=None)
+    assert plain.isfinite().all()
+    w2[1, 1, 5], w2[1, 2, 70], w2[1, 3, 5], w2[1, 3, 6] = math.inf, -math.inf, math.inf, -math.inf
+    w2[0] = math.nan  # (nobody's)
+    got = ops.dense_moe(x, logits, w13, w2, 1, activation=None)
+    assert (got[:, 1] == math.inf).all() and (got[:, 2] == -math.inf).all() and got[:, 3].isnan().all()
+    others = [n for n in range(hidden) if n not in (1, 2, 3)]
+    assert torch.equal(got[:, others], plain[:, others])
+    w2[1] = 0.5
+    w2[1, 7], w2[1, 9, 130] = -0.25, 0.0
+    if dtype == torch.bfloat16:
+        w13[1, 130, 0] = w13[1, inter + 130, 0] = 2.0**100  # 9 * 2^200
+    else:
+        w13[1, 130, 0] = math.inf
+    got = ops.dense_moe(x, logits, w13, w2, 1, activation=None)
+    others = [n for n in range(hidden) if n not in (7, 9)]
+    assert (got[:, 7] == -math.inf).all() and got[:, 9].isnan().all() and (got[:, others] == math.inf).all()
