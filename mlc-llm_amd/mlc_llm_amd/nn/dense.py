@@ -96,6 +96,8 @@ class DenseMoE(nn.Module):
     def forward(self, x: torch.Tensor, gate: torch.Tensor) -> torch.Tensor:
         """x [..., hidden]; gate [tokens, num_local_experts] router logits."""
         tokens = x.reshape(-1, x.shape[-1]).contiguous()
+        if isinstance(gate, torch.Tensor) and tuple(gate.shape) != (len(tokens), self.num_local_experts):  # (a run of it would hide further rows)
+            raise ValueError(f"gate {tuple(gate.shape)} for {len(tokens)} tokens of {self.num_local_experts} experts")
         most = ops.DENSE_MOE_TOKENS
         parts = [(tokens[i : i + most], gate[i : i + most]) for i in range(0, max(len(tokens), 1), most)]
         out = [ops.dense_moe(t, g, self.e1_e3.weight, self.e2.weight, self.num_experts_per_tok, activation=self.activation,

@@ -60,3 +60,14 @@ def test_expert_layer_of_any_number_of_tokens(tokens):
         part = ops.dense_moe(x[0, i : i + 64], gate[i : i + 64], moe.e1_e3.weight, moe.e2.weight, 3, scoring="sigmoid", bias=moe.score_bias,
                              num_groups=4, top_groups=2, scale=2.0)
         assert torch.equal(y[0, i : i + 64], part)
+
+
+@pytest.mark.parametrize("shape", [(70, 4), (128, 4), (63, 4), (0, 4), (64,), (1, 64, 4), (64, 5)])
+@pytest.mark.parametrize("tokens", [0, 64, 128])
+def test_expert_layer_wants_a_row_of_logits_a_token(tokens, shape):
+    """Rows of logits that no token goes with are refused, whatever runs the layer cuts its tokens into."""
+    moe = layers.DenseMoE(8, 8, 4, 2)
+    if shape == (tokens, 4):
+        return
+    with pytest.raises(ValueError, match=rf"gate \({', '.join(map(str, shape))},?\) for {tokens} tokens of 4 experts"):
+        moe(torch.zeros(tokens, 8, dtype=torch.float16), torch.zeros(shape))
