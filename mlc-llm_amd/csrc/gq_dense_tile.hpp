@@ -320,7 +320,8 @@ hipError_t launch_tile(const DenseArgs& a, const DensePlan& plan, int part, hipS
     const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kern));
     if (e != hipSuccess) return e;
   }
-  note_kernel("dense_tile %dx%d%s, %d shares of K", BN * P, BM, GATED ? " gated" : "", splits);
+  if (part == 0) note_kernel("dense_tile %dx%d%s, %d shares of K", BN * P, BM, GATED ? " gated" : "", splits);
+  else note_kernel("dense_tile %dx%d%s, %d shares of K, rows of W from %lld on", BN * P, BM, GATED ? " gated" : "", splits, static_cast<long long>(plan.n_rest));
   const int64_t most = (0xffffffffll / (64 * kWaves) - 8) / (m_tiles * splits);  // columns of tiles a launch, likewise
   if (most < 1) return hipErrorNotSupported;
   for (int64_t t0 = 0; t0 < n_tiles; t0 += most) {

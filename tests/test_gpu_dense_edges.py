@@ -7,6 +7,7 @@ import torch
 
 import mlc_llm_amd as gq
 from mlc_llm_amd import ops
+from test_gpu_dense import close, gated_ref, linear_ref
 
 HALVES = [torch.float16, torch.bfloat16]
 pytestmark = pytest.mark.gpu
@@ -121,3 +122,37 @@ def test_infinities_of_the_second_product(t, experts, dtype):
     got = ops.dense_moe(x, logits, w13, w2, 1, activation=None)
     others = [n for n in range(hidden) if n not in (7, 9)]
     assert (got[:, 7] == -math.inf).all() and got[:, 9].isnan().all() and (got[:, others] == math.inf).all()
+
+
+# (rows of x, rows of W, K): tiles of the last round that another form takes, after whole rounds of 256 x 256 and 256 x 160 ones; columns and K that end inside tiles,
+# W's rows from which the other form works in the middle of both halves of a gated one
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("m,n,k", [(2048, 9002, 264), (2048, 9008, 520), (1030, 14504, 520), (777, 28674, 520), (2000, 28676, 1032), (200, 66008, 264)])
+def test_columns_that_another_form_takes(m, n, k, dtype):
+    g = torch.Generator(device="cuda").manual_seed(n + k)
+    x, w = (torch.randn(r, k, generator=g, device="cuda") for r in (m, n))
+    x, w = x.to(dtype), (w / k**0.5).to(dtype)
+    bias = torch.randn(n, generator=g, device="cuda").to(dtype)
+    residual = torch.randn(m, n, generator=g, device="cuda").to(dtype)
+    close(ops.dense_linear(x, w, bias, "gelu", residual), linear_ref(x, w, bias, "gelu", residual, dtype))
+    assert "rows of W from" in gq._lib.last_kernel()
+    close(ops.dense_linear(x, w, out_dtype=torch.float32), linear_ref(x, w, None, None, None, torch.float32))
+    close(ops.dense_linear_gated(x, w, bias), gated_ref(x, w, bias, "silu", dtype))
+    assert "rows of W from" in gq._lib.last_kernel() and "gated" in gq._lib.last_kernel()
+
+
+@pytest.mark.parametrize("m,n,k", [(2048, 9008, 264), (777, 28680, 520)])
+def test_columns_that_another_form_takes_in_a_graph(m, n, k):
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, w = (torch.randn(r, k, generator=g, device="cuda").to(torch.float16) for r in (m, n))
+    ops.dense_linear(x, w), ops.dense_linear_gated(x, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, b = ops.dense_linear(x, w, activation="relu"), ops.dense_linear_gated(x, w)
+        assert "rows of W from" in gq._lib.last_kernel()
+    for _ in range(3):
+        x.copy_(torch.randn(m, k, generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, ops.dense_linear(x, w, activation="relu")) and torch.equal(b, ops.dense_linear_gated(x, w))
