@@ -7,7 +7,7 @@ import torch
 
 import mlc_llm_amd as gq
 from mlc_llm_amd import ops
-from test_gpu_dense import close, gated_ref, linear_ref
+from test_gpu_dense import close, gated_ref, linear_ref, moe_ref
 
 HALVES = [torch.float16, torch.bfloat16]
 pytestmark = pytest.mark.gpu
@@ -156,3 +156,26 @@ def test_columns_that_another_form_takes_in_a_graph(m, n, k):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(a, ops.dense_linear(x, w, activation="relu")) and torch.equal(b, ops.dense_linear_gated(x, w))
+
+
+# x in registers with four, eight and sixteen experts a lane of the routing, the fullest tables last: 512 experts, 2048 slots
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t,hidden,inter,experts,k", [(64, 2048, 1024, 128, 8), (64, 1600, 1032, 200, 8), (64, 3600, 1024, 130, 5), (64, 1544, 1024, 300, 32), (64, 2048, 1024, 512, 32),
+                                                      (48, 4096, 1024, 70, 32), (64, 3592, 1024, 257, 9)])
+def test_x_in_registers_of_many_experts(t, hidden, inter, experts, k, dtype):
+    g = torch.Generator(device="cuda").manual_seed(hidden + experts)
+    x = torch.randn(t, hidden, generator=g, device="cuda").to(dtype)
+    w13 = torch.empty(experts, 2 * inter, hidden, dtype=dtype, device="cuda")
+    w2 = torch.empty(experts, hidden, inter, dtype=dtype, device="cuda")
+    for w in (w13, w2):
+        for part in w:
+            part.copy_(torch.randn(part.shape, generator=g, device="cuda") / part.shape[1] ** 0.5)
+    logits = torch.randn(t, experts, generator=g, device="cuda")
+    for skewed in (False, True):
+        if skewed:  # all tokens to the last experts
+            logits[:, -k:] += 20.0
+        weights, ids = ops.moe_gating(logits, k)
+        got = ops.dense_moe(x, logits, w13, w2, k)
+        assert gq._lib.last_kernel().endswith("x kept")
+        close(got, moe_ref(x, weights, ids, w13, w2, "silu", dtype))
+        assert torch.equal(got, ops.dense_moe(x, logits, w13, w2, k))
