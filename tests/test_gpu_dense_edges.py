@@ -118,6 +118,7 @@ def test_infinities_of_the_second_product(t, experts, dtype):
     if dtype == torch.bfloat16:
         w13[1, 130, 0] = w13[1, inter + 130, 0] = 2.0**100  # 9 * 2^200
     else:
+        w13[1, :, 0] = 100.0  # the others 9 * 10^4
         w13[1, 130, 0] = math.inf
     got = ops.dense_moe(x, logits, w13, w2, 1, activation=None)
     others = [n for n in range(hidden) if n not in (7, 9)]
@@ -179,3 +180,101 @@ def test_x_in_registers_of_many_experts(t, hidden, inter, experts, k, dtype):
         assert gq._lib.last_kernel().endswith("x kept")
         close(got, moe_ref(x, weights, ids, w13, w2, "silu", dtype))
         assert torch.equal(got, ops.dense_moe(x, logits, w13, w2, k))
+
+
+def _filled(g, dtype, *shape, scale=1.0):
+    """Normal numbers, a part of the rows at a time."""
+    w = torch.empty(shape, dtype=dtype, device="cuda")
+    for part in w.view(-1, shape[-1]).split(max(1, (1 << 27) // shape[-1])):
+        part.copy_(scale * torch.randn(part.shape, generator=g, device="cuda"))
+    return w
+
+
+def _whole(g, dtype, *shape):
+    """Whole numbers of at most 8."""
+    return _filled(g, dtype, *shape, scale=4.0).clamp_(-8, 8).round_()
+
+
+def _few(g, dtype, rows, k):
+    """Rows of 48 whole numbers of at most 8 among zeros, the last number of a row among them: products with _whole's are exact in float32, in any order."""
+    x = torch.zeros(rows, k, dtype=dtype, device="cuda")
+    at = torch.randint(0, k, (rows, 48), generator=g, device="cuda")
+    at[:, 0] = k - 1
+    return x.scatter_(1, at, _whole(g, dtype, rows, 48))
+
+
+LONGEST = (1 << 23) - 136
+
+
+@pytest.mark.parametrize("form", [-1, 0, 10])
+@pytest.mark.parametrize("m,n", [(1, 24), (7, 40), (12, 24), (60, 72), (300, 280)])
+def test_longest_rows(m, n, form):
+    """K just below the limit: a tile's offsets come near 2^32 bytes."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, w = _few(g, torch.bfloat16, m, LONGEST), _whole(g, torch.bfloat16, n, LONGEST)
+    want = torch.cat([r[:, r[0] != 0].double() @ w[:, r[0] != 0].double().t() for r in x.split(1)])
+    gq._lib.set_option("gemm_variant", form)
+    gq._lib.set_option("gemm_split_k", -1 if form < 0 else 1)
+    try:
+        assert torch.equal(ops.dense_linear(x, w, out_dtype=torch.float32).double(), want)
+        got = ops.dense_linear_gated(x, w, activation=None, out_dtype=torch.float32)
+        assert torch.equal(got.double(), want[:, : n // 2] * want[:, n // 2 :])
+    finally:
+        gq._lib.set_option("gemm_variant", -1)
+        gq._lib.set_option("gemm_split_k", -1)
+
+
+@pytest.mark.parametrize("t,hidden,inter,experts,k", [(3, LONGEST, 8, 3, 2), (64, LONGEST, 8, 2, 1), (5, 8, LONGEST, 3, 2), (64, 16, LONGEST, 2, 1)])
+def test_longest_rows_of_an_expert_layer(t, hidden, inter, experts, k):
+    g = torch.Generator(device="cuda").manual_seed(t)
+    dtype = torch.bfloat16
+    x = _few(g, dtype, t, hidden) if hidden > 48 else _whole(g, dtype, t, hidden)
+    w13 = _whole(g, dtype, experts, 2 * inter, hidden)
+    w2 = torch.zeros(experts, hidden, inter, dtype=dtype, device="cuda")  # two numbers other than 0 in a row, one of them in its last eight
+    w2.scatter_(2, torch.randint(0, inter, (experts, hidden, 1), generator=g, device="cuda"), 1.0)
+    w2.scatter_(2, torch.randint(inter - 8, inter, (experts, hidden, 1), generator=g, device="cuda"), -1.0)
+    logits = torch.full((t, experts), -60.0, device="cuda")
+    ids = torch.stack([torch.randperm(experts, generator=g, device="cuda")[:k] for _ in range(t)])
+    logits.scatter_(1, ids, 30.0)
+    want = torch.zeros(t, hidden, dtype=torch.float64, device="cuda")
+    for e in range(experts):
+        rows = (ids == e).any(1)
+        some = x[rows].ne(0).any(0)
+        gate, up = (x[rows][:, some].double() @ w13[e][:, some].double().t()).chunk(2, 1)
+        used = w2[e].ne(0).any(0)
+        want[rows] += (gate * up)[:, used] @ w2[e][:, used].double().t() / k
+    got = ops.dense_moe(x, logits, w13, w2, k, activation=None)
+    assert torch.equal(got, want.float().to(dtype))
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t,hidden,inter,experts,k", [(1, 256, 128, 8, 2), (16, 2048, 768, 16, 4), (64, 2048, 1024, 4, 2)])
+def test_output_of_an_expert_layer_in_place_of_x(t, hidden, inter, experts, k, dtype):
+    g = torch.Generator(device="cuda").manual_seed(hidden)
+    x, logits = _filled(g, dtype, t, hidden), torch.randn(t, experts, generator=g, device="cuda")
+    w13, w2 = _filled(g, dtype, experts, 2 * inter, hidden, scale=hidden**-0.5), _filled(g, dtype, experts, hidden, inter, scale=inter**-0.5)
+    want = ops.dense_moe(x, logits, w13, w2, k)
+    size = gq._lib.lib().mi355gq_dense_moe_workspace_bytes(t, hidden, inter, experts, k)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    gq._lib.call("mi355gq_dense_moe", x.data_ptr(), logits.data_ptr(), None, t, hidden, inter, experts, k, 0, 1, 1, 1, 1.0, ops._MODEL_DTYPES[logits.dtype],
+                 w13.data_ptr(), w2.data_ptr(), ops._activation("silu"), ops._MODEL_DTYPES[dtype], x.data_ptr(), ws.data_ptr(), size, ops._stream())
+    assert torch.equal(x, want)
+
+
+def test_two_expert_layers_at_once():
+    """Calls of two streams, each with scratch of its own."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    layers = []
+    for t, hidden, inter, experts, k, dtype in ((9, 1024, 776, 24, 3, torch.float16), (64, 2048, 1024, 8, 2, torch.bfloat16)):
+        args = [_filled(g, dtype, t, hidden), torch.randn(t, experts, generator=g, device="cuda"), _filled(g, dtype, experts, 2 * inter, hidden, scale=hidden**-0.5),
+                _filled(g, dtype, experts, hidden, inter, scale=inter**-0.5), k]
+        layers.append((args, ops.dense_moe(*args), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (args, _, stream) in enumerate(layers):
+            with torch.cuda.stream(stream):
+                got[i].append(ops.dense_moe(*args))
+    torch.cuda.synchronize()
+    for i, (_, want, _) in enumerate(layers):
+        assert all(torch.equal(y, want) for y in got[i])
