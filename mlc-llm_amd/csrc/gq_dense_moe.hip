@@ -51,14 +51,20 @@ inline double experts_chosen(int64_t T, int64_t experts, int64_t k) {
 // 16, and x, which comes half as often, goes straight into registers (each pair in the same memory): 8 experts of 4096 x 14336, 2 a token, 32 tokens 213 -> 200 us, 48 226 -> 213; 16
 // experts of 7168 x 2048, 4 a token, 32 tokens 110 -> 95; (16 tokens of 128 experts of 2048 x 768, 8 a token, would take 48 and take 46).
 inline int moe_eights(int64_t T, int64_t experts, int64_t k) { return T > 8 && T * k > 4 * experts ? 2 : 1; }
-// Workgroups that share the K (all chosen experts' inter) of sixteen columns in the second kernel: about one a unit (sixteen tokens
-// of 128 experts, 128 tiles: 131 us with two shares, 159 with one and 136 with four; 224 tiles: 212 with one, 219 with two).
+// Workgroups that share the K (all chosen experts' inter) of the columns of one in the second kernel: about one a unit.  About two, in up to four shares, where
+// segments have eight rows and less than two blocks a wave, which is as much arithmetic between loads (planes, joins) as loads, and a unit has the LDS for two.
+// The second kernel's us, with 1, 2, 4 and 8 shares: 128 experts, 8 a token, 16 tokens, 2048 x 768 97, 51.5, 47.9 and 49.5 (the rule: 4), 3584 x 768 102, 80, 80
+// and 77 (2), 1024 x 768 80, 45, 27 and 28 (4).  More blocks a wave: 16 tokens of 8 experts of 4096 x 14336 164 with 1 (the rule), 170 with 2; a token of 64
+// experts of 2048 x 1408 13.4, 10.7, 11.9 and 16.3 (2).  One a unit: 64 tokens of 128 experts of 2048 x 768 88 with 2 (the rule), 95 with 4.
 inline int moe_shares(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k) {
   if (options().gemm_split_k > 0) return options().gemm_split_k < 8 ? options().gemm_split_k : 8;
-  const int64_t tiles = moe_eights(T, experts, k) == 2 ? (hidden + 31) / 32 : (hidden + 15) / 16;
+  const bool eight = moe_eights(T, experts, k) == 1;
+  const int64_t tiles = eight ? (hidden + 15) / 16 : (hidden + 31) / 32;
   const double blocks = experts_chosen(T, experts, k) * static_cast<double>((inter + kStreamBlock - 1) / kStreamBlock);
   int s = 1;
   while (s < 8 && tiles * s < 200 && blocks / (2 * s) >= 4 * kWaves) s *= 2;
+  const bool two = eight && inter < 2 * kWaves * kStreamBlock && T * (512 + 16 * k) <= 16384;  // (80 KiB less two stages a wave)
+  while (two && s < 4 && tiles * s < 400 && blocks / (2 * s) >= 8 * kWaves) s *= 2;
   return s;
 }
 
