@@ -47,24 +47,20 @@ inline double experts_chosen(int64_t T, int64_t experts, int64_t k) {
   for (int64_t t = 0; t < T; ++t) none *= 1 - static_cast<double>(k) / static_cast<double>(experts);
   return static_cast<double>(experts) * (1 - none);
 }
-// Eights of rows of a segment: sixteen rows where experts have more than four on average.  The second kernel then takes 32 columns a workgroup and not
-// 16, and x, which comes half as often, goes straight into registers (each pair in the same memory): 8 experts of 4096 x 14336, 2 a token, 32 tokens 213 -> 200 us, 48 226 -> 213; 16
-// experts of 7168 x 2048, 4 a token, 32 tokens 110 -> 95; (16 tokens of 128 experts of 2048 x 768, 8 a token, would take 48 and take 46).
-inline int moe_eights(int64_t T, int64_t experts, int64_t k) { return T > 8 && T * k > 4 * experts ? 2 : 1; }
-// Workgroups that share the K (all chosen experts' inter) of the columns of one in the second kernel: about one a unit.  About two, in up to four shares, where
-// segments have eight rows and less than two blocks a wave, which is as much arithmetic between loads (planes, joins) as loads, and a unit has the LDS for two.
-// The second kernel's us, with 1, 2, 4 and 8 shares: 128 experts, 8 a token, 16 tokens, 2048 x 768 97, 51.5, 47.9 and 49.5 (the rule: 4), 3584 x 768 102, 80, 80
-// and 77 (2), 1024 x 768 80, 45, 27 and 28 (4).  More blocks a wave: 16 tokens of 8 experts of 4096 x 14336 164 with 1 (the rule), 170 with 2; a token of 64
-// experts of 2048 x 1408 13.4, 10.7, 11.9 and 16.3 (2).  One a unit: 64 tokens of 128 experts of 2048 x 768 88 with 2 (the rule), 95 with 4.
+// Eights of rows of a segment: sixteen rows but for one token, whose experts have one each.  The second kernel takes 16 columns a workgroup then, and 32 with
+// sixteen rows, where x, which comes half as often, goes straight into registers.  Its us with eights / sixteens: one token, 6 of 64 experts of 2048 x 1408, 10.5 /
+// 11.8, 2 of 8 of 4096 x 14336 37.9 / 40.7; 2 tokens, 8 of 64 of 3584 x 2560, 49.5 / 48.3; 4 tokens, 2 of 8 of 4096 x 14336, 105 / 102, 32 tokens 240 / 169; 16
+// tokens, 8 of 128 of 2048 x 768, 50 / 46, 64 tokens 93 / 73.
+inline int moe_eights(int64_t T) { return T > 1 ? 2 : 1; }
+// Workgroups that share the K (all chosen experts' inter) of the columns of one in the second kernel: about one a unit.  The second kernel's us with 1, 2,
+// 4 and 8 shares: one token of 64 experts of 2048 x 1408, 128 tiles, 13.4, 10.3, 11.8 and 16.3 (the rule: 2); 16 tokens of 128 of 2048 x 768, 64 tiles, 123, 67, 46
+// and 51 (4); 32 tokens of 16 of 7168 x 2048, 224 tiles, 87, 95, 98 and 106 (1).
 inline int moe_shares(int64_t T, int64_t hidden, int64_t inter, int64_t experts, int64_t k) {
   if (options().gemm_split_k > 0) return options().gemm_split_k < 8 ? options().gemm_split_k : 8;
-  const bool eight = moe_eights(T, experts, k) == 1;
-  const int64_t tiles = eight ? (hidden + 15) / 16 : (hidden + 31) / 32;
+  const int64_t tiles = moe_eights(T) == 2 ? (hidden + 31) / 32 : (hidden + 15) / 16;
   const double blocks = experts_chosen(T, experts, k) * static_cast<double>((inter + kStreamBlock - 1) / kStreamBlock);
   int s = 1;
   while (s < 8 && tiles * s < 200 && blocks / (2 * s) >= 4 * kWaves) s *= 2;
-  const bool two = eight && inter < 2 * kWaves * kStreamBlock && T * (512 + 16 * k) <= 16384;  // (80 KiB less two stages a wave)
-  while (two && s < 4 && tiles * s < 400 && blocks / (2 * s) >= 8 * kWaves) s *= 2;
   return s;
 }
 
@@ -73,17 +69,17 @@ inline int moe_blocks(int64_t hidden) { return static_cast<int>((hidden + kWaves
 // Whether the first kernel keeps x in registers, in segments of 32 rows, rather than load it beside W, in segments of 8 or 16.  It does where that
 // fits (4 blocks a wave, or 7 and 8) and a segment is long enough for the wait that each change of x is.  The first kernel's us, with W / kept
 // in the same memory:
-// 8 experts of 4096 x 14336, 2 a token, 4 tokens 204 / 204, 8 tokens 298 / 284, 32 348 / 328, 48 373 / 327, 64 553 / 323; 64 of 64 experts of 2048 x
-// 1408, 6 a token, 156 / 150; 128 experts of 2048 x 768, 8 a token, 16 tokens 99 / 108, 64 tokens 141 / 147.
+// 8 experts of 4096 x 14336, 2 a token, 4 tokens 194 / 193, 8 tokens 262 / 262, 16 285 / 280, 32 299 / 285, 48 324 / 290, 64 476 / 300; 64 of 64 experts of 2048 x
+// 1408, 6 a token, 127 / 127; 128 experts of 2048 x 768, 8 a token, 16 tokens 85 / 92, 64 tokens 137 / 138.
 inline bool moe_keeps(const DenseMoeArgs& a) {
   const int blocks = moe_blocks(a.hidden);
   return (blocks == 4 || blocks == 7 || blocks == 8) && a.T * a.k >= 2 * a.experts && a.inter >= 1024;
 }
 
 // Rows of a segment of the second kernel: 32 where the first one keeps x and experts have more than twelve on average (64 tokens, 2 of 8 experts of 4096
-// x 14336, 302 -> 232 us; 48 tokens would take 221 and take 213).
+// x 14336, 269 -> 235 us; 48 tokens would take 213 and take 191).
 inline int moe_down_rows(const DenseMoeArgs& a) {
-  return moe_keeps(a) && a.T * a.k > 12 * a.experts ? 32 : 8 * moe_eights(a.T, a.experts, a.k);
+  return moe_keeps(a) && a.T * a.k > 12 * a.experts ? 32 : 8 * moe_eights(a.T);
 }
 
 struct MoeTables {  // in LDS, in front of the rest
@@ -640,7 +636,7 @@ static hipError_t launch_up(const DenseMoeArgs& a, const MoeLayout& layout, int 
 
 template <bool BF, int XG, int C>
 static hipError_t launch_down(const DenseMoeArgs& a, const MoeLayout& layout, hipStream_t s) {
-  constexpr int D = 2;  // (two workgroups a unit with two blocks ahead, C 1: one with four was 1 to 10 % behind)
+  constexpr int D = 2;  // (three blocks ahead, C 1: one token of 64 experts of 2048 x 1408 10.5 -> 11.5 us)
   const int shares = moe_shares(a.T, a.hidden, a.inter, a.experts, a.k);
   const dim3 grid(static_cast<unsigned>((a.hidden + 16 * C - 1) / (16 * C)), static_cast<unsigned>(shares));
   note_kernel("dense_moe up to %d rows, %d shares%s", 8 * XG, shares, moe_keeps(a) ? ", x kept" : "");
@@ -674,14 +670,15 @@ static hipError_t launch(const DenseMoeArgs& a, hipStream_t s) {
   hipError_t e = hipErrorNotSupported;
   if (moe_keeps(a)) e = moe_blocks(a.hidden) == 4 ? up(four, four, four) : up(four, four, eight);
   if (e == hipErrorNotSupported) e = up(rows, four, none);
-  if (e == hipErrorNotSupported) e = up(rows, two, none);  // (many slots: their tables take the room)
+  if constexpr (XG == 2)
+    if (e == hipErrorNotSupported) e = up(rows, two, none);  // (many slots: their tables take the room)
   if (e != hipSuccess) return e;
-  if constexpr (XG == 1) return launch_down<BF, 1, 1>(a, layout, s);  // (8 tokens, or few an expert)
+  if constexpr (XG == 1) return launch_down<BF, 1, 1>(a, layout, s);  // (one token)
   else return down_rows == 32 ? launch_down<BF, 4, 2>(a, layout, s) : launch_down<BF, 2, 2>(a, layout, s);
 }
 
 hipError_t launch_dense_moe(const DenseMoeArgs& a, hipStream_t s) {
-  const int eights = moe_eights(a.T, a.experts, a.k);
+  const int eights = moe_eights(a.T);
   if (a.bf16) return eights == 1 ? launch<true, 1>(a, s) : launch<true, 2>(a, s);
   return eights == 1 ? launch<false, 1>(a, s) : launch<false, 2>(a, s);
 }
