@@ -73,8 +73,8 @@ __device__ __forceinline__ float dense_sigmoid(float v) {
 }
 
 // v Phi(v).  Phi(-a) = exp(-a^2 / 2) t P(t), t = 1 / (1 + 0.3 a), for a >= 0: the factor behind the exponential is smooth in t, and P is the
-// Chebyshev interpolation of degree 7 of it over 0 <= a <= 14, beyond which Phi(-a) is 0 in float32.  Relative error 5e-7 of Phi(-a), so
-// also far out on the negative side.  (The C library's erfc takes three times the instructions; the epilogue of 2048 x 14336 results of
+// Chebyshev interpolation of degree 7 of it over 0 <= a <= 14, beyond which Phi(-a) is 0 in float32.  t P(t) is good to 4.5e-7 of its value.  The exponential has its
+// argument in float32, which adds up to 2^-24 a^2 on the negative side: 1.5e-6 of Phi(-5) in all, 8e-6 of Phi(-12).  (The C library's erfc takes three times the instructions; the epilogue of 2048 x 14336 results of
 // a large product is otherwise idle time of its matrix cores.)
 __device__ __forceinline__ float dense_gelu(float v) {
   const float a = __builtin_fabsf(v), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3f, a, 1.0f));

@@ -2,14 +2,14 @@
 //
 //   y_t = sum over j of w_tj  W2[e_tj] h_tj,  h_tj = act(Wg[e_tj] x_t) * (Wu[e_tj] x_t),  (w, e)_t the routing of token t
 //
-// The first routes (every workgroup all tokens for itself: a microsecond, where a launch of its own and its results' way through memory
-// are three) and streams the gate and up rows of the experts that some token chose past these experts' tokens.  A row of w h, the
+// The first routes (every workgroup all tokens for itself: 2.7 us, where a launch of its own takes as long before its results' way through
+// memory) and streams the gate and up rows of the experts that some token chose past these experts' tokens.  A row of w h, the
 // weighted activation of one token and expert, goes to the workspace in float32.
 // The second streams the down rows past the same rows of w h, which go through the matrix instruction as two or three 16-bit planes (down_planes); what
 // comes out of an expert joins the sums of its tokens, which lie in LDS.  An expert meets the tokens that chose it alone, whatever W or the other tokens hold.
-// Bound by HBM.  Both kernels, us (of their bytes at 6.85 TB/s): one token, 6 of 64 experts of 2048 x 1408, 27.5 (15.2); 2 of 8 experts of 4096 x 14336,
-// 4 tokens 290 (283), 16 tokens 440 (411), 32 tokens 447 (411), 64 tokens 527 (411), where the way of x from the L2 counts beside W's; 16 tokens, 8
-// of 128 experts of 2048 x 768, 126 (114).  In memory that a process has given back and taken again all of these take 10 to 20 % more.
+// Bound by HBM.  Both kernels, us (of their bytes at 6.85 TB/s): one token, 6 of 64 experts of 2048 x 1408, 27.8 (15.2); 2 of 8 experts of 4096 x 14336,
+// 4 tokens 296 (283), 16 tokens 431 (411), 32 tokens 454 (411), 64 tokens 533 (411), where the way of x from the L2 counts beside W's; 16 tokens, 8
+// of 128 experts of 2048 x 768, 130 (118).  In memory that a process has given back and taken again all of these take 10 to 20 % more.
 #include "gq_dense_stream.hpp"
 #include "gq_gating.hpp"
 

@@ -111,7 +111,7 @@ DensePlan plan_of(int64_t rows, int64_t N, int64_t K, bool only_whole = false) {
   return best;
 }
 
-// The plan of a call, made for its workspace and needed again for its launch right behind: 2 us of arithmetic.
+// The plan of a call, made for its workspace and needed again for its launch right behind: 4 to 9 us of arithmetic, by sizes.
 DensePlan plan_for(int64_t rows, int64_t N, int64_t K) {
   struct Last {
     int64_t rows = 0, N, K;

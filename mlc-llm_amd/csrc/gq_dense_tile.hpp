@@ -1,7 +1,7 @@
 // Products with 16-bit weights of more than a few rows: tiles through LDS on v_mfma_f32_16x16x32.
 //
 // Large ones are bound by the matrix pipe and the card's power: 256 x 256 tiles of 8192 x 8192 x 8192 keep the pipe 66 % busy at 1.79 GHz, 1395 TFLOP/s;
-// 2048 rows of 28672 x 4096, gated, 364 us (1320 TFLOP/s), of 14336 x 4096 with bias and gelu 212.  The 32x32x16 instruction, with half the reads of operands, lets the
+// 2048 rows of 28672 x 4096, gated, 355 to 369 us, by card (1305 to 1355 TFLOP/s), of 14336 x 4096 with bias and gelu 205 to 218.  The 32x32x16 instruction, with half the reads of operands, lets the
 // clock fall further and came out 3 to 8 % slower.  Below some 200 rows the bound is HBM: 48 rows of 4096 x 14336 26.0 us (4.5 TB/s of weights, the join
 // included), 16 of 128256 x 4096 163 (6.4).
 #pragma once

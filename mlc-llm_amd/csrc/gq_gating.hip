@@ -1,4 +1,4 @@
-// Routing of 8-bit block-scaled expert layers: scores, selection in groups of experts, weights; the stable order of the
+// Routing of expert layers: scores, selection in groups of experts, weights; the stable order of the
 // slots by expert; the weighted sum over a token's experts.  Small integer and float32 work, bound by latency.
 #include "gq_gating.hpp"
 
