@@ -21,7 +21,7 @@ def _pow2(exponents):
     return 2.0 ** torch.as_tensor(exponents, dtype=torch.float64)
 
 
-# Whole numbers times powers of two.  x has 48 numbers other than 0 in a row, of at most 8, as W13's: a gate or an up value is at most 48 * 64 = 3072 units, most
+# Whole numbers times powers of two.  x has 48 numbers other than 0 in a row, of at most 8, as W13's: a gate or an up value is at most 48 * 64 units, most
 # are below 1000, and their product takes up to 23 bits.  Experts of equal logits weigh 1, 1/2 or 1/4.  A row of W2 has four numbers other than 0, so that all sums of
 # products stay below 2^24 units (asserted below) and are exact in float32, in any order.  The one rounding is the output's.
 def _layer(g, dtype, t, hidden, inter, experts, k, x_exp, gate_exp, up_exp, w2_exp, without=()):
